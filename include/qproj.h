@@ -236,6 +236,93 @@ int qproj_moe_ffn(qproj_ctx *ctx, const qproj_weight *gate_exps, const qproj_wei
                   const qproj_weight *down_exps, const float *x_dev, const int32_t *ids_dev,
                   const float *weights_dev, int64_t n_used, int64_t B, float *y_dev, int act);
 
+/* ---- between the q/k/v projections and the output projection ------------------------------------------------
+ * llama.cpp's build_attn reaches these through the same context.decode
+ * (/root/reference/inference/crates/icn-engine/src/lib.rs:2264): GGML_OP_ROPE on q and k, the copies of k and v into the
+ * cache, GGML_OP_FLASH_ATTN_EXT.  All rows are fp32, all pointers 16-byte aligned, strides multiples of 4 floats, nothing is
+ * allocated but once (see qproj_attention), nothing synchronises. */
+
+/* The rotation's frequencies in 64 bits, on the HOST: freqs[i] for pair i of n_dims / 2, and what cosines and sines are
+ * multiplied by.  A caller makes the table once per model and keeps it on the device.
+ *   freqs[i] = base^(-2i / n_dims) / factors[i] (factors may be null: 1), stretched by freq_scale (positions four times as
+ *   far: 0.25).  YaRN (ext_factor > 0): pairs that turn more than beta_fast times over n_ctx_orig tokens keep their
+ *   frequency, those of less than beta_slow turns are stretched, a ramp between; *magnitude = attn_factor *
+ *   (1 + 0.1 ln(1 / freq_scale)), and attn_factor without YaRN. */
+typedef struct qproj_rope_scaling {
+    double base;
+    double freq_scale;
+    const float *factors;
+    int64_t n_ctx_orig;
+    float ext_factor, attn_factor, beta_fast, beta_slow;
+} qproj_rope_scaling;
+int qproj_rope_frequencies(const qproj_rope_scaling *scaling, int64_t n_dims, double *freqs, float *magnitude);
+
+/* Rotation of the first n_dims values of every head (a multiple of 8; the rest of the head stays):
+ *   (a, b) -> magnitude * (a cos - b sin, a sin + b cos),   angle = pos[token] * freqs[i]
+ * PAIRS: a, b are values 2i, 2i + 1 (ggml's normal order); HALVES: values i, i + n_dims / 2 (NeoX order). */
+enum qproj_rope_mode { QPROJ_ROPE_PAIRS = 0, QPROJ_ROPE_HALVES = 1 };
+typedef struct qproj_rotation {
+    const int32_t *pos_dev;   /* [n_tokens] */
+    const double *freqs_dev;  /* [n_dims / 2], radians a position */
+    int64_t n_dims;
+    int mode;
+    float magnitude;
+} qproj_rotation;
+
+/* GGML_OP_ROPE: y = x rotated, rows of n_head heads of head_dim values (a multiple of 8, at most 1024), a token's row every
+ * x_stride / y_stride floats.  y may be x (with the same stride); any other overlap is not allowed.  Angles and products are
+ * taken in 64 bits and rounded once. */
+int qproj_rope(qproj_ctx *ctx, const qproj_rotation *rotation, const float *x_dev, int64_t x_stride, int64_t n_tokens,
+               int64_t n_head, int64_t head_dim, float *y_dev, int64_t y_stride);
+
+/* A cache of keys and values held in 4 bits (ggml's Q4_0: blocks of 32 values, d * (n - 8)), in pages that any sequence
+ * may use.  The four planes are device memory of the caller, who decides which page is whose:
+ *   codes  uint8 [n_pages][n_head_kv][page_tokens][head_dim / 2],  scales fp16 [n_pages][n_head_kv][page_tokens][head_dim / 32]
+ * page_tokens is 16, 32, 64, 128 or 256; head_dim is 64, 96, 128 or 256.  Values' codes lie in order, two a byte, the first in
+ * the low half; keys' codes in words of eight, word w of a row of B blocks holding values 8 * (w / B) .. + 7 of block
+ * w % B.  Write through qproj_kv_append; pages may be copied whole. */
+typedef struct qproj_kv_cache {
+    void *k_codes, *k_scales, *v_codes, *v_scales;
+    int64_t n_pages;
+    int64_t page_tokens;
+    int64_t n_head_kv;
+    int64_t head_dim;
+} qproj_kv_cache;
+
+/* Keys and values of n_tokens tokens (rows of n_head_kv heads every k_stride / v_stride floats) into the places
+ * slots_dev[i] = page * page_tokens + place in the page, the keys rotated on the way (rotation null: as they are).  Each block:
+ * d = its value of largest magnitude (the first of them) / -8, n = min(15, trunc(x / d + 8.5)), as ggml's
+ * quantize_row_q4_0; a block with a value that is not finite or whose scale passes fp16 is NaN as a whole.  A negative slot is
+ * left out (padding); one behind the cache is left out and reported by the next qproj_sync.  The slots of one call are
+ * distinct: of two tokens in one place neither is kept whole.
+ * q_dev (null: none) is rotated beside, in the same launch: n_head heads of head_dim, into q_out_dev as qproj_rope does. */
+int qproj_kv_append(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *k_dev, int64_t k_stride, const float *v_dev,
+                    int64_t v_stride, int64_t n_tokens, const int64_t *slots_dev, const qproj_rotation *rotation,
+                    const float *q_dev, int64_t q_stride, int64_t n_head, float *q_out_dev, int64_t q_out_stride);
+
+/* What the cache holds at n places, as fp32 [n][n_head_kv][head_dim] (k_out_dev or v_out_dev may be null): to save a sequence,
+ * or to move it.  Negative slots are rows of zeros; so are those behind the cache, which the next qproj_sync reports. */
+int qproj_kv_read(qproj_ctx *ctx, const qproj_kv_cache *kv, const int64_t *slots_dev, int64_t n, float *k_out_dev,
+                  float *v_out_dev);
+
+/* Attention of the newest tokens of n_seq sequences over their keys and values in the cache (their own among them).
+ *   rows q_start_dev[s] .. q_start_dev[s + 1] - 1 of q_dev are the last tokens of sequence s (at most max_q of them), which
+ *   has kv_len_dev[s] tokens in the cache: token t in page pages_dev[s * pages_stride + t / page_tokens];
+ *   the row at position p = kv_len - (rows of s behind it) - 1 sees tokens t <= p, and of those the last `window` (0: all);
+ *   y = sum_t softmax_t(scale * q . k_t) v_t,  keys and values as the cache holds them, fp32 throughout.
+ * n_head is a multiple of n_head_kv; head h reads key/value head h / (n_head / n_head_kv).  Rows that see nothing are zeros;
+ * rows before q_start_dev[0] and from q_start_dev[n_seq] on are left as they were.  Bounds on the device are checked there: q_start_dev has to ascend
+ * within [0, n_tokens] by at most max_q, kv_len_dev to lie in [0, pages_stride * page_tokens], the pages that are read in
+ * [0, n_pages); a sequence that breaks the first two is left out, the tokens of a bad page are not seen, and the next
+ * qproj_sync reports it.  Every value accumulates in fp32; operands go to the matrix cores as fp16 pairs of 22 bits.  The
+ * result of a row depends on what else is in the call only in the order of its sums.  y must not overlap q.
+ * Workspace: a fixed buffer of the context, allocated by its first call, which therefore cannot be captured into a graph;
+ * later ones can.  Two captured calls of one context share it: replay them on one stream, or one after the other. */
+int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens,
+                    int64_t n_head, int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q,
+                    const int32_t *pages_dev, int64_t pages_stride, float scale, int64_t window, float *y_dev,
+                    int64_t y_stride);
+
 /* Backend eligibility probe: what the reference's server asks of a GPU runtime before it offers the
  * backend pack that needs it (/root/reference/inference/crates/icn-server/src/cuda_driver.rs:343-401
  * inspect(): initialise, driver version, device count, one architecture string and one hardware label per

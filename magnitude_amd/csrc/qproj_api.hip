@@ -2,6 +2,7 @@
 #include "../../include/qproj.h"
 
 #include <dlfcn.h>
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -12,6 +13,7 @@
 #include <new>
 #include <string>
 
+#include "kv_cache.h"
 #include "qproj_internal.h"
 
 using namespace qproj;
@@ -81,7 +83,7 @@ struct qproj_ctx {
     size_t ws_bytes = 0;
     uint8_t *ws2 = nullptr;     // second scratch: gate and up outputs of the unfused FFN front end
     size_t ws2_bytes = 0;
-    int32_t *flag_dev = nullptr;  // raised by kernels that meet bad device-side input
+    int32_t *flag_dev = nullptr;  // raised by kernels that meet bad device-side input: [0] expert ids, [1] the cache's (kKvBad*)
 };
 
 struct qproj_weight {
@@ -835,13 +837,16 @@ int qproj_ctx_destroy(qproj_ctx *ctx) {
 int qproj_sync(qproj_ctx *ctx) {
     if (!ctx) return QPROJ_ERR_INVALID_ARG;
     QP_HIP(ctx, hipSetDevice(ctx->device));
-    int32_t flag = 0;
-    QP_HIP(ctx, hipMemcpyAsync(&flag, ctx->flag_dev, sizeof flag, hipMemcpyDeviceToHost, ctx->stream));
+    int32_t flag[2] = {0, 0};
+    QP_HIP(ctx, hipMemcpyAsync(flag, ctx->flag_dev, sizeof flag, hipMemcpyDeviceToHost, ctx->stream));
     QP_HIP(ctx, hipStreamSynchronize(ctx->stream));
-    if (flag) {
+    if (flag[0] || flag[1]) {
         QP_HIP(ctx, hipMemsetAsync(ctx->flag_dev, 0, sizeof flag, ctx->stream));
         QP_HIP(ctx, hipStreamSynchronize(ctx->stream));
-        return fail(ctx, QPROJ_ERR_INVALID_ARG, "expert id outside [0, n_expert) in a MUL_MAT_ID batch");
+        if (flag[0]) return fail(ctx, QPROJ_ERR_INVALID_ARG, "expert id outside [0, n_expert) in a MUL_MAT_ID batch");
+        if (flag[1] & kKvBadSlot) return fail(ctx, QPROJ_ERR_INVALID_ARG, "a slot behind the key/value cache");
+        if (flag[1] & kKvBadPage) return fail(ctx, QPROJ_ERR_INVALID_ARG, "a page outside [0, n_pages) in an attention call");
+        return fail(ctx, QPROJ_ERR_INVALID_ARG, "q_start or kv_len out of bounds in an attention call");
     }
     return QPROJ_OK;
 }
@@ -1624,6 +1629,216 @@ int qproj_moe_ffn(qproj_ctx *ctx, const qproj_weight *gate, const qproj_weight *
         QP_HIP(ctx, launch_gemv_q8act(gd, mt, (int)E, ctx->stream));
     QP_HIP(ctx, launch_moe_combine(e, weights_dev, B, n_used, d_model, y_dev, ctx->stream));
     return QPROJ_OK;
+}
+
+// ---- rotary positions, the paged 4-bit cache and attention over it ----
+
+static bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// rows of n_head heads of head_dim floats, a token's every `stride`: null if they can be taken, otherwise what is wrong
+static const char *bad_rows(const float *p, int64_t stride, int64_t n_head, int64_t head_dim) {
+    if (!p) return "null argument";
+    if (!aligned16(p)) return "rows must be 16-byte aligned";
+    if (stride < n_head * head_dim || stride % 4 != 0 || stride > (int64_t)1 << 40) return "a row stride must be a multiple of 4 floats and hold a row";
+    return nullptr;
+}
+
+static const char *bad_rotation(const qproj_rotation *r, int64_t head_dim) {
+    if (!r->pos_dev || !r->freqs_dev) return "null argument";
+    if (r->n_dims <= 0 || r->n_dims % 8 != 0 || r->n_dims > head_dim) return "n_dims must be a multiple of 8 within the head";
+    if (r->mode != QPROJ_ROPE_PAIRS && r->mode != QPROJ_ROPE_HALVES) return "unknown rotation mode";
+    return nullptr;
+}
+
+static const char *bad_cache(const qproj_kv_cache *kv, KvView *view) {
+    if (!kv || !kv->k_codes || !kv->k_scales || !kv->v_codes || !kv->v_scales) return "null argument";
+    if (!aligned16(kv->k_codes) || !aligned16(kv->k_scales) || !aligned16(kv->v_codes) || !aligned16(kv->v_scales)) return "the cache's planes must be 16-byte aligned";
+    if (kv->head_dim != 64 && kv->head_dim != 96 && kv->head_dim != 128 && kv->head_dim != 256) return "head_dim of a cache must be 64, 96, 128 or 256";
+    int shift = 4;
+    while (shift < 8 && (int64_t)1 << shift != kv->page_tokens) ++shift;
+    if ((int64_t)1 << shift != kv->page_tokens) return "page_tokens must be 16, 32, 64, 128 or 256";
+    if (kv->n_pages <= 0 || kv->n_pages > 0x7fffffff || kv->n_head_kv <= 0 || kv->n_head_kv > 1024) return "n_pages or n_head_kv out of range";
+    *view = KvView{static_cast<uint8_t *>(kv->k_codes), static_cast<uint16_t *>(kv->k_scales), static_cast<uint8_t *>(kv->v_codes),
+                   static_cast<uint16_t *>(kv->v_scales), kv->n_pages, shift, (int32_t)kv->n_head_kv, (int32_t)kv->head_dim};
+    return nullptr;
+}
+
+static int refuse(qproj_ctx *ctx, const char *call, const char *why) {
+    char buf[200];
+    snprintf(buf, sizeof buf, "%s: %s", call, why);
+    return fail(ctx, QPROJ_ERR_INVALID_ARG, buf);
+}
+
+constexpr int64_t kMostHeads = 4096, kMostTokens = 0x7fffffff;
+
+int qproj_rope_frequencies(const qproj_rope_scaling *s, int64_t n_dims, double *freqs, float *magnitude) {
+    if (!s || !freqs || !magnitude || n_dims <= 0 || n_dims % 2 != 0 || !(s->base > 1.0) || !(s->freq_scale > 0.0)) return QPROJ_ERR_INVALID_ARG;
+    const bool yarn = s->ext_factor > 0.f;
+    if (!(s->ext_factor >= 0.f && s->ext_factor <= 1.f) || (yarn && (s->n_ctx_orig <= 0 || !(s->beta_fast > 0.f) || !(s->beta_slow > 0.f)))) return QPROJ_ERR_INVALID_ARG;
+    double low = 0, high = 0;
+    if (yarn) {   // the pair that turns `beta` times over the tokens of training
+        const auto pair = [&](double beta) { return n_dims * log(s->n_ctx_orig / (beta * 2 * M_PI)) / (2 * log(s->base)); };
+        low = std::max(0.0, floor(pair(s->beta_fast)));
+        high = std::min(n_dims - 1.0, ceil(pair(s->beta_slow)));
+    }
+    for (int64_t i = 0; i < n_dims / 2; ++i) {
+        const double f = pow(s->base, -2.0 * i / n_dims) / (s->factors ? (double)s->factors[i] : 1.0);
+        double keep = 0;   // of the frequency as trained
+        if (yarn) keep = s->ext_factor * (1.0 - std::min(1.0, std::max(0.0, (i - low) / std::max(0.001, high - low))));
+        freqs[i] = f * s->freq_scale * (1.0 - keep) + f * keep;
+    }
+    *magnitude = (float)(s->attn_factor * (yarn ? 1.0 + 0.1 * log(1.0 / s->freq_scale) : 1.0));
+    return QPROJ_OK;
+}
+
+static void set_rotation(RopeKvJob &j, const qproj_rotation *r) {
+    j.pos = r->pos_dev;
+    j.freqs = r->freqs_dev;
+    j.n_dims = (int)r->n_dims;
+    j.halves = r->mode == QPROJ_ROPE_HALVES;
+    j.magnitude = r->magnitude;
+}
+
+int qproj_rope(qproj_ctx *ctx, const qproj_rotation *rotation, const float *x_dev, int64_t x_stride, int64_t n_tokens, int64_t n_head,
+               int64_t head_dim, float *y_dev, int64_t y_stride) {
+    const char *call = "qproj_rope";
+    if (!ctx) return QPROJ_ERR_INVALID_ARG;
+    if (!rotation) return refuse(ctx, call, "null argument");
+    if (n_tokens < 0 || n_tokens > kMostTokens || n_head <= 0 || n_head > kMostHeads) return refuse(ctx, call, "n_tokens or n_head out of range");
+    if (head_dim <= 0 || head_dim % 8 != 0 || head_dim > 1024) return refuse(ctx, call, "head_dim must be a multiple of 8, at most 1024");
+    if (const char *why = bad_rotation(rotation, head_dim)) return refuse(ctx, call, why);
+    if (const char *why = bad_rows(x_dev, x_stride, n_head, head_dim)) return refuse(ctx, call, why);
+    if (const char *why = bad_rows(y_dev, y_stride, n_head, head_dim)) return refuse(ctx, call, why);
+    if (x_dev == y_dev && x_stride != y_stride) return refuse(ctx, call, "y may be x with the same stride only");
+    if (!dry_run()) QP_HIP(ctx, hipSetDevice(ctx->device));
+    RopeKvJob j{};
+    set_rotation(j, rotation);
+    j.n_tokens = n_tokens;
+    j.q = x_dev;
+    j.q_out = y_dev;
+    j.q_stride = x_stride;
+    j.q_out_stride = y_stride;
+    j.n_head = n_head;
+    j.q_dim = (int)head_dim;
+    QP_HIP(ctx, launch_rope_kv(j, ctx->stream));
+    return QPROJ_OK;
+}
+
+int qproj_kv_append(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *k_dev, int64_t k_stride, const float *v_dev, int64_t v_stride,
+                    int64_t n_tokens, const int64_t *slots_dev, const qproj_rotation *rotation, const float *q_dev, int64_t q_stride,
+                    int64_t n_head, float *q_out_dev, int64_t q_out_stride) {
+    const char *call = "qproj_kv_append";
+    if (!ctx) return QPROJ_ERR_INVALID_ARG;
+    KvView view;
+    if (const char *why = bad_cache(kv, &view)) return refuse(ctx, call, why);
+    if (!slots_dev) return refuse(ctx, call, "null argument");
+    if (n_tokens < 0 || n_tokens > kMostTokens) return refuse(ctx, call, "n_tokens out of range");
+    if (const char *why = bad_rows(k_dev, k_stride, kv->n_head_kv, kv->head_dim)) return refuse(ctx, call, why);
+    if (const char *why = bad_rows(v_dev, v_stride, kv->n_head_kv, kv->head_dim)) return refuse(ctx, call, why);
+    if (rotation)
+        if (const char *why = bad_rotation(rotation, kv->head_dim)) return refuse(ctx, call, why);
+    if (q_dev) {
+        if (!rotation) return refuse(ctx, call, "queries without a rotation");
+        if (n_head <= 0 || n_head > kMostHeads) return refuse(ctx, call, "n_head out of range");
+        if (const char *why = bad_rows(q_dev, q_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
+        if (const char *why = bad_rows(q_out_dev, q_out_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
+        if (q_dev == q_out_dev && q_stride != q_out_stride) return refuse(ctx, call, "q_out may be q with the same stride only");
+    }
+    if (!dry_run()) QP_HIP(ctx, hipSetDevice(ctx->device));
+    RopeKvJob j{};
+    if (rotation) set_rotation(j, rotation);
+    j.n_tokens = n_tokens;
+    if (q_dev) {
+        j.q = q_dev;
+        j.q_out = q_out_dev;
+        j.q_stride = q_stride;
+        j.q_out_stride = q_out_stride;
+        j.n_head = n_head;
+        j.q_dim = (int)kv->head_dim;
+    }
+    j.kv = &view;
+    j.k = k_dev;
+    j.v = v_dev;
+    j.k_stride = k_stride;
+    j.v_stride = v_stride;
+    j.slots = slots_dev;
+    j.error = ctx->flag_dev + 1;
+    QP_HIP(ctx, launch_rope_kv(j, ctx->stream));
+    return QPROJ_OK;
+}
+
+int qproj_kv_read(qproj_ctx *ctx, const qproj_kv_cache *kv, const int64_t *slots_dev, int64_t n, float *k_out_dev, float *v_out_dev) {
+    const char *call = "qproj_kv_read";
+    if (!ctx) return QPROJ_ERR_INVALID_ARG;
+    KvView view;
+    if (const char *why = bad_cache(kv, &view)) return refuse(ctx, call, why);
+    if (!slots_dev) return refuse(ctx, call, "null argument");
+    if (n < 0 || n > kMostTokens) return refuse(ctx, call, "n out of range");
+    if (!aligned16(k_out_dev) || !aligned16(v_out_dev)) return refuse(ctx, call, "rows must be 16-byte aligned");
+    if (!k_out_dev && !v_out_dev) return QPROJ_OK;
+    if (!dry_run()) QP_HIP(ctx, hipSetDevice(ctx->device));
+    QP_HIP(ctx, launch_kv_read(view, slots_dev, n, k_out_dev, v_out_dev, ctx->flag_dev + 1, ctx->stream));
+    return QPROJ_OK;
+}
+
+int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens, int64_t n_head,
+                    int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q, const int32_t *pages_dev,
+                    int64_t pages_stride, float scale, int64_t window, float *y_dev, int64_t y_stride) {
+    const char *call = "qproj_attention";
+    if (!ctx) return QPROJ_ERR_INVALID_ARG;
+    KvView view;
+    if (const char *why = bad_cache(kv, &view)) return refuse(ctx, call, why);
+    if (!q_start_dev || !kv_len_dev || !pages_dev) return refuse(ctx, call, "null argument");
+    if (n_tokens < 0 || n_tokens > kMostTokens || n_seq < 0 || n_seq > 65536 || max_q < 0 || pages_stride < 0)
+        return refuse(ctx, call, "n_tokens, n_seq, max_q or pages_stride out of range");
+    if (pages_stride * kv->page_tokens > 0x7fffffff) return refuse(ctx, call, "a sequence must stay under 2^31 tokens");
+    if (n_head <= 0 || n_head > kMostHeads || n_head % kv->n_head_kv != 0) return refuse(ctx, call, "n_head must be a multiple of n_head_kv");
+    if (window < 0) return refuse(ctx, call, "negative window");
+    if (const char *why = bad_rows(q_dev, q_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
+    if (const char *why = bad_rows(y_dev, y_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
+    if (q_dev == y_dev) return refuse(ctx, call, "y must not be q");
+    if (!dry_run()) QP_HIP(ctx, hipSetDevice(ctx->device));
+    AttentionJob j{};
+    j.kv = &view;
+    j.q = q_dev;
+    j.y = y_dev;
+    j.q_stride = q_stride;
+    j.y_stride = y_stride;
+    j.n_tokens = n_tokens;
+    j.n_seq = n_seq;
+    j.n_head = (int)n_head;
+    j.q_start = q_start_dev;
+    j.kv_len = kv_len_dev;
+    j.pages = pages_dev;
+    j.max_q = std::min(max_q, n_tokens);
+    j.pages_stride = pages_stride;
+    j.scale = scale;
+    j.window = (int32_t)std::min<int64_t>(window, 0x7fffffff);
+    j.error = ctx->flag_dev + 1;
+    QP_HIP(ctx, launch_attention(j, ctx->stream));
+    return QPROJ_OK;
+}
+
+// For the tests: a context without a device, whose calls check their arguments and note their launches without making them.
+// From begin to end the calling thread is in the dry mode of qproj_plan_mul_mat.
+qproj_ctx *qproj_internal_dry_begin() {
+    qproj_ctx *ctx = new (std::nothrow) qproj_ctx();
+    if (!ctx) return nullptr;
+    ctx->flag_dev = reinterpret_cast<int32_t *>(uintptr_t(256));   // never dereferenced in a dry run
+    g_plan = new (std::nothrow) std::string();
+    set_dry_run(true);
+    return ctx;
+}
+int qproj_internal_dry_end(qproj_ctx *ctx, char *buf, size_t buf_bytes) {
+    set_dry_run(false);
+    std::string *text = g_plan;
+    g_plan = nullptr;
+    const size_t scratch_bytes = ctx ? ctx->ws_bytes : 0;
+    delete ctx;
+    if (!text) return QPROJ_ERR_OOM;
+    const int rc = finish_plan(*text, QPROJ_OK, scratch_bytes, buf, buf_bytes);
+    delete text;
+    return rc;
 }
 
 }  // extern "C"

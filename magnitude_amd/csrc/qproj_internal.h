@@ -308,4 +308,41 @@ hipError_t launch_gemm_stream(int n, const WeightView *w, const ActView &a, int6
 size_t q6k_tile_scratch_bytes(int64_t K, int64_t M, int64_t N);   // what launch_gemm_q6k_q8k asks of its scratch
 hipError_t launch_gemm_q6k_q8k(const WeightView &w, const ActView &a, int64_t M, float *y, const Scratch &scratch, hipStream_t s);
 
+// ---- rotary positions, the paged 4-bit cache and attention over it (kv_cache.h) ----
+struct KvView;
+struct RopeKvJob {
+    const int32_t *pos;
+    const double *freqs;
+    int n_dims;                 // 0: no rotation
+    int halves;
+    float magnitude;
+    int64_t n_tokens;
+    const float *q;             // null: no queries
+    float *q_out;
+    int64_t q_stride, q_out_stride;
+    int64_t n_head;
+    int q_dim;
+    const KvView *kv;           // null: queries only
+    const float *k, *v;
+    int64_t k_stride, v_stride;
+    const int64_t *slots;
+    int32_t *error;
+};
+hipError_t launch_rope_kv(const RopeKvJob &j, hipStream_t s);
+hipError_t launch_kv_read(const KvView &kv, const int64_t *slots, int64_t n, float *k_out, float *v_out, int32_t *error, hipStream_t s);
+struct AttentionJob {
+    const KvView *kv;
+    const float *q;
+    float *y;
+    int64_t q_stride, y_stride;
+    int64_t n_tokens, n_seq;
+    int n_head;
+    const int32_t *q_start, *kv_len, *pages;
+    int64_t max_q, pages_stride;
+    float scale;
+    int32_t window;
+    int32_t *error;
+};
+hipError_t launch_attention(const AttentionJob &j, hipStream_t s);
+
 }  // namespace qproj

@@ -62,6 +62,11 @@ SYMBOLS = {
     "qproj_moe_ffn": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i32]),
     "qproj_plan_mul_mat": (_i32, [_i32, _i64, _i32, C.POINTER(_i64), _i64, _i32, _i32, C.c_char_p, _sz]),
     "qproj_plan_moe_ffn": (_i32, [_i32, _i32, _i64, _i64, _i64, _i64, _i64, C.c_char_p, _sz]),
+    "qproj_rope_frequencies": (_i32, [_vp, _i64, _vp, _vp]),
+    "qproj_rope": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64]),
+    "qproj_kv_append": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64]),
+    "qproj_kv_read": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp]),
+    "qproj_attention": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, C.c_float, _i64, _vp, _i64]),
     "qproj_version": (C.c_char_p, []),
     "qproj_probe_eligibility": (_i32, [_vp]),
 }
@@ -75,6 +80,26 @@ class Eligibility(C.Structure):
                 ("architectures", (C.c_char * 32) * PROBE_MAX_DEVICES),
                 ("hardware_labels", (C.c_char * 256) * PROBE_MAX_DEVICES),
                 ("runtime_library", C.c_char * 1024), ("diagnostic", C.c_char * 244)]
+
+
+class RopeScaling(C.Structure):
+    """struct qproj_rope_scaling of include/qproj.h"""
+    _fields_ = [("base", C.c_double), ("freq_scale", C.c_double), ("factors", _vp), ("n_ctx_orig", _i64),
+                ("ext_factor", C.c_float), ("attn_factor", C.c_float), ("beta_fast", C.c_float), ("beta_slow", C.c_float)]
+
+
+class Rotation(C.Structure):
+    """struct qproj_rotation of include/qproj.h"""
+    _fields_ = [("pos_dev", _vp), ("freqs_dev", _vp), ("n_dims", _i64), ("mode", C.c_int), ("magnitude", C.c_float)]
+
+
+class KvPlanes(C.Structure):
+    """struct qproj_kv_cache of include/qproj.h"""
+    _fields_ = [("k_codes", _vp), ("k_scales", _vp), ("v_codes", _vp), ("v_scales", _vp), ("n_pages", _i64),
+                ("page_tokens", _i64), ("n_head_kv", _i64), ("head_dim", _i64)]
+
+
+ROPE_MODES = {"pairs": 0, "halves": 1}
 
 
 class QprojError(RuntimeError):
@@ -171,6 +196,24 @@ def plan_moe_ffn(gate_type: int, down_type: int, d_model: int, d_ff: int, n_expe
     return buf.value.decode()
 
 
+def rope_frequencies(n_dims: int, base: float = 10000.0, freq_scale: float = 1.0, factors: Optional[Sequence[float]] = None,
+                     n_ctx_orig: int = 0, ext_factor: float = 0.0, attn_factor: float = 1.0, beta_fast: float = 32.0,
+                     beta_slow: float = 1.0):
+    """(float64 array of n_dims / 2 radians a position, what cosines and sines are multiplied by): plain, stretched
+    (freq_scale), with factors a frequency, or YaRN (ext_factor > 0, n_ctx_orig tokens of training).  Needs no GPU."""
+    if factors is not None:
+        factors = np.ascontiguousarray(factors, dtype=np.float32)
+        if factors.shape != (n_dims // 2,):
+            raise ValueError("one factor a pair of values")
+    p = RopeScaling(base, freq_scale, 0 if factors is None else factors.ctypes.data, n_ctx_orig, ext_factor, attn_factor,
+                    beta_fast, beta_slow)
+    freqs, magnitude = np.empty(max(0, n_dims // 2), dtype=np.float64), C.c_float(0.0)
+    st = load_library().qproj_rope_frequencies(C.byref(p), n_dims, freqs.ctypes.data, C.byref(magnitude))
+    if st:
+        raise QprojError(st, f"qproj_rope_frequencies({n_dims} values, base {base}, freq_scale {freq_scale})")
+    return freqs, magnitude.value
+
+
 def row_bytes(qtype: int, k: int) -> int:
     return int(load_library().qproj_row_bytes(qtype, k))
 
@@ -203,6 +246,34 @@ class Weight:
             self.free()
         except Exception:
             pass
+
+
+class KvCache:
+    """Keys and values of many sequences in 4 bits, in pages: codes uint8 [n_pages, n_head_kv, page_tokens, head_dim / 2] and
+    scales float16 [n_pages, n_head_kv, page_tokens, head_dim / 32] of either.  The tensors stay the caller's; which page
+    is whose is too."""
+
+    def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor):
+        if k_codes.dim() != 4:
+            raise ValueError("codes must be [n_pages, n_head_kv, page_tokens, head_dim / 2]")
+        n_pages, n_head, page, half = k_codes.shape
+        self.n_pages, self.n_head, self.page_tokens, self.head_dim = n_pages, n_head, page, 2 * half
+        for t, dtype, width in ((k_codes, torch.uint8, half), (v_codes, torch.uint8, half),
+                                (k_scales, torch.float16, half // 16), (v_scales, torch.float16, half // 16)):
+            if t.dtype != dtype or tuple(t.shape) != (n_pages, n_head, page, width) or t.device != k_codes.device:
+                raise ValueError("codes are uint8 [n_pages, n_head_kv, page_tokens, head_dim / 2] and scales float16 "
+                                 "[..., head_dim / 32], all on one device")
+        self.tensors = (k_codes, k_scales, v_codes, v_scales)
+        self.device = k_codes.device
+        self._planes = KvPlanes(_ptr(k_codes), _ptr(k_scales), _ptr(v_codes), _ptr(v_scales), n_pages, page, n_head, 2 * half)
+        self._ref = C.byref(self._planes)
+
+    @classmethod
+    def zeros(cls, n_pages: int, page_tokens: int, n_head_kv: int, head_dim: int, device="cuda") -> "KvCache":
+        shape = (n_pages, n_head_kv, page_tokens)
+        codes, scales = [torch.zeros(shape + (head_dim // 2,), dtype=torch.uint8, device=device) for _ in "kv"], \
+                        [torch.zeros(shape + (head_dim // 32,), dtype=torch.float16, device=device) for _ in "kv"]
+        return cls(codes[0], scales[0], codes[1], scales[1])
 
 
 class Context:
@@ -504,6 +575,146 @@ class Context:
         self._check(self.lib.qproj_moe_ffn(self.handle, gate.handle, up.handle, down.handle,
                                            self._cptr(x), self._cptr(ids),
                                            self._cptr(weights), n_used, b, _ptr(y), act))
+        if sync:
+            self.sync()
+        return y
+
+    # ---- between the q/k/v projections and the output projection ---------------------------
+    def _on_device(self, t: torch.Tensor, dtype: torch.dtype, what: str) -> int:
+        """Address of a contiguous tensor of this context's device."""
+        if t.dtype != dtype:
+            raise ValueError(f"{what} must be {dtype}")
+        if not t.is_cuda or t.get_device() != self.device:
+            raise ValueError(f"{what} must be on cuda:{self.device}")
+        if not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous")
+        return t.data_ptr()
+
+    def _rows(self, t: torch.Tensor, what: str, heads: Optional[int] = None, dim: Optional[int] = None):
+        """(address, floats from token to token) of rows of heads [tokens, heads, dim]: a token's row is dense, the tokens
+        may lie apart (columns of a joined product)."""
+        if t.dim() != 3 or t.dtype != torch.float32:
+            raise ValueError(f"{what} must be float32 [tokens, heads, dim]")
+        n, h, d = t.shape
+        if (heads is not None and h != heads) or (dim is not None and d != dim):
+            raise ValueError(f"{what} must be [tokens, {heads if heads is not None else 'heads'}, {dim}]")
+        if not t.is_cuda or t.get_device() != self.device:
+            raise ValueError(f"{what} must be on cuda:{self.device}")
+        if n and h and d and (t.stride(2) != 1 or (h > 1 and t.stride(1) != d) or (n > 1 and t.stride(0) < h * d)):
+            raise ValueError(f"{what}: a token's heads must lie one after the other")
+        return t.data_ptr(), t.stride(0) if n > 1 else h * d
+
+    def _cache(self, kv: KvCache):
+        if kv.device.index != self.device:
+            raise ValueError(f"the cache must be on cuda:{self.device}")
+        return kv._ref
+
+    def _rotation(self, pos: torch.Tensor, freqs: torch.Tensor, mode: str, magnitude: float, tokens: int) -> Rotation:
+        if pos.numel() != tokens:
+            raise ValueError("one position a token")
+        return Rotation(self._on_device(pos, torch.int32, "pos"), self._on_device(freqs, torch.float64, "freqs"),
+                        2 * freqs.numel(), ROPE_MODES[mode], magnitude)
+
+    def rope(self, x: torch.Tensor, pos: torch.Tensor, freqs: torch.Tensor, mode: str = "pairs", magnitude: float = 1.0,
+             out: Optional[torch.Tensor] = None, sync: bool = True) -> torch.Tensor:
+        """GGML_OP_ROPE: x f32 [tokens, heads, dim]; pos i32 [tokens]; freqs f64 (rope_frequencies) turns the first
+        2 * len(freqs) values of every head, "pairs" of neighbours or "halves".  out may be x."""
+        n, h, d = x.shape if x.dim() == 3 else (0, 0, 0)
+        y = out if out is not None else torch.empty((n, h, d), dtype=torch.float32, device=x.device)
+        xp, xs = self._rows(x, "x")
+        yp, ys = self._rows(y, "out", h, d)
+        if y.shape[0] != n:
+            raise ValueError("out must be shaped as x")
+        r = self._rotation(pos, freqs, mode, magnitude, n)
+        if n == 0:
+            return y
+        if sync:
+            torch.cuda.current_stream(x.device).synchronize()
+        self._check(self.lib.qproj_rope(self.handle, C.byref(r), xp, xs, n, h, d, yp, ys))
+        if sync:
+            self.sync()
+        return y
+
+    def kv_append(self, kv: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pos: Optional[torch.Tensor] = None,
+                  freqs: Optional[torch.Tensor] = None, mode: str = "pairs", magnitude: float = 1.0,
+                  q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None, sync: bool = True):
+        """Keys and values f32 [tokens, n_head_kv, head_dim] into the cache at slots i64 [tokens] (page * page_tokens + place;
+        negative: left out), the keys rotated on the way where freqs is given (as rope does).  q [tokens, heads, head_dim]
+        is rotated beside them in the same launch and returned (q_out, which may be q)."""
+        n = k.shape[0]
+        if v.shape[0] != n or slots.numel() != n:
+            raise ValueError("k, v and slots must have as many tokens")
+        kp, ks = self._rows(k, "k", kv.n_head, kv.head_dim)
+        vp, vs = self._rows(v, "v", kv.n_head, kv.head_dim)
+        sp = self._on_device(slots, torch.int64, "slots")
+        r = None
+        if freqs is not None:
+            if pos is None:
+                raise ValueError("a rotation needs positions")
+            r = self._rotation(pos, freqs, mode, magnitude, n)
+        qp = qs = h = yp = ys = 0
+        if q is not None:
+            if r is None or q.shape[0] != n:
+                raise ValueError("q needs a rotation, and as many tokens as k")
+            qp, qs = self._rows(q, "q", None, kv.head_dim)
+            h = q.shape[1]
+            if q_out is None:
+                q_out = torch.empty((n, h, kv.head_dim), dtype=torch.float32, device=q.device)
+            yp, ys = self._rows(q_out, "q_out", h, kv.head_dim)
+            if q_out.shape[0] != n:
+                raise ValueError("q_out must be shaped as q")
+        if n == 0:
+            return q_out
+        if sync:
+            torch.cuda.current_stream(k.device).synchronize()
+        self._check(self.lib.qproj_kv_append(self.handle, self._cache(kv), kp, ks, vp, vs, n, sp, C.byref(r) if r is not None else None,
+                                             qp, qs, h, yp, ys))
+        if sync:
+            self.sync()
+        return q_out
+
+    def kv_read(self, kv: KvCache, slots: torch.Tensor, k_out: Optional[torch.Tensor] = None,
+                v_out: Optional[torch.Tensor] = None, sync: bool = True):
+        """What the cache holds at slots i64 [n]: keys and values f32 [n, n_head_kv, head_dim] (negative slots: zeros)."""
+        n = slots.numel()
+        sp = self._on_device(slots, torch.int64, "slots")
+        shape = (n, kv.n_head, kv.head_dim)
+        k_out, v_out = (t if t is not None else torch.empty(shape, dtype=torch.float32, device=slots.device) for t in (k_out, v_out))
+        if tuple(k_out.shape) != shape or tuple(v_out.shape) != shape:
+            raise ValueError(f"k_out and v_out must be {list(shape)}")
+        kp, vp = self._on_device(k_out, torch.float32, "k_out"), self._on_device(v_out, torch.float32, "v_out")
+        if n == 0:
+            return k_out, v_out
+        if sync:
+            torch.cuda.current_stream(slots.device).synchronize()
+        self._check(self.lib.qproj_kv_read(self.handle, self._cache(kv), sp, n, kp, vp))
+        if sync:
+            self.sync()
+        return k_out, v_out
+
+    def attention(self, kv: KvCache, q: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor,
+                  max_q: Optional[int] = None, scale: Optional[float] = None, window: int = 0,
+                  out: Optional[torch.Tensor] = None, sync: bool = True) -> torch.Tensor:
+        """Attention of the newest tokens of sequences over the cache: q f32 [tokens, heads, head_dim], rows q_start[s] ..
+        q_start[s + 1] - 1 (i32 [n_seq + 1]) the last ones of the kv_len[s] (i32 [n_seq]) tokens that sequence s has in its
+        pages (i32 [n_seq, most pages]).  max_q: the most rows a sequence has (default: all of them could be one's).
+        scale: 1 / sqrt(head_dim) by default; window: how many tokens back a row sees, itself among them (0: all)."""
+        qp, qs = self._rows(q, "q", None, kv.head_dim)
+        n, h = q.shape[0], q.shape[1]
+        if pages.dim() != 2 or q_start.numel() != pages.shape[0] + 1 or kv_len.numel() != pages.shape[0]:
+            raise ValueError("pages must be [n_seq, most pages], q_start [n_seq + 1] and kv_len [n_seq]")
+        y = out if out is not None else torch.empty((n, h, kv.head_dim), dtype=torch.float32, device=q.device)
+        yp, ys = self._rows(y, "out", h, kv.head_dim)
+        if y.shape[0] != n:
+            raise ValueError("out must be shaped as q")
+        args = [self._on_device(t, torch.int32, w) for t, w in ((q_start, "q_start"), (kv_len, "kv_len"), (pages, "pages"))]
+        if n == 0:
+            return y
+        if sync:
+            torch.cuda.current_stream(q.device).synchronize()
+        self._check(self.lib.qproj_attention(self.handle, self._cache(kv), qp, qs, n, h, pages.shape[0], args[0], args[1],
+                                             n if max_q is None else max_q, args[2], pages.shape[1],
+                                             kv.head_dim ** -0.5 if scale is None else scale, window, yp, ys))
         if sync:
             self.sync()
         return y

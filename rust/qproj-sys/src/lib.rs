@@ -20,6 +20,43 @@ pub const QPROJ_ELIGIBILITY_USABLE: c_int = 0;
 pub const QPROJ_ELIGIBILITY_ABSENT: c_int = 1;
 pub const QPROJ_ELIGIBILITY_FAILED: c_int = 2;
 
+pub const QPROJ_ROPE_PAIRS: c_int = 0;
+pub const QPROJ_ROPE_HALVES: c_int = 1;
+
+#[repr(C)]
+pub struct qproj_rope_scaling {
+    pub base: f64,
+    pub freq_scale: f64,
+    pub factors: *const f32,
+    pub n_ctx_orig: i64,
+    pub ext_factor: f32,
+    pub attn_factor: f32,
+    pub beta_fast: f32,
+    pub beta_slow: f32,
+}
+
+#[repr(C)]
+pub struct qproj_rotation {
+    pub pos_dev: *const i32,
+    pub freqs_dev: *const f64,
+    pub n_dims: i64,
+    pub mode: c_int,
+    pub magnitude: f32,
+}
+
+/// Four device planes of the caller's; see include/qproj.h for their layout
+#[repr(C)]
+pub struct qproj_kv_cache {
+    pub k_codes: *mut c_void,
+    pub k_scales: *mut c_void,
+    pub v_codes: *mut c_void,
+    pub v_scales: *mut c_void,
+    pub n_pages: i64,
+    pub page_tokens: i64,
+    pub n_head_kv: i64,
+    pub head_dim: i64,
+}
+
 /// struct qproj_eligibility of include/qproj.h
 #[repr(C)]
 pub struct qproj_eligibility {
@@ -88,6 +125,19 @@ extern "C" {
     pub fn qproj_moe_ffn(ctx: *mut qproj_ctx, gate: *const qproj_weight, up: *const qproj_weight,
                          down: *const qproj_weight, x_dev: *const f32, ids_dev: *const i32,
                          weights_dev: *const f32, n_used: i64, b: i64, y_dev: *mut f32, act: c_int) -> c_int;
+    pub fn qproj_rope_frequencies(scaling: *const qproj_rope_scaling, n_dims: i64, freqs: *mut f64, magnitude: *mut f32) -> c_int;
+    pub fn qproj_rope(ctx: *mut qproj_ctx, rotation: *const qproj_rotation, x_dev: *const f32, x_stride: i64,
+                      n_tokens: i64, n_head: i64, head_dim: i64, y_dev: *mut f32, y_stride: i64) -> c_int;
+    pub fn qproj_kv_append(ctx: *mut qproj_ctx, kv: *const qproj_kv_cache, k_dev: *const f32, k_stride: i64,
+                           v_dev: *const f32, v_stride: i64, n_tokens: i64, slots_dev: *const i64,
+                           rotation: *const qproj_rotation, q_dev: *const f32, q_stride: i64, n_head: i64,
+                           q_out_dev: *mut f32, q_out_stride: i64) -> c_int;
+    pub fn qproj_kv_read(ctx: *mut qproj_ctx, kv: *const qproj_kv_cache, slots_dev: *const i64, n: i64,
+                         k_out_dev: *mut f32, v_out_dev: *mut f32) -> c_int;
+    pub fn qproj_attention(ctx: *mut qproj_ctx, kv: *const qproj_kv_cache, q_dev: *const f32, q_stride: i64,
+                           n_tokens: i64, n_head: i64, n_seq: i64, q_start_dev: *const i32, kv_len_dev: *const i32,
+                           max_q: i64, pages_dev: *const i32, pages_stride: i64, scale: f32, window: i64,
+                           y_dev: *mut f32, y_stride: i64) -> c_int;
     pub fn qproj_version() -> *const c_char;
     pub fn qproj_probe_eligibility(out: *mut qproj_eligibility) -> c_int;
 }
