@@ -1,88 +1,779 @@
-// Attention over the paged 4-bit cache.
+// Attention over the paged 4-bit cache on the matrix cores.
 //
 //   y = sum_t softmax_t(scale * q . k_t) v_t over the tokens t <= p (the last `window` of them) of a sequence.
 //
-// A wave serves one row of one head: it goes over the tokens once with the running maximum and sum of the softmax.
+// Work.  An item is 16 or 32 rows (some new tokens x the query heads that share a key/value head) against the
+// tokens they see, in tiles of 64 tokens.  All tiles of all items lie in one line, head by head, and the workgroups of one round
+// take equal stretches of it, whatever the lengths of the sequences are: a stretch ends inside an item where it has to, its
+// sums go to the workspace, and attention_join_kernel adds the parts of the items that were cut.  The line is laid out
+// on the device (a scan over the lengths in every workgroup), so that a captured call follows the lengths.  Inside a
+// workgroup the four waves take tiles in turn, each with its own running maximum, sum and result; they meet once, at the
+// end of an item.  No barrier in the loop over tiles.
+//
+// A tile.  v_mfma_f32_16x16x32_f16 with tokens (then dimensions) as rows and queries as columns, so that a lane's column is
+// one query throughout: row statistics are a lane's own, and the probabilities come out of the first product in the
+// order in which the second takes them.
+//   scores   acc = sum over a block of 32 of n * q, in fp32; S += d_k * acc.  The codes n (0..15) go into the matrix cores as
+//            subnormal halves: a nibble in bits 0..3 is n * 2^-24 as it stands, one in bits 4..7 n * 2^-20, so a word of eight
+//            codes costs a shift and four ands.  q carries 2^-4 where that is; d_k * -8 * sum(q) over the blocks is one more product.
+//            q is scaled by a power of two of its row and split into two halves: 22 bits, two products.
+//   values   codes become n - 8 (1024 + n as half bits, less 1032), times the block's d: product and remainder of one
+//            multiplication are two halves that hold it exactly (4 x 11 bits), the largest d of a tile brought to 2^11..2^12 by a power
+//            of two that the result is kept in.  Probabilities split into two halves too: three products (low x low is under 2^-22).
+//   A lane needs eight tokens' codes of one dimension, memory holds one token's of all: ds_read_b64_tr_b4 turns 16 x 16 nibbles.
+// The running maximum of a row moves only when a score passes it by 2^2.5; until then nothing is rescaled.  Weights are 2^13 at
+// the maximum, so that as pairs of halves they keep 22 bits down to 2^-26 of it, and steps of 2^-37 of it below.
+//
+// Weights, sums, maxima and results are fp32; every value that goes to the matrix cores has 22 bits.
 #include "kv_cache.h"
+#include "lds_direct.h"
 #include "qproj_internal.h"
+
+#include <algorithm>
 
 namespace qproj {
 
 namespace {
 
-constexpr int kMostDims = 256;
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kTile = 64;            // tokens of a tile
+constexpr float kBias = 13.f;        // weights are 2^kBias at the running maximum
+constexpr float kSlack = 2.5f;       // a score may pass it by this before the row is rescaled: 2^15.5 < 65504
 
 struct AttentionArgs {
     KvView kv;
     const float *q;
     float *y;
-    int64_t q_stride, y_stride, pages_stride, n_tokens, n_seq, max_q;
+    int64_t q_stride, y_stride, pages_stride;
     const int32_t *q_start, *kv_len, *pages;
     int32_t *error;
-    float scale;
-    int32_t window, group;
+    float *parts;            // [workgroups][2] sums of items that were cut (part_floats each)
+    int32_t *joins;          // [workgroups][8] {first stretch (-1: nothing to join), last stretch, sequence, row tile, head}
+    float scale;             // times log2(e)
+    int32_t n_tokens, n_seq, max_q, window;
+    int32_t group;           // query heads of a key/value head
+    int32_t splits, split;   // they are served `split` at a time, in `splits` goes
+    int32_t tokens;          // new tokens of an item
+    int32_t row_tiles;       // items of a sequence, at most
 };
 
-__global__ __launch_bounds__(64) void attention_kernel(const AttentionArgs a) {
-    constexpr int kHeld = kMostDims / 64;
-    const int lane = threadIdx.x, head = blockIdx.y, kv_head = head / a.group, dim = a.kv.dim, blocks = dim / 32;
-    const int64_t row = blockIdx.x;
-    const auto bad = [&](int64_t s) {
-        const int64_t b = a.q_start[s], e = a.q_start[s + 1], n = a.kv_len[s];
-        return b < 0 || e < b || e > a.n_tokens || e - b > a.max_q || n < 0 || n > a.pages_stride << a.kv.page_shift;
+constexpr int part_floats(int dim, int cols) { return 16 * cols * (dim + 2); }
+
+struct Sequence {
+    int start, count, len;   // first row, rows, tokens in the cache; count 0 where there is nothing to do
+};
+
+__device__ __forceinline__ Sequence sequence(const AttentionArgs &a, int s, bool &bad) {
+    Sequence q;
+    q.start = a.q_start[s];
+    const int end = a.q_start[s + 1];
+    q.len = a.kv_len[s];
+    q.count = end - q.start;
+    bad = q.start < 0 || end < q.start || end > a.n_tokens || q.count > a.max_q || q.len < 0 || (int64_t)q.len > a.pages_stride << a.kv.page_shift;
+    if (bad) q.count = 0;
+    return q;
+}
+
+// the rows of an item and the tokens that any of them sees
+struct Item {
+    int seq, first, count;   // first row, its tokens
+    int lo, hi;              // positions of its first and last token; tokens [see, hi] are seen (hi < 0: none)
+    int see;
+};
+
+__device__ __forceinline__ Item item_of(const AttentionArgs &a, int s, const Sequence &q, int row_tile) {
+    Item it;
+    it.seq = s;
+    it.first = q.start + row_tile * a.tokens;
+    it.count = min(a.tokens, q.count - row_tile * a.tokens);
+    it.lo = q.len - q.count + row_tile * a.tokens;
+    it.hi = it.lo + it.count - 1;
+    it.see = a.window ? max(0, it.lo - a.window + 1) : 0;
+    return it;
+}
+
+__device__ __forceinline__ int item_tiles(const Item &it) { return it.count <= 0 ? 0 : it.hi < 0 ? 1 : it.hi / kTile - it.see / kTile + 1; }
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+__device__ __forceinline__ void wave_sync() {   // LDS of one wave: its operations go in order, the compiler has to keep to it
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {   // to nearest
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, half2v));
+}
+__device__ __forceinline__ float low_half(uint32_t v) { return (float)__builtin_bit_cast(half2v, v)[0]; }
+__device__ __forceinline__ float high_half(uint32_t v) { return (float)__builtin_bit_cast(half2v, v)[1]; }
+
+__device__ __forceinline__ float max_xor(float v) {   // over the lanes of a column: xor 16, xor 32
+    uint32_t x, y;
+    swap16(__float_as_uint(v), x, y);
+    v = fmaxf(__uint_as_float(x), __uint_as_float(y));
+    swap32(__float_as_uint(v), x, y);
+    return fmaxf(__uint_as_float(x), __uint_as_float(y));
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = dpp_max<0x140>(dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(v))));   // each row of 16 lanes
+    uint32_t x, y;
+    swap16(v, x, y);
+    v = max(x, y);
+    swap32(v, x, y);
+    return (uint32_t)uniform((int)max(x, y));
+}
+
+// where the transposing read finds 16-byte chunk `chunk` of a token's value codes: rows of 16 tokens that one read takes
+// together are 16 tokens apart, chunks are turned so that they fall into different banks
+template <int D>
+__device__ __forceinline__ int value_at(int token, int chunk) {
+    constexpr int kChunks = D / 32;
+    const int turn = (token >> 4) & 3;
+    int c = chunk;
+    if (D == 128) c = chunk ^ turn;
+    else if (D == 256) c = chunk ^ (turn | ((token >> 1) & 1) << 2);
+    else if (D == 64) c = chunk ^ (turn & 1);
+    else c = (chunk + turn) % kChunks;
+    return token * (D / 2) + c * 16;
+}
+
+template <int D, int NQ>
+struct WaveLds {
+    uint8_t v[kTile * D / 2];
+    uint16_t k_scale[kTile][D / 32];
+    uint16_t v_scale[D / 32][kTile];
+};
+
+template <int D, int NQ>
+struct SharedLds {
+    union {
+        WaveLds<D, NQ> wave[kWaves];
+        struct {
+            f32x4 o[kWaves / 2][D / 16 * NQ][64];
+            float m[kWaves / 2][NQ][64], l[kWaves / 2][NQ][64];
+        } meet;
     };
-    if (row == 0 && head == 0)
-        for (int64_t s = lane; s < a.n_seq; s += 64)
-            if (bad(s)) atomicOr(a.error, kKvBadRows);
-    int64_t seq = 0, start = 0, end = 0;
-    for (; seq < a.n_seq; ++seq) {
-        start = a.q_start[seq], end = a.q_start[seq + 1];
-        if (row >= start && row < end) break;
-    }
-    if (seq == a.n_seq || bad(seq)) return;
-    const int64_t len = a.kv_len[seq];
-    const int64_t p = len - (end - row);
-    float q[kHeld], o[kHeld];
-    for (int i = 0; i < kHeld; ++i) {
-        const int d = lane + 64 * i;
-        q[i] = d < dim ? a.q[row * a.q_stride + (int64_t)head * dim + d] * a.scale : 0.f;
-        o[i] = 0.f;
-    }
-    float m = -3e38f, l = 0.f;
-    for (int64_t t = a.window ? max((int64_t)0, p - a.window + 1) : 0; t <= p; ++t) {
-        const int64_t page = a.pages[seq * a.pages_stride + (t >> a.kv.page_shift)];
-        if (page < 0 || page >= a.kv.n_pages) {
-            if (lane == 0) atomicOr(a.error, kKvBadPage);
-            continue;
+    int32_t wave_total[kWaves];
+    int32_t found[4];   // sequence, row tile, tiles before the item, its tiles
+};
+
+// what a wave holds of an item
+template <int D, int NQ>
+struct Running {
+    f32x4 o[D / 16][NQ];   // [16 dimensions][16 queries]: lane's column is query lane % 16, rows 4 * (lane / 16) + r
+    float m[NQ], l[NQ];    // of the lane's column; l of the lane's own tokens only until the end
+};
+
+template <int D, int NQ>
+__device__ __forceinline__ void merge(Running<D, NQ> &a, const f32x4 *o, const float *m, const float *l, int lane) {
+#pragma unroll
+    for (int g = 0; g < NQ; ++g) {
+        const float mo = m[g * 64 + lane], top = fmaxf(a.m[g], mo);
+        const float fa = a.m[g] == top ? 1.f : __builtin_amdgcn_exp2f(a.m[g] - top), fo = mo == top ? 1.f : __builtin_amdgcn_exp2f(mo - top);
+        a.l[g] = a.l[g] * fa + l[g * 64 + lane] * fo;
+        a.m[g] = top;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+            const f32x4 x = o[(t * NQ + g) * 64 + lane];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a.o[t][g][r] = a.o[t][g][r] * fa + x[r] * fo;
         }
-        const int64_t at = kv_row(a.kv, page, kv_head, (int)(t & ((1 << a.kv.page_shift) - 1)));
-        float s = 0.f, v[kHeld];
-        for (int i = 0; i < kHeld; ++i) {
-            const int d = lane + 64 * i;
-            v[i] = 0.f;
-            if (d >= dim) continue;
-            const int b = d / 32, e = d / 8 % 4, j = d % 8;
-            const uint32_t kw = reinterpret_cast<const uint32_t *>(a.kv.k_codes + at * (dim / 2))[key_word(blocks, b, e)];
-            const uint32_t vw = reinterpret_cast<const uint32_t *>(a.kv.v_codes + at * (dim / 2))[value_word(b, e)];
-            s = fmaf(q[i], h2f(a.kv.k_scales[at * blocks + b]) * (float)((int)((kw >> (4 * j)) & 15) - 8), s);
-            v[i] = h2f(a.kv.v_scales[at * blocks + b]) * (float)((int)((vw >> (4 * j)) & 15) - 8);
+    }
+}
+
+// Tiles [from, to) of an item (in tiles from token 0 on), every kWaves-th of them
+template <int D, int NQ>
+__device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int kv_head, int head0, int heads, int from, int to, WaveLds<D, NQ> &lds,
+                                     Running<D, NQ> &st, int lane) {
+    constexpr int B = D / 32, RB = D / 2, T = D / 16;
+    constexpr int kLoads = (RB + 63) / 64;       // of 16 bytes a lane for 16 tokens' value codes
+    const int col = lane & 15, part = lane >> 4;
+    const KvView &kv = a.kv;
+    const int shift = kv.page_shift, mask = (1 << shift) - 1;
+
+#pragma unroll
+    for (int g = 0; g < NQ; ++g) {
+        st.m[g] = -INFINITY;
+        st.l[g] = 0.f;
+#pragma unroll
+        for (int t = 0; t < T; ++t) st.o[t][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (from >= to || it.hi < 0) return;
+
+    // page of the lane's token of a tile (a token outside what is seen: of the nearest one that is)
+    const int32_t *table = a.pages + (int64_t)it.seq * a.pages_stride;
+    const auto page_of = [&](int tile) {
+        const int t = min(max(tile * kTile + lane, it.see), it.hi);
+        return table[t >> shift];
+    };
+    int page = page_of(from), page_next = from + kWaves < to ? page_of(from + kWaves) : 0;
+
+    u32x4 v_raw[4][kLoads];
+    uint32_t k_raw[4][B];
+    uint32_t ks_raw[(B + 1) / 2], vs_raw[(B + 1) / 2];
+    int bad_groups;      // of the tile whose loads are in flight
+    int64_t rows[4];     // first row of its groups of 16 tokens
+
+    const auto place = [&](int tile) {   // rows of the tile whose pages have come
+        const int t = min(max(tile * kTile + lane, it.see), it.hi);
+        const bool bad = page < 0 || page >= kv.n_pages;
+        if (bad && t == tile * kTile + lane) atomicOr(a.error, kKvBadPage);
+        bad_groups = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int p = __builtin_amdgcn_readlane(bad ? -1 : page, 16 * g);
+            if (p < 0) bad_groups |= 1 << g;
+            rows[g] = (((int64_t)max(p, 0) * kv.n_head + kv_head) << shift) + ((tile * kTile + 16 * g) & mask);
         }
-        s = wave_sum(s);
-        const float top = fmaxf(m, s), back = expf(m - top), w = expf(s - top);
-        l = fmaf(l, back, w);
-        for (int i = 0; i < kHeld; ++i) o[i] = fmaf(o[i], back, w * v[i]);
-        m = top;
+    };
+    uint32_t v_off[kLoads], k_off = (uint32_t)(col * RB + part * B * 4), s_off = (uint32_t)(col * B * 2);
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) v_off[c] = (uint32_t)min(c * 64 + lane, RB - 1) * 16;
+    const auto load_v = [&]() {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const auto base = scalar_global(kv.v_codes + rows[g] * RB);
+#pragma unroll
+            for (int c = 0; c < kLoads; ++c) v_raw[g][c] = load_global<u32x4>(base, v_off[c]);
+        }
+        const int64_t row = part == 0 ? rows[0] : part == 1 ? rows[1] : part == 2 ? rows[2] : rows[3];
+        const uint8_t *ks = reinterpret_cast<const uint8_t *>(kv.k_scales) + row * (B * 2) + s_off;
+        const uint8_t *vs = reinterpret_cast<const uint8_t *>(kv.v_scales) + row * (B * 2) + s_off;
+        if (B == 3) {
+            const uint16_t *k3 = reinterpret_cast<const uint16_t *>(ks), *v3 = reinterpret_cast<const uint16_t *>(vs);
+            ks_raw[0] = k3[0] | (uint32_t)k3[1] << 16, ks_raw[1] = k3[2];
+            vs_raw[0] = v3[0] | (uint32_t)v3[1] << 16, vs_raw[1] = v3[2];
+        } else {
+#pragma unroll
+            for (int i = 0; i < B / 2; ++i) {
+                ks_raw[i] = reinterpret_cast<const uint32_t *>(ks)[i];
+                vs_raw[i] = reinterpret_cast<const uint32_t *>(vs)[i];
+            }
+        }
+    };
+    const auto load_k = [&]() {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const auto base = scalar_global(kv.k_codes + rows[g] * RB);
+            if constexpr (B == 2) {
+                const u32x2 w = load_global<u32x2>(base, k_off);
+                k_raw[g][0] = w[0], k_raw[g][1] = w[1];
+            } else if constexpr (B == 3) {
+#pragma unroll
+                for (int b = 0; b < B; ++b) k_raw[g][b] = load_global<uint32_t>(base, k_off + 4 * b);
+            } else {
+#pragma unroll
+                for (int b = 0; b < B; b += 4) {
+                    const u32x4 w = load_global<u32x4>(base, k_off + 4 * b);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) k_raw[g][b + i] = w[i];
+                }
+            }
+        }
+    };
+    place(from);
+    load_v();
+    load_k();
+
+    // queries: 22 bits of q * scale * log2(e), scaled by a power of two of the row
+    u32x4 q_hi[B][NQ], q_lo[B][NQ];
+    u32x4 q_sum[NQ];         // -8 * sum(q) of every block, in the accumulators' unit: two halves each, for one more product with the scales
+    int q_exp[NQ], pos[NQ];  // scores are acc * 2^q_exp; position of the column's row, -1: no row
+#pragma unroll
+    for (int g = 0; g < NQ; ++g) {
+        const int slot = g * 16 + col, token = slot / a.split, head = slot - token * a.split;
+        const bool live = token < it.count && head < heads;
+        pos[g] = live ? it.lo + token : -1;
+        const float *row = a.q + (int64_t)(it.first + (live ? token : 0)) * a.q_stride + (int64_t)(head0 + (live ? head : 0)) * D + 8 * part;
+        float x[B][8];
+        float most = 0.f;
+        bool whole = true;
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(row + 32 * b), hi = *reinterpret_cast<const f32x4 *>(row + 32 * b + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[b][j] = live ? lo[j] * a.scale : 0.f;
+                x[b][4 + j] = live ? hi[j] * a.scale : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                most = fmaxf(most, fabsf(x[b][j]));
+                whole = whole && fabsf(x[b][j]) <= 3.402823466e38f;
+            }
+        }
+        most = max_xor(whole ? most : INFINITY);
+        // (frexp: most = f * 2^e with f in [0.5, 1); 0 for zero, and where a value is not finite the row stays as it is: NaN comes of it)
+        const int e = most > 0.f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
+        q_exp[g] = e - 15 + 24;
+        float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int s = 15 - e - (i & 1 ? 4 : 0);
+                const float u = ldexpf(x[b][i], s), v = ldexpf(x[b][i + 4], s);
+                const uint32_t hi = half_pair(u, v), lo = half_pair(u - low_half(hi), v - high_half(hi));
+                q_hi[b][g][i] = hi;
+                q_lo[b][g][i] = lo;
+                sum += ((low_half(hi) + low_half(lo)) + (high_half(hi) + high_half(lo))) * (i & 1 ? 16.f : 1.f);
+            }
+            sums[b] = add_xor32(add_xor16(sum)) * (-8.f * 5.9604644775390625e-8f);
+        }
+        // element 8 * part + j multiplies scale (8 * part + j) % B4 of the token: high halves in the first B4 of them, then low ones
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = 0;
+            if constexpr (B <= 4) {
+                const int j = 2 * i, b = j % 4;
+                const uint32_t hi = half_pair(sums[b], sums[b + 1]);
+                w = part != 0 ? 0 : j < 4 ? hi : half_pair(sums[b] - low_half(hi), sums[b + 1] - high_half(hi));
+            } else {
+                const uint32_t hi = half_pair(sums[2 * i], sums[2 * i + 1]);
+                w = part == 0 ? hi : part == 1 ? half_pair(sums[2 * i] - low_half(hi), sums[2 * i + 1] - high_half(hi)) : 0;
+            }
+            q_sum[g][i] = w;
+        }
     }
-    for (int i = 0; i < kHeld; ++i) {
-        const int d = lane + 64 * i;
-        if (d < dim) a.y[row * a.y_stride + (int64_t)head * dim + d] = l != 0.f ? o[i] / l : 0.f;
+
+    int unit = 0;               // results are in units of 2^unit
+    uint32_t ceiling = 0;       // half bits that a tile's largest |d| stays under, 0: no tile with values yet
+    float base[NQ];             // what is taken off a score
+    uint32_t poison[NQ];        // blocks of values that are not finite and were seen
+#pragma unroll
+    for (int g = 0; g < NQ; ++g) base[g] = -kBias, poison[g] = 0;
+
+    for (int tile = from; tile < to; tile += kWaves) {
+        const int t0 = tile * kTile;
+        const int bad_now = bad_groups;
+        // ---- value codes and scales to LDS ----
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int c = 0; c < kLoads; ++c) {
+                const int i = c * 64 + lane, token = i / B, chunk = i - token * B;
+                if (RB % 64 == 0 || i < RB) *reinterpret_cast<u32x4 *>(lds.v + value_at<D>(16 * g + token, chunk)) = v_raw[g][c];
+            }
+        const int t = t0 + lane;
+        const bool live = t >= it.see && t <= it.hi && !((bad_now >> part) & 1);
+        uint32_t most = 0;
+        uint16_t vs[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            lds.k_scale[lane][b] = (uint16_t)(ks_raw[b / 2] >> (16 * (b & 1)));
+            vs[b] = live ? (uint16_t)(vs_raw[b / 2] >> (16 * (b & 1))) : 0;
+            most = max(most, (uint32_t)vs[b] & 0x7fffu);
+        }
+        uint64_t strange = __ballot(most >= 0x7c00u);
+        if (strange) {           // blocks that are not finite count as zeros here; who sees them gets NaN below
+            most = 0;
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+                if ((vs[b] & 0x7fffu) < 0x7c00u) most = max(most, (uint32_t)vs[b] & 0x7fffu);
+        }
+        // the tile's largest scale goes to 2^11 .. 2^12; a tile within a factor of 2^8 below keeps the unit of the one before
+        float shrink = 1.f;      // of what has been summed
+        if (__ballot(most >= ceiling) || (ceiling > 0x2400u && !__ballot(most >= ceiling - 0x2400u) && __ballot(most != 0))) {
+            const uint32_t top = wave_max(most);
+            if (top) {
+                const int e = __builtin_amdgcn_frexp_expf(h2f(top));     // top < 2^e
+                if (ceiling) shrink = ldexpf(1.f, unit - (e - 12));
+                unit = e - 12;
+                ceiling = e >= 16 ? 0x7c00u : e > -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);   // the bits of 2^e
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const bool fine = (vs[b] & 0x7fffu) < 0x7c00u;
+            lds.v_scale[b][lane] = fine ? f2h(ldexpf(h2f(vs[b]), -unit)) : 0;
+        }
+        uint64_t strange_of[B];
+        if (strange) {
+#pragma unroll
+            for (int b = 0; b < B; ++b) strange_of[b] = __ballot((vs[b] & 0x7fffu) >= 0x7c00u);
+        }
+        wave_sync();
+        // ---- the next tile's values and scales, and the page of the one behind ----
+        const bool more = tile + kWaves < to;
+        if (more) {
+            page = page_next;
+            if (tile + 2 * kWaves < to) page_next = page_of(tile + 2 * kWaves);
+            place(tile + kWaves);
+            load_v();
+        }
+        // ---- scores ----
+        f32x4 s[4][NQ];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint32_t d[2 * B];   // scales of the lane's four tokens, two a word
+#pragma unroll
+            for (int i = 0; i < 2 * B; i += 2) {
+                const u32x2 v = *reinterpret_cast<const u32x2 *>(&lds.k_scale[16 * g + 4 * part][0] + 2 * i);
+                d[i] = v[0], d[i + 1] = v[1];
+            }
+            u32x4 own;           // scales of the token whose codes the lane holds
+            if constexpr (B <= 4) {
+                const uint16_t *row = &lds.k_scale[16 * g + col][0];
+                own[0] = own[2] = B == 3 ? row[0] | (uint32_t)row[1] << 16 : *reinterpret_cast<const uint32_t *>(row);
+                own[1] = own[3] = B == 2 ? 0 : B == 3 ? row[2] : *reinterpret_cast<const uint32_t *>(row + 2);
+            } else {
+                own = *reinterpret_cast<const u32x4 *>(&lds.k_scale[16 * g + col][0]);
+            }
+#pragma unroll
+            for (int c = 0; c < NQ; ++c)
+                s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, own), __builtin_bit_cast(half8, q_sum[c]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const uint32_t w = k_raw[g][b], w8 = w >> 8;
+                const u32x4 n = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
+                const half8 codes = __builtin_bit_cast(half8, n);
+#pragma unroll
+                for (int c = 0; c < NQ; ++c) {
+                    f32x4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, __builtin_bit_cast(half8, q_hi[b][c]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, __builtin_bit_cast(half8, q_lo[b][c]), acc, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[g][c][r] = fmaf((r * B + b) & 1 ? high_half(d[(r * B + b) / 2]) : low_half(d[(r * B + b) / 2]), acc[r], s[g][c][r]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (more) load_k();
+        __builtin_amdgcn_sched_barrier(0);
+        // ---- weights ----
+        const bool edge = t0 + kTile - 1 > it.lo || (a.window && t0 <= it.hi - a.window) || t0 < it.see || bad_now;
+        u32x4 p_hi[2][NQ], p_lo[2][NQ];
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[g][c][r] = ldexpf(s[g][c][r], q_exp[c]);
+            if (edge) {
+                const int last = pos[c] - t0 - 4 * part, behind = a.window ? last - a.window : -kTile;   // of the lane's tokens 16 g + r
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const bool there = !((bad_now >> g) & 1);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        s[g][c][r] = 16 * g + r <= last && 16 * g + r > behind && there ? s[g][c][r] : -INFINITY;
+                }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) top = fmaxf(top, fmaxf(fmaxf(s[g][c][0], s[g][c][1]), fmaxf(s[g][c][2], s[g][c][3])));
+            float back = shrink;
+            if (__ballot(top > st.m[c] + kSlack)) {
+                const float m = fmaxf(st.m[c], max_xor(top));
+                const float f = m == st.m[c] ? 1.f : __builtin_amdgcn_exp2f(st.m[c] - m);
+                st.l[c] *= f;
+                back *= f;
+                st.m[c] = m;
+                base[c] = (m == -INFINITY ? 0.f : m) - kBias;
+            }
+            if (__ballot(back != 1.f)) {
+#pragma unroll
+                for (int x = 0; x < T; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) st.o[x][c][r] *= back;
+            }
+            if (strange) {
+#pragma unroll
+                for (int b = 0; b < B; ++b) {
+                    const uint64_t own = strange_of[b] >> (4 * part);     // bit 16 g + r: the lane's token r of group g
+                    bool hit = false;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) hit = hit || ((own >> (16 * g + r) & 1) && s[g][c][r] != -INFINITY);
+                    poison[c] |= (uint32_t)hit << b;
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[g][c][r] = __builtin_amdgcn_exp2f(s[g][c][r] - base[c]);
+                st.l[c] += (s[g][c][0] + s[g][c][1]) + (s[g][c][2] + s[g][c][3]);
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    const uint32_t hi = half_pair(s[g][c][r], s[g][c][r + 1]);
+                    p_hi[g / 2][c][(g & 1) * 2 + r / 2] = hi;
+                    p_lo[g / 2][c][(g & 1) * 2 + r / 2] = half_pair(s[g][c][r] - low_half(hi), s[g][c][r + 1] - high_half(hi));
+                }
+            }
+        }
+        // ---- values ----
+        // The lane's dimension is lane % 16 of 16; its eight tokens of either half of the tile are those of its scores.  It names the
+        // row that nibble lane % 16 of the result comes from: nibbles i and i + 4 of a word, which one and takes together, are neighbours.
+        const int jj = col & 7, k = (jj & 3) * 2 + (jj >> 2);
+        const int from_token = 32 * (col >> 3) + 16 * (k >> 2) + 4 * part + (k & 3);
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            u32x2 d[4];          // scales of the lane's tokens of a group of 16
+#pragma unroll
+            for (int g = 0; g < 4; ++g) d[g] = *reinterpret_cast<const u32x2 *>(&lds.v_scale[b][16 * g + 4 * part]);
+#pragma unroll
+            for (int x = 2 * b; x < 2 * b + 2; ++x) {
+                const i32x2 raw = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+                    (__attribute__((address_space(3))) i32x2 *)(lds.v + value_at<D>(from_token, b) + 8 * (x & 1)));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t w = (uint32_t)raw[h], w8 = w >> 8;
+                    const uint32_t n[4] = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
+                    u32x4 a_hi, a_lo;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const half2v big = __builtin_bit_cast(half2v, n[i] | 0x64006400u);   // 1024 + n, or 1024 + 16 n
+                        const half2v code = i & 1 ? __builtin_elementwise_fma(big, half2v{(_Float16)0.0625f, (_Float16)0.0625f}, half2v{(_Float16)-72.f, (_Float16)-72.f})
+                                                  : big - half2v{(_Float16)1032.f, (_Float16)1032.f};
+                        const half2v e = __builtin_bit_cast(half2v, (uint32_t)d[2 * h + (i >> 1)][i & 1]);
+                        const half2v hi = code * e;
+                        a_hi[i] = __builtin_bit_cast(uint32_t, hi);
+                        a_lo[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, e, -hi));
+                    }
+#pragma unroll
+                    for (int c = 0; c < NQ; ++c) {
+                        const half8 vh = __builtin_bit_cast(half8, a_hi), vl = __builtin_bit_cast(half8, a_lo);
+                        const half8 ph = __builtin_bit_cast(half8, p_hi[h][c]), pl = __builtin_bit_cast(half8, p_lo[h][c]);
+                        st.o[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, st.o[x][c], 0, 0, 0);
+                        st.o[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, st.o[x][c], 0, 0, 0);
+                        st.o[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, st.o[x][c], 0, 0, 0);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        wave_sync();
     }
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+        st.l[c] = add_xor32(add_xor16(st.l[c]));
+        uint32_t p = poison[c], u, w;
+        swap16(p, u, w);
+        p = u | w;
+        swap32(p, u, w);
+        p = u | w;
+#pragma unroll
+        for (int x = 0; x < T; ++x)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) st.o[x][c][r] = (p >> (x / 2)) & 1 ? NAN : ldexpf(st.o[x][c][r], unit);
+    }
+}
+
+// rows of an item from sums: lane's column of 16 queries, 4 dimensions of 16
+template <int D, int NQ>
+__device__ __forceinline__ float *out_row(const AttentionArgs &a, const Item &it, int head0, int heads, int g, int lane, bool &live) {
+    const int slot = g * 16 + (lane & 15), token = slot / a.split, head = slot - token * a.split;
+    live = token < it.count && head < heads;
+    return a.y + (int64_t)(it.first + (live ? token : 0)) * a.y_stride + (int64_t)(head0 + (live ? head : 0)) * D + 4 * (lane >> 4);
+}
+
+template <int D, int NQ>
+__global__ __launch_bounds__(kThreads, D * NQ <= 256 ? 2 : 1) void attention_kernel(const AttentionArgs a) {
+    constexpr int T = D / 16;
+    __shared__ __align__(16) SharedLds<D, NQ> lds;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
+    const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
+    // ---- the line of tiles: a thread counts those of `per` items of one head ----
+    int mine = 0;
+    for (int u = id * per; u < min(units, (id + 1) * per); ++u) {
+        const int s = u / a.row_tiles;
+        bool bad;
+        const Sequence q = sequence(a, s, bad);
+        if (bad && u == s * a.row_tiles && blockIdx.x == 0) atomicOr(a.error, kKvBadRows);
+        mine += item_tiles(item_of(a, s, q, u - s * a.row_tiles));
+    }
+    int before = mine;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+        const int o = __shfl_up(before, x);
+        if (lane >= x) before += o;
+    }
+    if (lane == 63) lds.wave_total[wave] = before;
+    before -= mine;
+    __syncthreads();
+    int head_tiles = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) before += lds.wave_total[w];
+        head_tiles += lds.wave_total[w];
+    }
+    head_tiles = uniform(head_tiles);
+    const int64_t total = (int64_t)head_tiles * a.kv.n_head * a.splits;
+    // stretches of equal length, whole turns of the waves; the workgroups of an XCD take neighbouring ones
+    const int groups = gridDim.x;
+    const int64_t stretch = std::max<int64_t>(1, (total + (int64_t)groups * kWaves - 1) / ((int64_t)groups * kWaves)) * kWaves;
+    const int active = (int)((total + stretch - 1) / stretch), per_xcd = (active + 7) / 8;
+    const int me = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+    int32_t *const join = a.joins + 8 * (int64_t)blockIdx.x;
+    if ((int)blockIdx.x / 8 >= per_xcd || me >= active) {
+        if (id == 0) join[0] = -1;
+        return;
+    }
+    int64_t at = me * stretch;
+    const int64_t end = std::min<int64_t>(total, at + stretch);
+    int join_from = -1, join_seq = 0, join_tile = 0, join_head = 0;
+
+    while (at < end) {
+        const int hv = (int)(at / head_tiles), off = (int)(at - (int64_t)hv * head_tiles);
+        if (off >= before && off < before + mine) {     // one thread
+            int b = before;
+            for (int u = id * per; u < min(units, (id + 1) * per); ++u) {
+                const int s = u / a.row_tiles;
+                bool bad;
+                const Sequence q = sequence(a, s, bad);
+                const int n = item_tiles(item_of(a, s, q, u - s * a.row_tiles));
+                if (off < b + n) {
+                    lds.found[0] = s;
+                    lds.found[1] = u - s * a.row_tiles;
+                    lds.found[2] = b;
+                    lds.found[3] = n;
+                    break;
+                }
+                b += n;
+            }
+        }
+        __syncthreads();
+        const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), first = uniform(lds.found[2]), tiles = uniform(lds.found[3]);
+        bool bad;
+        const Sequence q = sequence(a, seq, bad);
+        const Item it = item_of(a, seq, q, row_tile);
+        const int kv_head = hv / a.splits, go = hv - kv_head * a.splits;
+        const int head0 = kv_head * a.group + go * a.split, heads = min(a.split, a.group - go * a.split);
+        const int skip = off - first, take = (int)std::min<int64_t>(tiles - skip, end - at);
+        const int tile0 = it.hi < 0 ? 0 : it.see / kTile;
+
+        Running<D, NQ> st;
+        walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + skip + wave, tile0 + skip + take, lds.wave[wave], st, lane);
+        // ---- the waves' sums, two by two ----
+#pragma unroll
+        for (int half = kWaves / 2; half; half /= 2) {
+            __syncthreads();
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int g = 0; g < NQ; ++g) {
+                    lds.meet.m[wave - half][g][lane] = st.m[g];
+                    lds.meet.l[wave - half][g][lane] = st.l[g];
+#pragma unroll
+                    for (int t = 0; t < T; ++t) lds.meet.o[wave - half][t * NQ + g][lane] = st.o[t][g];
+                }
+            }
+            __syncthreads();
+            if (wave < half) merge<D, NQ>(st, &lds.meet.o[wave][0][0], &lds.meet.m[wave][0][0], &lds.meet.l[wave][0][0], lane);
+        }
+        const bool starts = skip == 0, ends = skip + take == tiles;
+        if (wave == 0) {
+            float *part = a.parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ);
+#pragma unroll
+            for (int g = 0; g < NQ; ++g) {
+                bool live;
+                float *y = out_row<D, NQ>(a, it, head0, heads, g, lane, live);
+                if (!live) continue;
+                if (starts && ends) {
+                    const float f = st.l[g] != 0.f ? 1.f / st.l[g] : 0.f;
+#pragma unroll
+                    for (int t = 0; t < T; ++t) *reinterpret_cast<f32x4 *>(y + 16 * t) = f32x4{st.o[t][g][0] * f, st.o[t][g][1] * f, st.o[t][g][2] * f, st.o[t][g][3] * f};
+                } else {
+#pragma unroll
+                    for (int t = 0; t < T; ++t) reinterpret_cast<f32x4 *>(part)[(t * NQ + g) * 64 + lane] = st.o[t][g];
+                    if (lane < 16) {
+                        part[16 * NQ * D + g * 16 + lane] = st.m[g];
+                        part[16 * NQ * D + (NQ + g) * 16 + lane] = st.l[g];
+                    }
+                }
+            }
+        }
+        if (ends && !starts) {
+            join_from = (int)((at - skip) / stretch);
+            join_seq = seq, join_tile = row_tile, join_head = hv;
+        }
+        at += take;
+        if (at < end) __syncthreads();
+    }
+    if (id == 0) {
+        join[0] = join_from;
+        join[1] = me;
+        join[2] = join_seq;
+        join[3] = join_tile;
+        join[4] = join_head;
+    }
+}
+
+// Items that were cut: the sums of stretches first .. last, a quarter of the dimensions a workgroup.
+template <int D, int NQ>
+__global__ __launch_bounds__(64 * NQ) void attention_join_kernel(const AttentionArgs a) {
+    constexpr int T = D / 16, kQuarter = T / 4;
+    const int32_t *j = a.joins + 8 * (int64_t)blockIdx.x;
+    const int first = j[0], last = j[1];
+    if (first < 0) return;
+    const int lane = threadIdx.x & 63, g = uniform(threadIdx.x >> 6);
+    bool bad;
+    const Sequence q = sequence(a, j[2], bad);
+    const Item it = item_of(a, j[2], q, j[3]);
+    const int kv_head = j[4] / a.splits, go = j[4] - kv_head * a.splits;
+    const int head0 = kv_head * a.group + go * a.split, heads = min(a.split, a.group - go * a.split);
+    bool live;
+    float *y = out_row<D, NQ>(a, it, head0, heads, g, lane, live);
+    if (!live) return;
+    const int64_t size = part_floats(D, NQ);
+    const auto part = [&](int w) { return a.parts + ((int64_t)w * 2 + (w == first ? 1 : 0)) * size; };
+    float m = -INFINITY, l = 0.f;
+    for (int w = first; w <= last; ++w) m = fmaxf(m, part(w)[16 * NQ * D + g * 16 + (lane & 15)]);
+    f32x4 o[kQuarter];
+#pragma unroll
+    for (int t = 0; t < kQuarter; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int w = first; w <= last; ++w) {
+        const float *p = part(w);
+        const float mw = p[16 * NQ * D + g * 16 + (lane & 15)], f = mw == m ? 1.f : __builtin_amdgcn_exp2f(mw - m);
+        l += p[16 * NQ * D + (NQ + g) * 16 + (lane & 15)] * f;
+#pragma unroll
+        for (int t = 0; t < kQuarter; ++t) {
+            const int x = blockIdx.y * kQuarter + t;
+            const f32x4 v = reinterpret_cast<const f32x4 *>(p)[(x * NQ + g) * 64 + lane];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][r] += v[r] * f;
+        }
+    }
+    const float f = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int t = 0; t < kQuarter; ++t)
+        *reinterpret_cast<f32x4 *>(y + 16 * (blockIdx.y * kQuarter + t)) = f32x4{o[t][0] * f, o[t][1] * f, o[t][2] * f, o[t][3] * f};
+}
+
+template <int D, int NQ>
+hipError_t launch(const AttentionArgs &a, int groups, hipStream_t s) {
+    hipLaunchKernelGGL((attention_kernel<D, NQ>), dim3(groups), dim3(kThreads), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || groups == 1) return e;
+    constexpr int T = D / 16, kQuarter = T / 4;
+    static_assert(T % kQuarter == 0, "whole parts of the dimensions");
+    hipLaunchKernelGGL((attention_join_kernel<D, NQ>), dim3(groups, T / kQuarter), dim3(64 * NQ), 0, s, a);
+    return hipGetLastError();
 }
 
 }  // namespace
 
+size_t attention_scratch_bytes(int cus) {
+    return (size_t)cus * 2 * ((size_t)2 * part_floats(256, 2) * 4 + 32);
+}
+
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
-    if (j.n_tokens == 0 || j.n_seq == 0) return hipSuccess;
+    if (j.n_tokens == 0 || j.n_seq == 0 || j.max_q == 0) return hipSuccess;
     AttentionArgs a{};
     a.kv = *j.kv;
     a.q = j.q;
@@ -90,22 +781,42 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     a.q_stride = j.q_stride;
     a.y_stride = j.y_stride;
     a.pages_stride = j.pages_stride;
-    a.n_tokens = j.n_tokens;
-    a.n_seq = j.n_seq;
-    a.max_q = j.max_q;
+    a.n_tokens = (int32_t)j.n_tokens;
+    a.n_seq = (int32_t)j.n_seq;
+    a.max_q = (int32_t)j.max_q;
     a.q_start = j.q_start;
     a.kv_len = j.kv_len;
     a.pages = j.pages;
     a.error = j.error;
-    a.scale = j.scale;
+    a.scale = j.scale * 1.44269504088896341f;
     a.window = j.window;
     a.group = j.n_head / j.kv->n_head;
+    const int cols = j.max_q * a.group <= 16 ? 1 : 2, rows = 16 * cols;
+    a.splits = (a.group + rows - 1) / rows;
+    a.split = (a.group + a.splits - 1) / a.splits;
+    a.tokens = rows / a.split;
+    a.row_tiles = (int32_t)((j.max_q + a.tokens - 1) / a.tokens);
+    // no more workgroups than there can be turns of tiles
+    const int64_t most = ((j.pages_stride << j.kv->page_shift) + kTile - 1) / kTile + 1;
+    const double turns = (double)most * a.n_seq * a.row_tiles * j.kv->n_head * a.splits / kWaves + 1;
+    const int groups = (int)std::min<double>(2.0 * j.cus, turns);
+    a.parts = reinterpret_cast<float *>(j.scratch);
+    a.joins = reinterpret_cast<int32_t *>(j.scratch + (size_t)groups * 2 * part_floats(a.kv.dim, cols) * 4);
     if (dry_run()) {
-        plan_note("attention_kernel: %lld tokens x %d heads, a wave each", (long long)j.n_tokens, j.n_head);
+        plan_note("attention_kernel<%d, %d>: %d heads in %d x %d of %d, %d tokens x %d a sequence of rows, grid %d x %d", a.kv.dim, cols, j.n_head, a.kv.n_head,
+                  a.splits, a.split, a.tokens, a.row_tiles, groups, kThreads);
         return hipSuccess;
     }
-    hipLaunchKernelGGL(attention_kernel, dim3((unsigned)j.n_tokens, (unsigned)j.n_head), dim3(64), 0, s, a);
-    return hipGetLastError();
+    if (cols == 1) {
+        if (a.kv.dim == 64) return launch<64, 1>(a, groups, s);
+        if (a.kv.dim == 96) return launch<96, 1>(a, groups, s);
+        if (a.kv.dim == 128) return launch<128, 1>(a, groups, s);
+        return launch<256, 1>(a, groups, s);
+    }
+    if (a.kv.dim == 64) return launch<64, 2>(a, groups, s);
+    if (a.kv.dim == 96) return launch<96, 2>(a, groups, s);
+    if (a.kv.dim == 128) return launch<128, 2>(a, groups, s);
+    return launch<256, 2>(a, groups, s);
 }
 
 }  // namespace qproj

@@ -83,6 +83,8 @@ struct qproj_ctx {
     size_t ws_bytes = 0;
     uint8_t *ws2 = nullptr;     // second scratch: gate and up outputs of the unfused FFN front end
     size_t ws2_bytes = 0;
+    uint8_t *attention_ws = nullptr;  // fixed scratch of qproj_attention, made by its first call and never moved (captured calls hold it)
+    int cus = 0;                      // compute units of the device
     int32_t *flag_dev = nullptr;  // raised by kernels that meet bad device-side input: [0] expert ids, [1] the cache's (kKvBad*)
 };
 
@@ -780,6 +782,7 @@ int qproj_ctx_create(int device, void *stream, qproj_ctx **out) {
     qproj_ctx *ctx = new (std::nothrow) qproj_ctx();
     if (!ctx) return QPROJ_ERR_OOM;
     ctx->device = device;
+    ctx->cus = p.multiProcessorCount;
     if (hipSetDevice(device) != hipSuccess) {
         delete ctx;
         return QPROJ_ERR_HIP;
@@ -828,6 +831,7 @@ int qproj_ctx_destroy(qproj_ctx *ctx) {
     }
     if (ctx->ws) (void)hipFree(ctx->ws);
     if (ctx->ws2) (void)hipFree(ctx->ws2);
+    if (ctx->attention_ws) (void)hipFree(ctx->attention_ws);
     if (ctx->flag_dev) (void)hipFree(ctx->flag_dev);
     if (ctx->own_stream) (void)hipStreamDestroy(ctx->stream);
     delete ctx;
@@ -1794,11 +1798,25 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
     if (pages_stride * kv->page_tokens > 0x7fffffff) return refuse(ctx, call, "a sequence must stay under 2^31 tokens");
     if (n_head <= 0 || n_head > kMostHeads || n_head % kv->n_head_kv != 0) return refuse(ctx, call, "n_head must be a multiple of n_head_kv");
     if (window < 0) return refuse(ctx, call, "negative window");
+    // (the device counts tiles of 64 tokens in 32 bits)
+    const double rows = (double)n_seq * ((double)std::min(max_q, n_tokens) * (double)(n_head / kv->n_head_kv) / 16 + 1);
+    if (rows * ((double)pages_stride * kv->page_tokens / 64 + 1) > 2e9) return refuse(ctx, call, "n_seq * max_q * pages_stride too large: give max_q, or make several calls");
     if (const char *why = bad_rows(q_dev, q_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
     if (const char *why = bad_rows(y_dev, y_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
     if (q_dev == y_dev) return refuse(ctx, call, "y must not be q");
-    if (!dry_run()) QP_HIP(ctx, hipSetDevice(ctx->device));
+    if (n_tokens == 0 || n_seq == 0) return QPROJ_OK;
+    if (!dry_run()) {
+        QP_HIP(ctx, hipSetDevice(ctx->device));
+        if (!ctx->attention_ws) {
+            hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+            QP_HIP(ctx, hipStreamIsCapturing(ctx->stream, &capture));
+            if (capture != hipStreamCaptureStatusNone) return fail(ctx, QPROJ_ERR_UNSUPPORTED, "qproj_attention: a context's first call allocates and cannot be captured");
+            QP_HIP(ctx, hipMalloc((void **)&ctx->attention_ws, attention_scratch_bytes(ctx->cus)));
+        }
+    }
     AttentionJob j{};
+    j.cus = dry_run() ? 256 : ctx->cus;
+    j.scratch = ctx->attention_ws;
     j.kv = &view;
     j.q = q_dev;
     j.y = y_dev;

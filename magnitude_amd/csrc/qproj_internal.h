@@ -342,7 +342,10 @@ struct AttentionJob {
     float scale;
     int32_t window;
     int32_t *error;
+    int cus;                    // compute units of the device
+    uint8_t *scratch;           // attention_scratch_bytes(cus)
 };
+size_t attention_scratch_bytes(int cus);
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s);
 
 }  // namespace qproj

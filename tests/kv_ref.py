@@ -66,15 +66,16 @@ def decode(n, scales):
 
 
 def attention(cache, q, q_start, kv_len, pages, scale, window=0, n_pages=None):
-    """cache: (k_codes, k_scales, v_codes, v_scales) as numpy arrays.  Returns (y, bound): y [tokens, heads, dim] with NaN in
-    rows of no sequence, and sum_t p_t |v_t| with the largest sum_d |q_d k_td| * scale of a row, for error bounds."""
+    """cache: (k_codes, k_scales, v_codes, v_scales) as numpy arrays.  Returns (y, (weight, steep, spread)): y [tokens, heads, dim] with NaN in
+    rows of no sequence, and for error bounds sum_t p_t |v_t| and, of a row, the largest of a token's sums over d of
+    scale * |q_d| * 8 * (the scale of the key's block), which the products with its codes stay under, and sum_t |v_t|."""
     k_codes, k_scales, v_codes, v_scales = cache
     page = k_codes.shape[2]
     heads_kv, dim = k_codes.shape[1], 2 * k_codes.shape[3]
     q = np.asarray(q, dtype=np.float64)
     group = q.shape[1] // heads_kv
     y = np.full(q.shape, np.nan)
-    weight, steep = np.zeros(q.shape), np.zeros(q.shape[:2])
+    weight, steep, spread = np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape)
     for s in range(len(kv_len)):
         t = np.arange(int(kv_len[s]))
         where = np.asarray(pages)[s][t // page]
@@ -83,6 +84,7 @@ def attention(cache, q, q_start, kv_len, pages, scale, window=0, n_pages=None):
         at = t % page
         k = decode(unpack_keys(k_codes[where, :, at]), k_scales[where, :, at])
         v = decode(unpack_values(v_codes[where, :, at]), v_scales[where, :, at])
+        most = 8 * np.repeat(np.abs(k_scales[where, :, at].astype(np.float64)), 32, axis=-1)
         for r in range(q_start[s], q_start[s + 1]):
             p = int(kv_len[s]) - (q_start[s + 1] - r)
             seen = t <= p
@@ -99,14 +101,19 @@ def attention(cache, q, q_start, kv_len, pages, scale, window=0, n_pages=None):
                     w /= w.sum()
                     y[r, h] = (w[:, None] * vs).sum(0)
                     weight[r, h] = (w[:, None] * np.abs(vs)).sum(0)
-                    steep[r, h] = (np.abs(ks) @ np.abs(q[r, h])).max() * abs(scale)
-    return y, weight, steep
+                    spread[r, h] = np.abs(vs).sum(0)
+                    steep[r, h] = (most[seen, h // group] @ np.abs(q[r, h])).max() * abs(scale)
+    return y, (weight, steep, spread)
 
 
-def allowed(weight, steep, dim, tokens):
-    """How far an fp32 result may be from the exact one.  A score is `dim` products of operands with 22 bits (a fp16 pair: off by
-    2^-22 of the row's largest at most) and fp32 sums of them: off by delta <= steep * (2^-21 + (dim + 16) * 2^-24).  A weight is
+def allowed(sizes, dim, tokens):
+    """How far an fp32 result may be from the exact one.  A score is `dim` products of q, kept in 22 bits (a fp16
+    pair: off by 2^-22 of itself, or of the row's largest over 2^15), with codes of 0 to 15 and, taken off, with 8: three times
+    what steep sums at most.  Their fp32 sums round at most dim + 16 times: delta <= 3 * steep * (2^-21 + (dim + 16) * 2^-24).  A weight is
     then off by a factor of exp(2 delta) at most, by its own rounding to 22 bits, the exponential's (2 ulp) and the running sums'
-    (a rounding every 16 tokens, and one a rescaling: fewer than tokens / 8 + 64)."""
-    delta = steep * (2.0 ** -21 + (dim + 16) * 2.0 ** -24)
-    return weight * (np.expm1(2 * delta)[..., None] + (tokens / 8 + 64) * 2.0 ** -24 + 2.0 ** -21) + 1e-37
+    (a rounding every 16 tokens, and one a rescaling: fewer than tokens / 8 + 64).  A weight that is under 2^-26 of the row's largest
+    is a multiple of 2^-37 of that, a value under 2^-25 of the largest near it a multiple of 2^-36 of that: what a dimension in which
+    the heavy tokens have zeros is off by."""
+    weight, steep, spread = sizes
+    delta = 3 * steep * (2.0 ** -21 + (dim + 16) * 2.0 ** -24)
+    return weight * (np.expm1(2 * delta)[..., None] + (tokens / 8 + 64) * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -36 * spread.max(-1, keepdims=True) + 1e-37

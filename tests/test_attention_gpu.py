@@ -213,18 +213,19 @@ def make_cache(rng, lens, page, kv_heads, dim, spare=3, scale=1.0):
 def check(ctx, kv, pages, q, q_start, kv_len, window=0, scale=None, **kw):
     dim = kv.head_dim
     s = dim ** -0.5 if scale is None else scale
-    want, weight, steep = kv_ref.attention(numpy_cache(kv), q, q_start, kv_len, pages, s, window)
+    want, sizes = kv_ref.attention(numpy_cache(kv), q, q_start, kv_len, pages, s, window)
     out = torch.full(q.shape, 7.5, device="cuda")
     got = ctx.attention(kv, dev(q), dev(np.array(q_start, np.int32)), dev(np.array(kv_len, np.int32)), dev(pages), scale=scale, window=window,
                         out=out, **kw).cpu().numpy()
     mine = ~np.isnan(want).all(-1)
     assert (got[~mine] == 7.5).all()                       # rows of no sequence stay as they were
-    bound = kv_ref.allowed(weight, steep, dim, max([1] + list(kv_len)))
+    bound = kv_ref.allowed(sizes, dim, max([1] + list(kv_len)))
     err = np.abs(got - want)[mine]
     worst = np.max(err / bound[mine]) if err.size else 0.0
     rel = np.linalg.norm(err) / max(1e-30, np.linalg.norm(want[mine])) if err.size else 0.0
     tell(f"   worst {worst:.3g} of what is allowed, {rel:.3g} of the norm")
-    assert worst <= 1.0 and rel <= 1e-5
+    # over all values: 1e-5, and where scores are steep two steps of an fp32 number of their size (it is an exponent: the weight is off by as much)
+    assert worst <= 1.0 and rel <= 1e-5 + sizes[1].max() * 2.0 ** -23
     return got
 
 
@@ -364,7 +365,7 @@ def test_bad_pages_and_bad_bounds_are_reported(ctx):
         torch.cuda.synchronize()
         with pytest.raises(QprojError):
             ctx.sync()
-        want, _, _ = kv_ref.attention(numpy_cache(kv), q, [0, 3, 5], [100, 60], wrong, 64 ** -0.5)     # its tokens are not seen
+        want, _ = kv_ref.attention(numpy_cache(kv), q, [0, 3, 5], [100, 60], wrong, 64 ** -0.5)     # its tokens are not seen
         np.testing.assert_allclose(out.cpu().numpy(), want, rtol=2e-4, atol=2e-5)
     ok = ctx.attention(kv, dev(q), dev(np.array([0, 3, 5], np.int32)), dev(np.array([100, 60], np.int32)), dev(pages)).cpu().numpy()
     for q_start, lens, max_q, left in (([0, 3, 6], [100, 60], 5, [0, 1, 2]), ([0, 3, 5], [100, -1], 5, [0, 1, 2]), ([0, 3, 5], [100, 1 << 20], 5, [0, 1, 2]),
@@ -510,8 +511,8 @@ def test_captured_steps(ctx):
         own.sync()
         torch.cuda.synchronize()
         assert torch.equal(y, eager_y) and torch.equal(q_out, eager_q), f"replay {i}"
-        want, weight, steep = kv_ref.attention(numpy_cache(kv), q_out.cpu().numpy(), [0, 1, 2], lens.cpu().numpy(), order, dim ** -0.5)
-        assert (np.abs(y.cpu().numpy() - want) <= kv_ref.allowed(weight, steep, dim, int(lens.max()))).all()
+        want, sizes = kv_ref.attention(numpy_cache(kv), q_out.cpu().numpy(), [0, 1, 2], lens.cpu().numpy(), order, dim ** -0.5)
+        assert (np.abs(y.cpu().numpy() - want) <= kv_ref.allowed(sizes, dim, int(lens.max()))).all()
     own.close()
 
 
