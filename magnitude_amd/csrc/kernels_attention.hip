@@ -138,6 +138,15 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return (uint32_t)uniform((int)max(x, y));
 }
 
+// keeps a value where it is computed: the compiler otherwise moves whole chains behind the next branch, and what feeds them stays
+// in registers that long
+__device__ __forceinline__ void pin(f32x4 &v) { asm volatile("" : "+v"(v)); }
+// an offset that the block it is used in sees as 32 bits: loads take it beside a scalar base
+__device__ __forceinline__ uint32_t local(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // where the transposing read finds 16-byte chunk `chunk` of a token's value codes: rows of 16 tokens that one read takes
 // together are 16 tokens apart, chunks are turned so that they fall into different banks
 template <int D>
@@ -155,7 +164,7 @@ __device__ __forceinline__ int value_at(int token, int chunk) {
 template <int D, int NQ>
 struct WaveLds {
     uint8_t v[kTile * D / 2];
-    uint16_t k_scale[kTile][D / 32];
+    uint16_t k_scale[D / 32][kTile];
     uint16_t v_scale[D / 32][kTile];
 };
 
@@ -168,8 +177,11 @@ struct SharedLds {
             float m[kWaves / 2][NQ][64], l[kWaves / 2][NQ][64];
         } meet;
     };
+    u32x4 q[D / 32][NQ][2][64];   // the item's queries as the matrix cores take them: high halves, low halves
+    u32x4 q_sum[NQ][64];          // -8 * sum(q) of every block, two halves each
+    float q_unit[NQ][64];         // scores are sums times this
     int32_t wave_total[kWaves];
-    int32_t found[4];   // sequence, row tile, tiles before the item, its tiles
+    int32_t found[4];             // sequence, row tile, turns before the item, its turns
 };
 
 // what a wave holds of an item
@@ -196,10 +208,73 @@ __device__ __forceinline__ void merge(Running<D, NQ> &a, const f32x4 *o, const f
     }
 }
 
-// Tiles [from, to) of an item (in tiles from token 0 on), every kWaves-th of them
+// 16 queries of an item for the matrix cores: 22 bits of q * scale * log2(e), the row scaled by a power of two
 template <int D, int NQ>
-__device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int kv_head, int head0, int heads, int from, int to, WaveLds<D, NQ> &lds,
-                                     Running<D, NQ> &st, int lane) {
+__device__ __forceinline__ void stage_queries(const AttentionArgs &a, const Item &it, int head0, int heads, int g, SharedLds<D, NQ> &lds, int lane) {
+    constexpr int B = D / 32;
+    const int col = lane & 15, part = lane >> 4;
+    const int slot = g * 16 + col, token = slot / a.split, head = slot - token * a.split;
+    const bool live = token < it.count && head < heads;
+    const float *row = a.q + (int64_t)(it.first + (live ? token : 0)) * a.q_stride + (int64_t)(head0 + (live ? head : 0)) * D + 8 * part;
+    f32x4 x[B][2];
+    float most = 0.f;
+    bool whole = true;
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            x[b][k] = *reinterpret_cast<const f32x4 *>(row + 32 * b + 4 * k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[b][k][j] = live ? x[b][k][j] * a.scale : 0.f;
+                most = fmaxf(most, fabsf(x[b][k][j]));
+                whole = whole && fabsf(x[b][k][j]) <= 3.402823466e38f;
+            }
+        }
+    most = max_xor(whole ? most : INFINITY);
+    // (frexp: most = f * 2^e with f in [0.5, 1); where a value is not finite the row stays as it is: NaN comes of it)
+    const int e = most > 0.f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
+    lds.q_unit[g][lane] = ldexpf(1.f, min(e - 15 + 24, 127));
+    float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+        float sum = 0.f;
+        u32x4 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = 15 - e - (i & 1 ? 4 : 0);
+            const float u = ldexpf(x[b][0][i], s), v = ldexpf(x[b][1][i], s);
+            hi[i] = half_pair(u, v);
+            lo[i] = half_pair(u - low_half(hi[i]), v - high_half(hi[i]));
+            sum += ((low_half(hi[i]) + low_half(lo[i])) + (high_half(hi[i]) + high_half(lo[i]))) * (i & 1 ? 16.f : 1.f);
+        }
+        lds.q[b][g][0][lane] = hi;
+        lds.q[b][g][1][lane] = lo;
+        sums[b] = add_xor32(add_xor16(sum)) * (-8.f * 5.9604644775390625e-8f);
+    }
+    // element 8 * part + j multiplies scale j of a token's: of up to four blocks the high halves, then the low ones; of eight the
+    // high halves in part 0, the low ones in part 1
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (B <= 4) {
+            const int b = 2 * i % 4;
+            const uint32_t hi = half_pair(sums[b], sums[b + 1]);
+            w[i] = part != 0 ? 0 : i < 2 ? hi : half_pair(sums[b] - low_half(hi), sums[b + 1] - high_half(hi));
+        } else {
+            const uint32_t hi = half_pair(sums[2 * i], sums[2 * i + 1]);
+            w[i] = part == 0 ? hi : part == 1 ? half_pair(sums[2 * i] - low_half(hi), sums[2 * i + 1] - high_half(hi)) : 0;
+        }
+    }
+    lds.q_sum[g][lane] = w;
+}
+
+// Tiles [from, to) of an item (in tiles from token 0 on), every kWaves-th of them.  One barrier of the workgroup, behind the
+// staged queries, whatever there is to do.
+template <int D, int NQ>
+__device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int kv_head, int head0, int heads, int from, int to, SharedLds<D, NQ> &shared,
+                                     int wave, Running<D, NQ> &st, int lane) {
+    WaveLds<D, NQ> &lds = shared.wave[wave];
     constexpr int B = D / 32, RB = D / 2, T = D / 16;
     constexpr int kLoads = (RB + 63) / 64;       // of 16 bytes a lane for 16 tokens' value codes
     const int col = lane & 15, part = lane >> 4;
@@ -213,7 +288,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
 #pragma unroll
         for (int t = 0; t < T; ++t) st.o[t][g] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if (from >= to || it.hi < 0) return;
+    const bool work = from < to && it.hi >= 0;
 
     // page of the lane's token of a tile (a token outside what is seen: of the nearest one that is)
     const int32_t *table = a.pages + (int64_t)it.seq * a.pages_stride;
@@ -221,7 +296,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         const int t = min(max(tile * kTile + lane, it.see), it.hi);
         return table[t >> shift];
     };
-    int page = page_of(from), page_next = from + kWaves < to ? page_of(from + kWaves) : 0;
+    int page = work ? page_of(from) : 0, page_next = work && from + kWaves < to ? page_of(from + kWaves) : 0;
 
     u32x4 v_raw[4][kLoads];
     uint32_t k_raw[4][B];
@@ -249,7 +324,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         for (int g = 0; g < 4; ++g) {
             const auto base = scalar_global(kv.v_codes + rows[g] * RB);
 #pragma unroll
-            for (int c = 0; c < kLoads; ++c) v_raw[g][c] = load_global<u32x4>(base, v_off[c]);
+            for (int c = 0; c < kLoads; ++c) v_raw[g][c] = load_global<u32x4>(base, local(v_off[c]));
         }
         const int64_t row = part == 0 ? rows[0] : part == 1 ? rows[1] : part == 2 ? rows[2] : rows[3];
         const uint8_t *ks = reinterpret_cast<const uint8_t *>(kv.k_scales) + row * (B * 2) + s_off;
@@ -271,86 +346,43 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         for (int g = 0; g < 4; ++g) {
             const auto base = scalar_global(kv.k_codes + rows[g] * RB);
             if constexpr (B == 2) {
-                const u32x2 w = load_global<u32x2>(base, k_off);
+                const u32x2 w = load_global<u32x2>(base, local(k_off));
                 k_raw[g][0] = w[0], k_raw[g][1] = w[1];
             } else if constexpr (B == 3) {
 #pragma unroll
-                for (int b = 0; b < B; ++b) k_raw[g][b] = load_global<uint32_t>(base, k_off + 4 * b);
+                for (int b = 0; b < B; ++b) k_raw[g][b] = load_global<uint32_t>(base, local(k_off) + 4 * b);
             } else {
 #pragma unroll
                 for (int b = 0; b < B; b += 4) {
-                    const u32x4 w = load_global<u32x4>(base, k_off + 4 * b);
+                    const u32x4 w = load_global<u32x4>(base, local(k_off) + 4 * b);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) k_raw[g][b + i] = w[i];
                 }
             }
         }
     };
-    place(from);
-    load_v();
-    load_k();
+    if (work) {
+        place(from);
+        load_v();
+        load_k();
+    }
+    for (int g = wave; g < NQ; g += kWaves) stage_queries<D, NQ>(a, it, head0, heads, g, shared, lane);
+    __syncthreads();
+    if (!work) return;
 
-    // queries: 22 bits of q * scale * log2(e), scaled by a power of two of the row
-    u32x4 q_hi[B][NQ], q_lo[B][NQ];
-    u32x4 q_sum[NQ];         // -8 * sum(q) of every block, in the accumulators' unit: two halves each, for one more product with the scales
-    int q_exp[NQ], pos[NQ];  // scores are acc * 2^q_exp; position of the column's row, -1: no row
+    int pos[NQ];                // position of the column's row, -1: no row
+    u32x4 q_sum[NQ];
+    float q_unit[NQ];
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
-        const int slot = g * 16 + col, token = slot / a.split, head = slot - token * a.split;
-        const bool live = token < it.count && head < heads;
-        pos[g] = live ? it.lo + token : -1;
-        const float *row = a.q + (int64_t)(it.first + (live ? token : 0)) * a.q_stride + (int64_t)(head0 + (live ? head : 0)) * D + 8 * part;
-        float x[B][8];
-        float most = 0.f;
-        bool whole = true;
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const f32x4 lo = *reinterpret_cast<const f32x4 *>(row + 32 * b), hi = *reinterpret_cast<const f32x4 *>(row + 32 * b + 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[b][j] = live ? lo[j] * a.scale : 0.f;
-                x[b][4 + j] = live ? hi[j] * a.scale : 0.f;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                most = fmaxf(most, fabsf(x[b][j]));
-                whole = whole && fabsf(x[b][j]) <= 3.402823466e38f;
-            }
-        }
-        most = max_xor(whole ? most : INFINITY);
-        // (frexp: most = f * 2^e with f in [0.5, 1); 0 for zero, and where a value is not finite the row stays as it is: NaN comes of it)
-        const int e = most > 0.f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
-        q_exp[g] = e - 15 + 24;
-        float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int s = 15 - e - (i & 1 ? 4 : 0);
-                const float u = ldexpf(x[b][i], s), v = ldexpf(x[b][i + 4], s);
-                const uint32_t hi = half_pair(u, v), lo = half_pair(u - low_half(hi), v - high_half(hi));
-                q_hi[b][g][i] = hi;
-                q_lo[b][g][i] = lo;
-                sum += ((low_half(hi) + low_half(lo)) + (high_half(hi) + high_half(lo))) * (i & 1 ? 16.f : 1.f);
-            }
-            sums[b] = add_xor32(add_xor16(sum)) * (-8.f * 5.9604644775390625e-8f);
-        }
-        // element 8 * part + j multiplies scale (8 * part + j) % B4 of the token: high halves in the first B4 of them, then low ones
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t w = 0;
-            if constexpr (B <= 4) {
-                const int j = 2 * i, b = j % 4;
-                const uint32_t hi = half_pair(sums[b], sums[b + 1]);
-                w = part != 0 ? 0 : j < 4 ? hi : half_pair(sums[b] - low_half(hi), sums[b + 1] - high_half(hi));
-            } else {
-                const uint32_t hi = half_pair(sums[2 * i], sums[2 * i + 1]);
-                w = part == 0 ? hi : part == 1 ? half_pair(sums[2 * i] - low_half(hi), sums[2 * i + 1] - high_half(hi)) : 0;
-            }
-            q_sum[g][i] = w;
-        }
+        const int slot = g * 16 + col, token = slot / a.split;
+        pos[g] = token < it.count && slot - token * a.split < heads ? it.lo + token : -1;
+        q_sum[g] = shared.q_sum[g][lane];
+        q_unit[g] = shared.q_unit[g][lane];
     }
+
+    uint32_t mask0 = 0x000f000fu, mask1 = 0x00f000f0u, magic = 0x64006400u;   // (in registers: and-or in one instruction)
+    asm volatile("" : "+v"(mask0), "+v"(mask1), "+s"(magic));
 
     int unit = 0;               // results are in units of 2^unit
     uint32_t ceiling = 0;       // half bits that a tile's largest |d| stays under, 0: no tile with values yet
@@ -376,7 +408,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         uint16_t vs[B];
 #pragma unroll
         for (int b = 0; b < B; ++b) {
-            lds.k_scale[lane][b] = (uint16_t)(ks_raw[b / 2] >> (16 * (b & 1)));
+            lds.k_scale[b][lane] = (uint16_t)(ks_raw[b / 2] >> (16 * (b & 1)));
             vs[b] = live ? (uint16_t)(vs_raw[b / 2] >> (16 * (b & 1))) : 0;
             most = max(most, (uint32_t)vs[b] & 0x7fffu);
         }
@@ -421,49 +453,49 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         f32x4 s[4][NQ];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            uint32_t d[2 * B];   // scales of the lane's four tokens, two a word
-#pragma unroll
-            for (int i = 0; i < 2 * B; i += 2) {
-                const u32x2 v = *reinterpret_cast<const u32x2 *>(&lds.k_scale[16 * g + 4 * part][0] + 2 * i);
-                d[i] = v[0], d[i + 1] = v[1];
-            }
             u32x4 own;           // scales of the token whose codes the lane holds
-            if constexpr (B <= 4) {
-                const uint16_t *row = &lds.k_scale[16 * g + col][0];
-                own[0] = own[2] = B == 3 ? row[0] | (uint32_t)row[1] << 16 : *reinterpret_cast<const uint32_t *>(row);
-                own[1] = own[3] = B == 2 ? 0 : B == 3 ? row[2] : *reinterpret_cast<const uint32_t *>(row + 2);
-            } else {
-                own = *reinterpret_cast<const u32x4 *>(&lds.k_scale[16 * g + col][0]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int b = B <= 4 ? 2 * i % 4 : 2 * i;
+                own[i] = b < B ? lds.k_scale[b][16 * g + col] | (b + 1 < B ? (uint32_t)lds.k_scale[b + 1 < B ? b + 1 : 0][16 * g + col] << 16 : 0) : 0;
             }
 #pragma unroll
             for (int c = 0; c < NQ; ++c)
                 s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, own), __builtin_bit_cast(half8, q_sum[c]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        }
 #pragma unroll
-            for (int b = 0; b < B; ++b) {
+        for (int b = 0; b < B; ++b) {
+            half8 qh[NQ], ql[NQ];
+#pragma unroll
+            for (int c = 0; c < NQ; ++c) {
+                qh[c] = __builtin_bit_cast(half8, shared.q[b][c][0][lane]);
+                ql[c] = __builtin_bit_cast(half8, shared.q[b][c][1][lane]);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const u32x2 d = *reinterpret_cast<const u32x2 *>(&lds.k_scale[b][16 * g + 4 * part]);
                 const uint32_t w = k_raw[g][b], w8 = w >> 8;
                 const u32x4 n = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
                 const half8 codes = __builtin_bit_cast(half8, n);
 #pragma unroll
                 for (int c = 0; c < NQ; ++c) {
-                    f32x4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, __builtin_bit_cast(half8, q_hi[b][c]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, __builtin_bit_cast(half8, q_lo[b][c]), acc, 0, 0, 0);
+                    f32x4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, ql[c], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, qh[c], acc, 0, 0, 0);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[g][c][r] = fmaf((r * B + b) & 1 ? high_half(d[(r * B + b) / 2]) : low_half(d[(r * B + b) / 2]), acc[r], s[g][c][r]);
+                    for (int r = 0; r < 4; ++r) s[g][c][r] = fmaf(r & 1 ? high_half(d[r / 2]) : low_half(d[r / 2]), acc[r], s[g][c][r]);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int c = 0; c < NQ; ++c) pin(s[g][c]);
         if (more) load_k();
-        __builtin_amdgcn_sched_barrier(0);
         // ---- weights ----
         const bool edge = t0 + kTile - 1 > it.lo || (a.window && t0 <= it.hi - a.window) || t0 < it.see || bad_now;
         u32x4 p_hi[2][NQ], p_lo[2][NQ];
 #pragma unroll
         for (int c = 0; c < NQ; ++c) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s[g][c][r] = ldexpf(s[g][c][r], q_exp[c]);
             if (edge) {
                 const int last = pos[c] - t0 - 4 * part, behind = a.window ? last - a.window : -kTile;   // of the lane's tokens 16 g + r
 #pragma unroll
@@ -477,6 +509,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
             float top = -INFINITY;
 #pragma unroll
             for (int g = 0; g < 4; ++g) top = fmaxf(top, fmaxf(fmaxf(s[g][c][0], s[g][c][1]), fmaxf(s[g][c][2], s[g][c][3])));
+            top *= q_unit[c];
             float back = shrink;
             if (__ballot(top > st.m[c] + kSlack)) {
                 const float m = fmaxf(st.m[c], max_xor(top));
@@ -493,27 +526,28 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                     for (int r = 0; r < 4; ++r) st.o[x][c][r] *= back;
             }
             if (strange) {
+                uint32_t seen = 0;      // bit 4 g + r: the lane's token r of group g
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) seen |= (s[g][c][r] != -INFINITY ? 1u : 0u) << (4 * g + r);
 #pragma unroll
                 for (int b = 0; b < B; ++b) {
-                    const uint64_t own = strange_of[b] >> (4 * part);     // bit 16 g + r: the lane's token r of group g
-                    bool hit = false;
-#pragma unroll
-                    for (int g = 0; g < 4; ++g)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) hit = hit || ((own >> (16 * g + r) & 1) && s[g][c][r] != -INFINITY);
-                    poison[c] |= (uint32_t)hit << b;
+                    const uint64_t own = strange_of[b] >> (4 * part);     // bit 16 g + r
+                    const uint32_t bits = (uint32_t)(own & 15) | (uint32_t)(own >> 12 & 0xf0) | (uint32_t)(own >> 24 & 0xf00) | (uint32_t)(own >> 36 & 0xf000);
+                    poison[c] |= (seen & bits ? 1u : 0u) << b;
                 }
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[g][c][r] = __builtin_amdgcn_exp2f(s[g][c][r] - base[c]);
+                for (int r = 0; r < 4; ++r) s[g][c][r] = __builtin_amdgcn_exp2f(fmaf(s[g][c][r], q_unit[c], -base[c]));
                 st.l[c] += (s[g][c][0] + s[g][c][1]) + (s[g][c][2] + s[g][c][3]);
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
                     const uint32_t hi = half_pair(s[g][c][r], s[g][c][r + 1]);
                     p_hi[g / 2][c][(g & 1) * 2 + r / 2] = hi;
-                    p_lo[g / 2][c][(g & 1) * 2 + r / 2] = half_pair(s[g][c][r] - low_half(hi), s[g][c][r + 1] - high_half(hi));
+                    p_lo[g / 2][c][(g & 1) * 2 + r / 2] = half_pair(fmaf(low_half(hi), -1.f, s[g][c][r]), fmaf(high_half(hi), -1.f, s[g][c][r + 1]));
                 }
             }
         }
@@ -534,11 +568,11 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t w = (uint32_t)raw[h], w8 = w >> 8;
-                    const uint32_t n[4] = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
+                    const uint32_t n[4] = {w & mask0 | magic, w & mask1 | magic, w8 & mask0 | magic, w8 & mask1 | magic};
                     u32x4 a_hi, a_lo;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const half2v big = __builtin_bit_cast(half2v, n[i] | 0x64006400u);   // 1024 + n, or 1024 + 16 n
+                        const half2v big = __builtin_bit_cast(half2v, n[i]);   // 1024 + n, or 1024 + 16 n
                         const half2v code = i & 1 ? __builtin_elementwise_fma(big, half2v{(_Float16)0.0625f, (_Float16)0.0625f}, half2v{(_Float16)-72.f, (_Float16)-72.f})
                                                   : big - half2v{(_Float16)1032.f, (_Float16)1032.f};
                         const half2v e = __builtin_bit_cast(half2v, (uint32_t)d[2 * h + (i >> 1)][i & 1]);
@@ -659,7 +693,7 @@ __global__ __launch_bounds__(kThreads, D * NQ <= 256 ? 2 : 1) void attention_ker
         const int tile0 = it.hi < 0 ? 0 : it.see / kTile;
 
         Running<D, NQ> st;
-        walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + skip + wave, tile0 + skip + take, lds.wave[wave], st, lane);
+        walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + skip + wave, tile0 + skip + take, lds, wave, st, lane);
         // ---- the waves' sums, two by two ----
 #pragma unroll
         for (int half = kWaves / 2; half; half /= 2) {
@@ -714,45 +748,65 @@ __global__ __launch_bounds__(kThreads, D * NQ <= 256 ? 2 : 1) void attention_ker
     }
 }
 
-// Items that were cut: the sums of stretches first .. last, a quarter of the dimensions a workgroup.
+constexpr int join_share(int tiles) { return tiles % 4 ? tiles / 2 : tiles / 4; }   // of the dimensions, in 16s
+
+// Items that were cut: the sums of stretches first .. last, added by four waves in turn.  A workgroup takes 16 queries and a share of
+// the dimensions.
 template <int D, int NQ>
-__global__ __launch_bounds__(64 * NQ) void attention_join_kernel(const AttentionArgs a) {
-    constexpr int T = D / 16, kQuarter = T / 4;
+__global__ __launch_bounds__(kThreads) void attention_join_kernel(const AttentionArgs a) {
+    constexpr int T = D / 16, kShare = join_share(T), kShares = T / kShare;
+    static_assert(T % kShare == 0, "whole shares");
+    __shared__ __align__(16) f32x4 sums[kWaves][kShare][64];
+    __shared__ float weights[kWaves][64];
     const int32_t *j = a.joins + 8 * (int64_t)blockIdx.x;
     const int first = j[0], last = j[1];
     if (first < 0) return;
-    const int lane = threadIdx.x & 63, g = uniform(threadIdx.x >> 6);
-    bool bad;
-    const Sequence q = sequence(a, j[2], bad);
-    const Item it = item_of(a, j[2], q, j[3]);
-    const int kv_head = j[4] / a.splits, go = j[4] - kv_head * a.splits;
-    const int head0 = kv_head * a.group + go * a.split, heads = min(a.split, a.group - go * a.split);
-    bool live;
-    float *y = out_row<D, NQ>(a, it, head0, heads, g, lane, live);
-    if (!live) return;
-    const int64_t size = part_floats(D, NQ);
-    const auto part = [&](int w) { return a.parts + ((int64_t)w * 2 + (w == first ? 1 : 0)) * size; };
-    float m = -INFINITY, l = 0.f;
-    for (int w = first; w <= last; ++w) m = fmaxf(m, part(w)[16 * NQ * D + g * 16 + (lane & 15)]);
-    f32x4 o[kQuarter];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15;
+    const int g = blockIdx.y / kShares, x0 = (blockIdx.y % kShares) * kShare;
+    const float *const cut = a.parts + ((int64_t)first * 2 + 1) * part_floats(D, NQ);   // (the first part is a stretch's second)
+    const int64_t size = 2 * part_floats(D, NQ);
+    const float *const rest = cut - part_floats(D, NQ);
+    const int parts = last - first + 1;
+    constexpr int kM = 16 * NQ * D, kL = kM + 16 * NQ;
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int w = lane >> 4; w < parts; w += 4) top = fmaxf(top, (w ? rest + w * size : cut)[kM + g * 16 + col]);
+    const float m = max_xor(top);
+    f32x4 o[kShare];
 #pragma unroll
-    for (int t = 0; t < kQuarter; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int w = first; w <= last; ++w) {
-        const float *p = part(w);
-        const float mw = p[16 * NQ * D + g * 16 + (lane & 15)], f = mw == m ? 1.f : __builtin_amdgcn_exp2f(mw - m);
-        l += p[16 * NQ * D + (NQ + g) * 16 + (lane & 15)] * f;
+    for (int t = 0; t < kShare; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+#pragma unroll 4
+    for (int w = wave; w < parts; w += kWaves) {
+        const float *p = w ? rest + w * size : cut;
+        const float mw = p[kM + g * 16 + col], f = mw == m ? 1.f : __builtin_amdgcn_exp2f(mw - m);
+        l += p[kL + g * 16 + col] * f;
 #pragma unroll
-        for (int t = 0; t < kQuarter; ++t) {
-            const int x = blockIdx.y * kQuarter + t;
-            const f32x4 v = reinterpret_cast<const f32x4 *>(p)[(x * NQ + g) * 64 + lane];
+        for (int t = 0; t < kShare; ++t) {
+            const f32x4 v = reinterpret_cast<const f32x4 *>(p)[((x0 + t) * NQ + g) * 64 + lane];
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[t][r] += v[r] * f;
         }
     }
-    const float f = l != 0.f ? 1.f / l : 0.f;
+    weights[wave][lane] = l;
 #pragma unroll
-    for (int t = 0; t < kQuarter; ++t)
-        *reinterpret_cast<f32x4 *>(y + 16 * (blockIdx.y * kQuarter + t)) = f32x4{o[t][0] * f, o[t][1] * f, o[t][2] * f, o[t][3] * f};
+    for (int t = 0; t < kShare; ++t) sums[wave][t][lane] = o[t];
+    __syncthreads();
+    if (wave >= kShare) return;
+    bool bad, live;
+    const Sequence q = sequence(a, j[2], bad);
+    const Item it = item_of(a, j[2], q, j[3]);
+    const int kv_head = j[4] / a.splits, go = j[4] - kv_head * a.splits;
+    float *y = out_row<D, NQ>(a, it, kv_head * a.group + go * a.split, min(a.split, a.group - go * a.split), g, lane, live);
+    if (!live) return;
+    const float sum = (weights[0][lane] + weights[1][lane]) + (weights[2][lane] + weights[3][lane]);
+    const float f = sum != 0.f ? 1.f / sum : 0.f;
+    for (int t = wave; t < kShare; t += kWaves) {
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = ((sums[0][t][lane][r] + sums[1][t][lane][r]) + (sums[2][t][lane][r] + sums[3][t][lane][r])) * f;
+        *reinterpret_cast<f32x4 *>(y + 16 * (x0 + t)) = v;
+    }
 }
 
 template <int D, int NQ>
@@ -760,9 +814,7 @@ hipError_t launch(const AttentionArgs &a, int groups, hipStream_t s) {
     hipLaunchKernelGGL((attention_kernel<D, NQ>), dim3(groups), dim3(kThreads), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || groups == 1) return e;
-    constexpr int T = D / 16, kQuarter = T / 4;
-    static_assert(T % kQuarter == 0, "whole parts of the dimensions");
-    hipLaunchKernelGGL((attention_join_kernel<D, NQ>), dim3(groups, T / kQuarter), dim3(64 * NQ), 0, s, a);
+    hipLaunchKernelGGL((attention_join_kernel<D, NQ>), dim3(groups, D / 16 / join_share(D / 16) * NQ), dim3(kThreads), 0, s, a);
     return hipGetLastError();
 }
 
