@@ -64,9 +64,12 @@ struct AttentionArgs {
     int32_t splits, split;   // they are served `split` at a time, in `splits` goes
     int32_t tokens;          // new tokens of an item
     int32_t row_tiles;       // items of a sequence, at most
+    int32_t start;           // turns that beginning an item costs
 };
 
 constexpr int part_floats(int dim, int cols) { return 16 * cols * (dim + 2); }
+
+constexpr int waves_per_simd(int dim, int cols) { return dim <= 128 && cols == 1 ? 3 : dim * cols <= 256 ? 2 : 1; }
 
 struct Sequence {
     int start, count, len;   // first row, rows, tokens in the cache; count 0 where there is nothing to do
@@ -101,7 +104,11 @@ __device__ __forceinline__ Item item_of(const AttentionArgs &a, int s, const Seq
     return it;
 }
 
-__device__ __forceinline__ int item_tiles(const Item &it) { return it.count <= 0 ? 0 : it.hi < 0 ? 1 : it.hi / kTile - it.see / kTile + 1; }
+// what an item takes of the line: a turn of the waves for every kWaves tiles, and `start` for staging its queries and adding its sums
+__device__ __forceinline__ int item_tiles(const Item &it) { return it.hi < 0 ? 1 : it.hi / kTile - it.see / kTile + 1; }
+__device__ __forceinline__ int item_turns(const AttentionArgs &a, const Item &it) {
+    return it.count <= 0 ? 0 : a.start + (item_tiles(it) + kWaves - 1) / kWaves;
+}
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -168,17 +175,19 @@ struct WaveLds {
     uint16_t v_scale[D / 32][kTile];
 };
 
+constexpr int meet_rounds(int dim) { return dim > 128 ? 2 : 1; }   // (so that two workgroups' LDS fit)
+
 template <int D, int NQ>
 struct SharedLds {
     union {
         WaveLds<D, NQ> wave[kWaves];
         struct {
-            f32x4 o[kWaves / 2][D / 16 * NQ][64];
-            float m[kWaves / 2][NQ][64], l[kWaves / 2][NQ][64];
+            f32x4 o[kWaves][D / 16 / meet_rounds(D)][64];
+            float m[kWaves][16], l[kWaves][16];
         } meet;
     };
     u32x4 q[D / 32][NQ][2][64];   // the item's queries as the matrix cores take them: high halves, low halves
-    u32x4 q_sum[NQ][64];          // -8 * sum(q) of every block, two halves each
+    u32x4 q_sum[NQ][D / 32 <= 4 ? 1 : 2][64];   // -8 * sum(q) of every block, two halves each
     float q_unit[NQ][64];         // scores are sums times this
     int32_t wave_total[kWaves];
     int32_t found[4];             // sequence, row tile, turns before the item, its turns
@@ -190,23 +199,6 @@ struct Running {
     f32x4 o[D / 16][NQ];   // [16 dimensions][16 queries]: lane's column is query lane % 16, rows 4 * (lane / 16) + r
     float m[NQ], l[NQ];    // of the lane's column; l of the lane's own tokens only until the end
 };
-
-template <int D, int NQ>
-__device__ __forceinline__ void merge(Running<D, NQ> &a, const f32x4 *o, const float *m, const float *l, int lane) {
-#pragma unroll
-    for (int g = 0; g < NQ; ++g) {
-        const float mo = m[g * 64 + lane], top = fmaxf(a.m[g], mo);
-        const float fa = a.m[g] == top ? 1.f : __builtin_amdgcn_exp2f(a.m[g] - top), fo = mo == top ? 1.f : __builtin_amdgcn_exp2f(mo - top);
-        a.l[g] = a.l[g] * fa + l[g * 64 + lane] * fo;
-        a.m[g] = top;
-#pragma unroll
-        for (int t = 0; t < D / 16; ++t) {
-            const f32x4 x = o[(t * NQ + g) * 64 + lane];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) a.o[t][g][r] = a.o[t][g][r] * fa + x[r] * fo;
-        }
-    }
-}
 
 // 16 queries of an item for the matrix cores: 22 bits of q * scale * log2(e), the row scaled by a power of two
 template <int D, int NQ>
@@ -252,21 +244,19 @@ __device__ __forceinline__ void stage_queries(const AttentionArgs &a, const Item
         lds.q[b][g][1][lane] = lo;
         sums[b] = add_xor32(add_xor16(sum)) * (-8.f * 5.9604644775390625e-8f);
     }
-    // element 8 * part + j multiplies scale j of a token's: of up to four blocks the high halves, then the low ones; of eight the
-    // high halves in part 0, the low ones in part 1
-    u32x4 w;
+    // up to four blocks: high halves, then low ones, against the scales twice; eight: two products
+    u32x4 hi, lo;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if constexpr (B <= 4) {
-            const int b = 2 * i % 4;
-            const uint32_t hi = half_pair(sums[b], sums[b + 1]);
-            w[i] = part != 0 ? 0 : i < 2 ? hi : half_pair(sums[b] - low_half(hi), sums[b + 1] - high_half(hi));
-        } else {
-            const uint32_t hi = half_pair(sums[2 * i], sums[2 * i + 1]);
-            w[i] = part == 0 ? hi : part == 1 ? half_pair(sums[2 * i] - low_half(hi), sums[2 * i + 1] - high_half(hi)) : 0;
-        }
+        hi[i] = half_pair(sums[2 * i], sums[2 * i + 1]);
+        lo[i] = half_pair(sums[2 * i] - low_half(hi[i]), sums[2 * i + 1] - high_half(hi[i]));
     }
-    lds.q_sum[g][lane] = w;
+    if constexpr (B <= 4) {
+        lds.q_sum[g][0][lane] = u32x4{hi[0], hi[1], lo[0], lo[1]};
+    } else {
+        lds.q_sum[g][0][lane] = hi;
+        lds.q_sum[g][1][lane] = lo;
+    }
 }
 
 // Tiles [from, to) of an item (in tiles from token 0 on), every kWaves-th of them.  One barrier of the workgroup, behind the
@@ -296,7 +286,9 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         const int t = min(max(tile * kTile + lane, it.see), it.hi);
         return table[t >> shift];
     };
-    int page = work ? page_of(from) : 0, page_next = work && from + kWaves < to ? page_of(from + kWaves) : 0;
+    const int last_tile = work ? from + (to - 1 - from) / kWaves * kWaves : from;   // of this wave
+    int page = work ? page_of(from) : 0, page_next = work ? page_of(min(from + kWaves, last_tile)) : 0;
+    bool bad_page = false;
 
     u32x4 v_raw[4][kLoads];
     uint32_t k_raw[4][B];
@@ -307,7 +299,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     const auto place = [&](int tile) {   // rows of the tile whose pages have come
         const int t = min(max(tile * kTile + lane, it.see), it.hi);
         const bool bad = page < 0 || page >= kv.n_pages;
-        if (bad && t == tile * kTile + lane) atomicOr(a.error, kKvBadPage);
+        bad_page = bad_page || (bad && t == tile * kTile + lane);
         bad_groups = 0;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -371,13 +363,14 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     if (!work) return;
 
     int pos[NQ];                // position of the column's row, -1: no row
-    u32x4 q_sum[NQ];
+    u32x4 q_sum[NQ][B <= 4 ? 1 : 2];
     float q_unit[NQ];
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
         const int slot = g * 16 + col, token = slot / a.split;
         pos[g] = token < it.count && slot - token * a.split < heads ? it.lo + token : -1;
-        q_sum[g] = shared.q_sum[g][lane];
+#pragma unroll
+        for (int i = 0; i < (B <= 4 ? 1 : 2); ++i) q_sum[g][i] = shared.q_sum[g][i][lane];
         q_unit[g] = shared.q_unit[g][lane];
     }
 
@@ -385,7 +378,6 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     asm volatile("" : "+v"(mask0), "+v"(mask1), "+s"(magic));
 
     int unit = 0;               // results are in units of 2^unit
-    uint32_t ceiling = 0;       // half bits that a tile's largest |d| stays under, 0: no tile with values yet
     float base[NQ];             // what is taken off a score
     uint32_t poison[NQ];        // blocks of values that are not finite and were seen
 #pragma unroll
@@ -405,12 +397,15 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         const int t = t0 + lane;
         const bool live = t >= it.see && t <= it.hi && !((bad_now >> part) & 1);
         uint32_t most = 0;
+        bool tiny = false;
         uint16_t vs[B];
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             lds.k_scale[b][lane] = (uint16_t)(ks_raw[b / 2] >> (16 * (b & 1)));
             vs[b] = live ? (uint16_t)(vs_raw[b / 2] >> (16 * (b & 1))) : 0;
-            most = max(most, (uint32_t)vs[b] & 0x7fffu);
+            const uint32_t size = (uint32_t)vs[b] & 0x7fffu;
+            most = max(most, size);
+            tiny = tiny || size - 1 < 0x3ffu;       // (zero is not)
         }
         uint64_t strange = __ballot(most >= 0x7c00u);
         if (strange) {           // blocks that are not finite count as zeros here; who sees them gets NaN below
@@ -419,21 +414,20 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
             for (int b = 0; b < B; ++b)
                 if ((vs[b] & 0x7fffu) < 0x7c00u) most = max(most, (uint32_t)vs[b] & 0x7fffu);
         }
-        // the tile's largest scale goes to 2^11 .. 2^12; a tile within a factor of 2^8 below keeps the unit of the one before
-        float shrink = 1.f;      // of what has been summed
-        if (__ballot(most >= ceiling) || (ceiling > 0x2400u && !__ballot(most >= ceiling - 0x2400u) && __ballot(most != 0))) {
+        // scales within 2^-14 .. 2^12 are taken as they are; otherwise the tile's largest goes to 2^11 .. 2^12
+        int unit_now = 0;
+        if (__ballot(most >= 0x6c00u || tiny)) {
             const uint32_t top = wave_max(most);
-            if (top) {
-                const int e = __builtin_amdgcn_frexp_expf(h2f(top));     // top < 2^e
-                if (ceiling) shrink = ldexpf(1.f, unit - (e - 12));
-                unit = e - 12;
-                ceiling = e >= 16 ? 0x7c00u : e > -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);   // the bits of 2^e
-            }
+            unit_now = top ? __builtin_amdgcn_frexp_expf(h2f(top)) - 12 : unit;     // top < 2^(unit + 12)
         }
+        const float shrink = unit_now == unit ? 1.f : ldexpf(1.f, unit - unit_now);  // of what has been summed
+        unit = unit_now;
+        if (unit == 0 && !strange) {
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const bool fine = (vs[b] & 0x7fffu) < 0x7c00u;
-            lds.v_scale[b][lane] = fine ? f2h(ldexpf(h2f(vs[b]), -unit)) : 0;
+            for (int b = 0; b < B; ++b) lds.v_scale[b][lane] = vs[b];
+        } else {
+#pragma unroll
+            for (int b = 0; b < B; ++b) lds.v_scale[b][lane] = (vs[b] & 0x7fffu) < 0x7c00u ? f2h(ldexpf(h2f(vs[b]), -unit)) : 0;
         }
         uint64_t strange_of[B];
         if (strange) {
@@ -441,27 +435,35 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
             for (int b = 0; b < B; ++b) strange_of[b] = __ballot((vs[b] & 0x7fffu) >= 0x7c00u);
         }
         wave_sync();
+        uint32_t own_scales[(B + 1) / 2];
+#pragma unroll
+        for (int i = 0; i < (B + 1) / 2; ++i) own_scales[i] = ks_raw[i];
         // ---- the next tile's values and scales, and the page of the one behind ----
-        const bool more = tile + kWaves < to;
-        if (more) {
-            page = page_next;
-            if (tile + 2 * kWaves < to) page_next = page_of(tile + 2 * kWaves);
-            place(tile + kWaves);
-            load_v();
-        }
+        // (behind the wave's last tile that tile again: loads that no branch surrounds are waited for one by one)
+        page = page_next;
+        page_next = page_of(min(tile + 2 * kWaves, last_tile));
+        place(min(tile + kWaves, last_tile));
+        load_v();
         // ---- scores ----
         f32x4 s[4][NQ];
+        // (-8 * sum(q) * d over the blocks: the lanes of part g hold the scales of group g's tokens, the others take no part)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            u32x4 own;           // scales of the token whose codes the lane holds
+            const auto own = [&](int i) { return part == g ? own_scales[i] : 0u; };
+            if constexpr (B <= 4) {
+                const uint32_t w0 = own(0), w1 = B > 2 ? own(1) : 0;
+                const u32x4 w = {w0, w1, w0, w1};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int b = B <= 4 ? 2 * i % 4 : 2 * i;
-                own[i] = b < B ? lds.k_scale[b][16 * g + col] | (b + 1 < B ? (uint32_t)lds.k_scale[b + 1 < B ? b + 1 : 0][16 * g + col] << 16 : 0) : 0;
+                for (int c = 0; c < NQ; ++c)
+                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, q_sum[c][0]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            } else {
+                const u32x4 w = {own(0), own(1), own(2), own(3)};
+#pragma unroll
+                for (int c = 0; c < NQ; ++c) {
+                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, q_sum[c][1]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, q_sum[c][0]), s[g][c], 0, 0, 0);
+                }
             }
-#pragma unroll
-            for (int c = 0; c < NQ; ++c)
-                s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, own), __builtin_bit_cast(half8, q_sum[c]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
         }
 #pragma unroll
         for (int b = 0; b < B; ++b) {
@@ -490,7 +492,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         for (int g = 0; g < 4; ++g)
 #pragma unroll
             for (int c = 0; c < NQ; ++c) pin(s[g][c]);
-        if (more) load_k();
+        load_k();
         // ---- weights ----
         const bool edge = t0 + kTile - 1 > it.lo || (a.window && t0 <= it.hi - a.window) || t0 < it.see || bad_now;
         u32x4 p_hi[2][NQ], p_lo[2][NQ];
@@ -594,6 +596,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         }
         wave_sync();
     }
+    if (bad_page) atomicOr(a.error, kKvBadPage);
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
         st.l[c] = add_xor32(add_xor16(st.l[c]));
@@ -618,19 +621,19 @@ __device__ __forceinline__ float *out_row(const AttentionArgs &a, const Item &it
 }
 
 template <int D, int NQ>
-__global__ __launch_bounds__(kThreads, D * NQ <= 256 ? 2 : 1) void attention_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_kernel(const AttentionArgs a) {
     constexpr int T = D / 16;
     __shared__ __align__(16) SharedLds<D, NQ> lds;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
     const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
-    // ---- the line of tiles: a thread counts those of `per` items of one head ----
+    // ---- the line of turns: a thread counts those of `per` items of one head ----
     int mine = 0;
     for (int u = id * per; u < min(units, (id + 1) * per); ++u) {
         const int s = u / a.row_tiles;
         bool bad;
         const Sequence q = sequence(a, s, bad);
         if (bad && u == s * a.row_tiles && blockIdx.x == 0) atomicOr(a.error, kKvBadRows);
-        mine += item_tiles(item_of(a, s, q, u - s * a.row_tiles));
+        mine += item_turns(a, item_of(a, s, q, u - s * a.row_tiles));
     }
     int before = mine;
 #pragma unroll
@@ -641,17 +644,17 @@ __global__ __launch_bounds__(kThreads, D * NQ <= 256 ? 2 : 1) void attention_ker
     if (lane == 63) lds.wave_total[wave] = before;
     before -= mine;
     __syncthreads();
-    int head_tiles = 0;
+    int head_turns = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         if (w < wave) before += lds.wave_total[w];
-        head_tiles += lds.wave_total[w];
+        head_turns += lds.wave_total[w];
     }
-    head_tiles = uniform(head_tiles);
-    const int64_t total = (int64_t)head_tiles * a.kv.n_head * a.splits;
-    // stretches of equal length, whole turns of the waves; the workgroups of an XCD take neighbouring ones
+    head_turns = uniform(head_turns);
+    const int64_t total = (int64_t)head_turns * a.kv.n_head * a.splits;
+    // stretches of equal length; the workgroups of an XCD take neighbouring ones
     const int groups = gridDim.x;
-    const int64_t stretch = std::max<int64_t>(1, (total + (int64_t)groups * kWaves - 1) / ((int64_t)groups * kWaves)) * kWaves;
+    const int64_t stretch = std::max<int64_t>(1, (total + groups - 1) / groups);
     const int active = (int)((total + stretch - 1) / stretch), per_xcd = (active + 7) / 8;
     const int me = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
     int32_t *const join = a.joins + 8 * (int64_t)blockIdx.x;
@@ -664,14 +667,14 @@ __global__ __launch_bounds__(kThreads, D * NQ <= 256 ? 2 : 1) void attention_ker
     int join_from = -1, join_seq = 0, join_tile = 0, join_head = 0;
 
     while (at < end) {
-        const int hv = (int)(at / head_tiles), off = (int)(at - (int64_t)hv * head_tiles);
+        const int hv = (int)(at / head_turns), off = (int)(at - (int64_t)hv * head_turns);
         if (off >= before && off < before + mine) {     // one thread
             int b = before;
             for (int u = id * per; u < min(units, (id + 1) * per); ++u) {
                 const int s = u / a.row_tiles;
                 bool bad;
                 const Sequence q = sequence(a, s, bad);
-                const int n = item_tiles(item_of(a, s, q, u - s * a.row_tiles));
+                const int n = item_turns(a, item_of(a, s, q, u - s * a.row_tiles));
                 if (off < b + n) {
                     lds.found[0] = s;
                     lds.found[1] = u - s * a.row_tiles;
@@ -683,57 +686,72 @@ __global__ __launch_bounds__(kThreads, D * NQ <= 256 ? 2 : 1) void attention_ker
             }
         }
         __syncthreads();
-        const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), first = uniform(lds.found[2]), tiles = uniform(lds.found[3]);
+        const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), first = uniform(lds.found[2]), turns = uniform(lds.found[3]) - a.start;
         bool bad;
         const Sequence q = sequence(a, seq, bad);
         const Item it = item_of(a, seq, q, row_tile);
         const int kv_head = hv / a.splits, go = hv - kv_head * a.splits;
         const int head0 = kv_head * a.group + go * a.split, heads = min(a.split, a.group - go * a.split);
-        const int skip = off - first, take = (int)std::min<int64_t>(tiles - skip, end - at);
-        const int tile0 = it.hi < 0 ? 0 : it.see / kTile;
+        // the stretch's turns of the item: none where it ends within the item's start
+        const int skip = off - first, take = (int)std::min<int64_t>(turns + a.start - skip, end - at);
+        const int turn0 = max(0, skip - a.start), turn1 = skip + take - a.start;
+        if (turn1 <= 0) break;
+        const int tile0 = it.hi < 0 ? 0 : it.see / kTile, tile1 = tile0 + min(turn1 * kWaves, item_tiles(it));
 
         Running<D, NQ> st;
-        walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + skip + wave, tile0 + skip + take, lds, wave, st, lane);
-        // ---- the waves' sums, two by two ----
+        walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + turn0 * kWaves + wave, tile1, lds, wave, st, lane);
+        // ---- the waves' sums: every wave adds a quarter of them ----
+        const bool starts = turn0 == 0, ends = turn1 == turns;
+        float *part = a.parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ);
+        constexpr int kMeet = T / meet_rounds(D);
 #pragma unroll
-        for (int half = kWaves / 2; half; half /= 2) {
-            __syncthreads();
-            if (wave >= half && wave < 2 * half) {
+        for (int g = 0; g < NQ; ++g) {
+            bool live;
+            float *y = out_row<D, NQ>(a, it, head0, heads, g, lane, live);
 #pragma unroll
-                for (int g = 0; g < NQ; ++g) {
-                    lds.meet.m[wave - half][g][lane] = st.m[g];
-                    lds.meet.l[wave - half][g][lane] = st.l[g];
-#pragma unroll
-                    for (int t = 0; t < T; ++t) lds.meet.o[wave - half][t * NQ + g][lane] = st.o[t][g];
+            for (int t0 = 0; t0 < T; t0 += kMeet) {
+                __syncthreads();
+                if (lane < 16) {
+                    lds.meet.m[wave][lane] = st.m[g];
+                    lds.meet.l[wave][lane] = st.l[g];
                 }
-            }
-            __syncthreads();
-            if (wave < half) merge<D, NQ>(st, &lds.meet.o[wave][0][0], &lds.meet.m[wave][0][0], &lds.meet.l[wave][0][0], lane);
-        }
-        const bool starts = skip == 0, ends = skip + take == tiles;
-        if (wave == 0) {
-            float *part = a.parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ);
 #pragma unroll
-            for (int g = 0; g < NQ; ++g) {
-                bool live;
-                float *y = out_row<D, NQ>(a, it, head0, heads, g, lane, live);
-                if (!live) continue;
-                if (starts && ends) {
-                    const float f = st.l[g] != 0.f ? 1.f / st.l[g] : 0.f;
+                for (int t = 0; t < kMeet; ++t) lds.meet.o[wave][t][lane] = st.o[t0 + t][g];
+                __syncthreads();
+                if (live) {
+                    float m = -INFINITY, l = 0.f, f[kWaves];
 #pragma unroll
-                    for (int t = 0; t < T; ++t) *reinterpret_cast<f32x4 *>(y + 16 * t) = f32x4{st.o[t][g][0] * f, st.o[t][g][1] * f, st.o[t][g][2] * f, st.o[t][g][3] * f};
-                } else {
+                    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, lds.meet.m[w][lane & 15]);
 #pragma unroll
-                    for (int t = 0; t < T; ++t) reinterpret_cast<f32x4 *>(part)[(t * NQ + g) * 64 + lane] = st.o[t][g];
-                    if (lane < 16) {
-                        part[16 * NQ * D + g * 16 + lane] = st.m[g];
-                        part[16 * NQ * D + (NQ + g) * 16 + lane] = st.l[g];
+                    for (int w = 0; w < kWaves; ++w) {
+                        const float mw = lds.meet.m[w][lane & 15];
+                        f[w] = mw == m ? 1.f : __builtin_amdgcn_exp2f(mw - m);
+                        l += lds.meet.l[w][lane & 15] * f[w];
+                    }
+                    const bool whole = starts && ends;
+                    const float unit = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
+                    for (int t = wave; t < kMeet; t += kWaves) {
+                        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int w = 0; w < kWaves; ++w) {
+                            const f32x4 x = lds.meet.o[w][t][lane];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) v[r] += x[r] * f[w];
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] *= unit;
+                        if (whole) *reinterpret_cast<f32x4 *>(y + 16 * (t0 + t)) = v;
+                        else reinterpret_cast<f32x4 *>(part)[((t0 + t) * NQ + g) * 64 + lane] = v;
+                    }
+                    if (!whole && wave == 0 && lane < 16) {
+                        part[16 * NQ * D + g * 16 + lane] = m;
+                        part[16 * NQ * D + (NQ + g) * 16 + lane] = l;
                     }
                 }
             }
         }
         if (ends && !starts) {
-            join_from = (int)((at - skip) / stretch);
+            join_from = (int)((at - skip + a.start) / stretch);
             join_seq = seq, join_tile = row_tile, join_head = hv;
         }
         at += take;
@@ -821,7 +839,7 @@ hipError_t launch(const AttentionArgs &a, int groups, hipStream_t s) {
 }  // namespace
 
 size_t attention_scratch_bytes(int cus) {
-    return (size_t)cus * 2 * ((size_t)2 * part_floats(256, 2) * 4 + 32);
+    return (size_t)cus * 3 * ((size_t)2 * part_floats(256, 2) * 4 + 32);   // (more than any instance takes)
 }
 
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
@@ -848,10 +866,12 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     a.split = (a.group + a.splits - 1) / a.splits;
     a.tokens = rows / a.split;
     a.row_tiles = (int32_t)((j.max_q + a.tokens - 1) / a.tokens);
-    // no more workgroups than there can be turns of tiles
+    const int groups_most = waves_per_simd(a.kv.dim, cols) * j.cus;
+    a.start = 2 * (int64_t)a.row_tiles * a.n_seq * a.kv.n_head * a.splits > groups_most ? 2 : 0;
+    // no more workgroups than there can be turns
     const int64_t most = ((j.pages_stride << j.kv->page_shift) + kTile - 1) / kTile + 1;
-    const double turns = (double)most * a.n_seq * a.row_tiles * j.kv->n_head * a.splits / kWaves + 1;
-    const int groups = (int)std::min<double>(2.0 * j.cus, turns);
+    const double turns = (double)most * a.n_seq * a.row_tiles * j.kv->n_head * a.splits / kWaves + (double)a.n_seq * a.row_tiles * j.kv->n_head * a.splits;
+    const int groups = (int)std::min<double>(groups_most, turns);
     a.parts = reinterpret_cast<float *>(j.scratch);
     a.joins = reinterpret_cast<int32_t *>(j.scratch + (size_t)groups * 2 * part_floats(a.kv.dim, cols) * 4);
     if (dry_run()) {
