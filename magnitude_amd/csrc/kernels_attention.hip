@@ -64,12 +64,11 @@ struct AttentionArgs {
     int32_t splits, split;   // they are served `split` at a time, in `splits` goes
     int32_t tokens;          // new tokens of an item
     int32_t row_tiles;       // items of a sequence, at most
-    int32_t start;           // turns that beginning an item costs
 };
 
 constexpr int part_floats(int dim, int cols) { return 16 * cols * (dim + 2); }
 
-constexpr int waves_per_simd(int dim, int cols) { return dim <= 128 && cols == 1 ? 3 : dim * cols <= 256 ? 2 : 1; }
+constexpr int waves_per_simd(int dim, int cols) { return dim * cols <= 256 ? 2 : 1; }
 
 struct Sequence {
     int start, count, len;   // first row, rows, tokens in the cache; count 0 where there is nothing to do
@@ -104,11 +103,9 @@ __device__ __forceinline__ Item item_of(const AttentionArgs &a, int s, const Seq
     return it;
 }
 
-// what an item takes of the line: a turn of the waves for every kWaves tiles, and `start` for staging its queries and adding its sums
 __device__ __forceinline__ int item_tiles(const Item &it) { return it.hi < 0 ? 1 : it.hi / kTile - it.see / kTile + 1; }
-__device__ __forceinline__ int item_turns(const AttentionArgs &a, const Item &it) {
-    return it.count <= 0 ? 0 : a.start + (item_tiles(it) + kWaves - 1) / kWaves;
-}
+// what an item takes of the line: a turn of the waves for every kWaves tiles
+__device__ __forceinline__ int item_turns(const Item &it) { return it.count <= 0 ? 0 : (item_tiles(it) + kWaves - 1) / kWaves; }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -189,8 +186,8 @@ struct SharedLds {
     u32x4 q[D / 32][NQ][2][64];   // the item's queries as the matrix cores take them: high halves, low halves
     u32x4 q_sum[NQ][D / 32 <= 4 ? 1 : 2][64];   // -8 * sum(q) of every block, two halves each
     float q_unit[NQ][64];         // scores are sums times this
-    int32_t wave_total[kWaves];
-    int32_t found[4];             // sequence, row tile, turns before the item, its turns
+    int32_t wave_turns[kWaves], wave_items[kWaves];
+    int32_t found[8];             // sequence, row tile, turns before the item, its turns, and the sequence's first row, rows, tokens
 };
 
 // what a wave holds of an item
@@ -627,33 +624,39 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
     const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
     // ---- the line of turns: a thread counts those of `per` items of one head ----
-    int mine = 0;
+    int turns_mine = 0, items_mine = 0;
     for (int u = id * per; u < min(units, (id + 1) * per); ++u) {
         const int s = u / a.row_tiles;
         bool bad;
         const Sequence q = sequence(a, s, bad);
         if (bad && u == s * a.row_tiles && blockIdx.x == 0) atomicOr(a.error, kKvBadRows);
-        mine += item_turns(a, item_of(a, s, q, u - s * a.row_tiles));
+        const int n = item_turns(item_of(a, s, q, u - s * a.row_tiles));
+        turns_mine += n;
+        items_mine += n > 0;
     }
-    int before = mine;
+    int turns_before = turns_mine, items_before = items_mine;
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) {
-        const int o = __shfl_up(before, x);
-        if (lane >= x) before += o;
+        const int o = __shfl_up(turns_before, x), p = __shfl_up(items_before, x);
+        if (lane >= x) turns_before += o, items_before += p;
     }
-    if (lane == 63) lds.wave_total[wave] = before;
-    before -= mine;
+    if (lane == 63) lds.wave_turns[wave] = turns_before, lds.wave_items[wave] = items_before;
+    turns_before -= turns_mine, items_before -= items_mine;
     __syncthreads();
-    int head_turns = 0;
+    int head_turns = 0, head_items = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) before += lds.wave_total[w];
-        head_turns += lds.wave_total[w];
+        if (w < wave) turns_before += lds.wave_turns[w], items_before += lds.wave_items[w];
+        head_turns += lds.wave_turns[w];
+        head_items += lds.wave_items[w];
     }
-    head_turns = uniform(head_turns);
-    const int64_t total = (int64_t)head_turns * a.kv.n_head * a.splits;
+    // Where there are more turns than workgroups, beginning an item (staging its queries, adding its sums) counts as a turn.
+    const int groups = gridDim.x, heads_all = a.kv.n_head * a.splits;
+    const int start = (int64_t)uniform(head_turns) * heads_all > groups ? 1 : 0;
+    const int before = turns_before + start * items_before, mine = turns_mine + start * items_mine;
+    head_turns = uniform(head_turns + start * head_items);
+    const int64_t total = (int64_t)head_turns * heads_all;
     // stretches of equal length; the workgroups of an XCD take neighbouring ones
-    const int groups = gridDim.x;
     const int64_t stretch = std::max<int64_t>(1, (total + groups - 1) / groups);
     const int active = (int)((total + stretch - 1) / stretch), per_xcd = (active + 7) / 8;
     const int me = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
@@ -674,27 +677,25 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
                 const int s = u / a.row_tiles;
                 bool bad;
                 const Sequence q = sequence(a, s, bad);
-                const int n = item_turns(a, item_of(a, s, q, u - s * a.row_tiles));
-                if (off < b + n) {
-                    lds.found[0] = s;
-                    lds.found[1] = u - s * a.row_tiles;
-                    lds.found[2] = b;
-                    lds.found[3] = n;
+                const int n = item_turns(item_of(a, s, q, u - s * a.row_tiles));
+                if (n > 0 && off < b + n + start) {
+                    const int found[7] = {s, u - s * a.row_tiles, b, n, q.start, q.count, q.len};
+#pragma unroll
+                    for (int i = 0; i < 7; ++i) lds.found[i] = found[i];
                     break;
                 }
-                b += n;
+                b += n > 0 ? n + start : 0;
             }
         }
         __syncthreads();
-        const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), first = uniform(lds.found[2]), turns = uniform(lds.found[3]) - a.start;
-        bool bad;
-        const Sequence q = sequence(a, seq, bad);
+        const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), first = uniform(lds.found[2]), turns = uniform(lds.found[3]);
+        const Sequence q = {uniform(lds.found[4]), uniform(lds.found[5]), uniform(lds.found[6])};
         const Item it = item_of(a, seq, q, row_tile);
         const int kv_head = hv / a.splits, go = hv - kv_head * a.splits;
         const int head0 = kv_head * a.group + go * a.split, heads = min(a.split, a.group - go * a.split);
         // the stretch's turns of the item: none where it ends within the item's start
-        const int skip = off - first, take = (int)std::min<int64_t>(turns + a.start - skip, end - at);
-        const int turn0 = max(0, skip - a.start), turn1 = skip + take - a.start;
+        const int skip = off - first, take = (int)std::min<int64_t>(turns + start - skip, end - at);
+        const int turn0 = max(0, skip - start), turn1 = skip + take - start;
         if (turn1 <= 0) break;
         const int tile0 = it.hi < 0 ? 0 : it.see / kTile, tile1 = tile0 + min(turn1 * kWaves, item_tiles(it));
 
@@ -751,7 +752,7 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
             }
         }
         if (ends && !starts) {
-            join_from = (int)((at - skip + a.start) / stretch);
+            join_from = (int)((at - skip + start) / stretch);
             join_seq = seq, join_tile = row_tile, join_head = hv;
         }
         at += take;
@@ -766,47 +767,64 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
     }
 }
 
+// Items that were cut: the sums of stretches first .. last.  A workgroup takes 16 queries and a share of the dimensions; its waves take
+// the parts in turn, four at a time (their loads go out together: a part comes from another XCD's memory), and meet once.
+constexpr int kJoinWaves = 8;
 constexpr int join_share(int tiles) { return tiles % 4 ? tiles / 2 : tiles / 4; }   // of the dimensions, in 16s
 
-// Items that were cut: the sums of stretches first .. last, added by four waves in turn.  A workgroup takes 16 queries and a share of
-// the dimensions.
 template <int D, int NQ>
-__global__ __launch_bounds__(kThreads) void attention_join_kernel(const AttentionArgs a) {
-    constexpr int T = D / 16, kShare = join_share(T), kShares = T / kShare;
+__global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const AttentionArgs a) {
+    constexpr int T = D / 16, kShare = join_share(T), kShares = T / kShare, kBatch = 4;
     static_assert(T % kShare == 0, "whole shares");
-    __shared__ __align__(16) f32x4 sums[kWaves][kShare][64];
-    __shared__ float weights[kWaves][64];
+    __shared__ __align__(16) f32x4 sums[kJoinWaves][kShare][64];
+    __shared__ float tops[kJoinWaves][16], weights[kJoinWaves][16];
     const int32_t *j = a.joins + 8 * (int64_t)blockIdx.x;
     const int first = j[0], last = j[1];
     if (first < 0) return;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15;
     const int g = blockIdx.y / kShares, x0 = (blockIdx.y % kShares) * kShare;
-    const float *const cut = a.parts + ((int64_t)first * 2 + 1) * part_floats(D, NQ);   // (the first part is a stretch's second)
-    const int64_t size = 2 * part_floats(D, NQ);
-    const float *const rest = cut - part_floats(D, NQ);
+    const int64_t size = part_floats(D, NQ);
     const int parts = last - first + 1;
+    const auto part = [&](int w) { return a.parts + ((int64_t)(first + w) * 2 + (w ? 0 : 1)) * size; };   // (the first is a stretch's second)
     constexpr int kM = 16 * NQ * D, kL = kM + 16 * NQ;
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int w = lane >> 4; w < parts; w += 4) top = fmaxf(top, (w ? rest + w * size : cut)[kM + g * 16 + col]);
-    const float m = max_xor(top);
     f32x4 o[kShare];
 #pragma unroll
     for (int t = 0; t < kShare; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-#pragma unroll 4
-    for (int w = wave; w < parts; w += kWaves) {
-        const float *p = w ? rest + w * size : cut;
-        const float mw = p[kM + g * 16 + col], f = mw == m ? 1.f : __builtin_amdgcn_exp2f(mw - m);
-        l += p[kL + g * 16 + col] * f;
+    float m = -INFINITY, l = 0.f;
+    for (int w0 = wave; w0 < parts; w0 += kBatch * kJoinWaves) {
+        float mw[kBatch], lw[kBatch];
+        f32x4 v[kBatch][kShare];
 #pragma unroll
-        for (int t = 0; t < kShare; ++t) {
-            const f32x4 v = reinterpret_cast<const f32x4 *>(p)[((x0 + t) * NQ + g) * 64 + lane];
+        for (int k = 0; k < kBatch; ++k) {       // (behind the last part the first of the batch again, with no weight)
+            const int w = w0 + k * kJoinWaves;
+            const float *p = part(w < parts ? w : w0);
+            mw[k] = p[kM + g * 16 + col];
+            lw[k] = p[kL + g * 16 + col];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[t][r] += v[r] * f;
+            for (int t = 0; t < kShare; ++t) v[k][t] = reinterpret_cast<const f32x4 *>(p)[((x0 + t) * NQ + g) * 64 + lane];
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) top = fmaxf(top, mw[k]);
+        const float back = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= back;
+#pragma unroll
+        for (int t = 0; t < kShare; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][r] *= back;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            if (w0 + k * kJoinWaves >= parts) break;
+            const float f = mw[k] == m ? 1.f : __builtin_amdgcn_exp2f(mw[k] - m);
+            l += lw[k] * f;
+#pragma unroll
+            for (int t = 0; t < kShare; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[t][r] += v[k][t][r] * f;
         }
     }
-    weights[wave][lane] = l;
+    if (lane < 16) tops[wave][lane] = m, weights[wave][lane] = l;
 #pragma unroll
     for (int t = 0; t < kShare; ++t) sums[wave][t][lane] = o[t];
     __syncthreads();
@@ -817,14 +835,19 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(const Attentio
     const int kv_head = j[4] / a.splits, go = j[4] - kv_head * a.splits;
     float *y = out_row<D, NQ>(a, it, kv_head * a.group + go * a.split, min(a.split, a.group - go * a.split), g, lane, live);
     if (!live) return;
-    const float sum = (weights[0][lane] + weights[1][lane]) + (weights[2][lane] + weights[3][lane]);
-    const float f = sum != 0.f ? 1.f / sum : 0.f;
-    for (int t = wave; t < kShare; t += kWaves) {
-        f32x4 v;
+    const int used = min(kJoinWaves, parts);
+    m = -INFINITY, l = 0.f;
+    for (int w = 0; w < used; ++w) m = fmaxf(m, tops[w][col]);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < used; ++w) {
+        const float f = tops[w][col] == m ? 1.f : __builtin_amdgcn_exp2f(tops[w][col] - m);
+        const f32x4 x = sums[w][wave][lane];
+        l += weights[w][col] * f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = ((sums[0][t][lane][r] + sums[1][t][lane][r]) + (sums[2][t][lane][r] + sums[3][t][lane][r])) * f;
-        *reinterpret_cast<f32x4 *>(y + 16 * (x0 + t)) = v;
+        for (int r = 0; r < 4; ++r) v[r] += x[r] * f;
     }
+    const float unit = l != 0.f ? 1.f / l : 0.f;
+    *reinterpret_cast<f32x4 *>(y + 16 * (x0 + wave)) = f32x4{v[0] * unit, v[1] * unit, v[2] * unit, v[3] * unit};
 }
 
 template <int D, int NQ>
@@ -832,14 +855,14 @@ hipError_t launch(const AttentionArgs &a, int groups, hipStream_t s) {
     hipLaunchKernelGGL((attention_kernel<D, NQ>), dim3(groups), dim3(kThreads), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || groups == 1) return e;
-    hipLaunchKernelGGL((attention_join_kernel<D, NQ>), dim3(groups, D / 16 / join_share(D / 16) * NQ), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((attention_join_kernel<D, NQ>), dim3(groups, D / 16 / join_share(D / 16) * NQ), dim3(64 * kJoinWaves), 0, s, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 size_t attention_scratch_bytes(int cus) {
-    return (size_t)cus * 3 * ((size_t)2 * part_floats(256, 2) * 4 + 32);   // (more than any instance takes)
+    return (size_t)cus * 2 * ((size_t)2 * part_floats(256, 2) * 4 + 32);   // (more than any instance takes)
 }
 
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
@@ -867,7 +890,6 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     a.tokens = rows / a.split;
     a.row_tiles = (int32_t)((j.max_q + a.tokens - 1) / a.tokens);
     const int groups_most = waves_per_simd(a.kv.dim, cols) * j.cus;
-    a.start = 2 * (int64_t)a.row_tiles * a.n_seq * a.kv.n_head * a.splits > groups_most ? 2 : 0;
     // no more workgroups than there can be turns
     const int64_t most = ((j.pages_stride << j.kv->page_shift) + kTile - 1) / kTile + 1;
     const double turns = (double)most * a.n_seq * a.row_tiles * j.kv->n_head * a.splits / kWaves + (double)a.n_seq * a.row_tiles * j.kv->n_head * a.splits;
