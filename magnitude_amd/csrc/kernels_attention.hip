@@ -371,8 +371,10 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         q_unit[g] = shared.q_unit[g][lane];
     }
 
-    uint32_t mask0 = 0x000f000fu, mask1 = 0x00f000f0u, magic = 0x64006400u;   // (in registers: and-or in one instruction)
-    asm volatile("" : "+v"(mask0), "+v"(mask1), "+s"(magic));
+    // (in registers, and unknown to the compiler: and-or in one instruction, half times -1 plus float in one)
+    uint32_t mask0 = 0x000f000fu, mask1 = 0x00f000f0u, magic = 0x64006400u;
+    float minus = -1.f;
+    asm volatile("" : "+v"(mask0), "+v"(mask1), "+s"(magic), "+s"(minus));
 
     int unit = 0;               // results are in units of 2^unit
     float base[NQ];             // what is taken off a score
@@ -462,28 +464,60 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                 }
             }
         }
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
+        // A step is a block of kStep groups of tokens.  Behind each of its products goes a piece of the next step's codes or of the
+        // previous step's sums, so that the matrix cores and the vector unit work at once; the barriers keep that order.
+        constexpr int kStep = NQ == 1 ? 4 : 2, kSteps = B * 4 / kStep;
+        {
+            half8 codes[2][kStep];
+            f32x4 acc[2][kStep][NQ];
+            u32x2 d[2][kStep];
             half8 qh[NQ], ql[NQ];
+            const auto code = [&](int step, int g) {
+                const uint32_t w = k_raw[step % (4 / kStep) * kStep + g][step / (4 / kStep)], w8 = w >> 8;
+                codes[step & 1][g] = __builtin_bit_cast(half8, u32x4{w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u});
+            };
+            const auto add = [&](int step, int g, int c) {
+                f32x4 &to = s[step % (4 / kStep) * kStep + g][c];
+                const u32x2 dk = d[step & 1][g];
 #pragma unroll
-            for (int c = 0; c < NQ; ++c) {
-                qh[c] = __builtin_bit_cast(half8, shared.q[b][c][0][lane]);
-                ql[c] = __builtin_bit_cast(half8, shared.q[b][c][1][lane]);
-            }
+                for (int r = 0; r < 4; ++r) to[r] = fmaf(r & 1 ? high_half(dk[r / 2]) : low_half(dk[r / 2]), acc[step & 1][g][c][r], to[r]);
+            };
+            const auto fetch = [&](int step) {
+                const int b = step / (4 / kStep), g0 = step % (4 / kStep) * kStep;
+                if (g0 == 0) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const u32x2 d = *reinterpret_cast<const u32x2 *>(&lds.k_scale[b][16 * g + 4 * part]);
-                const uint32_t w = k_raw[g][b], w8 = w >> 8;
-                const u32x4 n = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
-                const half8 codes = __builtin_bit_cast(half8, n);
+                    for (int c = 0; c < NQ; ++c) {
+                        qh[c] = __builtin_bit_cast(half8, shared.q[b][c][0][lane]);
+                        ql[c] = __builtin_bit_cast(half8, shared.q[b][c][1][lane]);
+                    }
+                }
 #pragma unroll
-                for (int c = 0; c < NQ; ++c) {
-                    f32x4 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, ql[c], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, qh[c], acc, 0, 0, 0);
+                for (int g = 0; g < kStep; ++g) d[step & 1][g] = *reinterpret_cast<const u32x2 *>(&lds.k_scale[b][16 * (g0 + g) + 4 * part]);
+            };
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[g][c][r] = fmaf(r & 1 ? high_half(d[r / 2]) : low_half(d[r / 2]), acc[r], s[g][c][r]);
+            for (int g = 0; g < kStep; ++g) code(0, g);
+#pragma unroll
+            for (int step = 0; step < kSteps; ++step) {
+                fetch(step);
+                constexpr int kProducts = 2 * kStep * NQ, kPieces = kStep + kStep * NQ;
+#pragma unroll
+                for (int i = 0; i < kProducts; ++i) {
+                    const int half = i / (kStep * NQ), g = i % (kStep * NQ) / NQ, c = i % NQ;
+                    f32x4 &to = acc[step & 1][g][c];
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes[step & 1][g], half ? qh[c] : ql[c], half ? to : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                    for (int x = i * kPieces / kProducts; x < (i + 1) * kPieces / kProducts; ++x) {
+                        if (x < kStep) {
+                            if (step + 1 < kSteps) code(step + 1, x);
+                        } else if (step > 0) {
+                            add(step - 1, (x - kStep) / NQ, (x - kStep) % NQ);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
+#pragma unroll
+            for (int x = 0; x < kStep * NQ; ++x) add(kSteps - 1, x / NQ, x % NQ);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g)
@@ -546,7 +580,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                 for (int r = 0; r < 4; r += 2) {
                     const uint32_t hi = half_pair(s[g][c][r], s[g][c][r + 1]);
                     p_hi[g / 2][c][(g & 1) * 2 + r / 2] = hi;
-                    p_lo[g / 2][c][(g & 1) * 2 + r / 2] = half_pair(fmaf(low_half(hi), -1.f, s[g][c][r]), fmaf(high_half(hi), -1.f, s[g][c][r + 1]));
+                    p_lo[g / 2][c][(g & 1) * 2 + r / 2] = half_pair(fmaf(low_half(hi), minus, s[g][c][r]), fmaf(high_half(hi), minus, s[g][c][r + 1]));
                 }
             }
         }
@@ -555,41 +589,75 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         // row that nibble lane % 16 of the result comes from: nibbles i and i + 4 of a word, which one and takes together, are neighbours.
         const int jj = col & 7, k = (jj & 3) * 2 + (jj >> 2);
         const int from_token = 32 * (col >> 3) + 16 * (k >> 2) + 4 * part + (k & 3);
+        // A step is kWide times 16 dimensions; behind each of its products goes a piece of the next step's values, made of codes and
+        // scales that were asked of LDS a step earlier.  A piece is one register of both halves in four instructions, and overlaps
+        // with its neighbours: none waits for the one before it.
+        constexpr int kWide = NQ == 1 ? 2 : 1, kRounds = T / kWide, kUnits = 8 * kWide;
+        {
+            u32x4 v_hi[2][kWide][2], v_lo[2][kWide][2];
+            i32x2 raw[2][kWide];
+            u32x2 d[2][4];       // scales of the lane's tokens of a group of 16
+            uint32_t big[kUnits];
+            half2v code[kUnits];
+            const auto fetch = [&](int step) {
+                const int b = step * kWide / 2;
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-            u32x2 d[4];          // scales of the lane's tokens of a group of 16
+                for (int k = 0; k < kWide; ++k)
+                    raw[step & 1][k] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+                        (__attribute__((address_space(3))) i32x2 *)(lds.v + value_at<D>(from_token, b) + 8 * ((step * kWide + k) & 1)));
 #pragma unroll
-            for (int g = 0; g < 4; ++g) d[g] = *reinterpret_cast<const u32x2 *>(&lds.v_scale[b][16 * g + 4 * part]);
+                for (int g = 0; g < 4; ++g) d[step & 1][g] = *reinterpret_cast<const u32x2 *>(&lds.v_scale[b][16 * g + 4 * part]);
+            };
+            // unit u: register u % 4 of half u / 4 % 2 of 16 dimensions u / 8
+            const auto lift = [&](int step, int u) {
+                const uint32_t w = (uint32_t)raw[step & 1][u / 8][u / 4 % 2];
+                big[u] = ((u & 2) ? w >> 8 : w) & ((u & 1) ? mask1 : mask0) | magic;         // 1024 + n, or 1024 + 16 n
+            };
+            const auto center = [&](int u) {
+                const half2v b = __builtin_bit_cast(half2v, big[u]);
+                code[u] = u & 1 ? __builtin_elementwise_fma(b, half2v{(_Float16)0.0625f, (_Float16)0.0625f}, half2v{(_Float16)-72.f, (_Float16)-72.f})
+                                : b - half2v{(_Float16)1032.f, (_Float16)1032.f};
+            };
+            const auto scale = [&](int step, int u) { return __builtin_bit_cast(half2v, (uint32_t)d[step & 1][2 * (u / 4 % 2) + (u % 4 >> 1)][u & 1]); };
+            const auto high = [&](int step, int u) { v_hi[step & 1][u / 8][u / 4 % 2][u % 4] = __builtin_bit_cast(uint32_t, code[u] * scale(step, u)); };
+            const auto low = [&](int step, int u) {
+                v_lo[step & 1][u / 8][u / 4 % 2][u % 4] =
+                    __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code[u], scale(step, u), -__builtin_bit_cast(half2v, (uint32_t)v_hi[step & 1][u / 8][u / 4 % 2][u % 4])));
+            };
+            const auto piece = [&](int step, int u) {
+                if (u == 0) {
+                    lift(step, 0);
+                    lift(step, 1);
+                    center(0);
+                }
+                if (u + 2 < kUnits) lift(step, u + 2);
+                high(step, u);
+                if (u + 1 < kUnits) center(u + 1);
+                low(step, u);
+            };
+            fetch(0);
+            fetch(1);
 #pragma unroll
-            for (int x = 2 * b; x < 2 * b + 2; ++x) {
-                const i32x2 raw = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                    (__attribute__((address_space(3))) i32x2 *)(lds.v + value_at<D>(from_token, b) + 8 * (x & 1)));
+            for (int u = 0; u < kUnits; ++u) piece(0, u);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t w = (uint32_t)raw[h], w8 = w >> 8;
-                    const uint32_t n[4] = {w & mask0 | magic, w & mask1 | magic, w8 & mask0 | magic, w8 & mask1 | magic};
-                    u32x4 a_hi, a_lo;
+            for (int step = 0; step < kRounds; ++step) {
+                if (step + 2 < kRounds) fetch(step + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                constexpr int kProducts = 6 * kWide * NQ;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const half2v big = __builtin_bit_cast(half2v, n[i]);   // 1024 + n, or 1024 + 16 n
-                        const half2v code = i & 1 ? __builtin_elementwise_fma(big, half2v{(_Float16)0.0625f, (_Float16)0.0625f}, half2v{(_Float16)-72.f, (_Float16)-72.f})
-                                                  : big - half2v{(_Float16)1032.f, (_Float16)1032.f};
-                        const half2v e = __builtin_bit_cast(half2v, (uint32_t)d[2 * h + (i >> 1)][i & 1]);
-                        const half2v hi = code * e;
-                        a_hi[i] = __builtin_bit_cast(uint32_t, hi);
-                        a_lo[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, e, -hi));
+                for (int x = 0; x < kProducts; ++x) {
+                    const int c = x % NQ, k = x / NQ % kWide, i = x / (NQ * kWide) % 3, h = x / (NQ * kWide * 3);
+                    const half8 v = __builtin_bit_cast(half8, i == 0 ? v_lo[step & 1][k][h] : v_hi[step & 1][k][h]);
+                    const half8 p = __builtin_bit_cast(half8, i == 1 ? p_lo[h][c] : p_hi[h][c]);
+                    f32x4 &o = st.o[step * kWide + k][c];
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, o, 0, 0, 0);
+                    if (step + 1 < kRounds) {
+#pragma unroll
+                        for (int u = x * kUnits / kProducts; u < (x + 1) * kUnits / kProducts; ++u) piece(step + 1, u);
                     }
-#pragma unroll
-                    for (int c = 0; c < NQ; ++c) {
-                        const half8 vh = __builtin_bit_cast(half8, a_hi), vl = __builtin_bit_cast(half8, a_lo);
-                        const half8 ph = __builtin_bit_cast(half8, p_hi[h][c]), pl = __builtin_bit_cast(half8, p_lo[h][c]);
-                        st.o[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph, st.o[x][c], 0, 0, 0);
-                        st.o[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl, st.o[x][c], 0, 0, 0);
-                        st.o[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph, st.o[x][c], 0, 0, 0);
-                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
         wave_sync();
     }
