@@ -198,21 +198,34 @@ struct Running {
 };
 
 // 16 queries of an item for the matrix cores: 22 bits of q * scale * log2(e), the row scaled by a power of two
+template <int D>
+struct Queries {
+    f32x4 x[D / 32][2];
+    bool live;
+};
+
+template <int D>
+__device__ __forceinline__ void load_queries(const AttentionArgs &a, const Item &it, int head0, int heads, int g, Queries<D> &q, int lane) {
+    const int slot = g * 16 + (lane & 15), token = slot / a.split, head = slot - token * a.split;
+    q.live = token < it.count && head < heads;
+    const float *row = a.q + (int64_t)(it.first + (q.live ? token : 0)) * a.q_stride + (int64_t)(head0 + (q.live ? head : 0)) * D + 8 * (lane >> 4);
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) q.x[b][k] = *reinterpret_cast<const f32x4 *>(row + 32 * b + 4 * k);
+}
+
 template <int D, int NQ>
-__device__ __forceinline__ void stage_queries(const AttentionArgs &a, const Item &it, int head0, int heads, int g, SharedLds<D, NQ> &lds, int lane) {
+__device__ __forceinline__ void stage_queries(const AttentionArgs &a, Queries<D> &q, int g, SharedLds<D, NQ> &lds, int lane) {
     constexpr int B = D / 32;
-    const int col = lane & 15, part = lane >> 4;
-    const int slot = g * 16 + col, token = slot / a.split, head = slot - token * a.split;
-    const bool live = token < it.count && head < heads;
-    const float *row = a.q + (int64_t)(it.first + (live ? token : 0)) * a.q_stride + (int64_t)(head0 + (live ? head : 0)) * D + 8 * part;
-    f32x4 x[B][2];
+    auto &x = q.x;
+    const bool live = q.live;
     float most = 0.f;
     bool whole = true;
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            x[b][k] = *reinterpret_cast<const f32x4 *>(row + 32 * b + 4 * k);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 x[b][k][j] = live ? x[b][k][j] * a.scale : 0.f;
@@ -291,18 +304,19 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     uint32_t k_raw[4][B];
     uint32_t ks_raw[(B + 1) / 2], vs_raw[(B + 1) / 2];
     int bad_groups;      // of the tile whose loads are in flight
-    int64_t rows[4];     // first row of its groups of 16 tokens
+    uint32_t rows[4];    // first row of its groups of 16 tokens
 
     const auto place = [&](int tile) {   // rows of the tile whose pages have come
-        const int t = min(max(tile * kTile + lane, it.see), it.hi);
-        const bool bad = page < 0 || page >= kv.n_pages;
-        bad_page = bad_page || (bad && t == tile * kTile + lane);
+        const int own = tile * kTile + lane, t = min(max(own, it.see), it.hi);
+        const bool bad = (uint32_t)page >= (uint32_t)kv.n_pages;
+        bad_page = bad_page || (bad && t == own);
         bad_groups = 0;
+        const uint32_t row = (((bad ? 0u : (uint32_t)page) * kv.n_head + kv_head) << shift) + (own & mask);
+        const uint64_t bad_lanes = __ballot(bad);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int p = __builtin_amdgcn_readlane(bad ? -1 : page, 16 * g);
-            if (p < 0) bad_groups |= 1 << g;
-            rows[g] = (((int64_t)max(p, 0) * kv.n_head + kv_head) << shift) + ((tile * kTile + 16 * g) & mask);
+            rows[g] = __builtin_amdgcn_readlane(row, 16 * g);
+            bad_groups |= (int)(bad_lanes >> (16 * g) & 1) << g;
         }
     };
     uint32_t v_off[kLoads], k_off = (uint32_t)(col * RB + part * B * 4), s_off = (uint32_t)(col * B * 2);
@@ -311,11 +325,11 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     const auto load_v = [&]() {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const auto base = scalar_global(kv.v_codes + rows[g] * RB);
+            const auto base = scalar_global(kv.v_codes + (uint64_t)rows[g] * RB);
 #pragma unroll
             for (int c = 0; c < kLoads; ++c) v_raw[g][c] = load_global<u32x4>(base, local(v_off[c]));
         }
-        const int64_t row = part == 0 ? rows[0] : part == 1 ? rows[1] : part == 2 ? rows[2] : rows[3];
+        const uint64_t row = part == 0 ? rows[0] : part == 1 ? rows[1] : part == 2 ? rows[2] : rows[3];
         const uint8_t *ks = reinterpret_cast<const uint8_t *>(kv.k_scales) + row * (B * 2) + s_off;
         const uint8_t *vs = reinterpret_cast<const uint8_t *>(kv.v_scales) + row * (B * 2) + s_off;
         if (B == 3) {
@@ -333,7 +347,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     const auto load_k = [&]() {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const auto base = scalar_global(kv.k_codes + rows[g] * RB);
+            const auto base = scalar_global(kv.k_codes + (uint64_t)rows[g] * RB);
             if constexpr (B == 2) {
                 const u32x2 w = load_global<u32x2>(base, local(k_off));
                 k_raw[g][0] = w[0], k_raw[g][1] = w[1];
@@ -350,12 +364,16 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
             }
         }
     };
+    // (loads come back in order: pages, then queries, then keys and values)
+    static_assert(NQ <= kWaves, "a wave stages 16 queries");
+    Queries<D> queries;
+    if (wave < NQ) load_queries<D>(a, it, head0, heads, wave, queries, lane);
     if (work) {
         place(from);
         load_v();
         load_k();
     }
-    for (int g = wave; g < NQ; g += kWaves) stage_queries<D, NQ>(a, it, head0, heads, g, shared, lane);
+    if (wave < NQ) stage_queries<D, NQ>(a, queries, wave, shared, lane);
     __syncthreads();
     if (!work) return;
 
@@ -718,27 +736,27 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         head_turns += lds.wave_turns[w];
         head_items += lds.wave_items[w];
     }
-    // Where there are more turns than workgroups, beginning an item (staging its queries, adding its sums) counts as a turn.
-    const int groups = gridDim.x, heads_all = a.kv.n_head * a.splits;
-    const int start = (int64_t)uniform(head_turns) * heads_all > groups ? 1 : 0;
+    // Where there are more turns than workgroups, beginning an item (staging its queries, adding its sums) counts as two turns.
+    const uint32_t groups = gridDim.x, heads_all = a.kv.n_head * a.splits;
+    const int start = (uint32_t)uniform(head_turns) * heads_all > groups ? 2 : 0;
     const int before = turns_before + start * items_before, mine = turns_mine + start * items_mine;
     head_turns = uniform(head_turns + start * head_items);
-    const int64_t total = (int64_t)head_turns * heads_all;
-    // stretches of equal length; the workgroups of an XCD take neighbouring ones
-    const int64_t stretch = std::max<int64_t>(1, (total + groups - 1) / groups);
-    const int active = (int)((total + stretch - 1) / stretch), per_xcd = (active + 7) / 8;
-    const int me = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+    const uint32_t total = (uint32_t)head_turns * heads_all;
+    // Stretches of one length or one more, as many as there are workgroups; those of an XCD are neighbours.
+    const uint32_t active = std::min(total, groups), per_xcd = (active + 7) / 8;
+    const uint32_t me = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
     int32_t *const join = a.joins + 8 * (int64_t)blockIdx.x;
-    if ((int)blockIdx.x / 8 >= per_xcd || me >= active) {
+    if (blockIdx.x / 8 >= per_xcd || me >= active) {
         if (id == 0) join[0] = -1;
         return;
     }
-    int64_t at = me * stretch;
-    const int64_t end = std::min<int64_t>(total, at + stretch);
+    const uint32_t length = total / active, longer = total - length * active;     // the first `longer` ones have one more
+    uint32_t at = me * length + std::min(me, longer);
+    const uint32_t end = at + length + (me < longer ? 1 : 0);
     int join_from = -1, join_seq = 0, join_tile = 0, join_head = 0;
 
     while (at < end) {
-        const int hv = (int)(at / head_turns), off = (int)(at - (int64_t)hv * head_turns);
+        const int hv = (int)(at / (uint32_t)head_turns), off = (int)(at - (uint32_t)hv * head_turns);
         if (off >= before && off < before + mine) {     // one thread
             int b = before;
             for (int u = id * per; u < min(units, (id + 1) * per); ++u) {
@@ -762,7 +780,7 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         const int kv_head = hv / a.splits, go = hv - kv_head * a.splits;
         const int head0 = kv_head * a.group + go * a.split, heads = min(a.split, a.group - go * a.split);
         // the stretch's turns of the item: none where it ends within the item's start
-        const int skip = off - first, take = (int)std::min<int64_t>(turns + start - skip, end - at);
+        const int skip = off - first, take = (int)std::min<uint32_t>(turns + start - skip, end - at);
         const int turn0 = max(0, skip - start), turn1 = skip + take - start;
         if (turn1 <= 0) break;
         const int tile0 = it.hi < 0 ? 0 : it.see / kTile, tile1 = tile0 + min(turn1 * kWaves, item_tiles(it));
@@ -820,7 +838,8 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
             }
         }
         if (ends && !starts) {
-            join_from = (int)((at - skip + start) / stretch);
+            const uint32_t from = at - skip + start, edge = longer * (length + 1);
+            join_from = (int)(from < edge ? from / (length + 1) : longer + (from - edge) / length);
             join_seq = seq, join_tile = row_tile, join_head = hv;
         }
         at += take;

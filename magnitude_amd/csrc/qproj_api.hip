@@ -1662,6 +1662,7 @@ static const char *bad_cache(const qproj_kv_cache *kv, KvView *view) {
     while (shift < 8 && (int64_t)1 << shift != kv->page_tokens) ++shift;
     if ((int64_t)1 << shift != kv->page_tokens) return "page_tokens must be 16, 32, 64, 128 or 256";
     if (kv->n_pages <= 0 || kv->n_pages > 0x7fffffff || kv->n_head_kv <= 0 || kv->n_head_kv > 1024) return "n_pages or n_head_kv out of range";
+    if (kv->n_pages > 0xffffffffll / (kv->page_tokens * kv->n_head_kv)) return "a cache must stay under 2^32 rows (n_pages * n_head_kv * page_tokens)";
     *view = KvView{static_cast<uint8_t *>(kv->k_codes), static_cast<uint16_t *>(kv->k_scales), static_cast<uint8_t *>(kv->v_codes),
                    static_cast<uint16_t *>(kv->v_scales), kv->n_pages, shift, (int32_t)kv->n_head_kv, (int32_t)kv->head_dim};
     return nullptr;
@@ -1798,8 +1799,8 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
     if (pages_stride * kv->page_tokens > 0x7fffffff) return refuse(ctx, call, "a sequence must stay under 2^31 tokens");
     if (n_head <= 0 || n_head > kMostHeads || n_head % kv->n_head_kv != 0) return refuse(ctx, call, "n_head must be a multiple of n_head_kv");
     if (window < 0) return refuse(ctx, call, "negative window");
-    // (the device counts tiles of 64 tokens in 32 bits)
-    const double rows = (double)n_seq * ((double)std::min(max_q, n_tokens) * (double)(n_head / kv->n_head_kv) / 16 + 1);
+    // (the device counts tiles of 64 tokens, of all heads, in 32 bits)
+    const double rows = (double)n_seq * ((double)std::min(max_q, n_tokens) * n_head / 16 + n_head);
     if (rows * ((double)pages_stride * kv->page_tokens / 64 + 1) > 2e9) return refuse(ctx, call, "n_seq * max_q * pages_stride too large: give max_q, or make several calls");
     if (const char *why = bad_rows(q_dev, q_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
     if (const char *why = bad_rows(y_dev, y_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
