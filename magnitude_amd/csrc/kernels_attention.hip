@@ -66,6 +66,20 @@ struct AttentionArgs {
     int32_t row_tiles;       // items of a sequence, at most
 };
 
+// The kernel's arguments, loaded where they are used from here on.  Kept in registers from the start they are more scalars than there are, and
+// the kernel's phases use different ones.
+__device__ __forceinline__ const AttentionArgs &fresh_arguments() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef const AttentionArgs __attribute__((address_space(4))) *arguments;
+    arguments p = (arguments)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const AttentionArgs *)p;
+#else
+    static AttentionArgs none;   // device-only; the host pass just has to parse it
+    return none;
+#endif
+}
+
 constexpr int part_floats(int dim, int cols) { return 16 * cols * (dim + 2); }
 
 constexpr int waves_per_simd(int dim, int cols) { return dim * cols <= 256 ? 2 : 1; }
@@ -129,6 +143,13 @@ __device__ __forceinline__ float max_xor(float v) {   // over the lanes of a col
     return fmaxf(__uint_as_float(x), __uint_as_float(y));
 }
 
+// 16 bytes a lane from `g` to l + 16 * lane, as global_to_lds16, but unseen by the compiler, which would wait for all loads in flight before
+// any read of that memory.  Loads come back in order: what follows a wait for a later load of the same wave finds the bytes there.
+__device__ __forceinline__ void global_to_lds16_unseen(const void *g, const void *l) {
+    const uint32_t to = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)l;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(g) : "memory");   // (m0: nothing else here reads it)
+}
+
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true));
@@ -151,23 +172,31 @@ __device__ __forceinline__ uint32_t local(uint32_t v) {
     return v;
 }
 
-// where the transposing read finds 16-byte chunk `chunk` of a token's value codes: rows of 16 tokens that one read takes
-// together are 16 tokens apart, chunks are turned so that they fall into different banks
+// Where the transposing read finds 16-byte chunk `chunk` of a token's value codes: the rows that one read takes together are 16 tokens
+// apart, their chunks are turned so that they fall into different banks.  chunk_at is the chunk that lies at a place.
+template <int D>
+__device__ __forceinline__ int chunk_turn(int token) {
+    const int turn = (token >> 4) & 3;
+    return D == 128 ? turn : D == 256 ? turn | ((token >> 1) & 1) << 2 : D == 64 ? turn & 1 : turn % 3;
+}
 template <int D>
 __device__ __forceinline__ int value_at(int token, int chunk) {
-    constexpr int kChunks = D / 32;
-    const int turn = (token >> 4) & 3;
-    int c = chunk;
-    if (D == 128) c = chunk ^ turn;
-    else if (D == 256) c = chunk ^ (turn | ((token >> 1) & 1) << 2);
-    else if (D == 64) c = chunk ^ (turn & 1);
-    else c = (chunk + turn) % kChunks;
-    return token * (D / 2) + c * 16;
+    const int turn = chunk_turn<D>(token);
+    return token * (D / 2) + (D == 96 ? (chunk + turn) % 3 : chunk ^ turn) * 16;
 }
+template <int D>
+__device__ __forceinline__ int chunk_at(int token, int place) {
+    const int turn = chunk_turn<D>(token);
+    return D == 96 ? (place + 3 - turn) % 3 : place ^ turn;
+}
+
+// Value codes go from memory to LDS directly.  Two tiles' worth of room where the rest leaves it: the next tile's codes are then asked for
+// while this tile's are still read, otherwise behind the scores.
+constexpr bool values_ahead(int dim) { return dim <= 128; }
 
 template <int D, int NQ>
 struct WaveLds {
-    uint8_t v[kTile * D / 2];
+    uint8_t v[values_ahead(D) ? 2 : 1][kTile * D / 2];
     uint16_t k_scale[D / 32][kTile];
     uint16_t v_scale[D / 32][kTile];
 };
@@ -186,6 +215,7 @@ struct SharedLds {
     u32x4 q[D / 32][NQ][2][64];   // the item's queries as the matrix cores take them: high halves, low halves
     u32x4 q_sum[NQ][D / 32 <= 4 ? 1 : 2][64];   // -8 * sum(q) of every block, two halves each
     float q_unit[NQ][64];         // scores are sums times this
+    int32_t line[kThreads][2];    // a thread's items on a head's line: turns before them, theirs
     int32_t wave_turns[kWaves], wave_items[kWaves];
     int32_t found[8];             // sequence, row tile, turns before the item, its turns, and the sequence's first row, rows, tokens
 };
@@ -276,7 +306,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                                      int wave, Running<D, NQ> &st, int lane) {
     WaveLds<D, NQ> &lds = shared.wave[wave];
     constexpr int B = D / 32, RB = D / 2, T = D / 16;
-    constexpr int kLoads = (RB + 63) / 64;       // of 16 bytes a lane for 16 tokens' value codes
+    constexpr bool kAhead = values_ahead(D);
     const int col = lane & 15, part = lane >> 4;
     const KvView &kv = a.kv;
     const int shift = kv.page_shift, mask = (1 << shift) - 1;
@@ -300,7 +330,6 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     int page = work ? page_of(from) : 0, page_next = work ? page_of(min(from + kWaves, last_tile)) : 0;
     bool bad_page = false;
 
-    u32x4 v_raw[4][kLoads];
     uint32_t k_raw[4][B];
     uint32_t ks_raw[(B + 1) / 2], vs_raw[(B + 1) / 2];
     int bad_groups;      // of the tile whose loads are in flight
@@ -319,16 +348,30 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
             bad_groups |= (int)(bad_lanes >> (16 * g) & 1) << g;
         }
     };
-    uint32_t v_off[kLoads], k_off = (uint32_t)(col * RB + part * B * 4), s_off = (uint32_t)(col * B * 2);
+    // chunk i * 64 + lane of the tile's value codes, in the order in which they lie in LDS
+    const uint32_t k_off = (uint32_t)(col * RB + part * B * 4), s_off = (uint32_t)(col * B * 2);
+    const auto chunk_offset = [&](int i) {
+        const int chunk = i * 64 + lane, token = chunk / B;
+        return (uint32_t)((token & 15) * RB + chunk_at<D>(token, chunk - token * B) * 16);
+    };
+    uint32_t v_off[D == 128 ? 1 : B];
 #pragma unroll
-    for (int c = 0; c < kLoads; ++c) v_off[c] = (uint32_t)min(c * 64 + lane, RB - 1) * 16;
-    const auto load_v = [&]() {
+    for (int i = 0; i < (D == 128 ? 1 : B); ++i) v_off[i] = chunk_offset(i);
+    const auto offset = [&](int i) { return D == 128 ? local(v_off[0]) ^ (uint32_t)(16 * i) : v_off[D == 128 ? 0 : i]; };   // (of 128: the turn alone)
+    const auto load_v = [&](int to_buffer, const uint32_t (&rows)[4]) {
+        uint8_t *const to = lds.v[to_buffer];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const auto base = scalar_global(kv.v_codes + (uint64_t)rows[g] * RB);
-#pragma unroll
-            for (int c = 0; c < kLoads; ++c) v_raw[g][c] = load_global<u32x4>(base, local(v_off[c]));
+        for (int i = 0; i < B; ++i) {
+            if (B >= 4) {            // 64 chunks are within one group of 16 tokens
+                global_to_lds16_unseen(kv.v_codes + (uint64_t)rows[i * 64 / (16 * B)] * RB + offset(i), to + i * 1024);
+            } else {                 // of two
+                const int group = (i * 64 + lane) / (16 * B);
+                const uint32_t row = group == 0 ? rows[0] : group == 1 ? rows[1] : group == 2 ? rows[2] : rows[3];
+                global_to_lds16_unseen(kv.v_codes + (uint64_t)row * RB + offset(i), to + i * 1024);
+            }
         }
+    };
+    const auto load_scales = [&]() {
         const uint64_t row = part == 0 ? rows[0] : part == 1 ? rows[1] : part == 2 ? rows[2] : rows[3];
         const uint8_t *ks = reinterpret_cast<const uint8_t *>(kv.k_scales) + row * (B * 2) + s_off;
         const uint8_t *vs = reinterpret_cast<const uint8_t *>(kv.v_scales) + row * (B * 2) + s_off;
@@ -370,7 +413,8 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     if (wave < NQ) load_queries<D>(a, it, head0, heads, wave, queries, lane);
     if (work) {
         place(from);
-        load_v();
+        if (kAhead) load_v(0, rows);
+        load_scales();
         load_k();
     }
     if (wave < NQ) stage_queries<D, NQ>(a, queries, wave, shared, lane);
@@ -378,14 +422,11 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     if (!work) return;
 
     int pos[NQ];                // position of the column's row, -1: no row
-    u32x4 q_sum[NQ][B <= 4 ? 1 : 2];
     float q_unit[NQ];
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
         const int slot = g * 16 + col, token = slot / a.split;
         pos[g] = token < it.count && slot - token * a.split < heads ? it.lo + token : -1;
-#pragma unroll
-        for (int i = 0; i < (B <= 4 ? 1 : 2); ++i) q_sum[g][i] = shared.q_sum[g][i][lane];
         q_unit[g] = shared.q_unit[g][lane];
     }
 
@@ -396,21 +437,15 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
 
     int unit = 0;               // results are in units of 2^unit
     float base[NQ];             // what is taken off a score
-    uint32_t poison[NQ];        // blocks of values that are not finite and were seen
+    uint32_t poison = 0;        // blocks of values that are not finite and were seen, 8 bits a column
 #pragma unroll
-    for (int g = 0; g < NQ; ++g) base[g] = -kBias, poison[g] = 0;
+    for (int g = 0; g < NQ; ++g) base[g] = -kBias;
 
+    int buffer = 0;
     for (int tile = from; tile < to; tile += kWaves) {
         const int t0 = tile * kTile;
         const int bad_now = bad_groups;
-        // ---- value codes and scales to LDS ----
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int c = 0; c < kLoads; ++c) {
-                const int i = c * 64 + lane, token = i / B, chunk = i - token * B;
-                if (RB % 64 == 0 || i < RB) *reinterpret_cast<u32x4 *>(lds.v + value_at<D>(16 * g + token, chunk)) = v_raw[g][c];
-            }
+        // ---- scales to LDS ----
         const int t = t0 + lane;
         const bool live = t >= it.see && t <= it.hi && !((bad_now >> part) & 1);
         uint32_t most = 0;
@@ -455,12 +490,13 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         uint32_t own_scales[(B + 1) / 2];
 #pragma unroll
         for (int i = 0; i < (B + 1) / 2; ++i) own_scales[i] = ks_raw[i];
+        const uint32_t rows_now[4] = {rows[0], rows[1], rows[2], rows[3]};
         // ---- the next tile's values and scales, and the page of the one behind ----
         // (behind the wave's last tile that tile again: loads that no branch surrounds are waited for one by one)
         page = page_next;
         page_next = page_of(min(tile + 2 * kWaves, last_tile));
         place(min(tile + kWaves, last_tile));
-        load_v();
+        load_scales();
         // ---- scores ----
         f32x4 s[4][NQ];
         // (-8 * sum(q) * d over the blocks: the lanes of part g hold the scales of group g's tokens, the others take no part)
@@ -472,13 +508,13 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                 const u32x4 w = {w0, w1, w0, w1};
 #pragma unroll
                 for (int c = 0; c < NQ; ++c)
-                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, q_sum[c][0]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, shared.q_sum[c][0][lane]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             } else {
                 const u32x4 w = {own(0), own(1), own(2), own(3)};
 #pragma unroll
                 for (int c = 0; c < NQ; ++c) {
-                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, q_sum[c][1]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, q_sum[c][0]), s[g][c], 0, 0, 0);
+                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, shared.q_sum[c][1][lane]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, shared.q_sum[c][0][lane]), s[g][c], 0, 0, 0);
                 }
             }
         }
@@ -541,6 +577,9 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         for (int g = 0; g < 4; ++g)
 #pragma unroll
             for (int c = 0; c < NQ; ++c) pin(s[g][c]);
+        // The keys' codes have come, so the values' have, which were asked for before them.
+        if (kAhead) load_v(buffer ^ 1, rows);
+        else load_v(0, rows_now);
         load_k();
         // ---- weights ----
         const bool edge = t0 + kTile - 1 > it.lo || (a.window && t0 <= it.hi - a.window) || t0 < it.see || bad_now;
@@ -586,7 +625,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                 for (int b = 0; b < B; ++b) {
                     const uint64_t own = strange_of[b] >> (4 * part);     // bit 16 g + r
                     const uint32_t bits = (uint32_t)(own & 15) | (uint32_t)(own >> 12 & 0xf0) | (uint32_t)(own >> 24 & 0xf00) | (uint32_t)(own >> 36 & 0xf000);
-                    poison[c] |= (seen & bits ? 1u : 0u) << b;
+                    poison |= (seen & bits ? 1u : 0u) << (8 * c + b);
                 }
             }
 #pragma unroll
@@ -605,6 +644,10 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         // ---- values ----
         // The lane's dimension is lane % 16 of 16; its eight tokens of either half of the tile are those of its scores.  It names the
         // row that nibble lane % 16 of the result comes from: nibbles i and i + 4 of a word, which one and takes together, are neighbours.
+        if (!kAhead) {           // the keys' loads, which went out behind the values', may still be on their way
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(B) : "memory");
+        }
         const int jj = col & 7, k = (jj & 3) * 2 + (jj >> 2);
         const int from_token = 32 * (col >> 3) + 16 * (k >> 2) + 4 * part + (k & 3);
         // A step is kWide times 16 dimensions; behind each of its products goes a piece of the next step's values, made of codes and
@@ -622,7 +665,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
 #pragma unroll
                 for (int k = 0; k < kWide; ++k)
                     raw[step & 1][k] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                        (__attribute__((address_space(3))) i32x2 *)(lds.v + value_at<D>(from_token, b) + 8 * ((step * kWide + k) & 1)));
+                        (__attribute__((address_space(3))) i32x2 *)(lds.v[buffer] + value_at<D>(from_token, b) + 8 * ((step * kWide + k) & 1)));
 #pragma unroll
                 for (int g = 0; g < 4; ++g) d[step & 1][g] = *reinterpret_cast<const u32x2 *>(&lds.v_scale[b][16 * g + 4 * part]);
             };
@@ -678,12 +721,14 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
             }
         }
         wave_sync();
+        if (kAhead) buffer ^= 1;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last codes asked for have to be in LDS before it is used for something else
     if (bad_page) atomicOr(a.error, kKvBadPage);
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
         st.l[c] = add_xor32(add_xor16(st.l[c]));
-        uint32_t p = poison[c], u, w;
+        uint32_t p = poison >> (8 * c) & 0xffu, u, w;
         swap16(p, u, w);
         p = u | w;
         swap32(p, u, w);
@@ -704,7 +749,8 @@ __device__ __forceinline__ float *out_row(const AttentionArgs &a, const Item &it
 }
 
 template <int D, int NQ>
-__global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_kernel(const AttentionArgs) {
+    const AttentionArgs &a = fresh_arguments();
     constexpr int T = D / 16;
     __shared__ __align__(16) SharedLds<D, NQ> lds;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
@@ -739,7 +785,8 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
     // Where there are more turns than workgroups, beginning an item (staging its queries, adding its sums) counts as two turns.
     const uint32_t groups = gridDim.x, heads_all = a.kv.n_head * a.splits;
     const int start = (uint32_t)uniform(head_turns) * heads_all > groups ? 2 : 0;
-    const int before = turns_before + start * items_before, mine = turns_mine + start * items_mine;
+    lds.line[id][0] = turns_before + start * items_before;   // (each thread's own: kept out of the registers that the tiles want)
+    lds.line[id][1] = turns_mine + start * items_mine;
     head_turns = uniform(head_turns + start * head_items);
     const uint32_t total = (uint32_t)head_turns * heads_all;
     // Stretches of one length or one more, as many as there are workgroups; those of an XCD are neighbours.
@@ -757,6 +804,7 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
 
     while (at < end) {
         const int hv = (int)(at / (uint32_t)head_turns), off = (int)(at - (uint32_t)hv * head_turns);
+        const int before = lds.line[id][0], mine = lds.line[id][1];
         if (off >= before && off < before + mine) {     // one thread
             int b = before;
             for (int u = id * per; u < min(units, (id + 1) * per); ++u) {
@@ -777,6 +825,7 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), first = uniform(lds.found[2]), turns = uniform(lds.found[3]);
         const Sequence q = {uniform(lds.found[4]), uniform(lds.found[5]), uniform(lds.found[6])};
         const Item it = item_of(a, seq, q, row_tile);
+        const AttentionArgs &a = fresh_arguments();
         const int kv_head = hv / a.splits, go = hv - kv_head * a.splits;
         const int head0 = kv_head * a.group + go * a.split, heads = min(a.split, a.group - go * a.split);
         // the stretch's turns of the item: none where it ends within the item's start
@@ -789,12 +838,13 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + turn0 * kWaves + wave, tile1, lds, wave, st, lane);
         // ---- the waves' sums: every wave adds a quarter of them ----
         const bool starts = turn0 == 0, ends = turn1 == turns;
-        float *part = a.parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ);
+        float *part = fresh_arguments().parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ);
         constexpr int kMeet = T / meet_rounds(D);
+        const AttentionArgs &b = fresh_arguments();
 #pragma unroll
         for (int g = 0; g < NQ; ++g) {
             bool live;
-            float *y = out_row<D, NQ>(a, it, head0, heads, g, lane, live);
+            float *y = out_row<D, NQ>(b, it, head0, heads, g, lane, live);
 #pragma unroll
             for (int t0 = 0; t0 < T; t0 += kMeet) {
                 __syncthreads();
