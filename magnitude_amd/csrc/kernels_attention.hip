@@ -216,7 +216,7 @@ struct SharedLds {
     u32x4 q_sum[NQ][D / 32 <= 4 ? 1 : 2][64];   // -8 * sum(q) of every block, two halves each
     float q_unit[NQ][64];         // scores are sums times this
     int32_t line[kThreads][2];    // a thread's items on a head's line: turns before them, theirs
-    int32_t wave_turns[kWaves], wave_items[kWaves];
+    int32_t waves[kWaves][3];     // a wave's: turns, items, the longest
     int32_t found[8];             // sequence, row tile, turns before the item, its turns, and the sequence's first row, rows, tokens
 };
 
@@ -756,7 +756,7 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
     const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
     // ---- the line of turns: a thread counts those of `per` items of one head ----
-    int turns_mine = 0, items_mine = 0;
+    int turns_mine = 0, items_mine = 0, longest = 0;
     for (int u = id * per; u < min(units, (id + 1) * per); ++u) {
         const int s = u / a.row_tiles;
         bool bad;
@@ -765,6 +765,7 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         const int n = item_turns(item_of(a, s, q, u - s * a.row_tiles));
         turns_mine += n;
         items_mine += n > 0;
+        longest = max(longest, n);
     }
     int turns_before = turns_mine, items_before = items_mine;
 #pragma unroll
@@ -772,38 +773,51 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         const int o = __shfl_up(turns_before, x), p = __shfl_up(items_before, x);
         if (lane >= x) turns_before += o, items_before += p;
     }
-    if (lane == 63) lds.wave_turns[wave] = turns_before, lds.wave_items[wave] = items_before;
+    longest = (int)wave_max((uint32_t)longest);
+    if (lane == 63) {
+        lds.waves[wave][0] = turns_before;
+        lds.waves[wave][1] = items_before;
+        lds.waves[wave][2] = longest;
+    }
     turns_before -= turns_mine, items_before -= items_mine;
     __syncthreads();
     int head_turns = 0, head_items = 0;
+    longest = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) turns_before += lds.wave_turns[w], items_before += lds.wave_items[w];
-        head_turns += lds.wave_turns[w];
-        head_items += lds.wave_items[w];
+        if (w < wave) turns_before += lds.waves[w][0], items_before += lds.waves[w][1];
+        head_turns += lds.waves[w][0];
+        head_items += lds.waves[w][1];
+        longest = max(longest, lds.waves[w][2]);
     }
-    // Where there are more turns than workgroups, beginning an item (staging its queries, adding its sums) counts as two turns.
+    head_turns = uniform(head_turns), head_items = uniform(head_items), longest = uniform(longest);
+    // Where there are more turns than workgroups, beginning an item (staging its queries, adding its sums) counts as two turns.  Where no item
+    // is longer than a workgroup's share, items stay whole and are dealt out, forwards and backwards in turn: an item is as long as its
+    // rows are far from the start of their sequence, so that long ones meet short ones.  Otherwise every workgroup has a stretch of the
+    // line, of one length or one more; those of an XCD are neighbours.
     const uint32_t groups = gridDim.x, heads_all = a.kv.n_head * a.splits;
-    const int start = (uint32_t)uniform(head_turns) * heads_all > groups ? 2 : 0;
-    lds.line[id][0] = turns_before + start * items_before;   // (each thread's own: kept out of the registers that the tiles want)
-    lds.line[id][1] = turns_mine + start * items_mine;
-    head_turns = uniform(head_turns + start * head_items);
-    const uint32_t total = (uint32_t)head_turns * heads_all;
-    // Stretches of one length or one more, as many as there are workgroups; those of an XCD are neighbours.
+    const int start = (uint32_t)head_turns * heads_all > groups ? 2 : 0;
+    const uint32_t share = ((uint32_t)(head_turns + start * head_items) * heads_all + groups - 1) / groups;
+    const bool whole_items = (uint32_t)(longest + start) <= share;
+    const int head_length = whole_items ? head_items : head_turns + start * head_items;
+    lds.line[id][0] = whole_items ? items_before : turns_before + start * items_before;   // (each thread's own: kept out of the registers
+    lds.line[id][1] = whole_items ? items_mine : turns_mine + start * items_mine;         // that the tiles want)
+    const uint32_t total = (uint32_t)head_length * heads_all;
     const uint32_t active = std::min(total, groups), per_xcd = (active + 7) / 8;
-    const uint32_t me = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+    const uint32_t me = whole_items ? blockIdx.x : (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
     int32_t *const join = a.joins + 8 * (int64_t)blockIdx.x;
-    if (blockIdx.x / 8 >= per_xcd || me >= active) {
+    if (me >= active || (!whole_items && blockIdx.x / 8 >= per_xcd)) {
         if (id == 0) join[0] = -1;
         return;
     }
-    const uint32_t length = total / active, longer = total - length * active;     // the first `longer` ones have one more
-    uint32_t at = me * length + std::min(me, longer);
-    const uint32_t end = at + length + (me < longer ? 1 : 0);
+    const uint32_t length = total / active, longer = total - length * active;     // the first `longer` stretches have one more
+    uint32_t at = whole_items ? me : me * length + std::min(me, longer);
+    const uint32_t end = whole_items ? total : at + length + (me < longer ? 1 : 0);
+    uint32_t round = 0;
     int join_from = -1, join_seq = 0, join_tile = 0, join_head = 0;
 
     while (at < end) {
-        const int hv = (int)(at / (uint32_t)head_turns), off = (int)(at - (uint32_t)hv * head_turns);
+        const int hv = (int)(at / (uint32_t)head_length), off = (int)(at - (uint32_t)hv * head_length);
         const int before = lds.line[id][0], mine = lds.line[id][1];
         if (off >= before && off < before + mine) {     // one thread
             int b = before;
@@ -811,14 +825,14 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
                 const int s = u / a.row_tiles;
                 bool bad;
                 const Sequence q = sequence(a, s, bad);
-                const int n = item_turns(item_of(a, s, q, u - s * a.row_tiles));
-                if (n > 0 && off < b + n + start) {
+                const int n = item_turns(item_of(a, s, q, u - s * a.row_tiles)), weight = n == 0 ? 0 : whole_items ? 1 : n + start;
+                if (off < b + weight) {
                     const int found[7] = {s, u - s * a.row_tiles, b, n, q.start, q.count, q.len};
 #pragma unroll
                     for (int i = 0; i < 7; ++i) lds.found[i] = found[i];
                     break;
                 }
-                b += n > 0 ? n + start : 0;
+                b += weight;
             }
         }
         __syncthreads();
@@ -830,7 +844,7 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         const int head0 = kv_head * a.group + go * a.split, heads = min(a.split, a.group - go * a.split);
         // the stretch's turns of the item: none where it ends within the item's start
         const int skip = off - first, take = (int)std::min<uint32_t>(turns + start - skip, end - at);
-        const int turn0 = max(0, skip - start), turn1 = skip + take - start;
+        const int turn0 = whole_items ? 0 : max(0, skip - start), turn1 = whole_items ? turns : skip + take - start;
         if (turn1 <= 0) break;
         const int tile0 = it.hi < 0 ? 0 : it.see / kTile, tile1 = tile0 + min(turn1 * kWaves, item_tiles(it));
 
@@ -892,7 +906,12 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
             join_from = (int)(from < edge ? from / (length + 1) : longer + (from - edge) / length);
             join_seq = seq, join_tile = row_tile, join_head = hv;
         }
-        at += take;
+        if (whole_items) {
+            ++round;
+            at = round * active + (round & 1 ? active - 1 - me : me);
+        } else {
+            at += take;
+        }
         if (at < end) __syncthreads();
     }
     if (id == 0) {
