@@ -5,7 +5,7 @@
 // Work.  An item is 16 or 32 rows (some new tokens x the query heads that share a key/value head) against the
 // tokens they see, in tiles of 64 tokens.  All tiles of all items lie in one line, head by head, and the workgroups of one round
 // take equal stretches of it, whatever the lengths of the sequences are: a stretch ends inside an item where it has to, its
-// sums go to the workspace, and attention_join_kernel adds the parts of the items that were cut.  The line is laid out
+// sums go to the workspace, and the workgroup that writes the last part of an item adds them.  The line is laid out
 // on the device (a scan over the lengths in every workgroup), so that a captured call follows the lengths.  Inside a
 // workgroup the four waves take tiles in turn, each with its own running maximum, sum and result; they meet once, at the
 // end of an item.  No barrier in the loop over tiles.
@@ -57,7 +57,9 @@ struct AttentionArgs {
     const int32_t *q_start, *kv_len, *pages;
     int32_t *error;
     float *parts;            // [workgroups][2] sums of items that were cut (part_floats each)
-    int32_t *joins;          // [workgroups][8] {first stretch (-1: nothing to join), last stretch, sequence, row tile, head}
+    uint32_t *arrived;       // [workgroups] parts written of the item that a stretch begins and does not end; zero between calls.  Null:
+                             // attention_join_kernel adds the parts
+    int32_t *joins;          // [workgroups][8] for it: {first stretch (-1: nothing to join), last stretch, sequence, row tile, head}
     float scale;             // times log2(e)
     int32_t n_tokens, n_seq, max_q, window;
     int32_t group;           // query heads of a key/value head
@@ -163,6 +165,17 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return (uint32_t)uniform((int)max(x, y));
 }
 
+// sums over the lanes up to each one
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);    // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 // keeps a value where it is computed: the compiler otherwise moves whole chains behind the next branch, and what feeds them stays
 // in registers that long
 __device__ __forceinline__ void pin(f32x4 &v) { asm volatile("" : "+v"(v)); }
@@ -217,6 +230,7 @@ struct SharedLds {
     float q_unit[NQ][64];         // scores are sums times this
     int32_t line[kThreads][2];    // a thread's items on a head's line: turns before them, theirs
     int32_t waves[kWaves][3];     // a wave's: turns, items, the longest
+    int32_t last;                 // whether the workgroup wrote the last part of an item
     int32_t found[8];             // sequence, row tile, turns before the item, its turns, and the sequence's first row, rows, tokens
 };
 
@@ -228,74 +242,78 @@ struct Running {
 };
 
 // 16 queries of an item for the matrix cores: 22 bits of q * scale * log2(e), the row scaled by a power of two
-template <int D>
+template <int D, int NQ>
 struct Queries {
-    f32x4 x[D / 32][2];
-    bool live;
+    f32x4 x[NQ][D / 32][2];
 };
 
-template <int D>
-__device__ __forceinline__ void load_queries(const AttentionArgs &a, const Item &it, int head0, int heads, int g, Queries<D> &q, int lane) {
-    const int slot = g * 16 + (lane & 15), token = slot / a.split, head = slot - token * a.split;
-    q.live = token < it.count && head < heads;
-    const float *row = a.q + (int64_t)(it.first + (q.live ? token : 0)) * a.q_stride + (int64_t)(head0 + (q.live ? head : 0)) * D + 8 * (lane >> 4);
+template <int D, int NQ>
+__device__ __forceinline__ void load_queries(const AttentionArgs &a, const Item &it, int head0, int heads, Queries<D, NQ> &q, int lane) {
 #pragma unroll
-    for (int b = 0; b < D / 32; ++b)
+    for (int g = 0; g < NQ; ++g) {
+        const int slot = g * 16 + (lane & 15), token = slot / a.split, head = slot - token * a.split;
+        const bool live = token < it.count && head < heads;
+        const float *row = a.q + (int64_t)(it.first + (live ? token : 0)) * a.q_stride + (int64_t)(head0 + (live ? head : 0)) * D + 8 * (lane >> 4);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) q.x[b][k] = *reinterpret_cast<const f32x4 *>(row + 32 * b + 4 * k);
+        for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) q.x[g][b][k] = *reinterpret_cast<const f32x4 *>(row + 32 * b + 4 * k);
+    }
 }
 
+// (every wave finds the rows' largest values; each then stages its share of the blocks)
 template <int D, int NQ>
-__device__ __forceinline__ void stage_queries(const AttentionArgs &a, Queries<D> &q, int g, SharedLds<D, NQ> &lds, int lane) {
+__device__ __forceinline__ void stage_queries(const AttentionArgs &a, const Item &it, int heads, Queries<D, NQ> &q, SharedLds<D, NQ> &lds, int wave, int lane) {
     constexpr int B = D / 32;
-    auto &x = q.x;
-    const bool live = q.live;
-    float most = 0.f;
-    bool whole = true;
 #pragma unroll
-    for (int b = 0; b < B; ++b)
+    for (int g = 0; g < NQ; ++g) {
+        auto &x = q.x[g];
+        const int slot = g * 16 + (lane & 15), token = slot / a.split;
+        const bool live = token < it.count && slot - token * a.split < heads;
+        float most = 0.f;
+        bool whole = true;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int b = 0; b < B; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[b][k][j] = live ? x[b][k][j] * a.scale : 0.f;
-                most = fmaxf(most, fabsf(x[b][k][j]));
-                whole = whole && fabsf(x[b][k][j]) <= 3.402823466e38f;
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[b][k][j] = live ? x[b][k][j] * a.scale : 0.f;
+                    most = fmaxf(most, fabsf(x[b][k][j]));
+                    whole = whole && fabsf(x[b][k][j]) <= 3.402823466e38f;
+                }
+        most = max_xor(whole ? most : INFINITY);
+        // (frexp: most = f * 2^e with f in [0.5, 1); where a value is not finite the row stays as it is: NaN comes of it)
+        const int e = most > 0.f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
+        if (wave == 0) lds.q_unit[g][lane] = ldexpf(1.f, min(e - 15 + 24, 127));
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            if (b % kWaves != wave) continue;
+            float sum = 0.f;
+            u32x4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int s = 15 - e - (i & 1 ? 4 : 0);
+                const float u = ldexpf(x[b][0][i], s), v = ldexpf(x[b][1][i], s);
+                hi[i] = half_pair(u, v);
+                lo[i] = half_pair(u - low_half(hi[i]), v - high_half(hi[i]));
+                sum += ((low_half(hi[i]) + low_half(lo[i])) + (high_half(hi[i]) + high_half(lo[i]))) * (i & 1 ? 16.f : 1.f);
             }
+            lds.q[b][g][0][lane] = hi;
+            lds.q[b][g][1][lane] = lo;
+            // of up to four blocks the sums' high halves, then the low ones, against the scales twice; of eight two products
+            const float s = add_xor32(add_xor16(sum)) * (-8.f * 5.9604644775390625e-8f);
+            const uint32_t h = half_pair(s, s), l = half_pair(s - low_half(h), 0.f);
+            uint16_t *to = reinterpret_cast<uint16_t *>(&lds.q_sum[g][0][lane]);
+            to[b] = (uint16_t)h;
+            if (B <= 4) to[4 + b] = (uint16_t)l;
+            else reinterpret_cast<uint16_t *>(&lds.q_sum[g][B <= 4 ? 0 : 1][lane])[b] = (uint16_t)l;
         }
-    most = max_xor(whole ? most : INFINITY);
-    // (frexp: most = f * 2^e with f in [0.5, 1); where a value is not finite the row stays as it is: NaN comes of it)
-    const int e = most > 0.f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
-    lds.q_unit[g][lane] = ldexpf(1.f, min(e - 15 + 24, 127));
-    float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (B < 4 && wave == kWaves - 1) {       // places of blocks that are not there
+            uint16_t *to = reinterpret_cast<uint16_t *>(&lds.q_sum[g][0][lane]);
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
-        float sum = 0.f;
-        u32x4 hi, lo;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int s = 15 - e - (i & 1 ? 4 : 0);
-            const float u = ldexpf(x[b][0][i], s), v = ldexpf(x[b][1][i], s);
-            hi[i] = half_pair(u, v);
-            lo[i] = half_pair(u - low_half(hi[i]), v - high_half(hi[i]));
-            sum += ((low_half(hi[i]) + low_half(lo[i])) + (high_half(hi[i]) + high_half(lo[i]))) * (i & 1 ? 16.f : 1.f);
+            for (int b = B; b < 4; ++b) to[b] = to[4 + b] = 0;
         }
-        lds.q[b][g][0][lane] = hi;
-        lds.q[b][g][1][lane] = lo;
-        sums[b] = add_xor32(add_xor16(sum)) * (-8.f * 5.9604644775390625e-8f);
-    }
-    // up to four blocks: high halves, then low ones, against the scales twice; eight: two products
-    u32x4 hi, lo;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        hi[i] = half_pair(sums[2 * i], sums[2 * i + 1]);
-        lo[i] = half_pair(sums[2 * i] - low_half(hi[i]), sums[2 * i + 1] - high_half(hi[i]));
-    }
-    if constexpr (B <= 4) {
-        lds.q_sum[g][0][lane] = u32x4{hi[0], hi[1], lo[0], lo[1]};
-    } else {
-        lds.q_sum[g][0][lane] = hi;
-        lds.q_sum[g][1][lane] = lo;
     }
 }
 
@@ -408,16 +426,15 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         }
     };
     // (loads come back in order: pages, then queries, then keys and values)
-    static_assert(NQ <= kWaves, "a wave stages 16 queries");
-    Queries<D> queries;
-    if (wave < NQ) load_queries<D>(a, it, head0, heads, wave, queries, lane);
+    Queries<D, NQ> queries;
+    load_queries<D, NQ>(a, it, head0, heads, queries, lane);
     if (work) {
         place(from);
         if (kAhead) load_v(0, rows);
         load_scales();
         load_k();
     }
-    if (wave < NQ) stage_queries<D, NQ>(a, queries, wave, shared, lane);
+    stage_queries<D, NQ>(a, it, heads, queries, shared, wave, lane);
     __syncthreads();
     if (!work) return;
 
@@ -740,6 +757,25 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     }
 }
 
+// Parts go from one workgroup to another past the caches of their XCDs: stores and loads of device scope, which reach the memory that all of
+// them share.  (With ordinary ones and fences, every fence writes back or drops a whole L2: a token of 131072 took 149 us, like this 45.)
+__device__ __forceinline__ void store_part(float *p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void store_part(f32x4 *p, f32x4 v) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        __hip_atomic_store(reinterpret_cast<uint64_t *>(p) + i, __builtin_bit_cast(uint64_t, f32x2{v[2 * i], v[2 * i + 1]}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float load_part(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ f32x4 load_part(const f32x4 *p) {
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const f32x2 x = __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<const uint64_t *>(p) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        v[2 * i] = x[0], v[2 * i + 1] = x[1];
+    }
+    return v;
+}
+
 // rows of an item from sums: lane's column of 16 queries, 4 dimensions of 16
 template <int D, int NQ>
 __device__ __forceinline__ float *out_row(const AttentionArgs &a, const Item &it, int head0, int heads, int g, int lane, bool &live) {
@@ -748,10 +784,118 @@ __device__ __forceinline__ float *out_row(const AttentionArgs &a, const Item &it
     return a.y + (int64_t)(it.first + (live ? token : 0)) * a.y_stride + (int64_t)(head0 + (live ? head : 0)) * D + 4 * (lane >> 4);
 }
 
+// The waves' sums of an item: every wave adds a quarter of the dimensions, and writes rows of the result, or a part of one.
+template <int D, int NQ>
+__device__ __forceinline__ void meet(const AttentionArgs &a, const Item &it, int head0, int heads, const Running<D, NQ> &st, bool whole, float *part, SharedLds<D, NQ> &lds,
+                                     int wave, int lane) {
+    constexpr int T = D / 16, kMeet = T / meet_rounds(D);
+#pragma unroll
+    for (int g = 0; g < NQ; ++g) {
+        bool live;
+        float *y = out_row<D, NQ>(a, it, head0, heads, g, lane, live);
+#pragma unroll
+        for (int t0 = 0; t0 < T; t0 += kMeet) {
+            __syncthreads();
+            if (lane < 16) {
+                lds.meet.m[wave][lane] = st.m[g];
+                lds.meet.l[wave][lane] = st.l[g];
+            }
+#pragma unroll
+            for (int t = 0; t < kMeet; ++t) lds.meet.o[wave][t][lane] = st.o[t0 + t][g];
+            __syncthreads();
+            if (live) {
+                float m = -INFINITY, l = 0.f, f[kWaves];
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) m = fmaxf(m, lds.meet.m[w][lane & 15]);
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    const float mw = lds.meet.m[w][lane & 15];
+                    f[w] = mw == m ? 1.f : __builtin_amdgcn_exp2f(mw - m);
+                    l += lds.meet.l[w][lane & 15] * f[w];
+                }
+                const float unit = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
+                for (int t = wave; t < kMeet; t += kWaves) {
+                    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int w = 0; w < kWaves; ++w) {
+                        const f32x4 x = lds.meet.o[w][t][lane];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] += x[r] * f[w];
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] *= unit;
+                    if (whole) *reinterpret_cast<f32x4 *>(y + 16 * (t0 + t)) = v;
+                    else store_part(reinterpret_cast<f32x4 *>(part) + ((t0 + t) * NQ + g) * 64 + lane, v);
+                }
+                if (!whole && wave == 0 && lane < 16) {
+                    store_part(part + 16 * NQ * D + g * 16 + lane, m);
+                    store_part(part + 16 * NQ * D + (NQ + g) * 16 + lane, l);
+                }
+            }
+        }
+    }
+}
+
+// An item that was cut into a few parts, which stretches first .. first + parts - 1 wrote: their sums.  The waves share the dimensions; a part
+// comes from far away, so several are asked for at a time.
+template <int D, int NQ>
+__device__ __forceinline__ void join_parts(const AttentionArgs &a, const Item &it, int head0, int heads, int first, int parts, SharedLds<D, NQ> &lds, int wave, int lane) {
+    constexpr int T = D / 16, kMine = (T + kWaves - 1) / kWaves, kBatch = 4, kM = 16 * NQ * D, kL = kM + 16 * NQ;
+    const int col = lane & 15;
+    const int64_t size = part_floats(D, NQ);
+    const auto part = [&](int w) { return a.parts + ((int64_t)(first + w) * 2 + (w ? 0 : 1)) * size; };   // (the first is a stretch's second)
+#pragma unroll
+    for (int g = 0; g < NQ; ++g) {
+        bool live;
+        float *y = out_row<D, NQ>(a, it, head0, heads, g, lane, live);
+        float m = -INFINITY;
+        for (int w = wave * 4 + (lane >> 4); live && w < parts; w += 4 * kWaves) m = fmaxf(m, load_part(part(w) + kM + g * 16 + col));
+        m = max_xor(m);
+        __syncthreads();
+        if (lane < 16) lds.meet.m[wave][lane] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, lds.meet.m[w][col]);
+        if (live) {
+            float l = 0.f;
+            f32x4 o[kMine];
+#pragma unroll
+            for (int t = 0; t < kMine; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int w0 = 0; w0 < parts; w0 += kBatch) {
+                float mw[kBatch], lw[kBatch];
+                f32x4 v[kBatch][kMine];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {       // (behind the last part that part again, with no weight)
+                    const float *p = part(min(w0 + k, parts - 1));
+                    mw[k] = load_part(p + kM + g * 16 + col);
+                    lw[k] = load_part(p + kL + g * 16 + col);
+#pragma unroll
+                    for (int t = 0; t < kMine; ++t) v[k][t] = load_part(reinterpret_cast<const f32x4 *>(p) + (min(t * kWaves + wave, T - 1) * NQ + g) * 64 + lane);
+                }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    if (w0 + k >= parts) break;
+                    const float f = mw[k] == m ? 1.f : __builtin_amdgcn_exp2f(mw[k] - m);
+                    l += lw[k] * f;
+#pragma unroll
+                    for (int t = 0; t < kMine; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[t][r] += v[k][t][r] * f;
+                }
+            }
+            const float unit = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+            for (int t = 0; t < kMine; ++t)
+                if (t * kWaves + wave < T)
+                    *reinterpret_cast<f32x4 *>(y + 16 * (t * kWaves + wave)) = f32x4{o[t][0] * unit, o[t][1] * unit, o[t][2] * unit, o[t][3] * unit};
+        }
+    }
+}
+
 template <int D, int NQ>
 __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_kernel(const AttentionArgs) {
     const AttentionArgs &a = fresh_arguments();
-    constexpr int T = D / 16;
+    fetch_arguments<void(AttentionArgs), sizeof(AttentionArgs)>();
     __shared__ __align__(16) SharedLds<D, NQ> lds;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
     const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
@@ -767,12 +911,7 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         items_mine += n > 0;
         longest = max(longest, n);
     }
-    int turns_before = turns_mine, items_before = items_mine;
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-        const int o = __shfl_up(turns_before, x), p = __shfl_up(items_before, x);
-        if (lane >= x) turns_before += o, items_before += p;
-    }
+    int turns_before = wave_scan(turns_mine), items_before = wave_scan(items_mine);
     longest = (int)wave_max((uint32_t)longest);
     if (lane == 63) {
         lds.waves[wave][0] = turns_before;
@@ -805,16 +944,15 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
     const uint32_t total = (uint32_t)head_length * heads_all;
     const uint32_t active = std::min(total, groups), per_xcd = (active + 7) / 8;
     const uint32_t me = whole_items ? blockIdx.x : (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
-    int32_t *const join = a.joins + 8 * (int64_t)blockIdx.x;
     if (me >= active || (!whole_items && blockIdx.x / 8 >= per_xcd)) {
-        if (id == 0) join[0] = -1;
+        if (id == 0 && !a.arrived) a.joins[8 * (int64_t)blockIdx.x] = -1;
         return;
     }
+    int join_from = -1, join_seq = 0, join_tile = 0, join_head = 0;
     const uint32_t length = total / active, longer = total - length * active;     // the first `longer` stretches have one more
     uint32_t at = whole_items ? me : me * length + std::min(me, longer);
     const uint32_t end = whole_items ? total : at + length + (me < longer ? 1 : 0);
     uint32_t round = 0;
-    int join_from = -1, join_seq = 0, join_tile = 0, join_head = 0;
 
     while (at < end) {
         const int hv = (int)(at / (uint32_t)head_length), off = (int)(at - (uint32_t)hv * head_length);
@@ -850,61 +988,31 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
 
         Running<D, NQ> st;
         walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + turn0 * kWaves + wave, tile1, lds, wave, st, lane);
-        // ---- the waves' sums: every wave adds a quarter of them ----
+        // ---- the waves' sums ----
         const bool starts = turn0 == 0, ends = turn1 == turns;
-        float *part = fresh_arguments().parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ);
-        constexpr int kMeet = T / meet_rounds(D);
-        const AttentionArgs &b = fresh_arguments();
-#pragma unroll
-        for (int g = 0; g < NQ; ++g) {
-            bool live;
-            float *y = out_row<D, NQ>(b, it, head0, heads, g, lane, live);
-#pragma unroll
-            for (int t0 = 0; t0 < T; t0 += kMeet) {
+        meet<D, NQ>(fresh_arguments(), it, head0, heads, st, starts && ends, fresh_arguments().parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ), lds, wave, lane);
+        const AttentionArgs &c = fresh_arguments();
+        if (!(starts && ends) && (c.arrived || ends)) {
+            const auto stretch_of = [&](uint32_t p) {
+                const uint32_t edge = longer * (length + 1);
+                return (int)(p < edge ? p / (length + 1) : longer + (p - edge) / length);
+            };
+            const int first = stretch_of(at - skip + start);
+            if (!c.arrived) {
+                join_from = first;
+                join_seq = seq, join_tile = row_tile, join_head = hv;
+            } else {
+                // The part is in memory before it is counted (the wait is for the stores); whoever counts the last one loads them after that.
+                const int parts = stretch_of(at - skip + start + turns - 1) - first + 1;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads();
-                if (lane < 16) {
-                    lds.meet.m[wave][lane] = st.m[g];
-                    lds.meet.l[wave][lane] = st.l[g];
-                }
-#pragma unroll
-                for (int t = 0; t < kMeet; ++t) lds.meet.o[wave][t][lane] = st.o[t0 + t][g];
+                if (id == 0) lds.last = __hip_atomic_fetch_add(c.arrived + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
                 __syncthreads();
-                if (live) {
-                    float m = -INFINITY, l = 0.f, f[kWaves];
-#pragma unroll
-                    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, lds.meet.m[w][lane & 15]);
-#pragma unroll
-                    for (int w = 0; w < kWaves; ++w) {
-                        const float mw = lds.meet.m[w][lane & 15];
-                        f[w] = mw == m ? 1.f : __builtin_amdgcn_exp2f(mw - m);
-                        l += lds.meet.l[w][lane & 15] * f[w];
-                    }
-                    const bool whole = starts && ends;
-                    const float unit = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
-                    for (int t = wave; t < kMeet; t += kWaves) {
-                        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int w = 0; w < kWaves; ++w) {
-                            const f32x4 x = lds.meet.o[w][t][lane];
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) v[r] += x[r] * f[w];
-                        }
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] *= unit;
-                        if (whole) *reinterpret_cast<f32x4 *>(y + 16 * (t0 + t)) = v;
-                        else reinterpret_cast<f32x4 *>(part)[((t0 + t) * NQ + g) * 64 + lane] = v;
-                    }
-                    if (!whole && wave == 0 && lane < 16) {
-                        part[16 * NQ * D + g * 16 + lane] = m;
-                        part[16 * NQ * D + (NQ + g) * 16 + lane] = l;
-                    }
+                if (lds.last) {
+                    if (id == 0) __hip_atomic_store(c.arrived + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
+                    join_parts<D, NQ>(c, it, head0, heads, first, parts, lds, wave, lane);
                 }
             }
-        }
-        if (ends && !starts) {
-            const uint32_t from = at - skip + start, edge = longer * (length + 1);
-            join_from = (int)(from < edge ? from / (length + 1) : longer + (from - edge) / length);
-            join_seq = seq, join_tile = row_tile, join_head = hv;
         }
         if (whole_items) {
             ++round;
@@ -914,23 +1022,24 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         }
         if (at < end) __syncthreads();
     }
-    if (id == 0) {
+    if (id == 0 && !fresh_arguments().arrived) {
+        int32_t *const join = fresh_arguments().joins + 8 * (int64_t)blockIdx.x;
         join[0] = join_from;
-        join[1] = me;
+        join[1] = (int32_t)me;
         join[2] = join_seq;
         join[3] = join_tile;
         join[4] = join_head;
     }
 }
 
-// Items that were cut: the sums of stretches first .. last.  A workgroup takes 16 queries and a share of the dimensions; its waves take
+// Items that were cut into many parts: the sums of stretches first .. last.  A workgroup takes 16 queries and a share of the dimensions; its waves take
 // the parts in turn, four at a time (their loads go out together: a part comes from another XCD's memory), and meet once.
 constexpr int kJoinWaves = 8;
-constexpr int join_share(int tiles) { return tiles % 4 ? tiles / 2 : tiles / 4; }   // of the dimensions, in 16s
+constexpr int join_share(int dim, int cols) { return dim / 16 % 4 || cols > 1 ? dim / 32 : dim / 64; }   // of the dimensions, in 16s: few workgroups, most have nothing to join
 
 template <int D, int NQ>
 __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const AttentionArgs a) {
-    constexpr int T = D / 16, kShare = join_share(T), kShares = T / kShare, kBatch = 4;
+    constexpr int T = D / 16, kShare = join_share(D, NQ), kShares = T / kShare, kBatch = 4;
     static_assert(T % kShare == 0, "whole shares");
     __shared__ __align__(16) f32x4 sums[kJoinWaves][kShare][64];
     __shared__ float tops[kJoinWaves][16], weights[kJoinWaves][16];
@@ -1010,16 +1119,17 @@ template <int D, int NQ>
 hipError_t launch(const AttentionArgs &a, int groups, hipStream_t s) {
     hipLaunchKernelGGL((attention_kernel<D, NQ>), dim3(groups), dim3(kThreads), 0, s, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || groups == 1) return e;
-    hipLaunchKernelGGL((attention_join_kernel<D, NQ>), dim3(groups, D / 16 / join_share(D / 16) * NQ), dim3(64 * kJoinWaves), 0, s, a);
+    if (e != hipSuccess || a.arrived) return e;
+    hipLaunchKernelGGL((attention_join_kernel<D, NQ>), dim3(groups, D / 16 / join_share(D, NQ) * NQ), dim3(64 * kJoinWaves), 0, s, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
-size_t attention_scratch_bytes(int cus) {
-    return (size_t)cus * 2 * ((size_t)2 * part_floats(256, 2) * 4 + 32);   // (more than any instance takes)
-}
+// counts of parts (zero before the first call; every call leaves them so), what the joining kernel is to do, then the parts
+static size_t arrived_bytes(int cus) { return ((size_t)cus * 2 * 4 + 255) / 256 * 256; }
+static size_t joins_bytes(int cus) { return (size_t)cus * 2 * 32; }
+size_t attention_scratch_bytes(int cus) { return arrived_bytes(cus) + joins_bytes(cus) + (size_t)cus * 2 * 2 * part_floats(256, 2) * 4; }
 
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     if (j.n_tokens == 0 || j.n_seq == 0 || j.max_q == 0) return hipSuccess;
@@ -1050,8 +1160,13 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     const int64_t most = ((j.pages_stride << j.kv->page_shift) + kTile - 1) / kTile + 1;
     const double turns = (double)most * a.n_seq * a.row_tiles * j.kv->n_head * a.splits / kWaves + (double)a.n_seq * a.row_tiles * j.kv->n_head * a.splits;
     const int groups = (int)std::min<double>(groups_most, turns);
-    a.parts = reinterpret_cast<float *>(j.scratch);
-    a.joins = reinterpret_cast<int32_t *>(j.scratch + (size_t)groups * 2 * part_floats(a.kv.dim, cols) * 4);
+    a.parts = reinterpret_cast<float *>(j.scratch + arrived_bytes(j.cus) + joins_bytes(j.cus));
+    // An item is cut into as many parts as there are workgroups for it, one or two more at its ends.  Up to eight, whoever writes the last part
+    // adds them: one launch.  More are added by a kernel whose workgroups share the work: for a token of 131072 (64 parts) 52 us against 60.
+    const double items = (double)a.n_seq * a.row_tiles * j.kv->n_head * a.splits;
+    const bool few_parts = groups <= 8 * items;
+    a.arrived = few_parts ? reinterpret_cast<uint32_t *>(j.scratch) : nullptr;
+    a.joins = reinterpret_cast<int32_t *>(j.scratch + arrived_bytes(j.cus));
     if (dry_run()) {
         plan_note("attention_kernel<%d, %d>: %d heads in %d x %d of %d, %d tokens x %d a sequence of rows, grid %d x %d", a.kv.dim, cols, j.n_head, a.kv.n_head,
                   a.splits, a.split, a.tokens, a.row_tiles, groups, kThreads);

@@ -1812,7 +1812,14 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
             hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
             QP_HIP(ctx, hipStreamIsCapturing(ctx->stream, &capture));
             if (capture != hipStreamCaptureStatusNone) return fail(ctx, QPROJ_ERR_UNSUPPORTED, "qproj_attention: a context's first call allocates and cannot be captured");
-            QP_HIP(ctx, hipMalloc((void **)&ctx->attention_ws, attention_scratch_bytes(ctx->cus)));
+            uint8_t *ws = nullptr;
+            QP_HIP(ctx, hipMalloc((void **)&ws, attention_scratch_bytes(ctx->cus)));
+            const hipError_t e = hipMemsetAsync(ws, 0, attention_scratch_bytes(ctx->cus), ctx->stream);
+            if (e != hipSuccess) {
+                (void)hipFree(ws);
+                return fail(ctx, QPROJ_ERR_HIP, "hipMemsetAsync", e);
+            }
+            ctx->attention_ws = ws;
         }
     }
     AttentionJob j{};
