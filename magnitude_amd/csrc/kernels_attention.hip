@@ -14,8 +14,10 @@
 // one query throughout: row statistics are a lane's own, and the probabilities come out of the first product in the
 // order in which the second takes them.
 //   scores   acc = sum over a block of 32 of n * q, in fp32; S += d_k * acc.  The codes n (0..15) go into the matrix cores as
-//            subnormal halves: a nibble in bits 0..3 is n * 2^-24 as it stands, one in bits 4..7 n * 2^-20, so a word of eight
-//            codes costs a shift and four ands.  q carries 2^-4 where that is; d_k * -8 * sum(q) over the blocks is one more product.
+//            subnormal halves: a nibble in bits 4..7 is n * 2^-20 as it stands, so a word of eight codes costs three shifts and
+//            four ands.  (The matrix cores line products up by their factors' exponents, a subnormal's being 2^-14, and drop what is
+//            24 bits below the largest: nibbles left in bits 0..3 saved two of the shifts and cost four bits, an error of 1.5e-5 of
+//            the result.)  -8 * sum(q) of a block is what its products begin with.
 //            q is scaled by a power of two of its row and split into two halves: 22 bits, two products.
 //   values   codes become n - 8 (1024 + n as half bits, less 1032), times the block's d: product and remainder of one
 //            multiplication are two halves that hold it exactly (4 x 11 bits), the largest d of a tile brought to 2^11..2^12 by a power
@@ -226,7 +228,7 @@ struct SharedLds {
         } meet;
     };
     u32x4 q[D / 32][NQ][2][64];   // the item's queries as the matrix cores take them: high halves, low halves
-    u32x4 q_sum[NQ][D / 32 <= 4 ? 1 : 2][64];   // -8 * sum(q) of every block, two halves each
+    f32x4 q_sum[D / 32][NQ][16];                // -8 * sum(q) of every block, once for each of a lane's four tokens
     float q_unit[NQ][64];         // scores are sums times this
     int32_t line[kThreads][2];    // a thread's items on a head's line: turns before them, theirs
     int32_t waves[kWaves][3];     // a wave's: turns, items, the longest
@@ -285,7 +287,7 @@ __device__ __forceinline__ void stage_queries(const AttentionArgs &a, const Item
         most = max_xor(whole ? most : INFINITY);
         // (frexp: most = f * 2^e with f in [0.5, 1); where a value is not finite the row stays as it is: NaN comes of it)
         const int e = most > 0.f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
-        if (wave == 0) lds.q_unit[g][lane] = ldexpf(1.f, min(e - 15 + 24, 127));
+        if (wave == 0) lds.q_unit[g][lane] = ldexpf(1.f, min(e - 15 + 20, 127));
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             if (b % kWaves != wave) continue;
@@ -293,26 +295,15 @@ __device__ __forceinline__ void stage_queries(const AttentionArgs &a, const Item
             u32x4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int s = 15 - e - (i & 1 ? 4 : 0);
-                const float u = ldexpf(x[b][0][i], s), v = ldexpf(x[b][1][i], s);
+                const float u = ldexpf(x[b][0][i], 15 - e), v = ldexpf(x[b][1][i], 15 - e);
                 hi[i] = half_pair(u, v);
                 lo[i] = half_pair(u - low_half(hi[i]), v - high_half(hi[i]));
-                sum += ((low_half(hi[i]) + low_half(lo[i])) + (high_half(hi[i]) + high_half(lo[i]))) * (i & 1 ? 16.f : 1.f);
+                sum += (low_half(hi[i]) + low_half(lo[i])) + (high_half(hi[i]) + high_half(lo[i]));
             }
             lds.q[b][g][0][lane] = hi;
             lds.q[b][g][1][lane] = lo;
-            // of up to four blocks the sums' high halves, then the low ones, against the scales twice; of eight two products
-            const float s = add_xor32(add_xor16(sum)) * (-8.f * 5.9604644775390625e-8f);
-            const uint32_t h = half_pair(s, s), l = half_pair(s - low_half(h), 0.f);
-            uint16_t *to = reinterpret_cast<uint16_t *>(&lds.q_sum[g][0][lane]);
-            to[b] = (uint16_t)h;
-            if (B <= 4) to[4 + b] = (uint16_t)l;
-            else reinterpret_cast<uint16_t *>(&lds.q_sum[g][B <= 4 ? 0 : 1][lane])[b] = (uint16_t)l;
-        }
-        if (B < 4 && wave == kWaves - 1) {       // places of blocks that are not there
-            uint16_t *to = reinterpret_cast<uint16_t *>(&lds.q_sum[g][0][lane]);
-#pragma unroll
-            for (int b = B; b < 4; ++b) to[b] = to[4 + b] = 0;
+            const float less = add_xor32(add_xor16(sum)) * (-8.f * 9.5367431640625e-7f);
+            if (lane < 16) lds.q_sum[b][g][lane] = f32x4{less, less, less, less};
         }
     }
 }
@@ -504,9 +495,6 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
             for (int b = 0; b < B; ++b) strange_of[b] = __ballot((vs[b] & 0x7fffu) >= 0x7c00u);
         }
         wave_sync();
-        uint32_t own_scales[(B + 1) / 2];
-#pragma unroll
-        for (int i = 0; i < (B + 1) / 2; ++i) own_scales[i] = ks_raw[i];
         const uint32_t rows_now[4] = {rows[0], rows[1], rows[2], rows[3]};
         // ---- the next tile's values and scales, and the page of the one behind ----
         // (behind the wave's last tile that tile again: loads that no branch surrounds are waited for one by one)
@@ -516,25 +504,10 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         load_scales();
         // ---- scores ----
         f32x4 s[4][NQ];
-        // (-8 * sum(q) * d over the blocks: the lanes of part g hold the scales of group g's tokens, the others take no part)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const auto own = [&](int i) { return part == g ? own_scales[i] : 0u; };
-            if constexpr (B <= 4) {
-                const uint32_t w0 = own(0), w1 = B > 2 ? own(1) : 0;
-                const u32x4 w = {w0, w1, w0, w1};
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
-                for (int c = 0; c < NQ; ++c)
-                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, shared.q_sum[c][0][lane]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-            } else {
-                const u32x4 w = {own(0), own(1), own(2), own(3)};
-#pragma unroll
-                for (int c = 0; c < NQ; ++c) {
-                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, shared.q_sum[c][1][lane]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                    s[g][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, w), __builtin_bit_cast(half8, shared.q_sum[c][0][lane]), s[g][c], 0, 0, 0);
-                }
-            }
-        }
+            for (int c = 0; c < NQ; ++c) s[g][c] = f32x4{0.f, 0.f, 0.f, 0.f};
         // A step is a block of kStep groups of tokens.  Behind each of its products goes a piece of the next step's codes or of the
         // previous step's sums, so that the matrix cores and the vector unit work at once; the barriers keep that order.
         constexpr int kStep = NQ == 1 ? 4 : 2, kSteps = B * 4 / kStep;
@@ -543,9 +516,10 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
             f32x4 acc[2][kStep][NQ];
             u32x2 d[2][kStep];
             half8 qh[NQ], ql[NQ];
+            f32x4 less[NQ];      // what the codes' 8 takes off a block's sum
             const auto code = [&](int step, int g) {
-                const uint32_t w = k_raw[step % (4 / kStep) * kStep + g][step / (4 / kStep)], w8 = w >> 8;
-                codes[step & 1][g] = __builtin_bit_cast(half8, u32x4{w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u});
+                const uint32_t w = k_raw[step % (4 / kStep) * kStep + g][step / (4 / kStep)], m = 0x00f000f0u;
+                codes[step & 1][g] = __builtin_bit_cast(half8, u32x4{(w << 4) & m, w & m, (w >> 4) & m, (w >> 8) & m});
             };
             const auto add = [&](int step, int g, int c) {
                 f32x4 &to = s[step % (4 / kStep) * kStep + g][c];
@@ -560,6 +534,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                     for (int c = 0; c < NQ; ++c) {
                         qh[c] = __builtin_bit_cast(half8, shared.q[b][c][0][lane]);
                         ql[c] = __builtin_bit_cast(half8, shared.q[b][c][1][lane]);
+                        less[c] = shared.q_sum[b][c][col];
                     }
                 }
 #pragma unroll
@@ -575,7 +550,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                 for (int i = 0; i < kProducts; ++i) {
                     const int half = i / (kStep * NQ), g = i % (kStep * NQ) / NQ, c = i % NQ;
                     f32x4 &to = acc[step & 1][g][c];
-                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes[step & 1][g], half ? qh[c] : ql[c], half ? to : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes[step & 1][g], half ? qh[c] : ql[c], half ? to : less[c], 0, 0, 0);
 #pragma unroll
                     for (int x = i * kPieces / kProducts; x < (i + 1) * kPieces / kProducts; ++x) {
                         if (x < kStep) {
@@ -689,7 +664,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
             // unit u: register u % 4 of half u / 4 % 2 of 16 dimensions u / 8
             const auto lift = [&](int step, int u) {
                 const uint32_t w = (uint32_t)raw[step & 1][u / 8][u / 4 % 2];
-                big[u] = ((u & 2) ? w >> 8 : w) & ((u & 1) ? mask1 : mask0) | magic;         // 1024 + n, or 1024 + 16 n
+                big[u] = (((u & 2) ? w >> 8 : w) & ((u & 1) ? mask1 : mask0)) | magic;         // 1024 + n, or 1024 + 16 n
             };
             const auto center = [&](int u) {
                 const half2v b = __builtin_bit_cast(half2v, big[u]);

@@ -65,16 +65,17 @@ def decode(n, scales):
         return (n.astype(np.float64) - 8) * np.repeat(scales.astype(np.float64), 32, axis=-1)
 
 
-def attention(cache, q, q_start, kv_len, pages, scale, window=0, n_pages=None):
+def attention(cache, q, q_start, kv_len, pages, scale, window=0, dtype=np.float64):
     """cache: (k_codes, k_scales, v_codes, v_scales) as numpy arrays.  Returns (y, (weight, steep, spread)): y [tokens, heads, dim] with NaN in
     rows of no sequence, and for error bounds sum_t p_t |v_t| and, of a row, the largest of a token's sums over d of
-    scale * |q_d| * 8 * (the scale of the key's block), which the products with its codes stay under, and sum_t |v_t|."""
+    scale * |q_d| * 8 * (the scale of the key's block), which the products with its codes stay under, and sum_t |v_t|.  In
+    another `dtype` the same statement with every number of that type."""
     k_codes, k_scales, v_codes, v_scales = cache
     page = k_codes.shape[2]
     heads_kv, dim = k_codes.shape[1], 2 * k_codes.shape[3]
-    q = np.asarray(q, dtype=np.float64)
+    q, scale = np.asarray(q, dtype=dtype), dtype(scale)
     group = q.shape[1] // heads_kv
-    y = np.full(q.shape, np.nan)
+    y = np.full(q.shape, np.nan, dtype=dtype)
     weight, steep, spread = np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape)
     for s in range(len(kv_len)):
         t = np.arange(int(kv_len[s]))
@@ -82,8 +83,8 @@ def attention(cache, q, q_start, kv_len, pages, scale, window=0, n_pages=None):
         good = (where >= 0) & (where < k_codes.shape[0])
         t, where = t[good], where[good]
         at = t % page
-        k = decode(unpack_keys(k_codes[where, :, at]), k_scales[where, :, at])
-        v = decode(unpack_values(v_codes[where, :, at]), v_scales[where, :, at])
+        k = decode(unpack_keys(k_codes[where, :, at]), k_scales[where, :, at]).astype(dtype)
+        v = decode(unpack_values(v_codes[where, :, at]), v_scales[where, :, at]).astype(dtype)
         most = 8 * np.repeat(np.abs(k_scales[where, :, at].astype(np.float64)), 32, axis=-1)
         for r in range(q_start[s], q_start[s + 1]):
             p = int(kv_len[s]) - (q_start[s + 1] - r)
