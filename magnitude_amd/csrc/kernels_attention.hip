@@ -13,11 +13,11 @@
 // A tile.  v_mfma_f32_16x16x32_f16 with tokens (then dimensions) as rows and queries as columns, so that a lane's column is
 // one query throughout: row statistics are a lane's own, and the probabilities come out of the first product in the
 // order in which the second takes them.
-//   scores   acc = sum over a block of 32 of n * q, in fp32; S += d_k * acc.  The codes n (0..15) go into the matrix cores as
-//            subnormal halves: a nibble in bits 4..7 is n * 2^-20 as it stands, so a word of eight codes costs three shifts and
-//            four ands.  (The matrix cores line products up by their factors' exponents, a subnormal's being 2^-14, and drop what is
-//            24 bits below the largest: nibbles left in bits 0..3 saved two of the shifts and cost four bits, an error of 1.5e-5 of
-//            the result.)  -8 * sum(q) of a block is what its products begin with.
+//   scores   acc = sum over a block of 32 of (n - 8) * q, in fp32; S += d_k * acc.  A word of eight codes becomes halves in a shift,
+//            four and-ors (1024 + n, or 1024 + 16 n for a nibble in bits 4..7) and four subtractions or fmas.  (Left as the subnormals
+//            that nibbles are as they stand, with 8 sum(q) taken off apart, they cost half of that, and 1 to 2% of the time less:
+//            but the matrix cores line products up by their factors' exponents, a subnormal's being 2^-14, and drop what lies 24 bits
+//            below the largest.  Results were off by 1.5e-5 of their size, now by 3e-7.)
 //            q is scaled by a power of two of its row and split into two halves: 22 bits, two products.
 //   values   codes become n - 8 (1024 + n as half bits, less 1032), times the block's d: product and remainder of one
 //            multiplication are two halves that hold it exactly (4 x 11 bits), the largest d of a tile brought to 2^11..2^12 by a power
@@ -228,7 +228,6 @@ struct SharedLds {
         } meet;
     };
     u32x4 q[D / 32][NQ][2][64];   // the item's queries as the matrix cores take them: high halves, low halves
-    f32x4 q_sum[D / 32][NQ][16];                // -8 * sum(q) of every block, once for each of a lane's four tokens
     float q_unit[NQ][64];         // scores are sums times this
     int32_t line[kThreads][2];    // a thread's items on a head's line: turns before them, theirs
     int32_t waves[kWaves][3];     // a wave's: turns, items, the longest
@@ -287,23 +286,19 @@ __device__ __forceinline__ void stage_queries(const AttentionArgs &a, const Item
         most = max_xor(whole ? most : INFINITY);
         // (frexp: most = f * 2^e with f in [0.5, 1); where a value is not finite the row stays as it is: NaN comes of it)
         const int e = most > 0.f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
-        if (wave == 0) lds.q_unit[g][lane] = ldexpf(1.f, min(e - 15 + 20, 127));
+        if (wave == 0) lds.q_unit[g][lane] = ldexpf(1.f, e - 15);
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             if (b % kWaves != wave) continue;
-            float sum = 0.f;
             u32x4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float u = ldexpf(x[b][0][i], 15 - e), v = ldexpf(x[b][1][i], 15 - e);
                 hi[i] = half_pair(u, v);
                 lo[i] = half_pair(u - low_half(hi[i]), v - high_half(hi[i]));
-                sum += (low_half(hi[i]) + low_half(lo[i])) + (high_half(hi[i]) + high_half(lo[i]));
             }
             lds.q[b][g][0][lane] = hi;
             lds.q[b][g][1][lane] = lo;
-            const float less = add_xor32(add_xor16(sum)) * (-8.f * 9.5367431640625e-7f);
-            if (lane < 16) lds.q_sum[b][g][lane] = f32x4{less, less, less, less};
         }
     }
 }
@@ -516,10 +511,14 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
             f32x4 acc[2][kStep][NQ];
             u32x2 d[2][kStep];
             half8 qh[NQ], ql[NQ];
-            f32x4 less[NQ];      // what the codes' 8 takes off a block's sum
             const auto code = [&](int step, int g) {
-                const uint32_t w = k_raw[step % (4 / kStep) * kStep + g][step / (4 / kStep)], m = 0x00f000f0u;
-                codes[step & 1][g] = __builtin_bit_cast(half8, u32x4{(w << 4) & m, w & m, (w >> 4) & m, (w >> 8) & m});
+                const uint32_t w = k_raw[step % (4 / kStep) * kStep + g][step / (4 / kStep)], w8 = w >> 8;
+                const half2v k1032 = {(_Float16)1032.f, (_Float16)1032.f}, k72 = {(_Float16)72.f, (_Float16)72.f}, k16th = {(_Float16)0.0625f, (_Float16)0.0625f};
+                const auto even = [&](uint32_t x) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (x & mask0) | magic) - k1032); };
+                const auto odd = [&](uint32_t x) {
+                    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, (x & mask1) | magic), k16th, -k72));
+                };
+                codes[step & 1][g] = __builtin_bit_cast(half8, u32x4{even(w), odd(w), even(w8), odd(w8)});
             };
             const auto add = [&](int step, int g, int c) {
                 f32x4 &to = s[step % (4 / kStep) * kStep + g][c];
@@ -534,7 +533,6 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                     for (int c = 0; c < NQ; ++c) {
                         qh[c] = __builtin_bit_cast(half8, shared.q[b][c][0][lane]);
                         ql[c] = __builtin_bit_cast(half8, shared.q[b][c][1][lane]);
-                        less[c] = shared.q_sum[b][c][col];
                     }
                 }
 #pragma unroll
@@ -550,7 +548,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                 for (int i = 0; i < kProducts; ++i) {
                     const int half = i / (kStep * NQ), g = i % (kStep * NQ) / NQ, c = i % NQ;
                     f32x4 &to = acc[step & 1][g][c];
-                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes[step & 1][g], half ? qh[c] : ql[c], half ? to : less[c], 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes[step & 1][g], half ? qh[c] : ql[c], half ? to : f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
                     for (int x = i * kPieces / kProducts; x < (i + 1) * kPieces / kProducts; ++x) {
                         if (x < kStep) {

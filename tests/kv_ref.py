@@ -109,12 +109,12 @@ def attention(cache, q, q_start, kv_len, pages, scale, window=0, dtype=np.float6
 
 def allowed(sizes, dim, tokens):
     """How far an fp32 result may be from the exact one.  A score is `dim` products of q, kept in 22 bits (a fp16
-    pair: off by 2^-22 of itself, or of the row's largest over 2^15), with codes of 0 to 15 and, taken off, with 8: three times
-    what steep sums at most.  Their fp32 sums round at most dim + 16 times: delta <= 3 * steep * (2^-21 + (dim + 16) * 2^-24).  A weight is
+    pair: off by 2^-22 of itself, or of the row's largest over 2^15), with codes of -8 to 7.  Their fp32 sums round at most
+    dim + 16 times: delta <= steep * (2^-21 + (dim + 16) * 2^-24).  A weight is
     then off by a factor of exp(2 delta) at most, by its own rounding to 22 bits, the exponential's (2 ulp) and the running sums'
     (a rounding every 16 tokens, and one a rescaling: fewer than tokens / 8 + 64).  A weight that is under 2^-26 of the row's largest
     is a multiple of 2^-37 of that, a value under 2^-25 of the largest near it a multiple of 2^-36 of that: what a dimension in which
     the heavy tokens have zeros is off by."""
     weight, steep, spread = sizes
-    delta = 3 * steep * (2.0 ** -21 + (dim + 16) * 2.0 ** -24)
+    delta = steep * (2.0 ** -21 + (dim + 16) * 2.0 ** -24)
     return weight * (np.expm1(2 * delta)[..., None] + (tokens / 8 + 64) * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -36 * spread.max(-1, keepdims=True) + 1e-37
