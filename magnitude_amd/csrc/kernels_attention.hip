@@ -872,18 +872,26 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
     __shared__ __align__(16) SharedLds<D, NQ> lds;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
     const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
-    // ---- the line of turns: a thread counts those of `per` items of one head ----
+    // a thread's `per` places of the line of one head's items, those that hold an item (a sequence has as many places as max_q allows)
+    const auto each_item = [&](auto &&f) {
+        for (int u = id * per; u < min(units, (id + 1) * per);) {
+            const int s = u / a.row_tiles, tile0 = u - s * a.row_tiles, tile1 = min(a.row_tiles, tile0 + min(units, (id + 1) * per) - u);
+            bool bad;
+            const Sequence q = sequence(a, s, bad);
+            if (bad && tile0 == 0 && blockIdx.x == 0) atomicOr(a.error, kKvBadRows);
+            for (int tile = tile0; tile < tile1 && tile * a.tokens < q.count; ++tile)
+                if (f(s, tile, q, item_turns(item_of(a, s, q, tile)))) return;
+            u += tile1 - tile0;
+        }
+    };
+    // ---- the line of turns ----
     int turns_mine = 0, items_mine = 0, longest = 0;
-    for (int u = id * per; u < min(units, (id + 1) * per); ++u) {
-        const int s = u / a.row_tiles;
-        bool bad;
-        const Sequence q = sequence(a, s, bad);
-        if (bad && u == s * a.row_tiles && blockIdx.x == 0) atomicOr(a.error, kKvBadRows);
-        const int n = item_turns(item_of(a, s, q, u - s * a.row_tiles));
+    each_item([&](int, int, const Sequence &, int n) {
         turns_mine += n;
-        items_mine += n > 0;
+        ++items_mine;
         longest = max(longest, n);
-    }
+        return false;
+    });
     int turns_before = wave_scan(turns_mine), items_before = wave_scan(items_mine);
     longest = (int)wave_max((uint32_t)longest);
     if (lane == 63) {
@@ -932,19 +940,17 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         const int before = lds.line[id][0], mine = lds.line[id][1];
         if (off >= before && off < before + mine) {     // one thread
             int b = before;
-            for (int u = id * per; u < min(units, (id + 1) * per); ++u) {
-                const int s = u / a.row_tiles;
-                bool bad;
-                const Sequence q = sequence(a, s, bad);
-                const int n = item_turns(item_of(a, s, q, u - s * a.row_tiles)), weight = n == 0 ? 0 : whole_items ? 1 : n + start;
-                if (off < b + weight) {
-                    const int found[7] = {s, u - s * a.row_tiles, b, n, q.start, q.count, q.len};
-#pragma unroll
-                    for (int i = 0; i < 7; ++i) lds.found[i] = found[i];
-                    break;
+            each_item([&](int s, int tile, const Sequence &q, int n) {
+                const int weight = whole_items ? 1 : n + start;
+                if (off >= b + weight) {
+                    b += weight;
+                    return false;
                 }
-                b += weight;
-            }
+                const int found[7] = {s, tile, b, n, q.start, q.count, q.len};
+#pragma unroll
+                for (int i = 0; i < 7; ++i) lds.found[i] = found[i];
+                return true;
+            });
         }
         __syncthreads();
         const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), first = uniform(lds.found[2]), turns = uniform(lds.found[3]);

@@ -13,12 +13,15 @@
 #include "kv_cache.h"
 #include "qproj_internal.h"
 
+#include <algorithm>
+
 namespace qproj {
 
 namespace {
 
 constexpr int kRopeThreads = 256;
 constexpr int kUnit = 8;   // values a thread takes
+constexpr int64_t kMostGrid = (int64_t)1 << 23;   // tokens of a launch: a grid has fewer than 2^32 threads in a direction
 
 struct RotateArgs {
     const int32_t *pos;
@@ -234,26 +237,42 @@ hipError_t launch_rope_kv(const RopeKvJob &j, hipStream_t s) {
     }
     if (j.kv && a.q_units % 4) return hipErrorInvalidValue;   // a block of the cache is four lanes of a quad
     const int units = a.q_units + 2 * a.kv_units;
-    const dim3 grid((unsigned)j.n_tokens, (unsigned)((units + kRopeThreads - 1) / kRopeThreads));
-    if (dry_run()) {
-        plan_note("rope_kv_kernel: %lld tokens, %d units of queries + 2 x %d of keys and values, grid %u x %u x %d", (long long)j.n_tokens, a.q_units,
-                  a.kv_units, grid.x, grid.y, kRopeThreads);
-        return hipSuccess;
+    for (int64_t left = j.n_tokens; left > 0; left -= kMostGrid) {
+        const dim3 grid((unsigned)std::min(left, kMostGrid), (unsigned)((units + kRopeThreads - 1) / kRopeThreads));
+        if (dry_run()) {
+            plan_note("rope_kv_kernel: %u tokens, %d units of queries + 2 x %d of keys and values, grid %u x %u x %d", grid.x, a.q_units, a.kv_units, grid.x,
+                      grid.y, kRopeThreads);
+        } else {
+            hipLaunchKernelGGL(rope_kv_kernel, grid, dim3(kRopeThreads), (size_t)a.r.half * sizeof(double2), s, a);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        a.r.pos += a.r.half ? kMostGrid : 0;
+        a.q += kMostGrid * (a.q ? a.q_stride : 0);
+        a.q_out += kMostGrid * (a.q ? a.q_out_stride : 0);
+        a.k += kMostGrid * (a.k ? a.k_stride : 0);
+        a.v += kMostGrid * (a.v ? a.v_stride : 0);
+        a.slots += a.slots ? kMostGrid : 0;
     }
-    hipLaunchKernelGGL(rope_kv_kernel, grid, dim3(kRopeThreads), (size_t)a.r.half * sizeof(double2), s, a);
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 hipError_t launch_kv_read(const KvView &kv, const int64_t *slots, int64_t n, float *k_out, float *v_out, int32_t *error, hipStream_t s) {
     if (n == 0) return hipSuccess;
     const int units = kv.n_head * kv.dim / kUnit;
-    const dim3 grid((unsigned)n, (unsigned)((2 * units + kRopeThreads - 1) / kRopeThreads));
-    if (dry_run()) {
-        plan_note("kv_read_kernel: %lld places, 2 x %d units, grid %u x %u x %d", (long long)n, units, grid.x, grid.y, kRopeThreads);
-        return hipSuccess;
+    const int64_t row = (int64_t)kv.n_head * kv.dim;
+    for (int64_t at = 0; at < n; at += kMostGrid) {
+        const dim3 grid((unsigned)std::min(n - at, kMostGrid), (unsigned)((2 * units + kRopeThreads - 1) / kRopeThreads));
+        if (dry_run()) {
+            plan_note("kv_read_kernel: %u places, 2 x %d units, grid %u x %u x %d", grid.x, units, grid.x, grid.y, kRopeThreads);
+            continue;
+        }
+        hipLaunchKernelGGL(kv_read_kernel, grid, dim3(kRopeThreads), 0, s, kv, slots + at, k_out ? k_out + at * row : nullptr,
+                           v_out ? v_out + at * row : nullptr, units, error);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(kv_read_kernel, grid, dim3(kRopeThreads), 0, s, kv, slots, k_out, v_out, units, error);
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 }  // namespace qproj

@@ -1793,15 +1793,18 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
     if (!ctx) return QPROJ_ERR_INVALID_ARG;
     KvView view;
     if (const char *why = bad_cache(kv, &view)) return refuse(ctx, call, why);
-    if (!q_start_dev || !kv_len_dev || !pages_dev) return refuse(ctx, call, "null argument");
+    if (!q_start_dev || (!kv_len_dev && n_seq) || (!pages_dev && n_seq && pages_stride)) return refuse(ctx, call, "null argument");
     if (n_tokens < 0 || n_tokens > kMostTokens || n_seq < 0 || n_seq > 65536 || max_q < 0 || pages_stride < 0)
         return refuse(ctx, call, "n_tokens, n_seq, max_q or pages_stride out of range");
     if (pages_stride * kv->page_tokens > 0x7fffffff) return refuse(ctx, call, "a sequence must stay under 2^31 tokens");
     if (n_head <= 0 || n_head > kMostHeads || n_head % kv->n_head_kv != 0) return refuse(ctx, call, "n_head must be a multiple of n_head_kv");
     if (window < 0) return refuse(ctx, call, "negative window");
-    // (the device counts tiles of 64 tokens, of all heads, in 32 bits)
-    const double rows = (double)n_seq * ((double)std::min(max_q, n_tokens) * n_head / 16 + n_head);
-    if (rows * ((double)pages_stride * kv->page_tokens / 64 + 1) > 2e9) return refuse(ctx, call, "n_seq * max_q * pages_stride too large: give max_q, or make several calls");
+    // The device numbers places for rows of a head, and turns of four tiles of 64 tokens of all heads, in 32 bits.  A sequence's rows of a
+    // key/value head are at most rows * group / 16 + 1 items, an item's turns a quarter of its tiles, one for the rest and two for its start.
+    const double most_q = (double)std::min(max_q, n_tokens);
+    const double items = std::min((double)n_seq * most_q, (double)n_tokens) * n_head / 16 + (double)n_seq * n_head;
+    if ((double)n_seq * (most_q + 1) > 2e9 || items * ((double)pages_stride * kv->page_tokens / 256 + 4) > 2e9)
+        return refuse(ctx, call, "too many rows times tokens (or n_seq times max_q) for one call");
     if (const char *why = bad_rows(q_dev, q_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
     if (const char *why = bad_rows(y_dev, y_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
     if (q_dev == y_dev) return refuse(ctx, call, "y must not be q");

@@ -612,6 +612,8 @@ class Context:
     def _rotation(self, pos: torch.Tensor, freqs: torch.Tensor, mode: str, magnitude: float, tokens: int) -> Rotation:
         if pos.numel() != tokens:
             raise ValueError("one position a token")
+        if mode not in ROPE_MODES:
+            raise ValueError(f"unknown rotation mode {mode!r}")
         return Rotation(self._on_device(pos, torch.int32, "pos"), self._on_device(freqs, torch.float64, "freqs"),
                         2 * freqs.numel(), ROPE_MODES[mode], magnitude)
 

@@ -136,20 +136,30 @@ def test_calls_that_are_taken_note_their_launches():
     assert dry.plan.count("rope_kv_kernel:") == 3 and dry.plan.count("kv_read_kernel:") == 2 and dry.plan.count("attention_kernel<") == 21
 
 
+def test_long_calls_become_launches_that_fit():
+    with Dry() as dry:
+        assert call(dry, "rope", rot=rotation(), n=(1 << 24) + 1) == 0
+        assert call(dry, "read", cache(), n=(1 << 23) + 1) == 0
+        # 64 sequences of 131072 tokens, one of them a prompt of 8192, and a token of a million
+        assert call(dry, "attention", cache(n_pages=1 << 20), n=8192 + 63, seqs=64, max_q=8192, ps=2048) == 0
+        assert call(dry, "attention", cache(n_pages=1 << 20), n=1, seqs=1, max_q=1, ps=1 << 14) == 0
+    assert dry.plan.count("rope_kv_kernel: 8388608 tokens") == 2 and dry.plan.count("rope_kv_kernel: 1 tokens") == 1
+    assert dry.plan.count("kv_read_kernel: 8388608 places") == 1 and dry.plan.count("kv_read_kernel: 1 places") == 1
+
 
 ROPE_BAD = [dict(x=None), dict(y=None), dict(x=BUF + 4), dict(y=BUF + 8), dict(xs=4092), dict(xs=4098), dict(ys=100), dict(n=-1), dict(n=1 << 31),
             dict(h=0), dict(h=5000, xs=1 << 20, ys=1 << 20), dict(d=0), dict(d=100), dict(d=2048, xs=1 << 17, ys=1 << 17),
             dict(x=BUF, y=BUF, xs=4096, ys=8192)]
 ROTATION_BAD = [dict(pos_dev=None), dict(freqs_dev=None), dict(n_dims=0), dict(n_dims=12), dict(n_dims=136), dict(n_dims=-8), dict(mode=2)]
 CACHE_BAD = [dict(k_codes=None), dict(v_scales=None), dict(k_scales=BUF + 2), dict(v_codes=BUF + 8), dict(n_pages=0), dict(n_pages=1 << 31),
-             dict(page_tokens=8), dict(page_tokens=48), dict(page_tokens=512), dict(page_tokens=0), dict(n_head_kv=0), dict(n_head_kv=-1),
+             dict(n_pages=1 << 23), dict(page_tokens=8), dict(page_tokens=48), dict(page_tokens=512), dict(page_tokens=0), dict(n_head_kv=0), dict(n_head_kv=-1),
              dict(head_dim=80), dict(head_dim=512), dict(head_dim=0)]
 APPEND_BAD = [dict(k=None), dict(v=None), dict(slots=None), dict(k=BUF + 4), dict(ks=1020), dict(vs=1026), dict(n=-1),
               dict(q=BUF, qs=4096, h=32, qo=None, qos=4096), dict(q=BUF, qs=4000, h=32, qo=BUF, qos=4096), dict(q=BUF, qs=4096, h=0, qo=BUF, qos=4096),
               dict(q=BUF, qs=4096, h=32, qo=BUF, qos=8192)]
 ATTENTION_BAD = [dict(q=None), dict(y=None), dict(start=None), dict(len=None), dict(pages=None), dict(q=BUF + 4), dict(y=BUF + 8), dict(qs=4092), dict(ys=4094),
                  dict(h=33), dict(h=0), dict(h=-8), dict(seqs=-1), dict(seqs=65537), dict(max_q=-1), dict(n=-1), dict(ps=-1), dict(ps=1 << 26), dict(window=-1),
-                 dict(y=BUF)]
+                 dict(y=BUF), dict(n=1 << 30, max_q=1 << 30, seqs=1, ps=1 << 20), dict(n=1 << 20, max_q=1 << 20, seqs=65536)]
 
 
 @pytest.mark.parametrize("name,bad", [("rope", b) for b in ROPE_BAD] + [("append", b) for b in APPEND_BAD] + [("attention", b) for b in ATTENTION_BAD] +

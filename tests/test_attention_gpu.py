@@ -252,6 +252,25 @@ ATTENTION = [  # dim, page, kv heads, group, [(tokens in the cache, new ones)], 
     (128, 16, 1, 4, [(400, 100), (90, 90)], 1),
     (128, 16, 1, 4, [(400, 30)], 64),
     (128, 64, 8, 1, [(9000, 1), (100, 1), (4097, 1)], 0),
+    # far more items than workgroups, all short: dealt out whole, several rounds
+    (64, 16, 8, 1, [(1 + 37 * i % 301, 1) for i in range(300)], 0),
+    (96, 32, 4, 4, [(64 + 11 * i % 190, 64) for i in range(20)], 0),
+    (256, 16, 4, 2, [(1 + 13 * i % 97, 1) for i in range(150)], 0),
+    # more items than can stay whole, one of them long: cut, also inside what an item's start counts for
+    (64, 64, 4, 4, [(3000, 1)] + [(1 + 29 * i % 257, 1) for i in range(200)], 0),
+    (128, 64, 4, 4, [(2000, 130)] + [(1 + 29 * i % 257, 1) for i in range(60)], 0),
+    # a few parts an item, added by the last of its workgroups, and many, which a launch of its own adds
+    (128, 64, 8, 4, [(1 + 700 * i, 1) for i in range(8)], 0),
+    (96, 128, 2, 3, [(6000, 1), (5, 1), (2000, 1)], 0),
+    (256, 64, 2, 4, [(5000, 20)], 0),
+    (256, 64, 1, 4, [(20000, 1)], 0),
+    (64, 256, 1, 8, [(30000, 3)], 0),
+    (96, 256, 1, 1, [(20000, 1)], 5000),
+    (64, 64, 2, 8, [(3000, 64)], 0),
+    # a prompt among tokens, and no max_q: mostly places without an item
+    (64, 64, 2, 4, [(50 + i, 1) for i in range(30)] + [(400, 300)] + [(0, 0)] * 5 + [(90 + i, 1) for i in range(10)], 0),
+    # the last page full to its end
+    (128, 16, 2, 4, [(256, 1), (64, 2)], 0),
 ]
 
 
@@ -518,6 +537,128 @@ def test_captured_steps(ctx):
     own.close()
 
 
+@pytest.mark.parametrize("seqs,group", [(1, 4), (1, 32), (24, 4)])     # joined by a launch of their own, of two columns, by the last workgroup
+def test_captured_attention_follows_the_lengths(seqs, group):
+    """recorded once, replayed with lengths from nothing to full pages: items cut into one part, a few and many"""
+    from magnitude_amd import Context
+    stream = torch.cuda.Stream()
+    own, other = Context(0, stream=stream.cuda_stream), Context(0)
+    rng = np.random.default_rng(15)
+    page, dim, most = 256, 128, 5000
+    kv, pages = make_cache(rng, [most] * seqs, page, 1, dim)
+    q, y = dev(rng.standard_normal((seqs, group, dim)).astype(np.float32)), torch.zeros((seqs, group, dim), device="cuda")
+    start, lens, p = dev(np.arange(seqs + 1, dtype=np.int32)), torch.full((seqs,), most, dtype=torch.int32, device="cuda"), dev(pages)
+    own.attention(kv, q, start, lens, p, max_q=1, out=y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        own.attention(kv, q, start, lens, p, max_q=1, out=y, sync=False)
+    for i in range(12):
+        n = rng.integers(0, most + 1, seqs) if i % 3 else np.full(seqs, (0, 1, most, 300)[i // 3])
+        with torch.cuda.stream(stream):
+            lens.copy_(dev(n.astype(np.int32)))
+            y.fill_(7.5)
+            graph.replay()
+        stream.synchronize()
+        assert torch.equal(y, other.attention(kv, q, start, lens, p, max_q=1)), f"replay {i}"
+        if i % 2:       # the same context's own work between replays
+            own.attention(kv, q, start, lens, p, max_q=1)
+        if i == 4:
+            want, sizes = kv_ref.attention(numpy_cache(kv), q.cpu().numpy(), np.arange(seqs + 1), n, pages, dim ** -0.5)
+            assert (np.abs(y.cpu().numpy() - want) <= kv_ref.allowed(sizes, dim, most)).all()
+    own.close()
+    other.close()
+
+
+def test_the_first_call_of_a_context_is_not_captured():
+    from magnitude_amd import Context, KvCache, QprojError
+    stream = torch.cuda.Stream()
+    own = Context(0, stream=stream.cuda_stream)
+    kv = KvCache.zeros(2, 16, 1, 64)
+    q, y, spare = (torch.zeros((1, 4, 64), device="cuda") for _ in range(3))
+    args = dev(np.array([0, 1], np.int32)), dev(np.array([3], np.int32)), dev(np.array([[1]], np.int32))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        spare.add_(1)
+        with pytest.raises(QprojError, match="captured"):
+            own.attention(kv, q, *args, out=y, sync=False)
+    graph.replay()                       # what was recorded beside stays whole
+    torch.cuda.synchronize()
+    assert (spare == 1).all()
+    own.attention(kv, q, *args, out=y)   # and the context does too
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        own.attention(kv, q, *args, out=y, sync=False)
+    y.fill_(7.5)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not y.any()
+    own.close()
+
+
+def test_two_contexts_at_once():
+    """calls of two contexts on streams of their own, one cut into few parts and one into many, do not meet"""
+    from magnitude_amd import Context
+    rng = np.random.default_rng(16)
+    work = []
+    for lens, kv_heads in (([9000], 1), ([3000, 10, 700, 2000], 8)):
+        stream = torch.cuda.Stream()
+        kv, pages = make_cache(rng, lens, 64, kv_heads, 128)
+        q = dev(rng.standard_normal((len(lens), 4 * kv_heads, 128)).astype(np.float32))
+        args = kv, q, dev(np.arange(len(lens) + 1, dtype=np.int32)), dev(np.array(lens, np.int32)), dev(pages)
+        c = Context(0, stream=stream.cuda_stream)
+        work.append((c, args, c.attention(*args, max_q=1), [torch.zeros_like(q) for _ in range(20)]))
+    torch.cuda.synchronize()
+    for i in range(20):
+        for c, args, _, outs in work:
+            c.attention(*args, max_q=1, out=outs[i], sync=False)
+    for c, _, want, outs in work:
+        c.sync()
+        assert all(torch.equal(o, want) for o in outs)
+        c.close()
+
+
+def test_nothing_to_do(ctx):
+    kv, pages = make_cache(np.random.default_rng(17), [30], 16, 2, 64)
+    none = torch.zeros((0, 2, 64), device="cuda")
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    assert ctx.attention(kv, none, i32(0, 0), i32(30), dev(pages)).shape == (0, 2, 64)
+    y = torch.full((3, 2, 64), 7.5, device="cuda")
+    q = torch.zeros_like(y)
+    ctx.attention(kv, q, i32(0), i32(), dev(pages)[:0], out=y)                       # no sequence
+    assert (y == 7.5).all()
+    ctx.attention(kv, q, i32(0, 3), i32(0), dev(pages)[:, :0].contiguous(), out=y)   # no page, no token: rows of zeros
+    assert not y.any()
+    before = numpy_cache(kv)
+    ctx.kv_append(kv, none, none, torch.zeros(0, dtype=torch.int64, device="cuda"))
+    ctx.kv_append(kv, q, q, torch.full((3,), -1, dtype=torch.int64, device="cuda"))
+    assert all(np.array_equal(a, b) for a, b in zip(before, numpy_cache(kv)))
+
+
+def test_more_tokens_than_a_launch_has_workgroups(ctx):
+    from magnitude_amd import KvCache, rope_frequencies
+    n = (1 << 23) + 5
+    tell("rope of", n, "tokens")
+    x = torch.randn((n, 1, 8), device="cuda")
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    freqs = rope_frequencies(8)[0]
+    y = ctx.rope(x, pos, dev(freqs))
+    pick = np.r_[0:3, (1 << 23) - 3:n]
+    want = kv_ref.rotate(x[pick].cpu().numpy(), pick, freqs, "pairs", 1.0)
+    np.testing.assert_allclose(y[pick].cpu().numpy(), want, rtol=0, atol=2.0 ** -22 * np.abs(x[pick].cpu().numpy()).max())
+    tell("kv_append and kv_read of", n, "tokens")
+    kv = KvCache.zeros(n // 256 + 1, 256, 1, 64)
+    rows = torch.randn((n, 1, 64), device="cuda")
+    slots = torch.arange(n - 1, -1, -1, device="cuda")
+    ctx.kv_append(kv, rows, rows, slots)
+    k, v = ctx.kv_read(kv, slots)
+    assert torch.equal(k, v)
+    some = rows[pick]
+    small = KvCache.zeros(1, 16, 1, 64)
+    ctx.kv_append(small, some, some, torch.arange(len(pick), device="cuda"))
+    assert torch.equal(k[pick], ctx.kv_read(small, torch.arange(len(pick), device="cuda"))[0])
+
+
 def test_a_call_that_does_not_fit_its_tensors_is_refused(ctx):
     from magnitude_amd import KvCache, rope_frequencies
     kv = KvCache.zeros(4, 16, 2, 64)
@@ -537,7 +678,7 @@ def test_a_call_that_does_not_fit_its_tensors_is_refused(ctx):
     for i, f in enumerate(bad):
         with pytest.raises(ValueError):
             f()
-    with pytest.raises(KeyError):
+    with pytest.raises(ValueError):
         ctx.rope(x, pos, freqs, mode="neox")
     from magnitude_amd import QprojError
     with pytest.raises(QprojError):
