@@ -7,7 +7,8 @@ every step streams from HBM, not from the 256 MB Infinity Cache): per layer q/k/
 o, gate/up (one launch) in Q4_K and down in Q6_K, each preceded by the activation quantizer, in
 the ggml activation mode (the reference CPU path's arithmetic).  `value` is algorithmic GGUF bytes
 per step / time.  Extra legs report the dominant kernel against the HBM roofline, the int8-MFMA
-prefill GEMM (config 4), the MoE feed-forward (config 5) and the CPU oracle on the host cores.
+prefill GEMM (config 4), the MoE feed-forward (config 5) and the CPU oracle on the host cores; `attention`, which
+runs only when named, puts rotation, cache and attention between the projections.
 
     python bench.py --gpus 1 --steps 20 --warmup 3 [--legs step,roofline,verify,q8_0,prefill,moe,llama_bench,cpu]
 """
@@ -26,6 +27,7 @@ HBM_PEAK_GBS = 8000.0
 INT8_PEAK_TOPS = 5000.0
 Q4_K, Q6_K, Q8_0 = 12, 14, 8
 D_MODEL, D_KV, D_FF = 4096, 1024, 14336
+HEAD_DIM = 128
 
 
 def log(*a):
@@ -249,6 +251,9 @@ def compact_line(out, details_path=None):
         toks = {r["output"]["operation"].split(".")[1]: med(r["measurements"][1]["samples"]) for r in out["llama_bench"]}
         line["llama_bench_projections_only"] = {"pp512_tok_s": _r(toks.get("prompt-processing"), 0),
                                                 "tg128_tok_s": _r(toks.get("token-generation"), 1)}
+    if "attention" in out:
+        line["append_attention_us"] = {f"M{r['M']}_T{r['tokens']}": [_r(r["append_attention_us"], 1), _r(r["layer_us"], 1)]
+                                       for r in out["attention"]["rows"]}
     if details_path:
         line["details"] = details_path
     text = json.dumps(line, separators=(",", ":"))
@@ -318,7 +323,7 @@ def main():
     # ------------------------------------------------------------------ weights
     L = args.layers
     layers = []
-    need_layers = bool(legs & {"step", "roofline", "verify", "cpu", "llama_bench", "norm"})
+    need_layers = bool(legs & {"step", "roofline", "verify", "cpu", "llama_bench", "norm", "attention"})
     if need_layers:
         t0 = time.time()
         for l in range(L):
@@ -608,6 +613,70 @@ def main():
             log(f"[bench] norm + gate/up, M={m}: separate calls {row['separate_us']:.1f} us, one call {row['fused_us']:.1f} us per layer; "
                 f"with swiglu in the same call {row['fused_swiglu_us']:.1f} us")
         out["norm"] = res
+
+    # ------------------------------------------------------------------ attention leg (not among the default ones)
+    if "attention" in legs:
+        # What lies between the projections, and with it a layer as a decoder runs it: norm + q/k/v, rotation of q and k with
+        # the append to a 4-bit cache, attention, o, norm + gate/up + swiglu, down (residual sums apart).  Every layer has
+        # a cache of its own; rows are the last tokens of one sequence.
+        from magnitude_amd import KvCache, rope_frequencies
+        heads, kv_heads, dim, page = D_MODEL // HEAD_DIM, D_KV // HEAD_DIM, HEAD_DIM, 64
+        freqs, magnitude = rope_frequencies(dim, base=500000.0)
+        freqs = torch.from_numpy(freqs).to(dev)
+        gamma = torch.ones(D_MODEL, device=dev)
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+        res = []
+        for m, tokens in ((1, 512), (1, 8192), (1, 131072), (512, 512)):
+            caches = []
+            for _ in layers:
+                c = KvCache.zeros(tokens // page, page, kv_heads, dim, device=dev)
+                for i, t in enumerate(c.tensors):
+                    t.copy_(torch.rand(t.shape, generator=g, device=dev).mul_(0.05) if i % 2 else
+                            torch.randint(0, 256, t.shape, generator=g, dtype=torch.uint8, device=dev))
+                caches.append(c)
+            pages = torch.randperm(tokens // page, generator=g, device=dev).to(torch.int32).view(1, -1)
+            t = torch.arange(tokens - m, tokens, device=dev)
+            slots = pages[0, t // page].long() * page + t % page
+            pos, start, lens = t.to(torch.int32), i32([0, m]), i32([tokens])
+            xin = torch.randn((m, D_MODEL), generator=g, device=dev)
+            q, k, v, o = (torch.empty((m, n), device=dev) for n in (D_MODEL, D_KV, D_KV, D_MODEL))
+            qr, at = (torch.empty((m, heads, dim), device=dev) for _ in range(2))
+            h, d = torch.empty((m, D_FF), device=dev), torch.empty((m, D_MODEL), device=dev)
+            torch.cuda.synchronize()
+
+            def between(c):
+                ctx.kv_append(c, k.view(m, kv_heads, dim), v.view(m, kv_heads, dim), slots, pos=pos, freqs=freqs, magnitude=magnitude,
+                              q=q.view(m, heads, dim), q_out=qr, sync=False)
+                ctx.attention(c, qr, start, lens, pages, max_q=m, out=at, sync=False)
+
+            def around(lw, c=None):
+                ctx.rms_norm_mul_mat([lw["q"], lw["k"], lw["v"]], xin, gamma, 1e-5, ACT_GGML, outs=[q, k, v], sync=False)
+                if c is not None:
+                    between(c)
+                ctx.mul_mat_multi([lw["o"]], at.view(m, D_MODEL), ACT_GGML, outs=[o], sync=False)
+                ctx.ffn_gate_up(lw["gate"], lw["up"], o, ACT_GGML, gamma=gamma, eps=1e-5, out=h, sync=False)
+                ctx.mul_mat_multi([lw["down"]], h, ACT_GGML, outs=[d], sync=False)
+
+            row = {"M": m, "tokens": tokens}
+            at.zero_()
+            torch.cuda.synchronize()
+            for name, fn in (("layer_without_us", lambda: [around(lw) for lw in layers]), ("layer_us", lambda: [around(lw, c) for lw, c in zip(layers, caches)]),
+                             ("append_attention_us", lambda: [between(c) for c in caches])):
+                fn()
+                ctx.sync()
+                run = (None if args.no_graph else capture(torch, stream, fn)) or fn
+                for _ in range(MIN_WARMUP):
+                    run()
+                torch.cuda.synchronize()
+                st = summarize([s_ / L * 1e3 for s_ in timer.samples_ms(run, max(MIN_SAMPLES, args.steps))])
+                row[name], row["rel_mad_" + name] = st["median"], st["rel_mad"]
+            row["cache_bytes"] = tokens * kv_heads * dim * 9 // 8
+            row["GBps"] = row["cache_bytes"] / row["append_attention_us"] / 1e3
+            res.append(row)
+            log(f"[bench] attention M={m}, {tokens} tokens: append + attention {row['append_attention_us']:.1f} us, a layer "
+                f"{row['layer_us']:.1f} us (without them {row['layer_without_us']:.1f} us)")
+            del caches
+        out["attention"] = {"heads": heads, "heads_kv": kv_heads, "head_dim": dim, "cache": "4-bit, pages of 64", "rows": res}
 
     # ------------------------------------------------------------------ prefill leg (config 4)
     if "prefill" in legs:
