@@ -230,9 +230,10 @@ struct SharedLds {
     u32x4 q[D / 32][NQ][2][64];   // the item's queries as the matrix cores take them: high halves, low halves
     float q_unit[NQ][64];         // scores are sums times this
     int32_t line[kThreads][2];    // a thread's items on a head's line: turns before them, theirs
+    int32_t only[6][kThreads];    // where a thread has one place of the line: its item, as in `found`
     int32_t waves[kWaves][3];     // a wave's: turns, items, the longest
     int32_t last;                 // whether the workgroup wrote the last part of an item
-    int32_t found[8];             // sequence, row tile, turns before the item, its turns, and the sequence's first row, rows, tokens
+    int32_t found[8];             // sequence, row tile, its turns, the sequence's first row, rows, tokens, and what is before the item
 };
 
 // what a wave holds of an item
@@ -875,7 +876,7 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
     // a thread's `per` places of the line of one head's items, those that hold an item (a sequence has as many places as max_q allows)
     const auto each_item = [&](auto &&f) {
         for (int u = id * per; u < min(units, (id + 1) * per);) {
-            const int s = u / a.row_tiles, tile0 = u - s * a.row_tiles, tile1 = min(a.row_tiles, tile0 + min(units, (id + 1) * per) - u);
+            const int s = a.row_tiles == 1 ? u : u / a.row_tiles, tile0 = u - s * a.row_tiles, tile1 = min(a.row_tiles, tile0 + min(units, (id + 1) * per) - u);
             bool bad;
             const Sequence q = sequence(a, s, bad);
             if (bad && tile0 == 0 && blockIdx.x == 0) atomicOr(a.error, kKvBadRows);
@@ -886,7 +887,12 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
     };
     // ---- the line of turns ----
     int turns_mine = 0, items_mine = 0, longest = 0;
-    each_item([&](int, int, const Sequence &, int n) {
+    each_item([&](int s, int tile, const Sequence &q, int n) {
+        const int item[6] = {s, tile, n, q.start, q.count, q.len};
+        if (per == 1) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) lds.only[i][id] = item[i];
+        }
         turns_mine += n;
         ++items_mine;
         longest = max(longest, n);
@@ -940,24 +946,30 @@ __global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_ker
         const int before = lds.line[id][0], mine = lds.line[id][1];
         if (off >= before && off < before + mine) {     // one thread
             int b = before;
-            each_item([&](int s, int tile, const Sequence &q, int n) {
-                const int weight = whole_items ? 1 : n + start;
-                if (off >= b + weight) {
-                    b += weight;
-                    return false;
-                }
-                const int found[7] = {s, tile, b, n, q.start, q.count, q.len};
+            if (per == 1) {
 #pragma unroll
-                for (int i = 0; i < 7; ++i) lds.found[i] = found[i];
-                return true;
-            });
+                for (int i = 0; i < 6; ++i) lds.found[i] = lds.only[i][id];
+            } else {
+                each_item([&](int s, int tile, const Sequence &q, int n) {
+                    const int weight = whole_items ? 1 : n + start;
+                    if (off >= b + weight) {
+                        b += weight;
+                        return false;
+                    }
+                    const int item[6] = {s, tile, n, q.start, q.count, q.len};
+#pragma unroll
+                    for (int i = 0; i < 6; ++i) lds.found[i] = item[i];
+                    return true;
+                });
+            }
+            lds.found[6] = b;
         }
         __syncthreads();
-        const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), first = uniform(lds.found[2]), turns = uniform(lds.found[3]);
-        const Sequence q = {uniform(lds.found[4]), uniform(lds.found[5]), uniform(lds.found[6])};
+        const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), turns = uniform(lds.found[2]), first = uniform(lds.found[6]);
+        const Sequence q = {uniform(lds.found[3]), uniform(lds.found[4]), uniform(lds.found[5])};
         const Item it = item_of(a, seq, q, row_tile);
         const AttentionArgs &a = fresh_arguments();
-        const int kv_head = hv / a.splits, go = hv - kv_head * a.splits;
+        const int kv_head = a.splits == 1 ? hv : hv / a.splits, go = hv - kv_head * a.splits;
         const int head0 = kv_head * a.group + go * a.split, heads = min(a.split, a.group - go * a.split);
         // the stretch's turns of the item: none where it ends within the item's start
         const int skip = off - first, take = (int)std::min<uint32_t>(turns + start - skip, end - at);
