@@ -68,6 +68,7 @@ struct AttentionArgs {
     int32_t splits, split;   // they are served `split` at a time, in `splits` goes
     int32_t tokens;          // new tokens of an item
     int32_t row_tiles;       // items of a sequence, at most
+    int32_t cus;             // workgroups from this one on share a compute unit with an earlier one
 };
 
 // The kernel's arguments, loaded where they are used from here on.  Kept in registers from the start they are more scalars than there are, and
@@ -86,6 +87,8 @@ __device__ __forceinline__ const AttentionArgs &fresh_arguments() {
 
 constexpr int part_floats(int dim, int cols) { return 16 * cols * (dim + 2); }
 
+// (a third would fit where dim * cols <= 128, with the 168 registers that leaves: a token of 131072 took 59 us instead of 48, of 64-wide heads
+// 34 instead of 29; the vector units are busy with two)
 constexpr int waves_per_simd(int dim, int cols) { return dim * cols <= 256 ? 2 : 1; }
 
 struct Sequence {
@@ -413,6 +416,11 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         }
     };
     // (loads come back in order: pages, then queries, then keys and values)
+    // Of two waves of a SIMD the older one issues first whenever it can, and the younger one is left over: of 4096 prompt tokens the first
+    // 256 workgroups were done after 290 us, the others after 420.  So the younger ones go first every other tile; apart from that whoever
+    // multiplies values goes before whoever multiplies keys, which keeps the two in different phases, and what the waves meet for
+    // before everything.  (420 us became 400, 48 sequences 69 -> 65.)
+    __builtin_amdgcn_s_setprio(3);
     Queries<D, NQ> queries;
     load_queries<D, NQ>(a, it, head0, heads, queries, lane);
     if (work) {
@@ -446,9 +454,13 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     for (int g = 0; g < NQ; ++g) base[g] = -kBias;
 
     int buffer = 0;
+    const bool young = (int)blockIdx.x >= a.cus;
+    bool up = false;
     for (int tile = from; tile < to; tile += kWaves) {
         const int t0 = tile * kTile;
         const int bad_now = bad_groups;
+        up = young && !up;
+        if (up) __builtin_amdgcn_s_setprio(2); else __builtin_amdgcn_s_setprio(0);
         // ---- scales to LDS ----
         const int t = t0 + lane;
         const bool live = t >= it.see && t <= it.hi && !((bad_now >> part) & 1);
@@ -632,6 +644,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
                 }
             }
         }
+        if (!up) __builtin_amdgcn_s_setprio(1);
         // ---- values ----
         // The lane's dimension is lane % 16 of 16; its eight tokens of either half of the tile are those of its scores.  It names the
         // row that nibble lane % 16 of the result comes from: nibbles i and i + 4 of a word, which one and takes together, are neighbours.
@@ -714,6 +727,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
         wave_sync();
         if (kAhead) buffer ^= 1;
     }
+    __builtin_amdgcn_s_setprio(3);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the last codes asked for have to be in LDS before it is used for something else
     if (bad_page) atomicOr(a.error, kKvBadPage);
 #pragma unroll
@@ -1151,6 +1165,7 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     const int64_t most = ((j.pages_stride << j.kv->page_shift) + kTile - 1) / kTile + 1;
     const double turns = (double)most * a.n_seq * a.row_tiles * j.kv->n_head * a.splits / kWaves + (double)a.n_seq * a.row_tiles * j.kv->n_head * a.splits;
     const int groups = (int)std::min<double>(groups_most, turns);
+    a.cus = j.cus;
     a.parts = reinterpret_cast<float *>(j.scratch + arrived_bytes(j.cus) + joins_bytes(j.cus));
     // An item is cut into as many parts as there are workgroups for it, one or two more at its ends.  Up to eight, whoever writes the last part
     // adds them: one launch.  More are added by a kernel whose workgroups share the work: for a token of 131072 (64 parts) 52 us against 60.
