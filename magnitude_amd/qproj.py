@@ -264,7 +264,7 @@ class KvCache:
                 raise ValueError("codes are uint8 [n_pages, n_head_kv, page_tokens, head_dim / 2] and scales float16 "
                                  "[..., head_dim / 32], all on one device")
         self.tensors = (k_codes, k_scales, v_codes, v_scales)
-        self.device = k_codes.device
+        self.device, self.index = k_codes.device, k_codes.get_device()
         self._planes = KvPlanes(_ptr(k_codes), _ptr(k_scales), _ptr(v_codes), _ptr(v_scales), n_pages, page, n_head, 2 * half)
         self._ref = C.byref(self._planes)
 
@@ -287,6 +287,8 @@ class Context:
             raise QprojError(st, "qproj_ctx_create failed (is a gfx950 device visible?)")
         self.handle = h.value
         self.device = device
+        self._turn = Rotation()
+        self._turn_ref = C.byref(self._turn)
         self._held = []     # contiguous copies handed to launches that may still be pending (dropped in sync())
 
     def close(self) -> None:
@@ -582,9 +584,9 @@ class Context:
     # ---- between the q/k/v projections and the output projection ---------------------------
     def _on_device(self, t: torch.Tensor, dtype: torch.dtype, what: str) -> int:
         """Address of a contiguous tensor of this context's device."""
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise ValueError(f"{what} must be {dtype}")
-        if not t.is_cuda or t.get_device() != self.device:
+        if t.get_device() != self.device:       # (-1: on the host)
             raise ValueError(f"{what} must be on cuda:{self.device}")
         if not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous")
@@ -593,29 +595,35 @@ class Context:
     def _rows(self, t: torch.Tensor, what: str, heads: Optional[int] = None, dim: Optional[int] = None):
         """(address, floats from token to token) of rows of heads [tokens, heads, dim]: a token's row is dense, the tokens
         may lie apart (columns of a joined product)."""
-        if t.dim() != 3 or t.dtype != torch.float32:
+        shape = t.shape
+        if len(shape) != 3 or t.dtype is not torch.float32:
             raise ValueError(f"{what} must be float32 [tokens, heads, dim]")
-        n, h, d = t.shape
+        n, h, d = shape
         if (heads is not None and h != heads) or (dim is not None and d != dim):
             raise ValueError(f"{what} must be [tokens, {heads if heads is not None else 'heads'}, {dim}]")
-        if not t.is_cuda or t.get_device() != self.device:
+        if t.get_device() != self.device:
             raise ValueError(f"{what} must be on cuda:{self.device}")
+        if t.is_contiguous():
+            return t.data_ptr(), h * d
         if n and h and d and (t.stride(2) != 1 or (h > 1 and t.stride(1) != d) or (n > 1 and t.stride(0) < h * d)):
             raise ValueError(f"{what}: a token's heads must lie one after the other")
         return t.data_ptr(), t.stride(0) if n > 1 else h * d
 
     def _cache(self, kv: KvCache):
-        if kv.device.index != self.device:
+        if kv.index != self.device:
             raise ValueError(f"the cache must be on cuda:{self.device}")
         return kv._ref
 
-    def _rotation(self, pos: torch.Tensor, freqs: torch.Tensor, mode: str, magnitude: float, tokens: int) -> Rotation:
+    def _rotation(self, pos: torch.Tensor, freqs: torch.Tensor, mode: str, magnitude: float, tokens: int):
+        """Reference to the context's struct of a call's rotation (read by the call, not kept)."""
         if pos.numel() != tokens:
             raise ValueError("one position a token")
         if mode not in ROPE_MODES:
             raise ValueError(f"unknown rotation mode {mode!r}")
-        return Rotation(self._on_device(pos, torch.int32, "pos"), self._on_device(freqs, torch.float64, "freqs"),
-                        2 * freqs.numel(), ROPE_MODES[mode], magnitude)
+        r = self._turn
+        r.pos_dev, r.freqs_dev = self._on_device(pos, torch.int32, "pos"), self._on_device(freqs, torch.float64, "freqs")
+        r.n_dims, r.mode, r.magnitude = 2 * freqs.numel(), ROPE_MODES[mode], magnitude
+        return self._turn_ref
 
     def rope(self, x: torch.Tensor, pos: torch.Tensor, freqs: torch.Tensor, mode: str = "pairs", magnitude: float = 1.0,
              out: Optional[torch.Tensor] = None, sync: bool = True) -> torch.Tensor:
@@ -632,7 +640,7 @@ class Context:
             return y
         if sync:
             torch.cuda.current_stream(x.device).synchronize()
-        self._check(self.lib.qproj_rope(self.handle, C.byref(r), xp, xs, n, h, d, yp, ys))
+        self._check(self.lib.qproj_rope(self.handle, r, xp, xs, n, h, d, yp, ys))
         if sync:
             self.sync()
         return y
@@ -669,7 +677,7 @@ class Context:
             return q_out
         if sync:
             torch.cuda.current_stream(k.device).synchronize()
-        self._check(self.lib.qproj_kv_append(self.handle, self._cache(kv), kp, ks, vp, vs, n, sp, C.byref(r) if r is not None else None,
+        self._check(self.lib.qproj_kv_append(self.handle, self._cache(kv), kp, ks, vp, vs, n, sp, r,
                                              qp, qs, h, yp, ys))
         if sync:
             self.sync()
