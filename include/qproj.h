@@ -278,7 +278,8 @@ int qproj_rope(qproj_ctx *ctx, const qproj_rotation *rotation, const float *x_de
 /* A cache of keys and values held in 4 bits (ggml's Q4_0: blocks of 32 values, d * (n - 8)), in pages that any sequence
  * may use.  The four planes are device memory of the caller, who decides which page is whose:
  *   codes  uint8 [n_pages][n_head_kv][page_tokens][head_dim / 2],  scales fp16 [n_pages][n_head_kv][page_tokens][head_dim / 32]
- * page_tokens is 16, 32, 64, 128 or 256; head_dim is 64, 96, 128 or 256.  Values' codes lie in order, two a byte, the first in
+ * page_tokens is 16, 32, 64, 128 or 256; head_dim is 64, 96, 128 or 256; n_pages * n_head_kv * page_tokens stays under 2^32.
+ * Values' codes lie in order, two a byte, the first in
  * the low half; keys' codes in words of eight, word w of a row of B blocks holding values 8 * (w / B) .. + 7 of block
  * w % B.  Write through qproj_kv_append; pages may be copied whole. */
 typedef struct qproj_kv_cache {
@@ -314,10 +315,15 @@ int qproj_kv_read(qproj_ctx *ctx, const qproj_kv_cache *kv, const int64_t *slots
  * rows before q_start_dev[0] and from q_start_dev[n_seq] on are left as they were.  Bounds on the device are checked there: q_start_dev has to ascend
  * within [0, n_tokens] by at most max_q, kv_len_dev to lie in [0, pages_stride * page_tokens], the pages that are read in
  * [0, n_pages); a sequence that breaks the first two is left out, the tokens of a bad page are not seen, and the next
- * qproj_sync reports it.  Every value accumulates in fp32; operands go to the matrix cores as fp16 pairs of 22 bits.  The
- * result of a row depends on what else is in the call only in the order of its sums.  y must not overlap q.
- * Workspace: a fixed buffer of the context, allocated by its first call, which therefore cannot be captured into a graph;
- * later ones can.  Two captured calls of one context share it: replay them on one stream, or one after the other. */
+ * qproj_sync reports it.  Every value accumulates in fp32; queries, weights and values go to the matrix cores as fp16 pairs
+ * of 22 bits (of a row's largest query, down to 2^-37 of its largest weight and 2^-36 of the largest value near it).  A score
+ * past fp32 and a cached block that is not finite can make the rows that see them not finite, and no others.  The
+ * result of a row depends on what else is in the call only in the order of its sums; the same call gives the same bits.  y must
+ * not overlap q.  max_q should be what it says: it sizes the launch.  A call is refused where
+ * min(n_seq * max_q, n_tokens) * n_head / 8 + n_seq * n_head times pages_stride * page_tokens / 256 + 4 passes 2 * 10^9.
+ * Workspace: a fixed buffer of the context (17 MB on 256 compute units), allocated by its first call, which therefore cannot be
+ * captured into a graph (QPROJ_ERR_UNSUPPORTED); later ones can, and follow what the device arrays hold when they are replayed.
+ * All calls and replays of one context share it: they run one after the other, on the context's stream or ordered behind it. */
 int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens,
                     int64_t n_head, int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q,
                     const int32_t *pages_dev, int64_t pages_stride, float scale, int64_t window, float *y_dev,

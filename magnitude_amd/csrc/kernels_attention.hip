@@ -5,7 +5,8 @@
 // Work.  An item is 16 or 32 rows (some new tokens x the query heads that share a key/value head) against the
 // tokens they see, in tiles of 64 tokens.  All tiles of all items lie in one line, head by head, and the workgroups of one round
 // take equal stretches of it, whatever the lengths of the sequences are: a stretch ends inside an item where it has to, its
-// sums go to the workspace, and the workgroup that writes the last part of an item adds them.  The line is laid out
+// sums go to the workspace, and either the workgroup that writes the last part of an item adds them, or, where there are
+// many parts, a second kernel.  Items that are all short stay whole.  The line is laid out
 // on the device (a scan over the lengths in every workgroup), so that a captured call follows the lengths.  Inside a
 // workgroup the four waves take tiles in turn, each with its own running maximum, sum and result; they meet once, at the
 // end of an item.  No barrier in the loop over tiles.
@@ -27,6 +28,12 @@
 // the maximum, so that as pairs of halves they keep 22 bits down to 2^-26 of it, and steps of 2^-37 of it below.
 //
 // Weights, sums, maxima and results are fp32; every value that goes to the matrix cores has 22 bits.
+//
+// What bounds it, 32 heads of 128 on 8 (us a call): a token behind 131072 others 48, 151 MB of cache (3.1 TB/s; a copy moves
+// 5.1), 48 sequences of 100 to 8191 tokens 63, 232 MB (3.7 TB/s), 4096 prompt tokens 400, 137 Gflop (344 Tflop/s): the vector
+// units' and the matrix cores' issue slots.  A tile of 64 tokens and 16 (32) rows takes about 690 (870) vector instructions of four
+// cycles, two thirds of them to unpack its codes, and 80 (160) products of sixteen.  A short chat's token 11.6: the chain of
+// arguments, lengths, page, codes, one tile (2.2), the waves' meeting and the joining of two parts.
 #include "kv_cache.h"
 #include "lds_direct.h"
 #include "qproj_internal.h"
@@ -87,9 +94,9 @@ __device__ __forceinline__ const AttentionArgs &fresh_arguments() {
 
 constexpr int part_floats(int dim, int cols) { return 16 * cols * (dim + 2); }
 
-// (a third would fit where dim * cols <= 128, with the 168 registers that leaves: a token of 131072 took 59 us instead of 48, of 64-wide heads
-// 34 instead of 29; the vector units are busy with two)
-constexpr int waves_per_simd(int dim, int cols) { return dim * cols <= 256 ? 2 : 1; }
+// workgroups of a compute unit, waves of a SIMD (a third would fit where dim * cols <= 128, with the 168 registers that leaves: a token of
+// 131072 took 59 us instead of 48, of 64-wide heads 34 instead of 29; the vector units are busy with two)
+constexpr int kPerCu = 2;
 
 struct Sequence {
     int start, count, len;   // first row, rows, tokens in the cache; count 0 where there is nothing to do
@@ -881,7 +888,7 @@ __device__ __forceinline__ void join_parts(const AttentionArgs &a, const Item &i
 }
 
 template <int D, int NQ>
-__global__ __launch_bounds__(kThreads, waves_per_simd(D, NQ)) void attention_kernel(const AttentionArgs) {
+__global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const AttentionArgs) {
     const AttentionArgs &a = fresh_arguments();
     fetch_arguments<void(AttentionArgs), sizeof(AttentionArgs)>();
     __shared__ __align__(16) SharedLds<D, NQ> lds;
@@ -1132,9 +1139,11 @@ hipError_t launch(const AttentionArgs &a, int groups, hipStream_t s) {
 }  // namespace
 
 // counts of parts (zero before the first call; every call leaves them so), what the joining kernel is to do, then the parts
-static size_t arrived_bytes(int cus) { return ((size_t)cus * 2 * 4 + 255) / 256 * 256; }
-static size_t joins_bytes(int cus) { return (size_t)cus * 2 * 32; }
-size_t attention_scratch_bytes(int cus) { return arrived_bytes(cus) + joins_bytes(cus) + (size_t)cus * 2 * 2 * part_floats(256, 2) * 4; }
+static size_t arrived_bytes(int cus) { return ((size_t)cus * kPerCu * 4 + 255) / 256 * 256; }
+static size_t joins_bytes(int cus) { return (size_t)cus * kPerCu * 32; }
+size_t attention_scratch_bytes(int cus) {
+    return arrived_bytes(cus) + joins_bytes(cus) + (size_t)cus * kPerCu * 2 * std::max(part_floats(256, 1), part_floats(128, 2)) * 4;
+}
 
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     if (j.n_tokens == 0 || j.n_seq == 0 || j.max_q == 0) return hipSuccess;
@@ -1155,21 +1164,31 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     a.scale = j.scale * 1.44269504088896341f;
     a.window = j.window;
     a.group = j.n_head / j.kv->n_head;
-    const int cols = j.max_q * a.group <= 16 ? 1 : 2, rows = 16 * cols;
-    a.splits = (a.group + rows - 1) / rows;
-    a.split = (a.group + a.splits - 1) / a.splits;
-    a.tokens = rows / a.split;
-    a.row_tiles = (int32_t)((j.max_q + a.tokens - 1) / a.tokens);
-    const int groups_most = waves_per_simd(a.kv.dim, cols) * j.cus;
+    // 16 rows an item, or 32 of them that share the work of unpacking the codes.  Few rows of work leave most of the chip waiting for a turn of
+    // 32, which takes half as long again: 16 up to six turns of 16 rows (and two for their start) a workgroup.  Eight rows behind 4000
+    // tokens 14.1 us in sixteens and 17.7 in 32s, 64 rows 28.3 and 33.5; 128 rows 41.3 and 40.7, 128 behind 16000 122 and 103, 512
+    // prompt tokens 25.4 and 24.3, 1000 64 and 53.  Heads of 256 leave no registers for 32 at two waves a SIMD, and at one they were slower
+    // from 8 rows behind 1000 tokens (28 against 18.5 us) to 512 behind 32000 (838 against 804).
+    const int groups_most = kPerCu * j.cus;
+    const int64_t most_len = j.pages_stride << j.kv->page_shift;
+    double items = 0;
+    int cols = 1;
+    for (;; ++cols) {
+        const int rows = 16 * cols;
+        a.splits = (a.group + rows - 1) / rows;
+        a.split = (a.group + a.splits - 1) / a.splits;
+        a.tokens = rows / a.split;
+        a.row_tiles = (int32_t)((j.max_q + a.tokens - 1) / a.tokens);
+        items = std::min((double)a.n_seq * a.row_tiles, (double)a.n_tokens / a.tokens + a.n_seq) * j.kv->n_head * a.splits;
+        const int64_t seen = j.window ? std::min<int64_t>(most_len, (int64_t)j.window + a.tokens) : most_len;
+        if (cols == 2 || a.kv.dim > 128 || j.max_q * a.group <= 16 || items * ((double)seen / (kWaves * kTile) + 2) <= 6. * groups_most) break;
+    }
     // no more workgroups than there can be turns
-    const int64_t most = ((j.pages_stride << j.kv->page_shift) + kTile - 1) / kTile + 1;
-    const double turns = (double)most * a.n_seq * a.row_tiles * j.kv->n_head * a.splits / kWaves + (double)a.n_seq * a.row_tiles * j.kv->n_head * a.splits;
-    const int groups = (int)std::min<double>(groups_most, turns);
-    a.cus = j.cus;
+    const int64_t most = (most_len + kTile - 1) / kTile + 1;
+    const int groups = (int)std::max(1., std::min<double>(groups_most, items * ((double)most / kWaves + 1)));
     a.parts = reinterpret_cast<float *>(j.scratch + arrived_bytes(j.cus) + joins_bytes(j.cus));
     // An item is cut into as many parts as there are workgroups for it, one or two more at its ends.  Up to eight, whoever writes the last part
     // adds them: one launch.  More are added by a kernel whose workgroups share the work: for a token of 131072 (64 parts) 52 us against 60.
-    const double items = (double)a.n_seq * a.row_tiles * j.kv->n_head * a.splits;
     const bool few_parts = groups <= 8 * items;
     a.arrived = few_parts ? reinterpret_cast<uint32_t *>(j.scratch) : nullptr;
     a.joins = reinterpret_cast<int32_t *>(j.scratch + arrived_bytes(j.cus));
@@ -1186,8 +1205,7 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     }
     if (a.kv.dim == 64) return launch<64, 2>(a, groups, s);
     if (a.kv.dim == 96) return launch<96, 2>(a, groups, s);
-    if (a.kv.dim == 128) return launch<128, 2>(a, groups, s);
-    return launch<256, 2>(a, groups, s);
+    return launch<128, 2>(a, groups, s);
 }
 
 }  // namespace qproj

@@ -1800,9 +1800,9 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
     if (n_head <= 0 || n_head > kMostHeads || n_head % kv->n_head_kv != 0) return refuse(ctx, call, "n_head must be a multiple of n_head_kv");
     if (window < 0) return refuse(ctx, call, "negative window");
     // The device numbers places for rows of a head, and turns of four tiles of 64 tokens of all heads, in 32 bits.  A sequence's rows of a
-    // key/value head are at most rows * group / 16 + 1 items, an item's turns a quarter of its tiles, one for the rest and two for its start.
+    // key/value head are at most rows * group / 8 + 1 items, an item's turns a quarter of its tiles, one for the rest and two for its start.
     const double most_q = (double)std::min(max_q, n_tokens);
-    const double items = std::min((double)n_seq * most_q, (double)n_tokens) * n_head / 16 + (double)n_seq * n_head;
+    const double items = std::min((double)n_seq * most_q, (double)n_tokens) * n_head / 8 + (double)n_seq * n_head;
     if ((double)n_seq * (most_q + 1) > 2e9 || items * ((double)pages_stride * kv->page_tokens / 256 + 4) > 2e9)
         return refuse(ctx, call, "too many rows times tokens (or n_seq times max_q) for one call");
     if (const char *why = bad_rows(q_dev, q_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);

@@ -170,6 +170,41 @@ impl Context {
                            Activation::Ggml as c_int)
         })
     }
+
+    /// Keys and values `[n][n_head_kv][head_dim]` into the cache at `slots` (i64 on the device), the keys rotated; queries
+    /// `[n][n_head][head_dim]` rotated beside them into `q_out`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn kv_append(&self, kv: &sys::qproj_kv_cache, k: DevicePtr, v: DevicePtr, n: i64, slots: DevicePtr,
+                     rotation: &sys::qproj_rotation, q: DevicePtr, n_head: i64, q_out: DevicePtr) -> Result<()> {
+        let (row, q_row) = (kv.n_head_kv * kv.head_dim, n_head * kv.head_dim);
+        self.check(unsafe {
+            sys::qproj_kv_append(self.raw, kv, k.0.cast(), row, v.0.cast(), row, n, slots.0.cast(), rotation, q.0.cast(), q_row, n_head,
+                                 q_out.0.cast(), q_row)
+        })
+    }
+
+    /// Attention of the newest tokens of `n_seq` sequences over their tokens in the cache; see `qproj_attention`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn attention(&self, kv: &sys::qproj_kv_cache, q: DevicePtr, n: i64, n_head: i64, n_seq: i64, q_start: DevicePtr,
+                     kv_len: DevicePtr, max_q: i64, pages: DevicePtr, pages_stride: i64, scale: f32, window: i64, y: DevicePtr) -> Result<()> {
+        let row = n_head * kv.head_dim;
+        self.check(unsafe {
+            sys::qproj_attention(self.raw, kv, q.0.cast(), row, n, n_head, n_seq, q_start.0.cast(), kv_len.0.cast(), max_q,
+                                 pages.0.cast(), pages_stride, scale, window, y.0.cast(), row)
+        })
+    }
+}
+
+/// The frequencies of a rotation's `n_dims / 2` pairs and what cosines and sines are multiplied by.
+pub fn rope_frequencies(scaling: &sys::qproj_rope_scaling, n_dims: i64) -> Result<(Vec<f64>, f32)> {
+    let mut freqs = vec![0f64; (n_dims.max(0) / 2) as usize];
+    let mut magnitude = 0f32;
+    let st = unsafe { sys::qproj_rope_frequencies(scaling, n_dims, freqs.as_mut_ptr(), &mut magnitude) };
+    if st == sys::QPROJ_OK {
+        Ok((freqs, magnitude))
+    } else {
+        Err(QprojError { status: st, message: "rope_frequencies".into() })
+    }
 }
 
 /// Scratch bytes a `mul_mat` of this shape needs at most (what `mul_mat_noalloc` holds against its fixed buffer).

@@ -136,6 +136,21 @@ def test_calls_that_are_taken_note_their_launches():
     assert dry.plan.count("rope_kv_kernel:") == 3 and dry.plan.count("kv_read_kernel:") == 2 and dry.plan.count("attention_kernel<") == 21
 
 
+def test_rows_are_taken_sixteen_or_32_at_a_time():
+    """few rows of work: 16; many: 32, unless a head is 256 wide"""
+    def plan(dim=128, **kw):
+        with Dry() as dry:
+            assert call(dry, "attention", cache(n_pages=1 << 16, head_dim=dim), qs=32 * dim, ys=32 * dim, **kw) == 0
+        return dry.plan.split(":")[0]
+    one, token = dict(seqs=1, n=8, max_q=8), dict(seqs=1, n=1, max_q=1)
+    assert plan(ps=64, **one) == "attention_kernel<128, 1>" and plan(ps=2048, **one) == "attention_kernel<128, 2>"
+    assert plan(ps=2048, **token) == "attention_kernel<128, 1>" and plan(ps=2048, window=1000, **one) == "attention_kernel<128, 1>"
+    assert plan(seqs=1, n=4096, max_q=4096, ps=64) == "attention_kernel<128, 2>" and plan(dim=96, seqs=1, n=4096, max_q=4096, ps=64) == "attention_kernel<96, 2>"
+    assert plan(dim=256, seqs=1, n=4096, max_q=4096, ps=64) == "attention_kernel<256, 1>"
+    # a table that one of many sequences needs, and a max_q that one of them has
+    assert plan(seqs=64, n=64 + 100, max_q=100, ps=4) == "attention_kernel<128, 1>"
+
+
 def test_long_calls_become_launches_that_fit():
     with Dry() as dry:
         assert call(dry, "rope", rot=rotation(), n=(1 << 24) + 1) == 0

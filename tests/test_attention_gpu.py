@@ -210,24 +210,32 @@ def make_cache(rng, lens, page, kv_heads, dim, spare=3, scale=1.0):
     return kv, pages
 
 
+def wide(pages, kv):
+    """the same table with room for so many pages that rows are taken 32 at a time (where there are more than 16 of a head at all)"""
+    columns = -(-6 * 2 * 256 * 300 // (kv.page_tokens * kv.n_head * len(pages))) + 1
+    return np.pad(pages, ((0, 0), (0, columns)), constant_values=-7)
+
+
 def check(ctx, kv, pages, q, q_start, kv_len, window=0, scale=None, **kw):
+    """of the call in both its forms: 16 and 32 rows at a time"""
     dim = kv.head_dim
     s = dim ** -0.5 if scale is None else scale
     want, sizes = kv_ref.attention(numpy_cache(kv), q, q_start, kv_len, pages, s, window)
-    out = torch.full(q.shape, 7.5, device="cuda")
-    got = ctx.attention(kv, dev(q), dev(np.array(q_start, np.int32)), dev(np.array(kv_len, np.int32)), dev(pages), scale=scale, window=window,
-                        out=out, **kw).cpu().numpy()
     mine = ~np.isnan(want).all(-1)
-    assert (got[~mine] == 7.5).all()                       # rows of no sequence stay as they were
-    bound = kv_ref.allowed(sizes, dim, max([1] + list(kv_len)))
-    err = np.abs(got - want)[mine]
-    worst = np.max(err / bound[mine]) if err.size else 0.0
-    rel = np.linalg.norm(err) / max(1e-30, np.linalg.norm(want[mine])) if err.size else 0.0
     plain = kv_ref.attention(numpy_cache(kv), q, q_start, kv_len, pages, s, window, dtype=np.float32)[0]
-    usual = np.linalg.norm((plain - want)[mine]) / max(1e-30, np.linalg.norm(want[mine])) if err.size else 0.0
-    tell(f"   worst {worst:.3g} of what is allowed, {rel:.3g} of the norm, in fp32 {usual:.3g}")
-    # over all values: half as much again as the statement in fp32, or 16 steps of an fp32 number
-    assert worst <= 1.0 and rel <= max(1.5 * usual, 2.0 ** -20)
+    bound = kv_ref.allowed(sizes, dim, max([1] + list(kv_len)))[mine]
+    usual = np.linalg.norm((plain - want)[mine]) / max(1e-30, np.linalg.norm(want[mine])) if mine.any() else 0.0
+    for table in (wide(pages, kv), pages):
+        out = torch.full(q.shape, 7.5, device="cuda")
+        got = ctx.attention(kv, dev(q), dev(np.array(q_start, np.int32)), dev(np.array(kv_len, np.int32)), dev(table), scale=scale, window=window,
+                            out=out, **kw).cpu().numpy()
+        assert (got[~mine] == 7.5).all()                       # rows of no sequence stay as they were
+        err = np.abs(got - want)[mine]
+        worst = np.max(err / bound) if err.size else 0.0
+        rel = np.linalg.norm(err) / max(1e-30, np.linalg.norm(want[mine])) if err.size else 0.0
+        tell(f"   worst {worst:.3g} of what is allowed, {rel:.3g} of the norm, in fp32 {usual:.3g}")
+        # over all values: half as much again as the statement in fp32, or 16 steps of an fp32 number
+        assert worst <= 1.0 and rel <= max(1.5 * usual, 2.0 ** -20)
     return got
 
 
@@ -251,6 +259,8 @@ ATTENTION = [  # dim, page, kv heads, group, [(tokens in the cache, new ones)], 
     (64, 128, 2, 7, [(1500, 187)], 300),
     (128, 16, 1, 4, [(400, 100), (90, 90)], 1),
     (128, 16, 1, 4, [(400, 30)], 64),
+    (128, 64, 8, 4, [(700, 700)], 100),
+    (64, 128, 4, 7, [(1200, 500)], 200),
     (128, 64, 8, 1, [(9000, 1), (100, 1), (4097, 1)], 0),
     # far more items than workgroups, all short: dealt out whole, several rounds
     (64, 16, 8, 1, [(1 + 37 * i % 301, 1) for i in range(300)], 0),
@@ -327,15 +337,17 @@ def test_queries_of_every_size(ctx):
     check(ctx, kv, pages, (q * 3e4).astype(np.float32), [0, 7], [150])
 
 
-@pytest.mark.parametrize("dim,new,group", [(128, 1, 4), (128, 70, 4), (64, 9, 2), (256, 3, 1)])
-def test_blocks_that_are_not_finite_reach_only_who_sees_them(ctx, dim, new, group):
+@pytest.mark.parametrize("dim,new,group,rows", [(128, 1, 4, 16), (128, 70, 4, 16), (128, 70, 4, 32), (64, 9, 2, 16), (64, 9, 2, 32), (96, 20, 3, 32), (256, 3, 1, 16)])
+def test_blocks_that_are_not_finite_reach_only_who_sees_them(ctx, dim, new, group, rows):
     rng = np.random.default_rng(8)
     length = 200
     kv, pages = make_cache(rng, [length, 90], 16, 2, dim)
     clean = [t.clone() for t in kv.tensors]
     q = rng.standard_normal((new + 1, 2 * group, dim)).astype(np.float32)
     q_start, lens = [0, new, new + 1], [length, 90]
-    base = check(ctx, kv, pages, q, q_start, lens)
+    check(ctx, kv, pages, q, q_start, lens)
+    table = dev(wide(pages, kv) if rows == 32 else pages)
+    base = ctx.attention(kv, dev(q), dev(np.array(q_start, np.int32)), dev(np.array(lens, np.int32)), table).cpu().numpy()
     page_of = lambda s, t: (int(pages[s, t // 16]), t % 16)
 
     def poison(t, value, s=0):
@@ -355,7 +367,7 @@ def test_blocks_that_are_not_finite_reach_only_who_sees_them(ctx, dim, new, grou
             if u not in used:
                 for plane in (1, 3):
                     kv.tensors[plane][u] = value
-        got = ctx.attention(kv, dev(q), dev(np.array(q_start, np.int32)), dev(np.array(lens, np.int32)), dev(pages)).cpu().numpy()
+        got = ctx.attention(kv, dev(q), dev(np.array(q_start, np.int32)), dev(np.array(lens, np.int32)), table).cpu().numpy()
         hit = np.zeros(got.shape, bool)
         hit[new - 1, :group] = True
         hit[new - 1, group:, 32:64] = True
@@ -537,7 +549,7 @@ def test_captured_steps(ctx):
     own.close()
 
 
-@pytest.mark.parametrize("seqs,group", [(1, 4), (1, 32), (24, 4)])     # joined by a launch of their own, of two columns, by the last workgroup
+@pytest.mark.parametrize("seqs,group", [(1, 4), (1, 32), (24, 4)])     # joined by a launch of their own, by the last workgroup (of two halves of the heads, of many sequences)
 def test_captured_attention_follows_the_lengths(seqs, group):
     """recorded once, replayed with lengths from nothing to full pages: items cut into one part, a few and many"""
     from magnitude_amd import Context
