@@ -906,6 +906,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
             u += tile1 - tile0;
         }
     };
+    if (id < 8) lds.found[id] = 0;      // (lengths that another stream changes meanwhile find no item: nothing, and not anything)
     // ---- the line of turns ----
     int turns_mine = 0, items_mine = 0, longest = 0;
     each_item([&](int s, int tile, const Sequence &q, int n) {
