@@ -29,7 +29,7 @@
 //
 // Weights, sums, maxima and results are fp32; every value that goes to the matrix cores has 22 bits.
 //
-// What bounds it, 32 heads of 128 on 8 (us a call): a token behind 131072 others 48, 151 MB of cache (3.1 TB/s; a copy moves
+// What bounds it, 32 heads of 128 on 8 (us a call): a token behind 131072 others 45, 151 MB of cache (3.3 TB/s; a copy moves
 // 5.1), 48 sequences of 100 to 8191 tokens 63, 232 MB (3.7 TB/s), 4096 prompt tokens 400, 137 Gflop (344 Tflop/s): the vector
 // units' and the matrix cores' issue slots.  A tile of 64 tokens and 16 (32) rows takes about 690 (870) vector instructions of four
 // cycles, two thirds of them to unpack its codes, and 80 (160) products of sixteen.  A short chat's token 11.6: the chain of
@@ -68,7 +68,7 @@ struct AttentionArgs {
     float *parts;            // [workgroups][2] sums of items that were cut (part_floats each)
     uint32_t *arrived;       // [workgroups] parts written of the item that a stretch begins and does not end; zero between calls.  Null:
                              // attention_join_kernel adds the parts
-    int32_t *joins;          // [workgroups][8] for it: {first stretch (-1: nothing to join), last stretch, sequence, row tile, head}
+    int32_t *joins;          // [heads][n_seq][row_tiles][2] for it: of every item its first stretch (-1: nothing to join) and its last
     float scale;             // times log2(e)
     int32_t n_tokens, n_seq, max_q, window;
     int32_t group;           // query heads of a key/value head
@@ -956,11 +956,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
     const uint32_t total = (uint32_t)head_length * heads_all;
     const uint32_t active = std::min(total, groups), per_xcd = (active + 7) / 8;
     const uint32_t me = whole_items ? blockIdx.x : (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
-    if (me >= active || (!whole_items && blockIdx.x / 8 >= per_xcd)) {
-        if (id == 0 && !a.arrived) a.joins[8 * (int64_t)blockIdx.x] = -1;
-        return;
-    }
-    int join_from = -1, join_seq = 0, join_tile = 0, join_head = 0;
+    if (me >= active || (!whole_items && blockIdx.x / 8 >= per_xcd)) return;
     const uint32_t length = total / active, longer = total - length * active;     // the first `longer` stretches have one more
     uint32_t at = whole_items ? me : me * length + std::min(me, longer);
     const uint32_t end = whole_items ? total : at + length + (me < longer ? 1 : 0);
@@ -1008,26 +1004,26 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         const bool starts = turn0 == 0, ends = turn1 == turns;
         meet<D, NQ>(fresh_arguments(), it, head0, heads, st, starts && ends, fresh_arguments().parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ), lds, wave, lane);
         const AttentionArgs &c = fresh_arguments();
-        if (!(starts && ends) && (c.arrived || ends)) {
-            const auto stretch_of = [&](uint32_t p) {
-                const uint32_t edge = longer * (length + 1);
-                return (int)(p < edge ? p / (length + 1) : longer + (p - edge) / length);
-            };
-            const int first = stretch_of(at - skip + start);
-            if (!c.arrived) {
-                join_from = first;
-                join_seq = seq, join_tile = row_tile, join_head = hv;
-            } else {
-                // The part is in memory before it is counted (the wait is for the stores); whoever counts the last one loads them after that.
-                const int parts = stretch_of(at - skip + start + turns - 1) - first + 1;
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                __syncthreads();
-                if (id == 0) lds.last = __hip_atomic_fetch_add(c.arrived + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
-                __syncthreads();
-                if (lds.last) {
-                    if (id == 0) __hip_atomic_store(c.arrived + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
-                    join_parts<D, NQ>(c, it, head0, heads, first, parts, lds, wave, lane);
-                }
+        const auto stretch_of = [&](uint32_t p) {
+            const uint32_t edge = longer * (length + 1);
+            return (int)(p < edge ? p / (length + 1) : longer + (p - edge) / length);
+        };
+        if (!c.arrived) {            // whoever writes an item's end says what is to be joined
+            if (ends && id == 0) {
+                int32_t *const join = c.joins + 2 * ((int64_t)hv * c.n_seq * c.row_tiles + seq * c.row_tiles + row_tile);
+                join[0] = starts ? -1 : stretch_of(at - skip + start);
+                join[1] = (int32_t)me;
+            }
+        } else if (!(starts && ends)) {
+            // The part is in memory before it is counted (the wait is for the stores); whoever counts the last one loads them after that.
+            const int first = stretch_of(at - skip + start), parts = stretch_of(at - skip + start + turns - 1) - first + 1;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (id == 0) lds.last = __hip_atomic_fetch_add(c.arrived + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
+            __syncthreads();
+            if (lds.last) {
+                if (id == 0) __hip_atomic_store(c.arrived + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
+                join_parts<D, NQ>(c, it, head0, heads, first, parts, lds, wave, lane);
             }
         }
         if (whole_items) {
@@ -1038,51 +1034,39 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         }
         if (at < end) __syncthreads();
     }
-    if (id == 0 && !fresh_arguments().arrived) {
-        int32_t *const join = fresh_arguments().joins + 8 * (int64_t)blockIdx.x;
-        join[0] = join_from;
-        join[1] = (int32_t)me;
-        join[2] = join_seq;
-        join[3] = join_tile;
-        join[4] = join_head;
-    }
 }
 
-// Items that were cut into many parts: the sums of stretches first .. last.  A workgroup takes 16 queries and a share of the dimensions; its waves take
-// the parts in turn, four at a time (their loads go out together: a part comes from another XCD's memory), and meet once.
+// Items that were cut into many parts: the sums of stretches first .. last.  A workgroup takes 16 queries and 16
+// dimensions; its waves take the parts in turn, four at a time (their loads go out together: a part comes from another XCD's memory), and meet once.
 constexpr int kJoinWaves = 8;
-constexpr int join_share(int dim, int cols) { return dim / 16 % 4 || cols > 1 ? dim / 32 : dim / 64; }   // of the dimensions, in 16s: few workgroups, most have nothing to join
 
 template <int D, int NQ>
 __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const AttentionArgs a) {
-    constexpr int T = D / 16, kShare = join_share(D, NQ), kShares = T / kShare, kBatch = 4;
-    static_assert(T % kShare == 0, "whole shares");
-    __shared__ __align__(16) f32x4 sums[kJoinWaves][kShare][64];
+    constexpr int kBatch = 4, kM = 16 * NQ * D, kL = kM + 16 * NQ;
+    __shared__ __align__(16) f32x4 sums[kJoinWaves][64];
     __shared__ float tops[kJoinWaves][16], weights[kJoinWaves][16];
-    const int32_t *j = a.joins + 8 * (int64_t)blockIdx.x;
-    const int first = j[0], last = j[1];
-    if (first < 0) return;
+    const int32_t *j = a.joins + 2 * (int64_t)blockIdx.x;
+    const int first = j[0], last = j[1], units = a.n_seq * a.row_tiles;
+    const int hv = blockIdx.x / units, s = (blockIdx.x - hv * units) / a.row_tiles, row_tile = blockIdx.x - hv * units - s * a.row_tiles;
+    bool bad, live;
+    const Sequence q = sequence(a, s, bad);
+    const Item it = item_of(a, s, q, row_tile);
+    if (it.count <= 0 || first < 0) return;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15;
-    const int g = blockIdx.y / kShares, x0 = (blockIdx.y % kShares) * kShare;
-    const int64_t size = part_floats(D, NQ);
-    const int parts = last - first + 1;
-    const auto part = [&](int w) { return a.parts + ((int64_t)(first + w) * 2 + (w ? 0 : 1)) * size; };   // (the first is a stretch's second)
-    constexpr int kM = 16 * NQ * D, kL = kM + 16 * NQ;
-    f32x4 o[kShare];
-#pragma unroll
-    for (int t = 0; t < kShare; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int x = blockIdx.y / NQ, g = blockIdx.y % NQ, parts = last - first + 1;
+    const auto part = [&](int w) { return a.parts + ((int64_t)(first + w) * 2 + (w ? 0 : 1)) * part_floats(D, NQ); };   // (the first is a stretch's second)
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     for (int w0 = wave; w0 < parts; w0 += kBatch * kJoinWaves) {
         float mw[kBatch], lw[kBatch];
-        f32x4 v[kBatch][kShare];
+        f32x4 v[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {       // (behind the last part the first of the batch again, with no weight)
             const int w = w0 + k * kJoinWaves;
             const float *p = part(w < parts ? w : w0);
             mw[k] = p[kM + g * 16 + col];
             lw[k] = p[kL + g * 16 + col];
-#pragma unroll
-            for (int t = 0; t < kShare; ++t) v[k][t] = reinterpret_cast<const f32x4 *>(p)[((x0 + t) * NQ + g) * 64 + lane];
+            v[k] = reinterpret_cast<const f32x4 *>(p)[(x * NQ + g) * 64 + lane];
         }
         float top = m;
 #pragma unroll
@@ -1091,52 +1075,44 @@ __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const A
         m = top;
         l *= back;
 #pragma unroll
-        for (int t = 0; t < kShare; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[t][r] *= back;
+        for (int r = 0; r < 4; ++r) o[r] *= back;
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
             if (w0 + k * kJoinWaves >= parts) break;
             const float f = mw[k] == m ? 1.f : __builtin_amdgcn_exp2f(mw[k] - m);
             l += lw[k] * f;
 #pragma unroll
-            for (int t = 0; t < kShare; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[t][r] += v[k][t][r] * f;
+            for (int r = 0; r < 4; ++r) o[r] += v[k][r] * f;
         }
     }
     if (lane < 16) tops[wave][lane] = m, weights[wave][lane] = l;
-#pragma unroll
-    for (int t = 0; t < kShare; ++t) sums[wave][t][lane] = o[t];
+    sums[wave][lane] = o;
     __syncthreads();
-    if (wave >= kShare) return;
-    bool bad, live;
-    const Sequence q = sequence(a, j[2], bad);
-    const Item it = item_of(a, j[2], q, j[3]);
-    const int kv_head = j[4] / a.splits, go = j[4] - kv_head * a.splits;
+    if (wave != 0) return;
+    const int kv_head = hv / a.splits, go = hv - kv_head * a.splits;
     float *y = out_row<D, NQ>(a, it, kv_head * a.group + go * a.split, min(a.split, a.group - go * a.split), g, lane, live);
     if (!live) return;
     const int used = min(kJoinWaves, parts);
     m = -INFINITY, l = 0.f;
     for (int w = 0; w < used; ++w) m = fmaxf(m, tops[w][col]);
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int w = 0; w < used; ++w) {
         const float f = tops[w][col] == m ? 1.f : __builtin_amdgcn_exp2f(tops[w][col] - m);
-        const f32x4 x = sums[w][wave][lane];
+        const f32x4 v = sums[w][lane];
         l += weights[w][col] * f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] += x[r] * f;
+        for (int r = 0; r < 4; ++r) o[r] += v[r] * f;
     }
     const float unit = l != 0.f ? 1.f / l : 0.f;
-    *reinterpret_cast<f32x4 *>(y + 16 * (x0 + wave)) = f32x4{v[0] * unit, v[1] * unit, v[2] * unit, v[3] * unit};
+    *reinterpret_cast<f32x4 *>(y + 16 * x) = f32x4{o[0] * unit, o[1] * unit, o[2] * unit, o[3] * unit};
 }
 
 template <int D, int NQ>
-hipError_t launch(const AttentionArgs &a, int groups, hipStream_t s) {
+hipError_t launch(const AttentionArgs &a, int groups, int places, hipStream_t s) {
     hipLaunchKernelGGL((attention_kernel<D, NQ>), dim3(groups), dim3(kThreads), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.arrived) return e;
-    hipLaunchKernelGGL((attention_join_kernel<D, NQ>), dim3(groups, D / 16 / join_share(D, NQ) * NQ), dim3(64 * kJoinWaves), 0, s, a);
+    hipLaunchKernelGGL((attention_join_kernel<D, NQ>), dim3(places, D / 16 * NQ), dim3(64 * kJoinWaves), 0, s, a);
     return hipGetLastError();
 }
 
@@ -1144,7 +1120,7 @@ hipError_t launch(const AttentionArgs &a, int groups, hipStream_t s) {
 
 // counts of parts (zero before the first call; every call leaves them so), what the joining kernel is to do, then the parts
 static size_t arrived_bytes(int cus) { return ((size_t)cus * kPerCu * 4 + 255) / 256 * 256; }
-static size_t joins_bytes(int cus) { return (size_t)cus * kPerCu * 32; }
+static size_t joins_bytes(int cus) { return (size_t)cus * kPerCu * 8; }
 size_t attention_scratch_bytes(int cus) {
     return arrived_bytes(cus) + joins_bytes(cus) + (size_t)cus * kPerCu * 2 * std::max(part_floats(256, 1), part_floats(128, 2)) * 4;
 }
@@ -1192,9 +1168,12 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     const int groups = (int)std::max(1., std::min<double>(groups_most, items * ((double)most / kWaves + 1)));
     a.parts = reinterpret_cast<float *>(j.scratch + arrived_bytes(j.cus) + joins_bytes(j.cus));
     // An item is cut into as many parts as there are workgroups for it, one or two more at its ends.  Up to eight, whoever writes the last part
-    // adds them: one launch.  More are added by a kernel whose workgroups share the work: for a token of 131072 (64 parts) 52 us against 60,
-    // for five rows behind 2000 tokens 17.4 against 19.1; a short chat's token, with two, 12.8 against 15.1.
-    const bool few_parts = groups <= 8 * items;
+    // adds them: one launch.  More are added by a kernel whose workgroups share the work: for a token of 131072 (64 parts) 45 us against 56,
+    // of 8192 13.8 against 19.0, for eight rows behind 6000 17.2 against 22.1; a short chat's token, with two, 14.0 against 11.9.  (Up to five
+    // instead of eight: 0.6% more over 50 drawn calls, up to three 2%.)
+    // (the joins' list has a place for every item there could be, fewer than groups / 8)
+    const int64_t places = (int64_t)a.n_seq * a.row_tiles * j.kv->n_head * a.splits;
+    const bool few_parts = groups <= 8 * places;
     a.arrived = few_parts ? reinterpret_cast<uint32_t *>(j.scratch) : nullptr;
     a.joins = reinterpret_cast<int32_t *>(j.scratch + arrived_bytes(j.cus));
     if (dry_run()) {
@@ -1203,14 +1182,14 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
         return hipSuccess;
     }
     if (cols == 1) {
-        if (a.kv.dim == 64) return launch<64, 1>(a, groups, s);
-        if (a.kv.dim == 96) return launch<96, 1>(a, groups, s);
-        if (a.kv.dim == 128) return launch<128, 1>(a, groups, s);
-        return launch<256, 1>(a, groups, s);
+        if (a.kv.dim == 64) return launch<64, 1>(a, groups, (int)places, s);
+        if (a.kv.dim == 96) return launch<96, 1>(a, groups, (int)places, s);
+        if (a.kv.dim == 128) return launch<128, 1>(a, groups, (int)places, s);
+        return launch<256, 1>(a, groups, (int)places, s);
     }
-    if (a.kv.dim == 64) return launch<64, 2>(a, groups, s);
-    if (a.kv.dim == 96) return launch<96, 2>(a, groups, s);
-    return launch<128, 2>(a, groups, s);
+    if (a.kv.dim == 64) return launch<64, 2>(a, groups, (int)places, s);
+    if (a.kv.dim == 96) return launch<96, 2>(a, groups, (int)places, s);
+    return launch<128, 2>(a, groups, (int)places, s);
 }
 
 }  // namespace qproj

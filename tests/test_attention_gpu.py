@@ -275,6 +275,7 @@ ATTENTION = [  # dim, page, kv heads, group, [(tokens in the cache, new ones)], 
     (256, 64, 2, 4, [(5000, 20)], 0),
     (256, 64, 1, 4, [(20000, 1)], 0),
     (64, 256, 1, 8, [(30000, 3)], 0),
+    (128, 64, 1, 4, [(0, 0), (20000, 1), (0, 0), (5, 1)], 0),
     (96, 256, 1, 1, [(20000, 1)], 5000),
     (64, 64, 2, 8, [(3000, 64)], 0),
     # a prompt among tokens, and no max_q: mostly places without an item
