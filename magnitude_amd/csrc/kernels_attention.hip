@@ -297,7 +297,7 @@ __device__ __forceinline__ void stage_queries(const AttentionArgs &a, const Item
         most = max_xor(whole ? most : INFINITY);
         // (frexp: most = f * 2^e with f in [0.5, 1); where a value is not finite the row stays as it is: NaN comes of it)
         const int e = most > 0.f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
-        if (wave == 0) lds.q_unit[g][lane] = ldexpf(1.f, e - 15);
+        if (wave == 0) lds.q_unit[g][lane] = ldexpf(1.f, max(e - 15, -126));    // (not 0, which masked scores are multiplied by; such scores are 0)
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             if (b % kWaves != wave) continue;

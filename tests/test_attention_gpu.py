@@ -338,6 +338,15 @@ def test_queries_of_every_size(ctx):
     check(ctx, kv, pages, (q * 3e4).astype(np.float32), [0, 7], [150])
 
 
+def test_queries_next_to_nothing(ctx):
+    """so small that the unit of their scores would be zero: weights are equal, tokens that are masked stay so"""
+    rng = np.random.default_rng(18)
+    kv, pages = make_cache(rng, [100, 70], 16, 2, 128)
+    for size in (1e-36, 1e-40, 1e-43, 1e-45, 0.0):
+        q = (np.sign(rng.standard_normal((40, 8, 128))) * size).astype(np.float32)
+        check(ctx, kv, pages, q, [0, 1, 40], [100, 70])
+
+
 @pytest.mark.parametrize("dim,new,group,rows", [(128, 1, 4, 16), (128, 70, 4, 16), (128, 70, 4, 32), (64, 9, 2, 16), (64, 9, 2, 32), (96, 20, 3, 32), (256, 3, 1, 16)])
 def test_blocks_that_are_not_finite_reach_only_who_sees_them(ctx, dim, new, group, rows):
     rng = np.random.default_rng(8)
