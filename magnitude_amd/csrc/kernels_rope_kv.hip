@@ -23,7 +23,6 @@ namespace {
 
 constexpr int kRopeThreads = 256;
 constexpr int kUnit = 8;   // values a thread takes
-constexpr int64_t kManyTokens = 1024;
 constexpr int64_t kMostGrid = (int64_t)1 << 23;   // tokens of a launch: a grid has fewer than 2^32 threads in a direction
 
 struct RotateArgs {
@@ -136,14 +135,34 @@ __device__ __forceinline__ uint32_t quantize_unit(float4 lo, float4 hi, int eigh
     return word;
 }
 
-// 8 values of a key or a value into the cache; four neighbouring lanes take a block: q_units, kv_units and the workgroup are multiples of 4
-__device__ __forceinline__ void append_unit(const RopeKvArgs &a, const double2 *cs, int64_t token, int unit) {
+__global__ __launch_bounds__(kRopeThreads) void rope_kv_kernel(const RopeKvArgs a) {
+    extern __shared__ __align__(16) double2 cs[];
+    const int64_t token = blockIdx.x;
+    if (a.r.half) {
+        const double pos = (double)a.r.pos[token], mag = (double)a.r.magnitude;
+        for (int i = threadIdx.x; i < a.r.half; i += kRopeThreads) {
+            double turns = pos * a.r.freqs[i] * 0.15915494309189533577;   // 1 / 2 pi
+            turns -= rint(turns);
+            double s, c;
+            sincospi(2.0 * turns, &s, &c);
+            cs[i] = make_double2(c * mag, s * mag);
+        }
+        __syncthreads();
+    }
+    int unit = blockIdx.y * kRopeThreads + threadIdx.x;
+    if (unit < a.q_units) {
+        rotate_unit(a, cs, token, unit);
+        return;
+    }
+    unit -= a.q_units;
+    if (unit >= 2 * a.kv_units) return;
     const bool key = unit < a.kv_units;
     if (!key) unit -= a.kv_units;
     const int64_t slot = a.slots[token];
     const bool outside = slot >= a.kv.n_pages << a.kv.page_shift;
     if (outside && unit == 0) atomicOr(a.error, kKvBadSlot);
     if (slot < 0 || outside) return;
+    // four neighbouring lanes take a block: q_units, kv_units and the workgroup are multiples of 4
     const int blocks = a.kv.dim / 32, eighth = unit & 3, block = (unit >> 2) % blocks, head = (unit >> 2) / blocks;
     const int d = 32 * block + 8 * eighth;
     const float *row = (key ? a.k + token * a.k_stride : a.v + token * a.v_stride) + (int64_t)head * a.kv.dim;
@@ -161,27 +180,6 @@ __device__ __forceinline__ void append_unit(const RopeKvArgs &a, const double2 *
     uint8_t *codes = (key ? a.kv.k_codes : a.kv.v_codes) + at * (a.kv.dim / 2);
     reinterpret_cast<uint32_t *>(codes)[key ? key_word(blocks, block, eighth) : value_word(block, eighth)] = word;
     if (eighth == 0) (key ? a.kv.k_scales : a.kv.v_scales)[at * blocks + block] = scale;
-}
-
-__global__ __launch_bounds__(kRopeThreads) void rope_kv_kernel(const RopeKvArgs a) {
-    extern __shared__ __align__(16) double2 cs[];
-    const int64_t token = blockIdx.x;
-    if (a.r.half) {
-        const double pos = (double)a.r.pos[token], mag = (double)a.r.magnitude;
-        for (int i = threadIdx.x; i < a.r.half; i += kRopeThreads) {
-            double turns = pos * a.r.freqs[i] * 0.15915494309189533577;   // 1 / 2 pi
-            turns -= rint(turns);
-            double s, c;
-            sincospi(2.0 * turns, &s, &c);
-            cs[i] = make_double2(c * mag, s * mag);
-        }
-        __syncthreads();
-    }
-    const int total = a.q_units + 2 * a.kv_units;
-    for (int unit = blockIdx.y * kRopeThreads + threadIdx.x; unit < total; unit += gridDim.y * kRopeThreads) {
-        if (unit < a.q_units) rotate_unit(a, cs, token, unit);
-        else append_unit(a, cs, token, unit - a.q_units);
-    }
 }
 
 // rows of the cache as fp32 values; places outside it (and negative ones) are zeros
@@ -241,11 +239,8 @@ hipError_t launch_rope_kv(const RopeKvJob &j, hipStream_t s) {
     }
     if (j.kv && a.q_units % 4) return hipErrorInvalidValue;   // a block of the cache is four lanes of a quad
     const int units = a.q_units + 2 * a.kv_units;
-    // Few tokens: a thread for every unit.  Many: two workgroups a token, which take its cosines and sines once and several units each: 2048
-    // tokens of 40 heads 14.1 us instead of 14.7, 4096 tokens' append and read 48.1 instead of 49.7; one a token 14.4 and 49.0.
-    const int groups = (units + kRopeThreads - 1) / kRopeThreads;
     for (int64_t left = j.n_tokens; left > 0; left -= kMostGrid) {
-        const dim3 grid((unsigned)std::min(left, kMostGrid), (unsigned)(left >= kManyTokens ? std::min(2, groups) : groups));
+        const dim3 grid((unsigned)std::min(left, kMostGrid), (unsigned)((units + kRopeThreads - 1) / kRopeThreads));
         if (dry_run()) {
             plan_note("rope_kv_kernel: %u tokens, %d units of queries + 2 x %d of keys and values, grid %u x %u x %d", grid.x, a.q_units, a.kv_units, grid.x,
                       grid.y, kRopeThreads);
