@@ -73,6 +73,7 @@ struct AttentionArgs {
     int32_t n_tokens, n_seq, max_q, window;
     int32_t group;           // query heads of a key/value head
     int32_t splits, split;   // they are served `split` at a time, in `splits` goes
+    uint32_t split_part;     // 2^16 / split, rounded up
     int32_t tokens;          // new tokens of an item
     int32_t row_tiles;       // items of a sequence, at most
     int32_t cus;             // workgroups from this one on share a compute unit with an earlier one
@@ -97,6 +98,18 @@ constexpr int part_floats(int dim, int cols) { return 16 * cols * (dim + 2); }
 // workgroups of a compute unit, waves of a SIMD (a third would fit where dim * cols <= 128, with the 168 registers that leaves: a token of
 // 131072 took 59 us instead of 48, of 64-wide heads 34 instead of 29; the vector units are busy with two)
 constexpr int kPerCu = 2;
+
+// a row's token: slot / split, of slots under 64 (the fraction is off by less than 2^-10, the quotient's distance from the next is 2^-5 at least)
+__device__ __forceinline__ int token_of(const AttentionArgs &a, int slot) { return (int)((uint32_t)slot * a.split_part >> 16); }
+
+// a / b of numbers under 2^31: a quotient in fp32, off by 2^-22 of itself, then what it misses by, then one (a third of the instructions of /)
+__device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b) {
+    const float part = __builtin_amdgcn_rcpf((float)b);
+    uint32_t q = (uint32_t)((float)a * part);
+    q += (uint32_t)(int)floorf((float)(int)(a - q * b) * part);
+    const int left = (int)(a - q * b);
+    return q + (left >= (int)b) - (left < 0);
+}
 
 struct Sequence {
     int start, count, len;   // first row, rows, tokens in the cache; count 0 where there is nothing to do
@@ -266,7 +279,7 @@ template <int D, int NQ>
 __device__ __forceinline__ void load_queries(const AttentionArgs &a, const Item &it, int head0, int heads, Queries<D, NQ> &q, int wave, int lane) {
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
-        const int slot = g * 16 + (lane & 15), token = slot / a.split, head = slot - token * a.split;
+        const int slot = g * 16 + (lane & 15), token = token_of(a, slot), head = slot - token * a.split;
         const bool live = token < it.count && head < heads;
         const float *row = a.q + (int64_t)(it.first + (live ? token : 0)) * a.q_stride + (int64_t)(head0 + (live ? head : 0)) * D + 8 * (lane >> 4);
 #pragma unroll
@@ -283,7 +296,7 @@ __device__ __forceinline__ void stage_queries(const AttentionArgs &a, const Item
     const int col = lane & 15;
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
-        const int slot = g * 16 + col, token = slot / a.split;
+        const int slot = g * 16 + col, token = token_of(a, slot);
         const bool live = token < it.count && slot - token * a.split < heads;
         float most = 0.f;
         bool whole = true;
@@ -457,7 +470,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     int pos[NQ];                // position of the column's row, -1: no row
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
-        const int slot = g * 16 + col, token = slot / a.split;
+        const int slot = g * 16 + col, token = token_of(a, slot);
         pos[g] = token < it.count && slot - token * a.split < heads ? it.lo + token : -1;
     }
 
@@ -786,7 +799,7 @@ __device__ __forceinline__ f32x4 load_part(const f32x4 *p) {
 // rows of an item from sums: lane's column of 16 queries, 4 dimensions of 16
 template <int D, int NQ>
 __device__ __forceinline__ float *out_row(const AttentionArgs &a, const Item &it, int head0, int heads, int g, int lane, bool &live) {
-    const int slot = g * 16 + (lane & 15), token = slot / a.split, head = slot - token * a.split;
+    const int slot = g * 16 + (lane & 15), token = token_of(a, slot), head = slot - token * a.split;
     live = token < it.count && head < heads;
     return a.y + (int64_t)(it.first + (live ? token : 0)) * a.y_stride + (int64_t)(head0 + (live ? head : 0)) * D + 4 * (lane >> 4);
 }
@@ -909,7 +922,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
     // a thread's `per` places of the line of one head's items, those that hold an item (a sequence has as many places as max_q allows)
     const auto each_item = [&](auto &&f) {
         for (int u = id * per; u < min(units, (id + 1) * per);) {
-            const int s = a.row_tiles == 1 ? u : u / a.row_tiles, tile0 = u - s * a.row_tiles, tile1 = min(a.row_tiles, tile0 + min(units, (id + 1) * per) - u);
+            const int s = a.row_tiles == 1 ? u : (int)quotient(u, a.row_tiles), tile0 = u - s * a.row_tiles, tile1 = min(a.row_tiles, tile0 + min(units, (id + 1) * per) - u);
             bool bad;
             const Sequence q = sequence(a, s, bad);
             if (bad && tile0 == 0 && blockIdx.x == 0) atomicOr(a.error, kKvBadRows);
@@ -960,8 +973,8 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
     // calls.  Cut where they could stay whole, 512 prompt tokens took 27.5 us instead of 23.3, 4096 410 instead of 402.)
     const uint32_t groups = gridDim.x, heads_all = a.kv.n_head * a.splits;
     const int start = (uint32_t)head_turns * heads_all > groups ? 2 : 0;
-    const uint32_t share = ((uint32_t)(head_turns + start * head_items) * heads_all + groups - 1) / groups;
-    const bool whole_items = (uint32_t)(longest + start) <= share;
+    // (as long as a share: ceil(line / groups))
+    const bool whole_items = (uint64_t)(uint32_t)(longest + start - 1) * groups < (uint32_t)(head_turns + start * head_items) * heads_all;
     const int head_length = whole_items ? head_items : head_turns + start * head_items;
     lds.line[id][0] = whole_items ? items_before : turns_before + start * items_before;   // (each thread's own: kept out of the registers
     lds.line[id][1] = whole_items ? items_mine : turns_mine + start * items_mine;         // that the tiles want)
@@ -969,13 +982,13 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
     const uint32_t active = std::min(total, groups), per_xcd = (active + 7) / 8;
     const uint32_t me = whole_items ? blockIdx.x : (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
     if (me >= active || (!whole_items && blockIdx.x / 8 >= per_xcd)) return;
-    const uint32_t length = total / active, longer = total - length * active;     // the first `longer` stretches have one more
+    const uint32_t length = quotient(total, active), longer = total - length * active;     // the first `longer` stretches have one more
     uint32_t at = whole_items ? me : me * length + std::min(me, longer);
     const uint32_t end = whole_items ? total : at + length + (me < longer ? 1 : 0);
     uint32_t round = 0;
 
     while (at < end) {
-        const int hv = (int)(at / (uint32_t)head_length), off = (int)(at - (uint32_t)hv * head_length);
+        const int hv = (int)quotient(at, (uint32_t)head_length), off = (int)(at - (uint32_t)hv * head_length);
         const int before = lds.line[id][0], mine = lds.line[id][1];
         if (off >= before && off < before + mine) {     // one thread
             int b = before;
@@ -1018,7 +1031,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         const AttentionArgs &c = fresh_arguments();
         const auto stretch_of = [&](uint32_t p) {
             const uint32_t edge = longer * (length + 1);
-            return (int)(p < edge ? p / (length + 1) : longer + (p - edge) / length);
+            return (int)(p < edge ? quotient(p, length + 1) : longer + quotient(p - edge, length));
         };
         if (!c.arrived) {            // whoever writes an item's end says what is to be joined
             if (ends && id == 0) {
@@ -1169,6 +1182,7 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
         const int rows = 16 * cols;
         a.splits = (a.group + rows - 1) / rows;
         a.split = (a.group + a.splits - 1) / a.splits;
+        a.split_part = (65536 + a.split - 1) / a.split;
         a.tokens = rows / a.split;
         a.row_tiles = (int32_t)((j.max_q + a.tokens - 1) / a.tokens);
         items = std::min((double)a.n_seq * a.row_tiles, (double)a.n_tokens / a.tokens + a.n_seq) * j.kv->n_head * a.splits;
