@@ -103,19 +103,23 @@ constexpr int kPerCu = 2;
 __device__ __forceinline__ int token_of(const AttentionArgs &a, int slot) { return (int)((uint32_t)slot * a.split_part >> 16); }
 
 // a / b of numbers under 2^31: a quotient in fp32, off by 2^-22 of itself, then what it misses by, then one (a third of the instructions of /)
-__device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b) {
+__host__ __device__ __forceinline__ uint32_t quotient(uint32_t a, uint32_t b) {
+#if defined(__HIP_DEVICE_COMPILE__)
     const float part = __builtin_amdgcn_rcpf((float)b);
     uint32_t q = (uint32_t)((float)a * part);
     q += (uint32_t)(int)floorf((float)(int)(a - q * b) * part);
     const int left = (int)(a - q * b);
     return q + (left >= (int)b) - (left < 0);
+#else
+    return a / b;
+#endif
 }
 
 struct Sequence {
     int start, count, len;   // first row, rows, tokens in the cache; count 0 where there is nothing to do
 };
 
-__device__ __forceinline__ Sequence sequence(const AttentionArgs &a, int s, bool &bad) {
+__host__ __device__ __forceinline__ Sequence sequence(const AttentionArgs &a, int s, bool &bad) {
     Sequence q;
     q.start = a.q_start[s];
     const int end = a.q_start[s + 1];
@@ -133,7 +137,7 @@ struct Item {
     int see;
 };
 
-__device__ __forceinline__ Item item_of(const AttentionArgs &a, int s, const Sequence &q, int row_tile) {
+__host__ __device__ __forceinline__ Item item_of(const AttentionArgs &a, int s, const Sequence &q, int row_tile) {
     Item it;
     it.seq = s;
     it.first = q.start + row_tile * a.tokens;
@@ -144,9 +148,80 @@ __device__ __forceinline__ Item item_of(const AttentionArgs &a, int s, const Seq
     return it;
 }
 
-__device__ __forceinline__ int item_tiles(const Item &it) { return it.hi < 0 ? 1 : it.hi / kTile - it.see / kTile + 1; }
+__host__ __device__ __forceinline__ int item_tiles(const Item &it) { return it.hi < 0 ? 1 : it.hi / kTile - it.see / kTile + 1; }
 // what an item takes of the line: a turn of the waves for every kWaves tiles
-__device__ __forceinline__ int item_turns(const Item &it) { return it.count <= 0 ? 0 : (item_tiles(it) + kWaves - 1) / kWaves; }
+__host__ __device__ __forceinline__ int item_turns(const Item &it) { return it.count <= 0 ? 0 : (item_tiles(it) + kWaves - 1) / kWaves; }
+
+// Thread `id`'s places of the line of one head's items, `per` of them: f(sequence, row tile, rows, turns) of those that hold an item (a sequence has
+// as many places as max_q allows), until one returns true.  outside(sequence) of sequences that break the bounds.
+template <typename F, typename G>
+__host__ __device__ __forceinline__ void each_item(const AttentionArgs &a, int id, int units, int per, F &&f, G &&outside) {
+    for (int u = id * per; u < min(units, (id + 1) * per);) {
+        const int s = a.row_tiles == 1 ? u : (int)quotient(u, a.row_tiles), tile0 = u - s * a.row_tiles, tile1 = min(a.row_tiles, tile0 + min(units, (id + 1) * per) - u);
+        bool bad;
+        const Sequence q = sequence(a, s, bad);
+        if (bad && tile0 == 0) outside(s);
+        for (int tile = tile0; tile < tile1 && tile * a.tokens < q.count; ++tile)
+            if (f(s, tile, q, item_turns(item_of(a, s, q, tile)))) return;
+        u += tile1 - tile0;
+    }
+}
+
+// What a call's workgroups share out: the turns of all heads' items in one line, head by head.
+struct Line {
+    int start;               // what beginning an item counts as, in turns
+    bool whole;              // items stay whole: the line is one of items
+    int head_length;         // of one head
+    uint32_t total, active;  // of all; stretches, as many as workgroups have one
+    uint32_t length, longer; // a stretch's; the first `longer` have one more
+};
+
+__host__ __device__ __forceinline__ Line line_of(int head_turns, int head_items, int longest, uint32_t heads, uint32_t groups) {
+    // Where there are more turns than workgroups, beginning an item (staging its queries, adding its sums) counts as two turns.  Where no item
+    // is longer than a workgroup's share, items stay whole and are dealt out, forwards and backwards in turn: an item is as long as its
+    // rows are far from the start of their sequence, so that long ones meet short ones.  Otherwise every workgroup has a stretch of the
+    // line, of one length or one more; those of an XCD are neighbours.  (Without the charge 48 sequences took 67 us instead of 64.5, four
+    // with eight new tokens 32.6 instead of 28.3, heads of 64 behind 100000 tokens 31 instead of 29.4, but 64 of 2000 tokens 14.3 instead of
+    // 16.2; always charged, one of 8000 13.4 instead of 12.0; half of it, or from two turns a workgroup on, 1% more over 60 drawn
+    // calls.  Cut where they could stay whole, 512 prompt tokens took 27.5 us instead of 23.3, 4096 410 instead of 402.)
+    Line l;
+    l.start = (uint32_t)head_turns * heads > groups ? 2 : 0;
+    // (as long as a share: ceil(line / groups))
+    l.whole = (uint64_t)(uint32_t)(longest + l.start - 1) * groups < (uint32_t)(head_turns + l.start * head_items) * heads;
+    l.head_length = l.whole ? head_items : head_turns + l.start * head_items;
+    l.total = (uint32_t)l.head_length * heads;
+    l.active = l.total < groups ? l.total : groups;
+    l.length = l.active ? quotient(l.total, l.active) : 0;
+    l.longer = l.total - l.length * l.active;
+    return l;
+}
+
+// The stretch of a workgroup; those with none get a number behind the last.  Workgroups b, b + 8, ... are on one XCD: they have neighbours, and
+// those before `active` have every stretch once whatever the grid is.
+__host__ __device__ __forceinline__ uint32_t stretch_of_block(uint32_t block, uint32_t active) {
+    const uint32_t xcd = block % 8, rest = active % 8;
+    return block < active ? xcd * (active / 8) + (xcd < rest ? xcd : rest) + block / 8 : active;
+}
+
+// the stretch that has position p of the line
+__host__ __device__ __forceinline__ uint32_t stretch_at(const Line &l, uint32_t p) {
+    const uint32_t edge = l.longer * (l.length + 1);
+    return p < edge ? quotient(p, l.length + 1) : l.longer + quotient(p - edge, l.length);
+}
+
+// what a stretch takes of an item that it reaches at place `skip`, with `left` of the stretch to go: turns [from, to); none where it ends within
+// the item's start (to <= 0)
+struct Piece {
+    int take, from, to;
+};
+__host__ __device__ __forceinline__ Piece piece_of(const Line &l, int skip, int turns, uint32_t left) {
+    Piece p;
+    const uint32_t rest = (uint32_t)(turns + l.start - skip);
+    p.take = (int)(rest < left ? rest : left);
+    p.from = l.whole ? 0 : max(0, skip - l.start);
+    p.to = l.whole ? turns : skip + p.take - l.start;
+    return p;
+}
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -919,22 +994,10 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
     __shared__ __align__(16) SharedLds<D, NQ> lds;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
     const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
-    // a thread's `per` places of the line of one head's items, those that hold an item (a sequence has as many places as max_q allows)
-    const auto each_item = [&](auto &&f) {
-        for (int u = id * per; u < min(units, (id + 1) * per);) {
-            const int s = a.row_tiles == 1 ? u : (int)quotient(u, a.row_tiles), tile0 = u - s * a.row_tiles, tile1 = min(a.row_tiles, tile0 + min(units, (id + 1) * per) - u);
-            bool bad;
-            const Sequence q = sequence(a, s, bad);
-            if (bad && tile0 == 0 && blockIdx.x == 0) atomicOr(a.error, kKvBadRows);
-            for (int tile = tile0; tile < tile1 && tile * a.tokens < q.count; ++tile)
-                if (f(s, tile, q, item_turns(item_of(a, s, q, tile)))) return;
-            u += tile1 - tile0;
-        }
-    };
     if (id < 8) lds.found[id] = 0;      // (lengths that another stream changes meanwhile find no item: nothing, and not anything)
     // ---- the line of turns ----
     int turns_mine = 0, items_mine = 0, longest = 0;
-    each_item([&](int s, int tile, const Sequence &q, int n) {
+    each_item(a, id, units, per, [&](int s, int tile, const Sequence &q, int n) {
         const int item[6] = {s, tile, n, q.start, q.count, q.len};
         if (per == 1) {
 #pragma unroll
@@ -944,6 +1007,8 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         ++items_mine;
         longest = max(longest, n);
         return false;
+    }, [&](int) {
+        if (blockIdx.x == 0) atomicOr(a.error, kKvBadRows);
     });
     int turns_before = wave_scan(turns_mine), items_before = wave_scan(items_mine);
     longest = (int)wave_max((uint32_t)longest);
@@ -964,31 +1029,17 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         longest = max(longest, lds.waves[w][2]);
     }
     head_turns = uniform(head_turns), head_items = uniform(head_items), longest = uniform(longest);
-    // Where there are more turns than workgroups, beginning an item (staging its queries, adding its sums) counts as two turns.  Where no item
-    // is longer than a workgroup's share, items stay whole and are dealt out, forwards and backwards in turn: an item is as long as its
-    // rows are far from the start of their sequence, so that long ones meet short ones.  Otherwise every workgroup has a stretch of the
-    // line, of one length or one more; those of an XCD are neighbours.  (Without the charge 48 sequences took 67 us instead of 64.5, four
-    // with eight new tokens 32.6 instead of 28.3, heads of 64 behind 100000 tokens 31 instead of 29.4, but 64 of 2000 tokens 14.3 instead of
-    // 16.2; always charged, one of 8000 13.4 instead of 12.0; half of it, or from two turns a workgroup on, 1% more over 60 drawn
-    // calls.  Cut where they could stay whole, 512 prompt tokens took 27.5 us instead of 23.3, 4096 410 instead of 402.)
-    const uint32_t groups = gridDim.x, heads_all = a.kv.n_head * a.splits;
-    const int start = (uint32_t)head_turns * heads_all > groups ? 2 : 0;
-    // (as long as a share: ceil(line / groups))
-    const bool whole_items = (uint64_t)(uint32_t)(longest + start - 1) * groups < (uint32_t)(head_turns + start * head_items) * heads_all;
-    const int head_length = whole_items ? head_items : head_turns + start * head_items;
-    lds.line[id][0] = whole_items ? items_before : turns_before + start * items_before;   // (each thread's own: kept out of the registers
-    lds.line[id][1] = whole_items ? items_mine : turns_mine + start * items_mine;         // that the tiles want)
-    const uint32_t total = (uint32_t)head_length * heads_all;
-    const uint32_t active = std::min(total, groups), per_xcd = (active + 7) / 8;
-    const uint32_t me = whole_items ? blockIdx.x : (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
-    if (me >= active || (!whole_items && blockIdx.x / 8 >= per_xcd)) return;
-    const uint32_t length = quotient(total, active), longer = total - length * active;     // the first `longer` stretches have one more
-    uint32_t at = whole_items ? me : me * length + std::min(me, longer);
-    const uint32_t end = whole_items ? total : at + length + (me < longer ? 1 : 0);
+    const Line line = line_of(head_turns, head_items, longest, a.kv.n_head * a.splits, gridDim.x);
+    lds.line[id][0] = line.whole ? items_before : turns_before + line.start * items_before;   // (each thread's own: kept out of the registers
+    lds.line[id][1] = line.whole ? items_mine : turns_mine + line.start * items_mine;         // that the tiles want)
+    const uint32_t me = line.whole ? blockIdx.x : stretch_of_block(blockIdx.x, line.active);
+    if (me >= line.active) return;
+    uint32_t at = line.whole ? me : me * line.length + std::min(me, line.longer);
+    const uint32_t end = line.whole ? line.total : at + line.length + (me < line.longer ? 1 : 0);
     uint32_t round = 0;
 
     while (at < end) {
-        const int hv = (int)quotient(at, (uint32_t)head_length), off = (int)(at - (uint32_t)hv * head_length);
+        const int hv = (int)quotient(at, (uint32_t)line.head_length), off = (int)(at - (uint32_t)hv * line.head_length);
         const int before = lds.line[id][0], mine = lds.line[id][1];
         if (off >= before && off < before + mine) {     // one thread
             int b = before;
@@ -996,8 +1047,8 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
 #pragma unroll
                 for (int i = 0; i < 6; ++i) lds.found[i] = lds.only[i][id];
             } else {
-                each_item([&](int s, int tile, const Sequence &q, int n) {
-                    const int weight = whole_items ? 1 : n + start;
+                each_item(a, id, units, per, [&](int s, int tile, const Sequence &q, int n) {
+                    const int weight = line.whole ? 1 : n + line.start;
                     if (off >= b + weight) {
                         b += weight;
                         return false;
@@ -1006,7 +1057,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
 #pragma unroll
                     for (int i = 0; i < 6; ++i) lds.found[i] = item[i];
                     return true;
-                });
+                }, [](int) {});
             }
             lds.found[6] = b;
         }
@@ -1017,31 +1068,26 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         const AttentionArgs &a = fresh_arguments();
         const int kv_head = a.splits == 1 ? hv : hv / a.splits, go = hv - kv_head * a.splits;
         const int head0 = kv_head * a.group + go * a.split, heads = min(a.split, a.group - go * a.split);
-        // the stretch's turns of the item: none where it ends within the item's start
-        const int skip = off - first, take = (int)std::min<uint32_t>(turns + start - skip, end - at);
-        const int turn0 = whole_items ? 0 : max(0, skip - start), turn1 = whole_items ? turns : skip + take - start;
-        if (turn1 <= 0) break;
-        const int tile0 = it.hi < 0 ? 0 : it.see / kTile, tile1 = tile0 + min(turn1 * kWaves, item_tiles(it));
+        const int skip = off - first;
+        const Piece piece = piece_of(line, skip, turns, end - at);
+        if (piece.to <= 0) break;
+        const int tile0 = it.hi < 0 ? 0 : it.see / kTile, tile1 = tile0 + min(piece.to * kWaves, item_tiles(it));
 
         Running<D, NQ> st;
-        walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + turn0 * kWaves + wave, tile1, lds, wave, st, lane);
+        walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + piece.from * kWaves + wave, tile1, lds, wave, st, lane);
         // ---- the waves' sums ----
-        const bool starts = turn0 == 0, ends = turn1 == turns;
+        const bool starts = piece.from == 0, ends = piece.to == turns;
         meet<D, NQ>(fresh_arguments(), it, head0, heads, st, starts && ends, fresh_arguments().parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ), lds, wave, lane);
         const AttentionArgs &c = fresh_arguments();
-        const auto stretch_of = [&](uint32_t p) {
-            const uint32_t edge = longer * (length + 1);
-            return (int)(p < edge ? quotient(p, length + 1) : longer + quotient(p - edge, length));
-        };
         if (!c.arrived) {            // whoever writes an item's end says what is to be joined
             if (ends && id == 0) {
                 int32_t *const join = c.joins + 2 * ((int64_t)hv * c.n_seq * c.row_tiles + seq * c.row_tiles + row_tile);
-                join[0] = starts ? -1 : stretch_of(at - skip + start);
+                join[0] = starts ? -1 : (int32_t)stretch_at(line, at - skip + line.start);
                 join[1] = (int32_t)me;
             }
         } else if (!(starts && ends)) {
             // The part is in memory before it is counted (the wait is for the stores); whoever counts the last one loads them after that.
-            const int first = stretch_of(at - skip + start), parts = stretch_of(at - skip + start + turns - 1) - first + 1;
+            const int first = (int)stretch_at(line, at - skip + line.start), parts = (int)stretch_at(line, at - skip + line.start + turns - 1) - first + 1;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             if (id == 0) lds.last = __hip_atomic_fetch_add(c.arrived + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
@@ -1051,11 +1097,11 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
                 join_parts<D, NQ>(c, it, head0, heads, first, parts, lds, wave, lane);
             }
         }
-        if (whole_items) {
+        if (line.whole) {
             ++round;
-            at = round * active + (round & 1 ? active - 1 - me : me);
+            at = round * line.active + (round & 1 ? line.active - 1 - me : me);
         } else {
-            at += take;
+            at += piece.take;
         }
         if (at < end) __syncthreads();
     }
@@ -1216,6 +1262,82 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     if (a.kv.dim == 64) return launch<64, 2>(a, groups, (int)places, s);
     if (a.kv.dim == 96) return launch<96, 2>(a, groups, (int)places, s);
     return launch<128, 2>(a, groups, (int)places, s);
+}
+
+// For the tests: the pieces of the line that every workgroup of a call takes, in the order in which it takes them, worked out on the host by the
+// kernel's own arithmetic.  A piece is {workgroup, head, sequence, row tile, its turns from, to, all the item's turns, first and last stretch of the item}.
+// Their number, or -1 where a workgroup would not come to an end.
+int64_t attention_pieces(const AttentionJob &j, int64_t most_len, int tokens, int heads, int groups, int32_t *out, int64_t room) {
+    AttentionArgs a{};
+    a.pages_stride = most_len;      // (pages of one token)
+    a.n_tokens = (int32_t)j.n_tokens, a.n_seq = (int32_t)j.n_seq, a.max_q = (int32_t)j.max_q, a.window = j.window;
+    a.q_start = j.q_start, a.kv_len = j.kv_len;
+    a.tokens = tokens;
+    a.row_tiles = (a.max_q + tokens - 1) / tokens;
+    const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
+    struct Thread { int turns_before, items_before, turns, items, only[3]; } threads[kThreads];
+    int head_turns = 0, head_items = 0, longest = 0;
+    for (int id = 0; id < kThreads; ++id) {
+        Thread &t = threads[id];
+        t = Thread{head_turns, head_items, 0, 0, {0, 0, 0}};
+        each_item(a, id, units, per, [&](int s, int tile, const Sequence &, int n) {
+            t.only[0] = s, t.only[1] = tile, t.only[2] = n;
+            t.turns += n;
+            ++t.items;
+            longest = max(longest, n);
+            return false;
+        }, [](int) {});
+        head_turns += t.turns, head_items += t.items;
+    }
+    const Line line = line_of(head_turns, head_items, longest, heads, groups);
+    int64_t pieces = 0;
+    for (int block = 0; block < groups; ++block) {
+        const uint32_t me = line.whole ? block : stretch_of_block(block, line.active);
+        if (me >= line.active) continue;
+        uint32_t at = line.whole ? me : me * line.length + std::min(me, line.longer);
+        const uint32_t end = line.whole ? line.total : at + line.length + (me < line.longer ? 1 : 0);
+        uint32_t round = 0;
+        int found[4] = {0, 0, 0, 0};
+        for (int64_t steps = 0; at < end; ++steps) {
+            if (steps > line.total) return -1;
+            const int hv = (int)quotient(at, (uint32_t)line.head_length), off = (int)(at - (uint32_t)hv * line.head_length);
+            for (int id = 0; id < kThreads; ++id) {
+                const Thread &t = threads[id];
+                int b = line.whole ? t.items_before : t.turns_before + line.start * t.items_before;
+                if (off < b || off >= b + (line.whole ? t.items : t.turns + line.start * t.items)) continue;
+                if (per == 1) {
+                    found[0] = t.only[0], found[1] = t.only[1], found[2] = t.only[2];
+                } else {
+                    each_item(a, id, units, per, [&](int s, int tile, const Sequence &, int n) {
+                        const int weight = line.whole ? 1 : n + line.start;
+                        if (off >= b + weight) {
+                            b += weight;
+                            return false;
+                        }
+                        found[0] = s, found[1] = tile, found[2] = n;
+                        return true;
+                    }, [](int) {});
+                }
+                found[3] = b;
+            }
+            const int turns = found[2], skip = off - found[3];
+            const Piece piece = piece_of(line, skip, turns, end - at);
+            if (piece.to <= 0) break;
+            const uint32_t first = line.whole ? me : stretch_at(line, at - skip + line.start), last = line.whole ? me : stretch_at(line, at - skip + line.start + turns - 1);
+            if (pieces < room) {
+                const int32_t row[9] = {block, hv, found[0], found[1], piece.from, piece.to, turns, (int32_t)first, (int32_t)last};
+                for (int i = 0; i < 9; ++i) out[9 * pieces + i] = row[i];
+            }
+            ++pieces;
+            if (line.whole) {
+                ++round;
+                at = round * line.active + (round & 1 ? line.active - 1 - me : me);
+            } else {
+                at += piece.take;
+            }
+        }
+    }
+    return pieces;
 }
 
 }  // namespace qproj

@@ -1,0 +1,110 @@
+"""How attention's work is shared out among workgroups, on the CPU: the grid from the plan of a call on a context without a device, the
+pieces from the kernel's own arithmetic compiled for the host.  Every turn of every item has to be taken by one workgroup."""
+import ctypes as C
+import re
+
+import numpy as np
+import pytest
+
+from test_attention_cpu import Dry, cache, call
+
+
+def plan(heads_kv, group, n, seqs, max_q, table_pages, page, dim=128, window=0):
+    """(tokens of an item, heads of the line, workgroups) of the launch of such a call"""
+    heads = heads_kv * group
+    with Dry() as dry:
+        assert call(dry, "attention", cache(n_pages=max(1, seqs * table_pages), page_tokens=page, n_head_kv=heads_kv, head_dim=dim), h=heads, qs=heads * dim,
+                    ys=heads * dim, n=n, seqs=seqs, max_q=max_q, ps=table_pages, window=window) == 0
+    m = re.search(r"heads in (\d+) x (\d+) of \d+, (\d+) tokens x (\d+) a sequence of rows, grid (\d+) x", dry.plan)
+    kv, splits, tokens, _, grid = (int(v) for v in m.groups())
+    return tokens, kv * splits, grid
+
+
+def pieces(q_start, kv_len, n, max_q, most_len, window, tokens, heads, grid):
+    """[workgroup, head, sequence, row tile, from, to, turns, first stretch, last stretch] of every piece"""
+    from magnitude_amd import qproj
+    f = qproj.load_library().qproj_internal_attention_pieces
+    f.restype, f.argtypes = C.c_int64, [C.c_void_p, C.c_void_p] + [C.c_int64] * 8 + [C.c_void_p, C.c_int64]
+    start, lens = np.ascontiguousarray(q_start, np.int32), np.ascontiguousarray(kv_len, np.int32)
+    room = 1 << 16
+    out = np.zeros((room, 9), np.int32)
+    got = f(start.ctypes.data, lens.ctypes.data, len(lens), n, max_q, most_len, window, tokens, heads, grid, out.ctypes.data, room)
+    assert 0 <= got <= room, "a workgroup does not come to an end"
+    return out[:got]
+
+
+def items(q_start, kv_len, tokens, window):
+    """{(sequence, row tile): turns}, from the definition: rows at positions lo .. hi see tokens max(0, lo - window + 1) .. hi, 256 of them a turn from
+    a multiple of 64 on"""
+    got = {}
+    for s in range(len(kv_len)):
+        count = q_start[s + 1] - q_start[s]
+        for tile in range(-(-count // tokens)):
+            lo = kv_len[s] - count + tile * tokens
+            hi = lo + min(tokens, count - tile * tokens) - 1
+            see = max(0, lo - window + 1) if window else 0
+            got[s, tile] = 1 if hi < 0 else -(-(hi // 64 - see // 64 + 1) // 4)
+    return got
+
+
+def check(heads_kv, group, seqs, page, spare=0, window=0, max_q=None, dim=128):
+    """seqs: (tokens in the cache, new ones)"""
+    lens, q_start = [n for n, _ in seqs], np.cumsum([0] + [m for _, m in seqs]).tolist()
+    n, max_q = q_start[-1], max_q or max(m for _, m in seqs)
+    table = max(-(-v // page) for v in lens) + spare
+    tokens, heads, grid = plan(heads_kv, group, n, len(seqs), max_q, table, page, dim, window)
+    got = pieces(q_start, lens, n, max_q, table * page, window, tokens, heads, grid)
+    want = items(q_start, lens, tokens, window)
+    assert (got[:, 0] < grid).all()
+    taken = {}
+    for row in got.tolist():
+        taken.setdefault(tuple(row[1:4]), []).append(row)
+    assert set(taken) == {(h, s, t) for h in range(heads) for s, t in want}
+    for (h, s, t), parts in taken.items():
+        parts.sort(key=lambda r: r[4])
+        assert parts[0][6] == want[s, t] and parts[0][4] == 0 and parts[-1][5] == want[s, t]
+        assert all(a[5] == b[4] for a, b in zip(parts, parts[1:]))                       # one after the other, nothing between
+        assert all(r[7:] == parts[0][7:] for r in parts) and len(parts) == parts[0][8] - parts[0][7] + 1     # as many as the item is said to have
+        assert len({r[0] for r in parts}) == len(parts)
+    return len(got)
+
+
+def test_every_stretch_has_one_workgroup():
+    """the numbering reaches each of `active` stretches once from any grid that has as many workgroups"""
+    for active in range(1, 700):
+        # one head, one sequence that needs exactly `active` turns, in a table of exactly its pages
+        for grid in {active, active + 1, active + 5, 1024}:
+            got = pieces([0, 1], [256 * active - 3], 1, 1, 256 * active, 0, 16, 1, grid)
+            assert sorted(got[:, 4]) == list(range(active)) and len(set(got[:, 0])) == active
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("spare", [0, 1, 300])
+def test_every_length_of_one_token(page, spare):
+    for heads_kv, group in ((1, 4), (1, 32), (2, 7), (3, 1), (4, 8), (5, 3), (7, 2), (8, 4)):
+        for length in list(range(1, 4000, 137)) + [255, 256, 257, 512, 513, 1025, 1300, 1537, 2049, 2100, 9000, 22604]:
+            check(heads_kv, group, [(length, 1)], page, spare)
+
+
+@pytest.mark.parametrize("heads_kv", range(1, 9))
+def test_shapes(heads_kv):
+    rng = np.random.default_rng(heads_kv)
+    for group in list(range(1, 17)) + [71]:
+        for _ in range(12):
+            most = int(np.exp(rng.uniform(0, np.log(9000))))
+            rows = int(rng.choice([1, 1, 2, 8, 27, 64]))
+            seqs = [(int(rng.integers(0, most + 1)), int(rng.integers(0 if rows > 1 else 1, rows + 1))) for _ in range(rng.integers(1, 7))]
+            if rng.random() < 0.5:
+                seqs = [(most, rows)] * len(seqs)
+            seqs[0] = (max(1, seqs[0][0]), max(1, seqs[0][1]))
+            check(heads_kv, group, seqs, int(rng.choice([16, 64, 256])), int(rng.choice([0, 0, 1, 500])), int(rng.choice([0, 0, 1, 100, 5000])),
+                  dim=int(rng.choice([64, 128, 256])))
+
+
+def test_many_sequences():
+    """more places than threads, so that the line is searched again for every item"""
+    rng = np.random.default_rng(9)
+    for n in (255, 256, 257, 700):
+        check(2, 4, [(int(v), 1) for v in rng.integers(1, 600, n)], 16)
+        check(1, 4, [(30000, 1)] + [(int(v), 1) for v in rng.integers(1, 600, n - 1)], 16, window=7000)
+    check(2, 4, [(int(v), 40) for v in rng.integers(0, 600, 30)] + [(2000, 300)], 16, max_q=331)

@@ -1,0 +1,70 @@
+"""Attention where the grid has hardly more workgroups than the call has stretches of work, against plain statements in 64 bits (kv_ref.py): tables
+of exactly the pages that are needed, few heads, lengths on both sides of what a turn takes."""
+import numpy as np
+import pytest
+import torch
+
+import kv_ref
+from test_attention_gpu import check, dev, make_cache, numpy_cache, tell
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    """one context for all calls, one after the other"""
+    from magnitude_amd import Context
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    c = Context(0)
+    yield c
+    c.close()
+
+
+def exact_table(rng, lens, page, kv_heads, dim):
+    kv, pages = make_cache(rng, lens, page, kv_heads, dim)
+    return kv, np.ascontiguousarray(pages[:, :max(1, max(-(-n // page) for n in lens))])
+
+
+@pytest.mark.parametrize("length", [257, 513, 1025, 1300, 1537, 2049, 2100, 9000])
+@pytest.mark.parametrize("kv_heads,group,dim,page", [(1, 4, 128, 64), (2, 7, 64, 16), (3, 1, 96, 32), (4, 8, 128, 64), (5, 3, 256, 16), (1, 71, 128, 64)])
+def test_a_token_in_a_table_of_its_pages(ctx, kv_heads, group, dim, page, length):
+    tell("a token", kv_heads, group, dim, page, length)
+    rng = np.random.default_rng(length + kv_heads)
+    kv, pages = exact_table(rng, [length], page, kv_heads, dim)
+    q = rng.standard_normal((1, kv_heads * group, dim)).astype(np.float32)
+    check(ctx, kv, pages, q, [0, 1], [length], max_q=1)
+
+
+@pytest.mark.parametrize("kv_heads,lens,new", [(1, [2100] * 2, 1), (1, [1100] * 3, 1), (2, [1300] * 3, 1), (1, [777] * 5, 1), (3, [1025, 900], 1), (1, [1500], 9),
+                                               (2, [700, 650, 600], 4), (4, [1550], 1), (1, [1900], 27)])
+def test_few_sequences_of_like_lengths(ctx, kv_heads, lens, new):
+    tell("few sequences", kv_heads, lens, new)
+    rng = np.random.default_rng(sum(lens) + kv_heads)
+    kv, pages = exact_table(rng, lens, 64, kv_heads, 128)
+    q_start = np.arange(len(lens) + 1) * new
+    q = rng.standard_normal((q_start[-1], kv_heads * 4, 128)).astype(np.float32)
+    check(ctx, kv, pages, q, q_start, lens, max_q=new)
+    check(ctx, kv, pages, q, q_start, lens, window=500, max_q=new)
+
+
+def test_two_contexts_at_once_have_the_right_results():
+    from magnitude_amd import Context
+    rng = np.random.default_rng(16)
+    work = []
+    for lens, kv_heads in (([9000], 1), ([3000, 10, 700, 2000], 8), ([1300], 2)):
+        stream = torch.cuda.Stream()
+        kv, pages = exact_table(rng, lens, 64, kv_heads, 128)
+        q = rng.standard_normal((len(lens), 4 * kv_heads, 128)).astype(np.float32)
+        start = np.arange(len(lens) + 1, dtype=np.int32)
+        want, sizes = kv_ref.attention(numpy_cache(kv), q, start, lens, pages, 128 ** -0.5)
+        args = kv, dev(q), dev(start), dev(np.array(lens, np.int32)), dev(pages)
+        work.append((Context(0, stream=stream.cuda_stream), args, want, kv_ref.allowed(sizes, 128, max(lens)), [torch.zeros_like(args[1]) for _ in range(10)]))
+    torch.cuda.synchronize()
+    for i in range(10):
+        for c, args, _, _, outs in work:
+            c.attention(*args, max_q=1, out=outs[i], sync=False)
+    for c, _, want, bound, outs in work:
+        c.sync()
+        for o in outs:
+            assert (np.abs(o.cpu().numpy() - want) <= bound).all()
+        c.close()
