@@ -144,7 +144,7 @@ __host__ __device__ __forceinline__ Item item_of(const AttentionArgs &a, int s, 
     it.count = min(a.tokens, q.count - row_tile * a.tokens);
     it.lo = q.len - q.count + row_tile * a.tokens;
     it.hi = it.lo + it.count - 1;
-    it.see = a.window ? max(0, it.lo - a.window + 1) : 0;
+    it.see = a.window && it.lo >= a.window ? it.lo - a.window + 1 : 0;     // (lo is negative where a sequence has more rows than tokens)
     return it;
 }
 

@@ -1842,7 +1842,7 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
     j.max_q = std::min(max_q, n_tokens);
     j.pages_stride = pages_stride;
     j.scale = scale;
-    j.window = (int32_t)std::min<int64_t>(window, 0x7fffffff);
+    j.window = window < pages_stride * kv->page_tokens ? (int32_t)window : 0;    // (a window as long as a sequence can be hides nothing)
     j.error = ctx->flag_dev + 1;
     QP_HIP(ctx, launch_attention(j, ctx->stream));
     return QPROJ_OK;

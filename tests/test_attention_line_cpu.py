@@ -108,3 +108,17 @@ def test_many_sequences():
         check(2, 4, [(int(v), 1) for v in rng.integers(1, 600, n)], 16)
         check(1, 4, [(30000, 1)] + [(int(v), 1) for v in rng.integers(1, 600, n - 1)], 16, window=7000)
     check(2, 4, [(int(v), 40) for v in rng.integers(0, 600, 30)] + [(2000, 300)], 16, max_q=331)
+
+
+@pytest.mark.parametrize("window", [1, 2, 1 << 20, (1 << 31) - 2, (1 << 31) - 1])
+def test_windows_of_any_size_behind_more_rows_than_tokens(window):
+    """rows that stand before the first token: position minus window must not leave 32 bits"""
+    q_start, lens = [0, 8, 40, 41], [3, 0, 700]
+    for tokens in (1, 4, 16):
+        got = pieces(q_start, lens, 41, 32, 1024, window, tokens, 2, 64)
+        want = items(q_start, lens, tokens, window)
+        for (s, t), turns in want.items():
+            for head in range(2):
+                mine = got[(got[:, 1:4] == (head, s, t)).all(1)]
+                assert (mine[:, 6] == turns).all() and (mine[:, 5] - mine[:, 4]).sum() == turns
+        assert len({tuple(r) for r in got[:, 1:4].tolist()}) == 2 * len(want)

@@ -68,3 +68,15 @@ def test_two_contexts_at_once_have_the_right_results():
         for o in outs:
             assert (np.abs(o.cpu().numpy() - want) <= bound).all()
         c.close()
+
+
+@pytest.mark.parametrize("window", [47, 48, 49, (1 << 31) - 1, 1 << 31, 1 << 62])
+def test_windows_of_any_size(ctx, window):
+    """as long as a sequence can be and longer, where rows stand before the first token"""
+    tell("window", window)
+    rng = np.random.default_rng(21)
+    lens, q_start = [3, 0, 40, 48], [0, 8, 12, 13, 33]
+    kv, pages = exact_table(rng, lens, 16, 2, 128)
+    q = rng.standard_normal((33, 8, 128)).astype(np.float32)
+    got = check(ctx, kv, pages, q, q_start, lens, window=window)
+    assert not got[:5].any() and got[5:8].any() and not got[8:12].any() and got[12:].any()
