@@ -203,10 +203,11 @@ __host__ __device__ __forceinline__ uint32_t stretch_of_block(uint32_t block, ui
     return block < active ? xcd * (active / 8) + (xcd < rest ? xcd : rest) + block / 8 : active;
 }
 
-// the stretch that has position p of the line
+// the stretch that has position p of the line (the last one of what lies behind: where lengths change during a call, an item may seem to reach there)
 __host__ __device__ __forceinline__ uint32_t stretch_at(const Line &l, uint32_t p) {
-    const uint32_t edge = l.longer * (l.length + 1);
-    return p < edge ? quotient(p, l.length + 1) : l.longer + quotient(p - edge, l.length);
+    const uint32_t edge = l.longer * (l.length + 1), last = l.active - 1;
+    const uint32_t at = p < edge ? quotient(p, l.length + 1) : l.longer + quotient(p - edge, l.length);
+    return at < last ? at : last;
 }
 
 // what a stretch takes of an item that it reaches at place `skip`, with `left` of the stretch to go: turns [from, to); none where it ends within
@@ -331,7 +332,8 @@ struct SharedLds {
     int32_t only[6][kThreads];    // where a thread has one place of the line: its item, as in `found`
     int32_t waves[kWaves][3];     // a wave's: turns, items, the longest
     int32_t last;                 // whether the workgroup wrote the last part of an item
-    int32_t found[8];             // sequence, row tile, its turns, the sequence's first row, rows, tokens, and what is before the item
+    int32_t found[8];             // sequence, row tile, its turns, the sequence's first row, rows, tokens, what is before the item; the place of the line
+                                  // that was looked for, and one
 };
 
 // what a wave holds of an item
@@ -994,7 +996,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
     __shared__ __align__(16) SharedLds<D, NQ> lds;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
     const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
-    if (id < 8) lds.found[id] = 0;      // (lengths that another stream changes meanwhile find no item: nothing, and not anything)
+    if (id == 0) lds.found[7] = 0;
     // ---- the line of turns ----
     int turns_mine = 0, items_mine = 0, longest = 0;
     each_item(a, id, units, per, [&](int s, int tile, const Sequence &q, int n) {
@@ -1046,6 +1048,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
             if (per == 1) {
 #pragma unroll
                 for (int i = 0; i < 6; ++i) lds.found[i] = lds.only[i][id];
+                lds.found[7] = (int)at + 1;
             } else {
                 each_item(a, id, units, per, [&](int s, int tile, const Sequence &q, int n) {
                     const int weight = line.whole ? 1 : n + line.start;
@@ -1056,12 +1059,14 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
                     const int item[6] = {s, tile, n, q.start, q.count, q.len};
 #pragma unroll
                     for (int i = 0; i < 6; ++i) lds.found[i] = item[i];
+                    lds.found[7] = (int)at + 1;
                     return true;
                 }, [](int) {});
             }
             lds.found[6] = b;
         }
         __syncthreads();
+        if (uniform(lds.found[7]) != (int)at + 1) break;    // lengths that another stream changes meanwhile: no item is there any more
         const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), turns = uniform(lds.found[2]), first = uniform(lds.found[6]);
         const Sequence q = {uniform(lds.found[3]), uniform(lds.found[4]), uniform(lds.found[5])};
         const Item it = item_of(a, seq, q, row_tile);
@@ -1266,8 +1271,8 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
 
 // For the tests: the pieces of the line that every workgroup of a call takes, in the order in which it takes them, worked out on the host by the
 // kernel's own arithmetic.  A piece is {workgroup, head, sequence, row tile, its turns from, to, all the item's turns, first and last stretch of the item}.
-// Their number, or -1 where a workgroup would not come to an end.
-int64_t attention_pieces(const AttentionJob &j, int64_t most_len, int tokens, int heads, int groups, int32_t *out, int64_t room) {
+// Their number, or -1 where a workgroup would not come to an end.  kv_len_later: what the lengths are when an item is looked for.
+int64_t attention_pieces(const AttentionJob &j, const int32_t *kv_len_later, int64_t most_len, int tokens, int heads, int groups, int32_t *out, int64_t room) {
     AttentionArgs a{};
     a.pages_stride = most_len;      // (pages of one token)
     a.n_tokens = (int32_t)j.n_tokens, a.n_seq = (int32_t)j.n_seq, a.max_q = (int32_t)j.max_q, a.window = j.window;
@@ -1290,6 +1295,7 @@ int64_t attention_pieces(const AttentionJob &j, int64_t most_len, int tokens, in
         head_turns += t.turns, head_items += t.items;
     }
     const Line line = line_of(head_turns, head_items, longest, heads, groups);
+    a.kv_len = kv_len_later;
     int64_t pieces = 0;
     for (int block = 0; block < groups; ++block) {
         const uint32_t me = line.whole ? block : stretch_of_block(block, line.active);
@@ -1297,7 +1303,7 @@ int64_t attention_pieces(const AttentionJob &j, int64_t most_len, int tokens, in
         uint32_t at = line.whole ? me : me * line.length + std::min(me, line.longer);
         const uint32_t end = line.whole ? line.total : at + line.length + (me < line.longer ? 1 : 0);
         uint32_t round = 0;
-        int found[4] = {0, 0, 0, 0};
+        int found[5] = {0, 0, 0, 0, 0};
         for (int64_t steps = 0; at < end; ++steps) {
             if (steps > line.total) return -1;
             const int hv = (int)quotient(at, (uint32_t)line.head_length), off = (int)(at - (uint32_t)hv * line.head_length);
@@ -1306,7 +1312,7 @@ int64_t attention_pieces(const AttentionJob &j, int64_t most_len, int tokens, in
                 int b = line.whole ? t.items_before : t.turns_before + line.start * t.items_before;
                 if (off < b || off >= b + (line.whole ? t.items : t.turns + line.start * t.items)) continue;
                 if (per == 1) {
-                    found[0] = t.only[0], found[1] = t.only[1], found[2] = t.only[2];
+                    found[0] = t.only[0], found[1] = t.only[1], found[2] = t.only[2], found[4] = (int)at + 1;
                 } else {
                     each_item(a, id, units, per, [&](int s, int tile, const Sequence &, int n) {
                         const int weight = line.whole ? 1 : n + line.start;
@@ -1314,12 +1320,13 @@ int64_t attention_pieces(const AttentionJob &j, int64_t most_len, int tokens, in
                             b += weight;
                             return false;
                         }
-                        found[0] = s, found[1] = tile, found[2] = n;
+                        found[0] = s, found[1] = tile, found[2] = n, found[4] = (int)at + 1;
                         return true;
                     }, [](int) {});
                 }
                 found[3] = b;
             }
+            if (found[4] != (int)at + 1) break;
             const int turns = found[2], skip = off - found[3];
             const Piece piece = piece_of(line, skip, turns, end - at);
             if (piece.to <= 0) break;

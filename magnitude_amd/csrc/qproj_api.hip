@@ -1870,8 +1870,9 @@ int qproj_internal_dry_end(qproj_ctx *ctx, char *buf, size_t buf_bytes) {
     return rc;
 }
 
-// For the tests: which workgroup of an attention call takes what, worked out on the host (attention_pieces).  q_start and kv_len are host arrays.
-int64_t qproj_internal_attention_pieces(const int32_t *q_start, const int32_t *kv_len, int64_t n_seq, int64_t n_tokens, int64_t max_q, int64_t most_len, int64_t window,
+// For the tests: which workgroup of an attention call takes what, worked out on the host (attention_pieces).  q_start and kv_len are host arrays;
+// kv_len_later (null: kv_len) stands in it where a workgroup looks for its items.
+int64_t qproj_internal_attention_pieces(const int32_t *q_start, const int32_t *kv_len, const int32_t *kv_len_later, int64_t n_seq, int64_t n_tokens, int64_t max_q, int64_t most_len, int64_t window,
                                         int64_t tokens, int64_t heads, int64_t groups, int32_t *out, int64_t room) {
     AttentionJob j{};
     j.q_start = q_start;
@@ -1880,7 +1881,7 @@ int64_t qproj_internal_attention_pieces(const int32_t *q_start, const int32_t *k
     j.n_tokens = n_tokens;
     j.max_q = max_q;
     j.window = (int32_t)window;
-    return attention_pieces(j, most_len, (int)tokens, (int)heads, (int)groups, out, room);
+    return attention_pieces(j, kv_len_later ? kv_len_later : kv_len, most_len, (int)tokens, (int)heads, (int)groups, out, room);
 }
 
 }  // extern "C"

@@ -347,6 +347,6 @@ struct AttentionJob {
 };
 size_t attention_scratch_bytes(int cus);
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s);
-int64_t attention_pieces(const AttentionJob &j, int64_t most_len, int tokens, int heads, int groups, int32_t *out, int64_t room);   // for the tests
+int64_t attention_pieces(const AttentionJob &j, const int32_t *kv_len_later, int64_t most_len, int tokens, int heads, int groups, int32_t *out, int64_t room);   // for the tests
 
 }  // namespace qproj

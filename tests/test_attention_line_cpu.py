@@ -20,15 +20,16 @@ def plan(heads_kv, group, n, seqs, max_q, table_pages, page, dim=128, window=0):
     return tokens, kv * splits, grid
 
 
-def pieces(q_start, kv_len, n, max_q, most_len, window, tokens, heads, grid):
+def pieces(q_start, kv_len, n, max_q, most_len, window, tokens, heads, grid, later=None):
     """[workgroup, head, sequence, row tile, from, to, turns, first stretch, last stretch] of every piece"""
     from magnitude_amd import qproj
     f = qproj.load_library().qproj_internal_attention_pieces
-    f.restype, f.argtypes = C.c_int64, [C.c_void_p, C.c_void_p] + [C.c_int64] * 8 + [C.c_void_p, C.c_int64]
+    f.restype, f.argtypes = C.c_int64, [C.c_void_p] * 3 + [C.c_int64] * 8 + [C.c_void_p, C.c_int64]
     start, lens = np.ascontiguousarray(q_start, np.int32), np.ascontiguousarray(kv_len, np.int32)
+    later = lens if later is None else np.ascontiguousarray(later, np.int32)
     room = 1 << 16
     out = np.zeros((room, 9), np.int32)
-    got = f(start.ctypes.data, lens.ctypes.data, len(lens), n, max_q, most_len, window, tokens, heads, grid, out.ctypes.data, room)
+    got = f(start.ctypes.data, lens.ctypes.data, later.ctypes.data, len(lens), n, max_q, most_len, window, tokens, heads, grid, out.ctypes.data, room)
     assert 0 <= got <= room, "a workgroup does not come to an end"
     return out[:got]
 
@@ -122,3 +123,22 @@ def test_windows_of_any_size_behind_more_rows_than_tokens(window):
                 mine = got[(got[:, 1:4] == (head, s, t)).all(1)]
                 assert (mine[:, 6] == turns).all() and (mine[:, 5] - mine[:, 4]).sum() == turns
         assert len({tuple(r) for r in got[:, 1:4].tolist()}) == 2 * len(want)
+
+
+@pytest.mark.parametrize("seqs,most", [(300, 400), (300, 20000), (257, 60000), (600, 3000), (40, 9000)])
+def test_lengths_that_change_during_a_call(seqs, most):
+    """what a workgroup finds where it looks again is not what it counted: it comes to an end all the same, and stays among the stretches there are"""
+    rng = np.random.default_rng(seqs + most)
+    for i in range(60):
+        lens, later = rng.integers(0, most + 1, seqs), rng.integers(0, most + 1, seqs)
+        if i % 4 == 1:
+            later = np.minimum(later, lens)
+        if i % 4 == 2:
+            later = np.maximum(later, lens)
+        if i % 4 == 3:
+            later = np.where(rng.random(seqs) < 0.01, later, lens)
+        heads, grid = int(rng.integers(1, 9)), int(rng.choice([7, 64, 256, 512]))
+        got = pieces(np.arange(seqs + 1), lens, seqs, 1, most, 0, 4, heads, grid, later)
+        assert (got[:, 0] < grid).all() and (got[:, 1] < heads).all() and (got[:, 2] < seqs).all()
+        assert (0 <= got[:, 4]).all() and (got[:, 4] < got[:, 5]).all() and (got[:, 5] <= got[:, 6]).all()
+        assert (0 <= got[:, 7]).all() and (got[:, 7] <= got[:, 8]).all() and (got[:, 8] < grid).all()
