@@ -332,8 +332,7 @@ struct SharedLds {
     int32_t only[6][kThreads];    // where a thread has one place of the line: its item, as in `found`
     int32_t waves[kWaves][3];     // a wave's: turns, items, the longest
     int32_t last;                 // whether the workgroup wrote the last part of an item
-    int32_t found[8];             // sequence, row tile, its turns, the sequence's first row, rows, tokens, what is before the item; the place of the line
-                                  // that was looked for, and one
+    int32_t found[7];             // sequence, row tile, its turns, the sequence's first row, rows, tokens, and what is before the item (-1: it is gone)
 };
 
 // what a wave holds of an item
@@ -996,7 +995,6 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
     __shared__ __align__(16) SharedLds<D, NQ> lds;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
     const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
-    if (id == 0) lds.found[7] = 0;
     // ---- the line of turns ----
     int turns_mine = 0, items_mine = 0, longest = 0;
     each_item(a, id, units, per, [&](int s, int tile, const Sequence &q, int n) {
@@ -1048,8 +1046,8 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
             if (per == 1) {
 #pragma unroll
                 for (int i = 0; i < 6; ++i) lds.found[i] = lds.only[i][id];
-                lds.found[7] = (int)at + 1;
             } else {
+                bool there = false;
                 each_item(a, id, units, per, [&](int s, int tile, const Sequence &q, int n) {
                     const int weight = line.whole ? 1 : n + line.start;
                     if (off >= b + weight) {
@@ -1059,15 +1057,16 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
                     const int item[6] = {s, tile, n, q.start, q.count, q.len};
 #pragma unroll
                     for (int i = 0; i < 6; ++i) lds.found[i] = item[i];
-                    lds.found[7] = (int)at + 1;
+                    there = true;
                     return true;
                 }, [](int) {});
+                if (!there) b = -1;      // (lengths that another stream changes meanwhile)
             }
             lds.found[6] = b;
         }
         __syncthreads();
-        if (uniform(lds.found[7]) != (int)at + 1) break;    // lengths that another stream changes meanwhile: no item is there any more
         const int seq = uniform(lds.found[0]), row_tile = uniform(lds.found[1]), turns = uniform(lds.found[2]), first = uniform(lds.found[6]);
+        if (first < 0) break;
         const Sequence q = {uniform(lds.found[3]), uniform(lds.found[4]), uniform(lds.found[5])};
         const Item it = item_of(a, seq, q, row_tile);
         const AttentionArgs &a = fresh_arguments();
@@ -1303,7 +1302,7 @@ int64_t attention_pieces(const AttentionJob &j, const int32_t *kv_len_later, int
         uint32_t at = line.whole ? me : me * line.length + std::min(me, line.longer);
         const uint32_t end = line.whole ? line.total : at + line.length + (me < line.longer ? 1 : 0);
         uint32_t round = 0;
-        int found[5] = {0, 0, 0, 0, 0};
+        int found[4] = {0, 0, 0, 0};
         for (int64_t steps = 0; at < end; ++steps) {
             if (steps > line.total) return -1;
             const int hv = (int)quotient(at, (uint32_t)line.head_length), off = (int)(at - (uint32_t)hv * line.head_length);
@@ -1312,21 +1311,24 @@ int64_t attention_pieces(const AttentionJob &j, const int32_t *kv_len_later, int
                 int b = line.whole ? t.items_before : t.turns_before + line.start * t.items_before;
                 if (off < b || off >= b + (line.whole ? t.items : t.turns + line.start * t.items)) continue;
                 if (per == 1) {
-                    found[0] = t.only[0], found[1] = t.only[1], found[2] = t.only[2], found[4] = (int)at + 1;
+                    found[0] = t.only[0], found[1] = t.only[1], found[2] = t.only[2];
                 } else {
+                    bool there = false;
                     each_item(a, id, units, per, [&](int s, int tile, const Sequence &, int n) {
                         const int weight = line.whole ? 1 : n + line.start;
                         if (off >= b + weight) {
                             b += weight;
                             return false;
                         }
-                        found[0] = s, found[1] = tile, found[2] = n, found[4] = (int)at + 1;
+                        found[0] = s, found[1] = tile, found[2] = n;
+                        there = true;
                         return true;
                     }, [](int) {});
+                    if (!there) b = -1;
                 }
                 found[3] = b;
             }
-            if (found[4] != (int)at + 1) break;
+            if (found[3] < 0) break;
             const int turns = found[2], skip = off - found[3];
             const Piece piece = piece_of(line, skip, turns, end - at);
             if (piece.to <= 0) break;
