@@ -314,7 +314,8 @@ int qproj_kv_read(qproj_ctx *ctx, const qproj_kv_cache *kv, const int64_t *slots
  * n_head is a multiple of n_head_kv; head h reads key/value head h / (n_head / n_head_kv).  Rows that see nothing are zeros;
  * rows before q_start_dev[0] and from q_start_dev[n_seq] on are left as they were.  Bounds on the device are checked there: q_start_dev has to ascend
  * within [0, n_tokens] by at most max_q, kv_len_dev to lie in [0, pages_stride * page_tokens], the pages that are read in
- * [0, n_pages); a sequence that breaks the first two is left out, the tokens of a bad page are not seen, and the next
+ * [0, n_pages); a sequence that breaks the first two is left out (where q_start falls and others share rows, all
+ * of them may be), the tokens of a bad page are not seen, and the next
  * qproj_sync reports it.  Every value accumulates in fp32; queries, weights and values go to the matrix cores as fp16 pairs
  * of 22 bits (of a row's largest query, down to 2^-37 of its largest weight and 2^-36 of the largest value near it).  A score
  * past fp32 and a cached block that is not finite can make the rows that see them not finite, and no others.  The

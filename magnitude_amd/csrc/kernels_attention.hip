@@ -76,6 +76,7 @@ struct AttentionArgs {
     uint32_t split_part;     // 2^16 / split, rounded up
     int32_t tokens;          // new tokens of an item
     int32_t row_tiles;       // items of a sequence, at most
+    int32_t most_items;      // of a head: as many as sequences that share no rows can have.  Their turns can be counted in 32 bits
     int32_t cus;             // workgroups from this one on share a compute unit with an earlier one
 };
 
@@ -1029,6 +1030,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         longest = max(longest, lds.waves[w][2]);
     }
     head_turns = uniform(head_turns), head_items = uniform(head_items), longest = uniform(longest);
+    if (head_items > a.most_items) return;      // (q_start falls somewhere: reported above)
     const Line line = line_of(head_turns, head_items, longest, a.kv.n_head * a.splits, gridDim.x);
     lds.line[id][0] = line.whole ? items_before : turns_before + line.start * items_before;   // (each thread's own: kept out of the registers
     lds.line[id][1] = line.whole ? items_mine : turns_mine + line.start * items_mine;         // that the tiles want)
@@ -1235,6 +1237,7 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
         a.split_part = (65536 + a.split - 1) / a.split;
         a.tokens = rows / a.split;
         a.row_tiles = (int32_t)((j.max_q + a.tokens - 1) / a.tokens);
+        a.most_items = a.n_tokens / a.tokens + a.n_seq;
         items = std::min((double)a.n_seq * a.row_tiles, (double)a.n_tokens / a.tokens + a.n_seq) * j.kv->n_head * a.splits;
         const int64_t seen = j.window ? std::min<int64_t>(most_len, (int64_t)j.window + a.tokens) : most_len;
         if (cols == 2 || a.kv.dim > 128 || j.max_q * a.group <= 16 || items * ((double)seen / (kWaves * kTile) + 2) <= 6. * groups_most) break;
@@ -1278,6 +1281,7 @@ int64_t attention_pieces(const AttentionJob &j, const int32_t *kv_len_later, int
     a.q_start = j.q_start, a.kv_len = j.kv_len;
     a.tokens = tokens;
     a.row_tiles = (a.max_q + tokens - 1) / tokens;
+    a.most_items = a.n_tokens / tokens + a.n_seq;
     const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
     struct Thread { int turns_before, items_before, turns, items, only[3]; } threads[kThreads];
     int head_turns = 0, head_items = 0, longest = 0;
@@ -1293,6 +1297,7 @@ int64_t attention_pieces(const AttentionJob &j, const int32_t *kv_len_later, int
         }, [](int) {});
         head_turns += t.turns, head_items += t.items;
     }
+    if (head_items > a.most_items) return 0;
     const Line line = line_of(head_turns, head_items, longest, heads, groups);
     a.kv_len = kv_len_later;
     int64_t pieces = 0;

@@ -27,7 +27,7 @@ def pieces(q_start, kv_len, n, max_q, most_len, window, tokens, heads, grid, lat
     f.restype, f.argtypes = C.c_int64, [C.c_void_p] * 3 + [C.c_int64] * 8 + [C.c_void_p, C.c_int64]
     start, lens = np.ascontiguousarray(q_start, np.int32), np.ascontiguousarray(kv_len, np.int32)
     later = lens if later is None else np.ascontiguousarray(later, np.int32)
-    room = 1 << 16
+    room = 1 << 17
     out = np.zeros((room, 9), np.int32)
     got = f(start.ctypes.data, lens.ctypes.data, later.ctypes.data, len(lens), n, max_q, most_len, window, tokens, heads, grid, out.ctypes.data, room)
     assert 0 <= got <= room, "a workgroup does not come to an end"
@@ -142,3 +142,14 @@ def test_lengths_that_change_during_a_call(seqs, most):
         assert (got[:, 0] < grid).all() and (got[:, 1] < heads).all() and (got[:, 2] < seqs).all()
         assert (0 <= got[:, 4]).all() and (got[:, 4] < got[:, 5]).all() and (got[:, 5] <= got[:, 6]).all()
         assert (0 <= got[:, 7]).all() and (got[:, 7] <= got[:, 8]).all() and (got[:, 8] < grid).all()
+
+
+@pytest.mark.parametrize("seqs,rows,most", [(64, 8192, 1 << 23), (33, 100, 1 << 28), (41, 100, 1 << 28), (9, 60000, 1 << 20), (3, 50, 3000)])
+def test_sequences_that_share_rows(seqs, rows, most):
+    """q_start that falls again and again: the sequences between are within bounds one by one, together they can be more than 32 bits count"""
+    for tokens in (1, 4, 8):
+        assert len(pieces([rows * (i % 2) for i in range(seqs + 1)], [most] * seqs, rows, rows, most, 0, tokens, 8, 512)) == 0
+    # one that falls among others that do not: the others are taken
+    start = np.array([0, 3, 2, 5, 9], np.int32)
+    got = pieces(start, [700, 700, 300, 900], 9, 9, 1024, 0, 4, 2, 64)
+    assert {tuple(r) for r in got[:, 1:4].tolist()} == {(h, s, t) for h in range(2) for s, t in items(start.tolist(), [700, 700, 300, 900], 4, 0)}

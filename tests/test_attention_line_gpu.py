@@ -80,3 +80,31 @@ def test_windows_of_any_size(ctx, window):
     q = rng.standard_normal((33, 8, 128)).astype(np.float32)
     got = check(ctx, kv, pages, q, q_start, lens, window=window)
     assert not got[:5].any() and got[5:8].any() and not got[8:12].any() and got[12:].any()
+
+
+def test_sequences_that_share_rows_are_reported(ctx):
+    from magnitude_amd import QprojError
+    rng = np.random.default_rng(22)
+    lens = [700, 700, 300, 900]
+    kv, pages = exact_table(rng, lens, 64, 2, 128)
+    q = rng.standard_normal((9, 8, 128)).astype(np.float32)
+    i32 = lambda a: dev(np.array(a, np.int32))
+    out = torch.full(q.shape, 7.5, device="cuda")
+    tell("q_start falls among others")
+    with pytest.raises(QprojError, match="q_start or kv_len"):
+        ctx.attention(kv, dev(q), i32([0, 3, 2, 5, 9]), i32(lens), dev(pages), out=out)
+    got = out.cpu().numpy()
+    for s, rows in ((0, [0, 1]), (2, [3, 4]), (3, [5, 6, 7, 8])):
+        a, b = [0, 3, 2, 5, 9][s], [0, 3, 2, 5, 9][s + 1]
+        want, sizes = kv_ref.attention(numpy_cache(kv), q[a:b], [0, b - a], lens[s:s + 1], pages[s:s + 1], 128 ** -0.5)
+        bound = kv_ref.allowed(sizes, 128, lens[s])
+        assert (np.abs(got[rows] - want[[r - a for r in rows]]) <= bound[[r - a for r in rows]]).all()
+    # so many shared rows behind so many tokens that 32 bits do not count them: nothing is done
+    tell("q_start falls again and again")
+    kv, _ = make_cache(rng, [256], 256, 8, 128)
+    q = torch.zeros((100, 32, 128), device="cuda")
+    out = torch.full(q.shape, 7.5, device="cuda")
+    with pytest.raises(QprojError, match="q_start or kv_len"):
+        ctx.attention(kv, q, i32([100 * (i % 2) for i in range(42)]), i32([1 << 28] * 41), torch.zeros((41, 1 << 20), dtype=torch.int32, device="cuda"), out=out)
+    assert (out == 7.5).all()
+    ctx.sync()
