@@ -325,7 +325,8 @@ int qproj_kv_read(qproj_ctx *ctx, const qproj_kv_cache *kv, const int64_t *slots
  * Workspace: a fixed buffer of the context (17 MB on 256 compute units), allocated by its first call, which therefore cannot be
  * captured into a graph (QPROJ_ERR_UNSUPPORTED); later ones can, and follow what the device arrays hold when they are replayed.
  * All calls and replays of one context share it: they run one after the other, on the context's stream or ordered behind it.
- * What the device arrays hold must stay while a call runs (lengths that change meanwhile leave that call's rows undefined, and nothing else). */
+ * What the device arrays hold must stay while a call runs.  (Calls that run at once, or whose lengths change meanwhile, have rows of any values; the
+ * calls after them are not touched by it.) */
 int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens,
                     int64_t n_head, int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q,
                     const int32_t *pages_dev, int64_t pages_stride, float scale, int64_t window, float *y_dev,

@@ -66,8 +66,9 @@ struct AttentionArgs {
     const int32_t *q_start, *kv_len, *pages;
     int32_t *error;
     float *parts;            // [workgroups][2] sums of items that were cut (part_floats each)
-    uint32_t *arrived;       // [workgroups] parts written of the item that a stretch begins and does not end; zero between calls.  Null:
-                             // attention_join_kernel adds the parts
+    uint32_t *calls;         // [slots] how many calls have counted parts; a workgroup's own and those no workgroup has go on by one in every such call
+    uint64_t *arrived;       // [2][slots] parts written of the item that a stretch begins and does not end, and above them the call that counts them;
+                             // calls use either half in turn.  Null: attention_join_kernel adds the parts
     int32_t *joins;          // [heads][n_seq][row_tiles][2] for it: of every item its first stretch (-1: nothing to join) and its last
     float scale;             // times log2(e)
     int32_t n_tokens, n_seq, max_q, window;
@@ -76,6 +77,8 @@ struct AttentionArgs {
     uint32_t split_part;     // 2^16 / split, rounded up
     int32_t tokens;          // new tokens of an item
     int32_t row_tiles;       // items of a sequence, at most
+    int32_t slots;           // workgroups that a grid can have
+    int32_t slots_each;      // of those that this grid does not have, a workgroup's share
     int32_t most_items;      // of a head: as many as sequences that share no rows can have.  Their turns can be counted in 32 bits
     int32_t cus;             // workgroups from this one on share a compute unit with an earlier one
 };
@@ -254,6 +257,12 @@ __device__ __forceinline__ void global_to_lds16_unseen(const void *g, const void
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(g) : "memory");   // (m0: nothing else here reads it)
 }
 
+// the same of 4 bytes, to l + 4 * lane
+__device__ __forceinline__ void global_to_lds4_unseen(const void *g, const void *l) {
+    const uint32_t to = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)l;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(g) : "memory");
+}
+
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true));
@@ -333,6 +342,7 @@ struct SharedLds {
     int32_t only[6][kThreads];    // where a thread has one place of the line: its item, as in `found`
     int32_t waves[kWaves][3];     // a wave's: turns, items, the longest
     int32_t last;                 // whether the workgroup wrote the last part of an item
+    uint32_t call;                // the call's number, where parts are counted, less kFirstCall; for the first wave
     int32_t found[7];             // sequence, row tile, its turns, the sequence's first row, rows, tokens, and what is before the item (-1: it is gone)
 };
 
@@ -873,6 +883,33 @@ __device__ __forceinline__ f32x4 load_part(const f32x4 *p) {
     return v;
 }
 
+// One more part of an item is written; how many there are.  The call before has left the word at this call's number and no part.  A word that holds
+// anything else (calls of one context that ran at once, lengths that changed during a call) is begun anew by whoever meets it first, and each
+// part is counted once all the same: those that met the old word come here again, those that come later find the new one.
+__device__ __forceinline__ uint32_t arrive(uint64_t *word, uint32_t call) {
+    const uint64_t was = __hip_atomic_fetch_add(word, (uint64_t)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if ((uint32_t)(was >> 32) == call) return (uint32_t)was + 1;
+    uint64_t now = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), next;
+    do {
+        next = (uint32_t)(now >> 32) == call ? now + 1 : ((uint64_t)call << 32) + 1;
+    } while (!__hip_atomic_compare_exchange_strong(word, &now, next, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    return (uint32_t)next;
+}
+
+// What a workgroup of a call that counts parts does once: the next call's words, in the half that this call does not use, and the calls' number.  Its
+// slots are its own and its share of those that the grid has no workgroup for, so that every slot goes on whatever the grids are; and by an addition,
+// so that calls which ran at once, and may have spoiled each other's results, leave all numbers alike.
+__device__ __forceinline__ void advance(const AttentionArgs &a, uint32_t call) {
+    uint64_t *const next = a.arrived + (call & 1 ? 0 : a.slots);
+    for (uint32_t i = threadIdx.x; i <= (uint32_t)a.slots_each; i += 64) {
+        const uint32_t slot = i ? gridDim.x + blockIdx.x * a.slots_each + i - 1 : blockIdx.x;
+        if (slot >= (uint32_t)a.slots) break;
+        __hip_atomic_store(next + slot, (uint64_t)(call + 1) << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_fetch_add(a.calls + slot, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+constexpr uint32_t kFirstCall = 0x9e3779b9u;     // (the number of a call that finds zeros: no word of zeros is taken for counted)
+
 // rows of an item from sums: lane's column of 16 queries, 4 dimensions of 16
 template <int D, int NQ>
 __device__ __forceinline__ float *out_row(const AttentionArgs &a, const Item &it, int head0, int heads, int g, int lane, bool &live) {
@@ -1018,6 +1055,19 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         lds.waves[wave][1] = items_before;
         lds.waves[wave][2] = longest;
     }
+    // (behind the lengths, which would be waited for with it, and to LDS, where it takes no register while tiles are worked on)
+    const bool counted = a.arrived != nullptr;
+    if (counted && id == 0) global_to_lds4_unseen(a.calls + blockIdx.x, &lds.call);
+    const auto call = [&]() {     // behind a wait for the wave's loads
+        return (uint32_t)uniform((int)*(volatile uint32_t *)&lds.call) + kFirstCall;
+    };
+    bool advanced = !counted || wave != 0;
+    const auto leave = [&](const AttentionArgs &a) {
+        if (advanced) return;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        advance(a, call());
+        advanced = true;
+    };
     turns_before -= turns_mine, items_before -= items_mine;
     __syncthreads();
     int head_turns = 0, head_items = 0;
@@ -1030,12 +1080,12 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         longest = max(longest, lds.waves[w][2]);
     }
     head_turns = uniform(head_turns), head_items = uniform(head_items), longest = uniform(longest);
-    if (head_items > a.most_items) return;      // (q_start falls somewhere: reported above)
+    if (head_items > a.most_items) return leave(a);      // (q_start falls somewhere: reported above)
     const Line line = line_of(head_turns, head_items, longest, a.kv.n_head * a.splits, gridDim.x);
     lds.line[id][0] = line.whole ? items_before : turns_before + line.start * items_before;   // (each thread's own: kept out of the registers
     lds.line[id][1] = line.whole ? items_mine : turns_mine + line.start * items_mine;         // that the tiles want)
     const uint32_t me = line.whole ? blockIdx.x : stretch_of_block(blockIdx.x, line.active);
-    if (me >= line.active) return;
+    if (me >= line.active) return leave(a);
     uint32_t at = line.whole ? me : me * line.length + std::min(me, line.longer);
     const uint32_t end = line.whole ? line.total : at + line.length + (me < line.longer ? 1 : 0);
     uint32_t round = 0;
@@ -1081,6 +1131,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
 
         Running<D, NQ> st;
         walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + piece.from * kWaves + wave, tile1, lds, wave, st, lane);
+        leave(fresh_arguments());       // (here, so that nothing waits for it)
         // ---- the waves' sums ----
         const bool starts = piece.from == 0, ends = piece.to == turns;
         meet<D, NQ>(fresh_arguments(), it, head0, heads, st, starts && ends, fresh_arguments().parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ), lds, wave, lane);
@@ -1096,12 +1147,9 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
             const int first = (int)stretch_at(line, at - skip + line.start), parts = (int)stretch_at(line, at - skip + line.start + turns - 1) - first + 1;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (id == 0) lds.last = __hip_atomic_fetch_add(c.arrived + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
+            if (id == 0) lds.last = arrive(c.arrived + (call() & 1 ? c.slots : 0) + first, call()) == (uint32_t)parts;
             __syncthreads();
-            if (lds.last) {
-                if (id == 0) __hip_atomic_store(c.arrived + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next call
-                join_parts<D, NQ>(c, it, head0, heads, first, parts, lds, wave, lane);
-            }
+            if (lds.last) join_parts<D, NQ>(c, it, head0, heads, first, parts, lds, wave, lane);
         }
         if (line.whole) {
             ++round;
@@ -1111,6 +1159,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         }
         if (at < end) __syncthreads();
     }
+    leave(fresh_arguments());
 }
 
 // Items that were cut into many parts: the sums of stretches first .. last.  A workgroup takes 16 queries and 16
@@ -1195,12 +1244,15 @@ hipError_t launch(const AttentionArgs &a, int groups, int places, hipStream_t s)
 
 }  // namespace
 
-// counts of parts (zero before the first call; every call leaves them so), what the joining kernel is to do, then the parts
-static size_t arrived_bytes(int cus) { return ((size_t)cus * kPerCu * 4 + 255) / 256 * 256; }
+// numbers of calls and counts of parts, what the joining kernel is to do, then the parts; zeros before the first call
+static size_t counts_bytes(int cus) { return (size_t)cus * kPerCu * 2 * 8; }
+static size_t calls_bytes(int cus) { return ((size_t)cus * kPerCu * 4 + 255) / 256 * 256; }
 static size_t joins_bytes(int cus) { return (size_t)cus * kPerCu * 8; }
+static size_t head_bytes(int cus) { return counts_bytes(cus) + calls_bytes(cus) + joins_bytes(cus); }
 size_t attention_scratch_bytes(int cus) {
-    return arrived_bytes(cus) + joins_bytes(cus) + (size_t)cus * kPerCu * 2 * std::max(part_floats(256, 1), part_floats(128, 2)) * 4;
+    return head_bytes(cus) + (size_t)cus * kPerCu * 2 * std::max(part_floats(256, 1), part_floats(128, 2)) * 4;
 }
+size_t attention_counts_bytes(int cus) { return counts_bytes(cus); }
 
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     if (j.n_tokens == 0 || j.n_seq == 0 || j.max_q == 0) return hipSuccess;
@@ -1245,7 +1297,9 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     // no more workgroups than there can be turns
     const int64_t most = (most_len + kTile - 1) / kTile + 1;
     const int groups = (int)std::max(1., std::min<double>(groups_most, items * ((double)most / kWaves + 1)));
-    a.parts = reinterpret_cast<float *>(j.scratch + arrived_bytes(j.cus) + joins_bytes(j.cus));
+    a.parts = reinterpret_cast<float *>(j.scratch + head_bytes(j.cus));
+    a.slots = groups_most;
+    a.slots_each = (groups_most - groups + groups - 1) / groups;
     // An item is cut into as many parts as there are workgroups for it, one or two more at its ends.  Up to eight, whoever writes the last part
     // adds them: one launch.  More are added by a kernel whose workgroups share the work: for a token of 131072 (64 parts) 45 us against 56,
     // of 8192 13.8 against 19.0, for eight rows behind 6000 17.2 against 22.1; a short chat's token, with two, 14.0 against 11.9.  (Up to five
@@ -1253,8 +1307,9 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     // (the joins' list has a place for every item there could be, fewer than groups / 8)
     const int64_t places = (int64_t)a.n_seq * a.row_tiles * j.kv->n_head * a.splits;
     const bool few_parts = groups <= 8 * places;
-    a.arrived = few_parts ? reinterpret_cast<uint32_t *>(j.scratch) : nullptr;
-    a.joins = reinterpret_cast<int32_t *>(j.scratch + arrived_bytes(j.cus));
+    a.arrived = few_parts ? reinterpret_cast<uint64_t *>(j.scratch) : nullptr;
+    a.calls = reinterpret_cast<uint32_t *>(j.scratch + counts_bytes(j.cus));
+    a.joins = reinterpret_cast<int32_t *>(j.scratch + counts_bytes(j.cus) + calls_bytes(j.cus));
     if (dry_run()) {
         plan_note("attention_kernel<%d, %d>: %d heads in %d x %d of %d, %d tokens x %d a sequence of rows, grid %d x %d", a.kv.dim, cols, j.n_head, a.kv.n_head,
                   a.splits, a.split, a.tokens, a.row_tiles, groups, kThreads);

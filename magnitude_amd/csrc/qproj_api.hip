@@ -1884,4 +1884,17 @@ int64_t qproj_internal_attention_pieces(const int32_t *q_start, const int32_t *k
     return attention_pieces(j, kv_len_later ? kv_len_later : kv_len, most_len, (int)tokens, (int)heads, (int)groups, out, room);
 }
 
+// For the tests: sets the counts of parts of a context whose attention has run to `words`, over and over where there are more of them.
+int qproj_internal_attention_counts(qproj_ctx *ctx, const uint64_t *words, int64_t n) {
+    if (!ctx || !ctx->attention_ws || !words || n <= 0) return QPROJ_ERR_INVALID_ARG;
+    const size_t count = attention_counts_bytes(ctx->cus) / 8;
+    uint64_t *all = new (std::nothrow) uint64_t[count];
+    if (!all) return QPROJ_ERR_OOM;
+    for (size_t i = 0; i < count; ++i) all[i] = words[i % n];
+    hipError_t e = hipStreamSynchronize(ctx->stream);
+    if (e == hipSuccess) e = hipMemcpy(ctx->attention_ws, all, count * 8, hipMemcpyHostToDevice);
+    delete[] all;
+    return e == hipSuccess ? QPROJ_OK : fail(ctx, QPROJ_ERR_HIP, "qproj_internal_attention_counts", e);
+}
+
 }  // extern "C"

@@ -346,6 +346,7 @@ struct AttentionJob {
     uint8_t *scratch;           // attention_scratch_bytes(cus)
 };
 size_t attention_scratch_bytes(int cus);
+size_t attention_counts_bytes(int cus);   // of its beginning: 64-bit counts of parts
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s);
 int64_t attention_pieces(const AttentionJob &j, const int32_t *kv_len_later, int64_t most_len, int tokens, int heads, int groups, int32_t *out, int64_t room);   // for the tests
 

@@ -108,3 +108,78 @@ def test_sequences_that_share_rows_are_reported(ctx):
         ctx.attention(kv, q, i32([100 * (i % 2) for i in range(42)]), i32([1 << 28] * 41), torch.zeros((41, 1 << 20), dtype=torch.int32, device="cuda"), out=out)
     assert (out == 7.5).all()
     ctx.sync()
+
+
+def set_counts(c, words):
+    """the counts of parts in a context's workspace, as a call that went wrong could have left them"""
+    import ctypes as C
+    f = c.lib.qproj_internal_attention_counts
+    f.restype, f.argtypes = C.c_int, [C.c_void_p, C.c_void_p, C.c_int64]
+    words = np.ascontiguousarray(words, np.uint64)
+    assert f(c.handle, words.ctypes.data, len(words)) == 0
+
+
+@pytest.mark.parametrize("kv_heads,lens,new", [(8, [500], 1), (2, [1300], 1), (4, [900, 2100, 333], 1), (1, [1500] * 24, 1), (2, [1200, 900], 8), (8, [700], 100)])
+def test_what_counts_of_parts_an_earlier_call_left_behind_is_nothing(kv_heads, lens, new):
+    from magnitude_amd import Context
+    tell("counts", kv_heads, lens, new)
+    rng = np.random.default_rng(sum(lens) + kv_heads)
+    kv, pages = exact_table(rng, lens, 64, kv_heads, 128)
+    q_start = np.arange(len(lens) + 1, dtype=np.int32) * new
+    q = rng.standard_normal((q_start[-1], 4 * kv_heads, 128)).astype(np.float32)
+    want, sizes = kv_ref.attention(numpy_cache(kv), q, q_start, lens, pages, 128 ** -0.5)
+    bound = kv_ref.allowed(sizes, 128, max(lens))
+    stream = torch.cuda.Stream()
+    c = Context(0, stream=stream.cuda_stream)
+    args = kv, dev(q), dev(q_start), dev(np.array(lens, np.int32)), dev(pages)
+    y = torch.full(q.shape, 7.5, device="cuda")
+    torch.cuda.synchronize()
+
+    def right(what):
+        c.sync()
+        assert (np.abs(y.cpu().numpy() - want) <= bound).all(), what
+        y.fill_(7.5)
+        torch.cuda.synchronize()
+
+    c.attention(*args, max_q=new, out=y, sync=False)
+    right("the first call")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        c.attention(*args, max_q=new, out=y, sync=False)
+    number = 0x9e3779b9 + 1        # of the next call.  (Its own number with a count is what only the call itself can have written.)
+    for kind in ("zeros", "ones", "random", "the call before, a count that carries into this one's number", "the call to come", "the call before"):
+        for how in ("an eager call", "a replay"):
+            if kind == "random":
+                words = rng.integers(0, 1 << 63, 999, dtype=np.uint64)
+            else:
+                words = [{"zeros": 0, "ones": (1 << 64) - 1}.get(kind, (number + (1 if "come" in kind else -1) << 32) + (0xffffffff if "carries" in kind else 3))]
+            set_counts(c, words)
+            if how == "a replay":
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            else:
+                c.attention(*args, max_q=new, out=y, sync=False)
+            right((kind, how))
+            c.attention(*args, max_q=new, out=y, sync=False)
+            right((kind, "the call after " + how))
+            number += 2
+    c.close()
+
+
+def test_grids_of_many_sizes_in_one_context():
+    """a call advances the words of the workgroups that it does not have, too"""
+    from magnitude_amd import Context
+    rng = np.random.default_rng(30)
+    c = Context(0)
+    work = []
+    for kv_heads, lens, new in ((8, [500], 1), (1, [1500] * 24, 1), (2, [1300], 1), (1, [70], 1), (4, [3000] * 9, 1), (1, [9000], 1), (8, [300], 64)):
+        kv, pages = exact_table(rng, lens, 64, kv_heads, 64)
+        q_start = np.arange(len(lens) + 1, dtype=np.int32) * new
+        q = rng.standard_normal((q_start[-1], 2 * kv_heads, 64)).astype(np.float32)
+        want, sizes = kv_ref.attention(numpy_cache(kv), q, q_start, lens, pages, 64 ** -0.5)
+        work.append(((kv, dev(q), dev(q_start), dev(np.array(lens, np.int32)), dev(pages)), new, want, kv_ref.allowed(sizes, 64, max(lens))))
+    for i in rng.integers(0, len(work), 80):
+        args, new, want, bound = work[i]
+        got = c.attention(*args, max_q=new)
+        assert (np.abs(got.cpu().numpy() - want) <= bound).all(), i
+    c.close()
