@@ -1059,7 +1059,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
     const bool counted = a.arrived != nullptr;
     if (counted && id == 0) global_to_lds4_unseen(a.calls + blockIdx.x, &lds.call);
     const auto call = [&]() {     // behind a wait for the wave's loads
-        return (uint32_t)uniform((int)*(volatile uint32_t *)&lds.call) + kFirstCall;
+        return (uint32_t)uniform((int)*(volatile __attribute__((address_space(3))) uint32_t *)&lds.call) + kFirstCall;
     };
     bool advanced = !counted || wave != 0;
     const auto leave = [&](const AttentionArgs &a) {
