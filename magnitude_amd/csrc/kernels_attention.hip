@@ -80,7 +80,7 @@ struct AttentionArgs {
     int32_t slots;           // workgroups that a grid can have
     int32_t slots_each;      // of those that this grid does not have, a workgroup's share
     int32_t most_items;      // of a head: as many as sequences that share no rows can have.  Their turns can be counted in 32 bits
-    int32_t cus;             // workgroups from this one on share a compute unit with an earlier one
+    int32_t young;           // workgroups from this one on go first every other tile
 };
 
 // The kernel's arguments, loaded where they are used from here on.  Kept in registers from the start they are more scalars than there are, and
@@ -539,7 +539,8 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     // Of two waves of a SIMD the older one issues first whenever it can, and the younger one is left over: of 4096 prompt tokens the first
     // 256 workgroups were done after 290 us, the others after 420.  So the younger ones go first every other tile; apart from that whoever
     // multiplies values goes before whoever multiplies keys, which keeps the two in different phases, and what the waves meet for
-    // before everything.  (420 us became 400, 48 sequences 69 -> 65.)
+    // before everything.  (No wave up 403.5 us, the younger ones 386.7, all of them 391; 512 prompt tokens 22.6, 21.5, 22.1; 48 sequences 66, 64, 64.5.
+    // Where one item is cut into many parts, all of them: a token of 131072 46.0 us against 46.9, of 32768 24.1 against 24.8.)
     __builtin_amdgcn_s_setprio(3);
     Queries<D, NQ> queries;
     load_queries<D, NQ>(a, it, head0, heads, queries, wave, lane);
@@ -573,7 +574,7 @@ __device__ __forceinline__ void walk(const AttentionArgs &a, const Item &it, int
     for (int g = 0; g < NQ; ++g) base[g] = -kBias;
 
     int buffer = 0;
-    const bool young = (int)blockIdx.x >= a.cus;
+    const bool young = (int)blockIdx.x >= a.young;
     bool up = false;
     for (int tile = from; tile < to; tile += kWaves) {
         const int t0 = tile * kTile;
@@ -1309,10 +1310,11 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
     const bool few_parts = groups <= 8 * places;
     a.arrived = few_parts ? reinterpret_cast<uint64_t *>(j.scratch) : nullptr;
     a.calls = reinterpret_cast<uint32_t *>(j.scratch + counts_bytes(j.cus));
+    a.young = few_parts ? j.cus : 0;      // (the second workgroups of the compute units, or all: see walk)
     a.joins = reinterpret_cast<int32_t *>(j.scratch + counts_bytes(j.cus) + calls_bytes(j.cus));
     if (dry_run()) {
-        plan_note("attention_kernel<%d, %d>: %d heads in %d x %d of %d, %d tokens x %d a sequence of rows, grid %d x %d", a.kv.dim, cols, j.n_head, a.kv.n_head,
-                  a.splits, a.split, a.tokens, a.row_tiles, groups, kThreads);
+        plan_note("attention_kernel<%d, %d>: %d heads in %d x %d of %d, %d tokens x %d a sequence of rows, grid %d x %d, first from %d on", a.kv.dim, cols, j.n_head, a.kv.n_head,
+                  a.splits, a.split, a.tokens, a.row_tiles, groups, kThreads, a.young);
         return hipSuccess;
     }
     if (cols == 1) {

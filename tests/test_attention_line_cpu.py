@@ -11,13 +11,17 @@ from test_attention_cpu import Dry, cache, call
 
 def plan(heads_kv, group, n, seqs, max_q, table_pages, page, dim=128, window=0):
     """(tokens of an item, heads of the line, workgroups) of the launch of such a call"""
+    m = re.search(r"heads in (\d+) x (\d+) of \d+, (\d+) tokens x (\d+) a sequence of rows, grid (\d+) x", plan_text(heads_kv, group, n, seqs, max_q, table_pages, page, dim, window))
+    kv, splits, tokens, _, grid = (int(v) for v in m.groups())
+    return tokens, kv * splits, grid
+
+
+def plan_text(heads_kv, group, n, seqs, max_q, table_pages, page, dim=128, window=0):
     heads = heads_kv * group
     with Dry() as dry:
         assert call(dry, "attention", cache(n_pages=max(1, seqs * table_pages), page_tokens=page, n_head_kv=heads_kv, head_dim=dim), h=heads, qs=heads * dim,
                     ys=heads * dim, n=n, seqs=seqs, max_q=max_q, ps=table_pages, window=window) == 0
-    m = re.search(r"heads in (\d+) x (\d+) of \d+, (\d+) tokens x (\d+) a sequence of rows, grid (\d+) x", dry.plan)
-    kv, splits, tokens, _, grid = (int(v) for v in m.groups())
-    return tokens, kv * splits, grid
+    return dry.plan
 
 
 def pieces(q_start, kv_len, n, max_q, most_len, window, tokens, heads, grid, later=None):
@@ -153,3 +157,10 @@ def test_sequences_that_share_rows(seqs, rows, most):
     start = np.array([0, 3, 2, 5, 9], np.int32)
     got = pieces(start, [700, 700, 300, 900], 9, 9, 1024, 0, 4, 2, 64)
     assert {tuple(r) for r in got[:, 1:4].tolist()} == {(h, s, t) for h in range(2) for s, t in items(start.tolist(), [700, 700, 300, 900], 4, 0)}
+
+
+def test_which_workgroups_go_first():
+    """the second ones of the compute units (256 on a context without a device); all where one item is cut into many parts"""
+    assert "first from 256 on" in plan_text(8, 4, 4096, 1, 4096, 64, 64)
+    assert "first from 256 on" in plan_text(8, 4, 48, 48, 1, 128, 64)
+    assert "first from 0 on" in plan_text(8, 4, 1, 1, 1, 2048, 64)
