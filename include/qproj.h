@@ -320,7 +320,7 @@ int qproj_kv_read(qproj_ctx *ctx, const qproj_kv_cache *kv, const int64_t *slots
  * of 22 bits (of a row's largest query, down to 2^-37 of its largest weight and 2^-36 of the largest value near it).  A score
  * past fp32 and a cached block that is not finite can make the rows that see them not finite, and no others.  The
  * result of a row depends on what else is in the call only in the order of its sums; the same call gives the same bits.  y must
- * not overlap q.  max_q should be what it says: it sizes the launch.  A call is refused where
+ * not overlap q.  max_q should be what it says: it sizes the launch.  Where n_tokens or n_seq is 0 nothing is looked at.  A call is refused where
  * min(n_seq * max_q, n_tokens) * n_head / 8 + n_seq * n_head times pages_stride * page_tokens / 256 + 4 passes 2 * 10^9.
  * Workspace: a fixed buffer of the context (17 MB on 256 compute units), allocated by its first call, which therefore cannot be
  * captured into a graph (QPROJ_ERR_UNSUPPORTED); later ones can, and follow what the device arrays hold when they are replayed.

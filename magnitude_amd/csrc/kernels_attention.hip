@@ -1256,7 +1256,7 @@ size_t attention_scratch_bytes(int cus) {
 size_t attention_counts_bytes(int cus) { return counts_bytes(cus); }
 
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
-    if (j.n_tokens == 0 || j.n_seq == 0 || j.max_q == 0) return hipSuccess;
+    if (j.n_tokens == 0 || j.n_seq == 0) return hipSuccess;     // (max_q 0: any row of a sequence is one too many, which the kernel reports)
     AttentionArgs a{};
     a.kv = *j.kv;
     a.q = j.q;
@@ -1289,7 +1289,7 @@ hipError_t launch_attention(const AttentionJob &j, hipStream_t s) {
         a.split = (a.group + a.splits - 1) / a.splits;
         a.split_part = (65536 + a.split - 1) / a.split;
         a.tokens = rows / a.split;
-        a.row_tiles = (int32_t)((j.max_q + a.tokens - 1) / a.tokens);
+        a.row_tiles = (int32_t)std::max<int64_t>(1, (j.max_q + a.tokens - 1) / a.tokens);
         a.most_items = a.n_tokens / a.tokens + a.n_seq;
         items = std::min((double)a.n_seq * a.row_tiles, (double)a.n_tokens / a.tokens + a.n_seq) * j.kv->n_head * a.splits;
         const int64_t seen = j.window ? std::min<int64_t>(most_len, (int64_t)j.window + a.tokens) : most_len;
@@ -1337,7 +1337,7 @@ int64_t attention_pieces(const AttentionJob &j, const int32_t *kv_len_later, int
     a.n_tokens = (int32_t)j.n_tokens, a.n_seq = (int32_t)j.n_seq, a.max_q = (int32_t)j.max_q, a.window = j.window;
     a.q_start = j.q_start, a.kv_len = j.kv_len;
     a.tokens = tokens;
-    a.row_tiles = (a.max_q + tokens - 1) / tokens;
+    a.row_tiles = std::max(1, (a.max_q + tokens - 1) / tokens);
     a.most_items = a.n_tokens / tokens + a.n_seq;
     const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
     struct Thread { int turns_before, items_before, turns, items, only[3]; } threads[kThreads];

@@ -164,3 +164,10 @@ def test_which_workgroups_go_first():
     assert "first from 256 on" in plan_text(8, 4, 4096, 1, 4096, 64, 64)
     assert "first from 256 on" in plan_text(8, 4, 48, 48, 1, 128, 64)
     assert "first from 0 on" in plan_text(8, 4, 1, 1, 1, 2048, 64)
+
+
+def test_no_rows_allowed_is_a_launch_that_looks():
+    """max_q 0: sequences without rows are fine, one with a row is reported by the kernel"""
+    assert "attention_kernel<" in plan_text(8, 4, 5, 3, 0, 10, 64)
+    assert len(pieces([0, 0, 0], [100, 0], 5, 0, 640, 0, 4, 8, 64)) == 0
+    assert len(pieces([0, 3, 5], [100, 60], 5, 0, 640, 0, 4, 8, 64)) == 0

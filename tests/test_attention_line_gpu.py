@@ -110,6 +110,17 @@ def test_sequences_that_share_rows_are_reported(ctx):
     ctx.sync()
 
 
+def test_more_rows_than_none_are_reported(ctx):
+    from magnitude_amd import QprojError
+    kv, pages = make_cache(np.random.default_rng(23), [100, 60], 16, 1, 64)
+    q, out = torch.zeros((5, 4, 64), device="cuda"), torch.full((5, 4, 64), 7.5, device="cuda")
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    ctx.attention(kv, q, i32(0, 0, 0), i32(100, 60), dev(pages), max_q=0, out=out)
+    with pytest.raises(QprojError, match="q_start or kv_len"):
+        ctx.attention(kv, q, i32(0, 0, 2), i32(100, 60), dev(pages), max_q=0, out=out)
+    assert (out == 7.5).all()
+
+
 def set_counts(c, words):
     """the counts of parts in a context's workspace, as a call that went wrong could have left them"""
     import ctypes as C
