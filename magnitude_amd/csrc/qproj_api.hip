@@ -847,10 +847,14 @@ int qproj_sync(qproj_ctx *ctx) {
     if (flag[0] || flag[1]) {
         QP_HIP(ctx, hipMemsetAsync(ctx->flag_dev, 0, sizeof flag, ctx->stream));
         QP_HIP(ctx, hipStreamSynchronize(ctx->stream));
-        if (flag[0]) return fail(ctx, QPROJ_ERR_INVALID_ARG, "expert id outside [0, n_expert) in a MUL_MAT_ID batch");
-        if (flag[1] & kKvBadSlot) return fail(ctx, QPROJ_ERR_INVALID_ARG, "a slot behind the key/value cache");
-        if (flag[1] & kKvBadPage) return fail(ctx, QPROJ_ERR_INVALID_ARG, "a page outside [0, n_pages) in an attention call");
-        return fail(ctx, QPROJ_ERR_INVALID_ARG, "q_start or kv_len out of bounds in an attention call");
+        const struct { int raised; const char *what; } all[] = {{flag[0], "expert id outside [0, n_expert) in a MUL_MAT_ID batch"},
+                                                                {flag[1] & kKvBadSlot, "a slot behind the key/value cache"},
+                                                                {flag[1] & kKvBadPage, "a page outside [0, n_pages) in an attention call"},
+                                                                {flag[1] & kKvBadRows, "q_start or kv_len out of bounds in an attention call"}};
+        char buf[300] = "";     // (what several calls have met since the last time is named once each)
+        for (const auto &f : all)
+            if (f.raised) snprintf(buf + strlen(buf), sizeof buf - strlen(buf), "%s%s", *buf ? "; " : "", f.what);
+        return fail(ctx, QPROJ_ERR_INVALID_ARG, buf);
     }
     return QPROJ_OK;
 }

@@ -121,6 +121,27 @@ def test_more_rows_than_none_are_reported(ctx):
     assert (out == 7.5).all()
 
 
+def test_everything_that_went_wrong_since_the_last_time_is_named(ctx):
+    from magnitude_amd import QprojError
+    kv, pages = make_cache(np.random.default_rng(24), [100, 60], 16, 1, 64)
+    x, q, out = torch.zeros((1, 1, 64), device="cuda"), torch.zeros((5, 4, 64), device="cuda"), torch.zeros((5, 4, 64), device="cuda")
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    slots, start, lens, wrong, table = torch.tensor([1 << 40], device="cuda"), i32(0, 3, 5), i32(100, 60), i32(100, -1), dev(pages)
+    bad = dev(np.full_like(pages, kv.n_pages))
+    torch.cuda.synchronize()
+    ctx.kv_append(kv, x, x, slots, sync=False)
+    ctx.attention(kv, q, start, wrong, table, out=out, sync=False)
+    with pytest.raises(QprojError, match="slot.*; q_start or kv_len"):
+        ctx.sync()
+    ctx.sync()
+    ctx.attention(kv, q, start, wrong, table, out=out, sync=False)
+    ctx.attention(kv, q, start, lens, bad, out=out, sync=False)
+    ctx.kv_append(kv, x, x, slots, sync=False)
+    with pytest.raises(QprojError, match="slot.*; a page.*; q_start or kv_len"):
+        ctx.sync()
+    ctx.sync()
+
+
 def set_counts(c, words):
     """the counts of parts in a context's workspace, as a call that went wrong could have left them"""
     import ctypes as C
