@@ -1097,8 +1097,11 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         if (off >= before && off < before + mine) {     // one thread
             int b = before;
             if (per == 1) {
+                int item[6];        // (read before any is written: one trip instead of six)
 #pragma unroll
-                for (int i = 0; i < 6; ++i) lds.found[i] = lds.only[i][id];
+                for (int i = 0; i < 6; ++i) item[i] = lds.only[i][id];
+#pragma unroll
+                for (int i = 0; i < 6; ++i) lds.found[i] = item[i];
             } else {
                 bool there = false;
                 each_item(a, id, units, per, [&](int s, int tile, const Sequence &q, int n) {
@@ -1132,7 +1135,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
 
         Running<D, NQ> st;
         walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + piece.from * kWaves + wave, tile1, lds, wave, st, lane);
-        leave(fresh_arguments());       // (here, so that nothing waits for it)
+        leave(a);                       // (here, so that nothing waits for it)
         // ---- the waves' sums ----
         const bool starts = piece.from == 0, ends = piece.to == turns;
         meet<D, NQ>(fresh_arguments(), it, head0, heads, st, starts && ends, fresh_arguments().parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ), lds, wave, lane);
@@ -1146,9 +1149,11 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         } else if (!(starts && ends)) {
             // The part is in memory before it is counted (the wait is for the stores); whoever counts the last one loads them after that.
             const int first = (int)stretch_at(line, at - skip + line.start), parts = (int)stretch_at(line, at - skip + line.start + turns - 1) - first + 1;
+            const uint32_t number = call();
+            uint64_t *const word = c.arrived + (number & 1 ? c.slots : 0) + first;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (id == 0) lds.last = arrive(c.arrived + (call() & 1 ? c.slots : 0) + first, call()) == (uint32_t)parts;
+            if (id == 0) lds.last = arrive(word, number) == (uint32_t)parts;
             __syncthreads();
             if (lds.last) join_parts<D, NQ>(c, it, head0, heads, first, parts, lds, wave, lane);
         }
