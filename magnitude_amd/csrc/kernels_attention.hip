@@ -1081,7 +1081,12 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const Atten
         longest = max(longest, lds.waves[w][2]);
     }
     head_turns = uniform(head_turns), head_items = uniform(head_items), longest = uniform(longest);
-    if (head_items > a.most_items) return leave(a);      // (q_start falls somewhere: reported above)
+    if (__builtin_expect(head_items > a.most_items, 0)) {      // (q_start falls somewhere: reported above)
+        const AttentionArgs &a = fresh_arguments();
+        if (!a.arrived)                                        // nothing is to be joined
+            for (int i = id; i < a.n_seq * a.row_tiles * a.kv.n_head * a.splits; i += kThreads) a.joins[2 * i] = -1;
+        return leave(a);
+    }
     const Line line = line_of(head_turns, head_items, longest, a.kv.n_head * a.splits, gridDim.x);
     lds.line[id][0] = line.whole ? items_before : turns_before + line.start * items_before;   // (each thread's own: kept out of the registers
     lds.line[id][1] = line.whole ? items_mine : turns_mine + line.start * items_mine;         // that the tiles want)

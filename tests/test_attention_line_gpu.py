@@ -110,6 +110,20 @@ def test_sequences_that_share_rows_are_reported(ctx):
     ctx.sync()
 
 
+def test_rows_of_a_call_that_is_left_out_are_not_joined(ctx):
+    """items cut into many parts, then a call with the same places whose sequences share too many rows: what was joined before is not again"""
+    from magnitude_amd import QprojError
+    rng = np.random.default_rng(25)
+    lens = [9000, 9000, 9000]
+    kv, pages = exact_table(rng, lens, 64, 1, 128)
+    q = rng.standard_normal((40, 4, 128)).astype(np.float32)
+    check(ctx, kv, pages, q, [0, 1, 2, 40], lens, max_q=40)
+    out = torch.full(q.shape, 7.5, device="cuda")
+    with pytest.raises(QprojError, match="q_start or kv_len"):
+        ctx.attention(kv, dev(q), dev(np.array([0, 40, 0, 40], np.int32)), dev(np.array(lens, np.int32)), dev(pages), max_q=40, out=out)
+    assert (out == 7.5).all()
+
+
 def test_more_rows_than_none_are_reported(ctx):
     from magnitude_amd import QprojError
     kv, pages = make_cache(np.random.default_rng(23), [100, 60], 16, 1, 64)
