@@ -312,21 +312,21 @@ int qproj_kv_read(qproj_ctx *ctx, const qproj_kv_cache *kv, const int64_t *slots
  *   the row at position p = kv_len - (rows of s behind it) - 1 sees tokens t <= p, and of those the last `window` (0: all);
  *   y = sum_t softmax_t(scale * q . k_t) v_t,  keys and values as the cache holds them, fp32 throughout.
  * n_head is a multiple of n_head_kv; head h reads key/value head h / (n_head / n_head_kv).  Rows that see nothing are zeros;
- * rows before q_start_dev[0] and from q_start_dev[n_seq] on are left as they were.  Bounds on the device are checked there: q_start_dev has to ascend
- * within [0, n_tokens] by at most max_q, kv_len_dev to lie in [0, pages_stride * page_tokens], the pages that are read in
- * [0, n_pages); a sequence that breaks the first two is left out (where q_start falls and others share rows, all
- * of them may be), the tokens of a bad page are not seen, and the next
- * qproj_sync reports it.  Every value accumulates in fp32; queries, weights and values go to the matrix cores as fp16 pairs
- * of 22 bits (of a row's largest query, down to 2^-37 of its largest weight and 2^-36 of the largest value near it).  A score
- * past fp32 and a cached block that is not finite can make the rows that see them not finite, and no others.  The
- * result of a row depends on what else is in the call only in the order of its sums; the same call gives the same bits.  y must
- * not overlap q.  max_q should be what it says: it sizes the launch.  Where n_tokens or n_seq is 0 nothing is looked at.  A call is refused where
+ * rows before q_start_dev[0] and from q_start_dev[n_seq] on are left as they were.  Bounds on the device are checked there:
+ * q_start_dev has to ascend within [0, n_tokens] by at most max_q, kv_len_dev to lie in [0, pages_stride * page_tokens], the
+ * pages that are read in [0, n_pages); a sequence that breaks the first two is left out (where q_start falls and others share
+ * rows, all of them may be), the tokens of a bad page are not seen, and the next qproj_sync reports it.  Where n_tokens or
+ * n_seq is 0 nothing is looked at.  Every value accumulates in fp32; queries, weights and values go to the matrix cores as
+ * fp16 pairs of 22 bits (of a row's largest query, down to 2^-37 of its largest weight and 2^-36 of the largest value near
+ * it).  A score past fp32 and a cached block that is not finite can make the rows that see them not finite, and no others.
+ * The result of a row depends on what else is in the call only in the order of its sums; the same call gives the same bits.
+ * y must not overlap q.  max_q should be what it says: it sizes the launch.  A call is refused where
  * min(n_seq * max_q, n_tokens) * n_head / 8 + n_seq * n_head times pages_stride * page_tokens / 256 + 4 passes 2 * 10^9.
  * Workspace: a fixed buffer of the context (17 MB on 256 compute units), allocated by its first call, which therefore cannot be
  * captured into a graph (QPROJ_ERR_UNSUPPORTED); later ones can, and follow what the device arrays hold when they are replayed.
  * All calls and replays of one context share it: they run one after the other, on the context's stream or ordered behind it.
- * What the device arrays hold must stay while a call runs.  (Calls that run at once, or whose lengths change meanwhile, have rows of any values; the
- * calls after them are not touched by it.) */
+ * What the device arrays hold must stay while a call runs.  Calls that run at once, or whose lengths change meanwhile, have
+ * rows of any values; the calls after them are not touched by it. */
 int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens,
                     int64_t n_head, int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q,
                     const int32_t *pages_dev, int64_t pages_stride, float scale, int64_t window, float *y_dev,

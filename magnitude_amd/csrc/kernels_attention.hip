@@ -29,10 +29,10 @@
 //
 // Weights, sums, maxima and results are fp32; every value that goes to the matrix cores has 22 bits.
 //
-// What bounds it, 32 heads of 128 on 8 (us a call): a token behind 131072 others 45, 151 MB of cache (3.4 TB/s; a copy moves
-// 5.1), 48 sequences of 100 to 8191 tokens 61, 232 MB (3.8 TB/s), 4096 prompt tokens 383, 137 Gflop (359 Tflop/s): the vector
+// What bounds it, 32 heads of 128 on 8 (us a call): a token behind 131072 others 45, 151 MB of cache (3.3 TB/s; a copy moves
+// 5.1), 48 sequences of 100 to 8191 tokens 62, 232 MB (3.8 TB/s), 4096 prompt tokens 386, 137 Gflop (356 Tflop/s): the vector
 // units' and the matrix cores' issue slots.  A tile of 64 tokens and 16 (32) rows takes about 690 (870) vector instructions of four
-// cycles, two thirds of them to unpack its codes, and 80 (160) products of sixteen.  A short chat's token 11.3: the chain of
+// cycles, two thirds of them to unpack its codes, and 80 (160) products of sixteen.  A short chat's token 11.5: the chain of
 // arguments, lengths, page, codes, one tile (2.2), the waves' meeting and the joining of two parts.
 #include "kv_cache.h"
 #include "lds_direct.h"
