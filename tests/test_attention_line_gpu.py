@@ -229,3 +229,45 @@ def test_grids_of_many_sizes_in_one_context():
         got = c.attention(*args, max_q=new)
         assert (np.abs(got.cpu().numpy() - want) <= bound).all(), i
     c.close()
+
+
+def test_calls_behind_each_other_of_many_grids():
+    """no wait between them: each finds the words of counts and the calls' number as the one before left them, eager or replayed"""
+    from magnitude_amd import Context
+    rng = np.random.default_rng(31)
+    stream = torch.cuda.Stream()
+    c = Context(0, stream=stream.cuda_stream)
+    work = []
+    for kv_heads, lens, new in ((8, [500], 1), (1, [1500] * 24, 1), (2, [1300], 1), (1, [70], 1), (4, [3000] * 9, 1), (1, [9000], 1), (8, [300], 64)):
+        kv, pages = exact_table(rng, lens, 64, kv_heads, 128)
+        q_start = np.arange(len(lens) + 1, dtype=np.int32) * new
+        q = rng.standard_normal((q_start[-1], 4 * kv_heads, 128)).astype(np.float32)
+        want, sizes = kv_ref.attention(numpy_cache(kv), q, q_start, lens, pages, 128 ** -0.5)
+        work.append(((kv, dev(q), dev(q_start), dev(np.array(lens, np.int32)), dev(pages)), new, want, kv_ref.allowed(sizes, 128, max(lens))))
+    order = rng.integers(0, len(work), 120)
+    outs = [torch.full(work[i][2].shape, 7.5, dtype=torch.float32, device="cuda") for i in order]
+    torch.cuda.synchronize()
+
+    def all_right(what):
+        c.sync()
+        for n, (i, out) in enumerate(zip(order, outs)):
+            assert (np.abs(out.cpu().numpy() - work[i][2]) <= work[i][3]).all(), (what, n, i)
+            out.fill_(7.5)
+        torch.cuda.synchronize()
+
+    def calls():
+        for i, out in zip(order, outs):
+            c.attention(*work[i][0], max_q=work[i][1], out=out, sync=False)
+
+    calls()
+    all_right("eager")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        calls()
+    for n in range(3):
+        with torch.cuda.stream(stream):
+            graph.replay()
+        all_right(f"replay {n}")
+        calls()
+        all_right("eager again")
+    c.close()
