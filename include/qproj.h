@@ -332,6 +332,17 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
                     const int32_t *pages_dev, int64_t pages_stride, float scale, int64_t window, float *y_dev,
                     int64_t y_stride);
 
+/* Attention of rows over tokens of another length: llama.cpp's build_attn over an encoder's states (llm_graph_input_attn_cross), and an
+ * encoder's own layers.  As qproj_attention, but every row q_start_dev[s] .. q_start_dev[s + 1] - 1 sees all kv_len_dev[s] tokens of its
+ * sequence, of which there may be fewer than rows:
+ *   y = sum_t softmax_t(scale * q . k_t) v_t,  t < kv_len.
+ * The states' keys and values are appended without a rotation; rows that look at the same states (beams of a request) are
+ * best given as rows of one sequence, which reads them once.  Bounds, errors, workspace and capture as for qproj_attention; rows of a
+ * sequence without tokens are zeros. */
+int qproj_cross_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens,
+                          int64_t n_head, int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q,
+                          const int32_t *pages_dev, int64_t pages_stride, float scale, float *y_dev, int64_t y_stride);
+
 /* Backend eligibility probe: what the reference's server asks of a GPU runtime before it offers the
  * backend pack that needs it (/root/reference/inference/crates/icn-server/src/cuda_driver.rs:343-401
  * inspect(): initialise, driver version, device count, one architecture string and one hardware label per

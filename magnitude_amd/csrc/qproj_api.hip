@@ -1790,13 +1790,11 @@ int qproj_kv_read(qproj_ctx *ctx, const qproj_kv_cache *kv, const int64_t *slots
     return QPROJ_OK;
 }
 
-int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens, int64_t n_head,
-                    int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q, const int32_t *pages_dev,
-                    int64_t pages_stride, float scale, int64_t window, float *y_dev, int64_t y_stride) {
-    const char *call = "qproj_attention";
-    if (!ctx) return QPROJ_ERR_INVALID_ARG;
-    KvView view;
-    if (const char *why = bad_cache(kv, &view)) return refuse(ctx, call, why);
+// What every attention call checks and hands to its kernel.  The job's n_tokens or n_seq are 0 where there is nothing to do.
+static int attention_job(qproj_ctx *ctx, const char *call, const qproj_kv_cache *kv, KvView *view, const float *q_dev, int64_t q_stride, int64_t n_tokens, int64_t n_head,
+                         int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q, const int32_t *pages_dev, int64_t pages_stride, float scale,
+                         int64_t window, float *y_dev, int64_t y_stride, AttentionJob *job) {
+    if (const char *why = bad_cache(kv, view)) return refuse(ctx, call, why);
     if (!q_start_dev || (!kv_len_dev && n_seq) || (!pages_dev && n_seq && pages_stride)) return refuse(ctx, call, "null argument");
     if (n_tokens < 0 || n_tokens > kMostTokens || n_seq < 0 || n_seq > 65536 || max_q < 0 || pages_stride < 0)
         return refuse(ctx, call, "n_tokens, n_seq, max_q or pages_stride out of range");
@@ -1812,13 +1810,18 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
     if (const char *why = bad_rows(q_dev, q_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
     if (const char *why = bad_rows(y_dev, y_stride, n_head, kv->head_dim)) return refuse(ctx, call, why);
     if (q_dev == y_dev) return refuse(ctx, call, "y must not be q");
+    job->n_tokens = n_tokens;
+    job->n_seq = n_seq;
     if (n_tokens == 0 || n_seq == 0) return QPROJ_OK;
     if (!dry_run()) {
         QP_HIP(ctx, hipSetDevice(ctx->device));
         if (!ctx->attention_ws) {
             hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
             QP_HIP(ctx, hipStreamIsCapturing(ctx->stream, &capture));
-            if (capture != hipStreamCaptureStatusNone) return fail(ctx, QPROJ_ERR_UNSUPPORTED, "qproj_attention: a context's first call allocates and cannot be captured");
+            if (capture != hipStreamCaptureStatusNone) {
+                refuse(ctx, call, "a context's first attention call allocates and cannot be captured");
+                return QPROJ_ERR_UNSUPPORTED;
+            }
             uint8_t *ws = nullptr;
             QP_HIP(ctx, hipMalloc((void **)&ws, attention_scratch_bytes(ctx->cus)));
             const hipError_t e = hipMemsetAsync(ws, 0, attention_scratch_bytes(ctx->cus), ctx->stream);
@@ -1829,16 +1832,14 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
             ctx->attention_ws = ws;
         }
     }
-    AttentionJob j{};
+    AttentionJob &j = *job;
     j.cus = dry_run() ? 256 : ctx->cus;
     j.scratch = ctx->attention_ws;
-    j.kv = &view;
+    j.kv = view;
     j.q = q_dev;
     j.y = y_dev;
     j.q_stride = q_stride;
     j.y_stride = y_stride;
-    j.n_tokens = n_tokens;
-    j.n_seq = n_seq;
     j.n_head = (int)n_head;
     j.q_start = q_start_dev;
     j.kv_len = kv_len_dev;
@@ -1848,7 +1849,32 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
     j.scale = scale;
     j.window = window < pages_stride * kv->page_tokens ? (int32_t)window : 0;    // (a window as long as a sequence can be hides nothing)
     j.error = ctx->flag_dev + 1;
+    return QPROJ_OK;
+}
+
+int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens, int64_t n_head,
+                    int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q, const int32_t *pages_dev,
+                    int64_t pages_stride, float scale, int64_t window, float *y_dev, int64_t y_stride) {
+    if (!ctx) return QPROJ_ERR_INVALID_ARG;
+    KvView view;
+    AttentionJob j{};
+    const int rc = attention_job(ctx, "qproj_attention", kv, &view, q_dev, q_stride, n_tokens, n_head, n_seq, q_start_dev, kv_len_dev, max_q, pages_dev, pages_stride, scale, window,
+                                 y_dev, y_stride, &j);
+    if (rc != QPROJ_OK) return rc;
     QP_HIP(ctx, launch_attention(j, ctx->stream));
+    return QPROJ_OK;
+}
+
+int qproj_cross_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens, int64_t n_head,
+                          int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q, const int32_t *pages_dev,
+                          int64_t pages_stride, float scale, float *y_dev, int64_t y_stride) {
+    if (!ctx) return QPROJ_ERR_INVALID_ARG;
+    KvView view;
+    AttentionJob j{};
+    const int rc = attention_job(ctx, "qproj_cross_attention", kv, &view, q_dev, q_stride, n_tokens, n_head, n_seq, q_start_dev, kv_len_dev, max_q, pages_dev, pages_stride, scale, 0,
+                                 y_dev, y_stride, &j);
+    if (rc != QPROJ_OK) return rc;
+    QP_HIP(ctx, launch_attention_all(j, ctx->stream));
     return QPROJ_OK;
 }
 

@@ -67,6 +67,7 @@ SYMBOLS = {
     "qproj_kv_append": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64]),
     "qproj_kv_read": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp]),
     "qproj_attention": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, C.c_float, _i64, _vp, _i64]),
+    "qproj_cross_attention": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, C.c_float, _vp, _i64]),
     "qproj_version": (C.c_char_p, []),
     "qproj_probe_eligibility": (_i32, [_vp]),
 }
@@ -702,13 +703,9 @@ class Context:
             self.sync()
         return k_out, v_out
 
-    def attention(self, kv: KvCache, q: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor,
-                  max_q: Optional[int] = None, scale: Optional[float] = None, window: int = 0,
-                  out: Optional[torch.Tensor] = None, sync: bool = True) -> torch.Tensor:
-        """Attention of the newest tokens of sequences over the cache: q f32 [tokens, heads, head_dim], rows q_start[s] ..
-        q_start[s + 1] - 1 (i32 [n_seq + 1]) the last ones of the kv_len[s] (i32 [n_seq]) tokens that sequence s has in its
-        pages (i32 [n_seq, most pages]).  max_q: the most rows a sequence has (default: all of them could be one's).
-        scale: 1 / sqrt(head_dim) by default; window: how many tokens back a row sees, itself among them (0: all)."""
+    def _attention_args(self, kv: KvCache, q: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor,
+                        max_q: Optional[int], scale: Optional[float], out: Optional[torch.Tensor]):
+        """(rows, an attention call's arguments up to the scale, those of its result, the result)"""
         qp, qs = self._rows(q, "q", None, kv.head_dim)
         n, h = q.shape[0], q.shape[1]
         if pages.dim() != 2 or q_start.numel() != pages.shape[0] + 1 or kv_len.numel() != pages.shape[0]:
@@ -717,14 +714,38 @@ class Context:
         yp, ys = self._rows(y, "out", h, kv.head_dim)
         if y.shape[0] != n:
             raise ValueError("out must be shaped as q")
-        args = [self._on_device(t, torch.int32, w) for t, w in ((q_start, "q_start"), (kv_len, "kv_len"), (pages, "pages"))]
+        i32 = torch.int32
+        return n, (self.handle, self._cache(kv), qp, qs, n, h, pages.shape[0], self._on_device(q_start, i32, "q_start"),
+                   self._on_device(kv_len, i32, "kv_len"), n if max_q is None else max_q, self._on_device(pages, i32, "pages"),
+                   pages.shape[1], kv.head_dim ** -0.5 if scale is None else scale), (yp, ys), y
+
+    def attention(self, kv: KvCache, q: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor,
+                  max_q: Optional[int] = None, scale: Optional[float] = None, window: int = 0,
+                  out: Optional[torch.Tensor] = None, sync: bool = True) -> torch.Tensor:
+        """Attention of the newest tokens of sequences over the cache: q f32 [tokens, heads, head_dim], rows q_start[s] ..
+        q_start[s + 1] - 1 (i32 [n_seq + 1]) the last ones of the kv_len[s] (i32 [n_seq]) tokens that sequence s has in its
+        pages (i32 [n_seq, most pages]).  max_q: the most rows a sequence has (default: all of them could be one's).
+        scale: 1 / sqrt(head_dim) by default; window: how many tokens back a row sees, itself among them (0: all)."""
+        n, head, tail, y = self._attention_args(kv, q, q_start, kv_len, pages, max_q, scale, out)
         if n == 0:
             return y
         if sync:
             torch.cuda.current_stream(q.device).synchronize()
-        self._check(self.lib.qproj_attention(self.handle, self._cache(kv), qp, qs, n, h, pages.shape[0], args[0], args[1],
-                                             n if max_q is None else max_q, args[2], pages.shape[1],
-                                             kv.head_dim ** -0.5 if scale is None else scale, window, yp, ys))
+        self._check(self.lib.qproj_attention(*head, window, *tail))
+        if sync:
+            self.sync()
+        return y
+
+    def cross_attention(self, kv: KvCache, q: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor,
+                        max_q: Optional[int] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                        sync: bool = True) -> torch.Tensor:
+        """As attention, but every row sees all kv_len[s] tokens of its sequence: a decoder's rows over an encoder's states."""
+        n, head, tail, y = self._attention_args(kv, q, q_start, kv_len, pages, max_q, scale, out)
+        if n == 0:
+            return y
+        if sync:
+            torch.cuda.current_stream(q.device).synchronize()
+        self._check(self.lib.qproj_cross_attention(*head, *tail))
         if sync:
             self.sync()
         return y

@@ -138,6 +138,10 @@ extern "C" {
                            n_tokens: i64, n_head: i64, n_seq: i64, q_start_dev: *const i32, kv_len_dev: *const i32,
                            max_q: i64, pages_dev: *const i32, pages_stride: i64, scale: f32, window: i64,
                            y_dev: *mut f32, y_stride: i64) -> c_int;
+    pub fn qproj_cross_attention(ctx: *mut qproj_ctx, kv: *const qproj_kv_cache, q_dev: *const f32, q_stride: i64,
+                                 n_tokens: i64, n_head: i64, n_seq: i64, q_start_dev: *const i32, kv_len_dev: *const i32,
+                                 max_q: i64, pages_dev: *const i32, pages_stride: i64, scale: f32, y_dev: *mut f32,
+                                 y_stride: i64) -> c_int;
     pub fn qproj_version() -> *const c_char;
     pub fn qproj_probe_eligibility(out: *mut qproj_eligibility) -> c_int;
 }

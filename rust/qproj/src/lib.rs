@@ -193,6 +193,17 @@ impl Context {
                                  pages.0.cast(), pages_stride, scale, window, y.0.cast(), row)
         })
     }
+
+    /// Attention of rows that see all tokens of their sequence, an encoder's states say; see `qproj_cross_attention`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn cross_attention(&self, kv: &sys::qproj_kv_cache, q: DevicePtr, n: i64, n_head: i64, n_seq: i64, q_start: DevicePtr,
+                           kv_len: DevicePtr, max_q: i64, pages: DevicePtr, pages_stride: i64, scale: f32, y: DevicePtr) -> Result<()> {
+        let row = n_head * kv.head_dim;
+        self.check(unsafe {
+            sys::qproj_cross_attention(self.raw, kv, q.0.cast(), row, n, n_head, n_seq, q_start.0.cast(), kv_len.0.cast(), max_q,
+                                       pages.0.cast(), pages_stride, scale, y.0.cast(), row)
+        })
+    }
 }
 
 /// The frequencies of a rotation's `n_dims / 2` pairs and what cosines and sines are multiplied by.

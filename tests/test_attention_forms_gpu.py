@@ -1,0 +1,127 @@
+"""Attention over the paged 4-bit cache in its other forms on the GPU, against plain statements in 64 bits (forms_ref.py)."""
+import numpy as np
+import pytest
+import torch
+
+import forms_ref
+from test_attention_gpu import dev, make_cache, numpy_cache, tell, wide
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from magnitude_amd import Context
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    c = Context(0)
+    yield c
+    c.close()
+
+
+def i32(a):
+    return dev(np.asarray(a, np.int32))
+
+
+def compare(got, want, plain, sizes, dim, tokens):
+    """`got` against the statement in 64 bits: every value within what is derived for it, all of them within half as much again as the statement
+    in fp32, or 16 steps of an fp32 number"""
+    mine = ~np.isnan(want).all(-1)
+    assert (got[~mine] == 7.5).all()                       # rows of no sequence stay as they were
+    got, want, plain, bound = got[mine], want[mine], plain[mine], forms_ref.allowed(sizes, dim, tokens)[mine]
+    if not want.size:
+        return
+    err, norm = np.abs(got - want), max(1e-30, np.linalg.norm(want))
+    worst, rel, usual = np.max(err / bound), np.linalg.norm(err) / norm, np.linalg.norm(plain - want) / norm
+    tell(f"   worst {worst:.3g} of what is allowed, {rel:.3g} of the norm, in fp32 {usual:.3g}")
+    assert worst <= 1.0 and rel <= max(1.5 * usual, 2.0 ** -20)
+
+
+# ---- rows that see everything ---------------------------------------------------------------------------------------------
+def check_cross(ctx, kv, pages, q, q_start, kv_len, scale=None, **kw):
+    """of the call in both its forms: 16 and 32 rows at a time"""
+    s = kv.head_dim ** -0.5 if scale is None else scale
+    want, sizes = forms_ref.attention(numpy_cache(kv), q, q_start, kv_len, pages, s, sees_all=True)
+    plain = forms_ref.attention(numpy_cache(kv), q, q_start, kv_len, pages, s, sees_all=True, dtype=np.float32)[0]
+    for table in (wide(pages, kv), pages):
+        out = torch.full(q.shape, 7.5, device="cuda")
+        got = ctx.cross_attention(kv, dev(q), i32(q_start), i32(kv_len), dev(table), scale=scale, out=out, **kw).cpu().numpy()
+        compare(got, want, plain, sizes, kv.head_dim, max([1] + list(kv_len)))
+    return got
+
+
+CROSS = [  # dim, page, kv heads, group, [(states, rows)]
+    (64, 64, 1, 1, [(1, 1)]),
+    (64, 64, 12, 1, [(1500, 1)]),
+    (128, 16, 8, 4, [(500, 1), (64, 1), (63, 1), (65, 1)]),
+    (96, 32, 2, 5, [(257, 3), (1, 7), (0, 2), (90, 0), (128, 1)]),
+    (128, 64, 2, 4, [(1601, 187)]),
+    (128, 64, 2, 4, [(5, 300), (200, 40)]),               # more rows than states
+    (256, 128, 1, 8, [(700, 3), (100, 50)]),
+    (64, 256, 1, 71, [(100, 2)]),
+    (128, 64, 1, 4, [(20000, 1)]),                        # many parts, joined by a launch of their own
+    (128, 64, 8, 4, [(1 + 700 * i, 1) for i in range(8)]),
+    (64, 16, 8, 1, [(1 + 37 * i % 301, 1 + i % 3) for i in range(150)]),
+    (96, 16, 1, 3, [(1300, 400)]),
+]
+
+
+@pytest.mark.parametrize("dim,page,kv_heads,group,seqs", CROSS)
+def test_cross_attention(ctx, dim, page, kv_heads, group, seqs):
+    tell("cross", dim, page, kv_heads, group, seqs)
+    rng = np.random.default_rng(dim + page + len(seqs))
+    lens = [n for n, _ in seqs]
+    kv, pages = make_cache(rng, lens, page, kv_heads, dim)
+    q_start = np.cumsum([0] + [m for _, m in seqs])
+    q = rng.standard_normal((q_start[-1], kv_heads * group, dim)).astype(np.float32)
+    check_cross(ctx, kv, pages, q, q_start, lens)
+    check_cross(ctx, kv, pages, q, q_start, lens, scale=1.0, max_q=max(m for _, m in seqs))
+
+
+def test_cross_rows_of_no_sequence_stay_and_rows_without_states_are_zeros(ctx):
+    rng = np.random.default_rng(21)
+    lens, q_start = [3, 0, 40, 0], [2, 10, 14, 14, 15]
+    kv, pages = make_cache(rng, lens, 16, 2, 64)
+    q = rng.standard_normal((20, 8, 64)).astype(np.float32)
+    got = check_cross(ctx, kv, pages, q, q_start, lens)
+    assert got[2:10].any(-1).all() and not got[10:15].any()
+
+
+def test_cross_blocks_that_are_not_finite_reach_every_row_of_their_sequence(ctx):
+    rng = np.random.default_rng(22)
+    kv, pages = make_cache(rng, [200, 90], 16, 2, 128)
+    q = rng.standard_normal((40, 8, 128)).astype(np.float32)
+    args = kv, dev(q), i32([0, 30, 40]), i32([200, 90]), dev(pages)
+    base = ctx.cross_attention(*args).cpu().numpy()
+    last = int(pages[0, 199 // 16]), 199 % 16
+    kv.tensors[3][last[0], 1, last[1], 1] = float("nan")          # a block of a value of head 1
+    for at in range(last[1] + 1, 16):                             # what lies behind the end is seen by nobody
+        kv.tensors[1][last[0], :, at] = float("nan")
+        kv.tensors[3][last[0], :, at] = float("nan")
+    got = ctx.cross_attention(*args).cpu().numpy()
+    assert np.isnan(got[:30, 4:, 32:64]).all()
+    np.testing.assert_array_equal(got[30:], base[30:])
+    np.testing.assert_array_equal(got[:30, :4], base[:30, :4])
+    np.testing.assert_array_equal(got[:30, 4:, :32], base[:30, 4:, :32])
+
+
+def test_cross_bad_pages_and_bounds_are_reported(ctx):
+    from magnitude_amd import QprojError
+    rng = np.random.default_rng(23)
+    kv, pages = make_cache(rng, [100, 60], 16, 1, 64)
+    q = rng.standard_normal((5, 4, 64)).astype(np.float32)
+    ok = ctx.cross_attention(kv, dev(q), i32([0, 3, 5]), i32([100, 60]), dev(pages)).cpu().numpy()
+    wrong = pages.copy()
+    wrong[0, 2] = kv.n_pages
+    out = torch.full(q.shape, 7.5, device="cuda")
+    with pytest.raises(QprojError, match="page"):
+        ctx.cross_attention(kv, dev(q), i32([0, 3, 5]), i32([100, 60]), dev(wrong), out=out)
+    want, sizes = forms_ref.attention(numpy_cache(kv), q, [0, 3, 5], [100, 60], wrong, 64 ** -0.5, sees_all=True)
+    assert (np.abs(out.cpu().numpy() - want) <= forms_ref.allowed(sizes, 64, 100)).all()
+    for q_start, lens, max_q, left in (([0, 3, 6], [100, 60], 5, [0, 1, 2]), ([0, 3, 5], [-1, 60], 5, [3, 4]), ([0, 3, 5], [100, 1 << 20], 5, [0, 1, 2]), ([0, 3, 5], [100, 60], 2, [3, 4])):
+        out = torch.full(q.shape, 7.5, device="cuda")
+        with pytest.raises(QprojError, match="q_start or kv_len"):
+            ctx.cross_attention(kv, dev(q), i32(q_start), i32(lens), dev(pages), max_q=max_q, out=out)
+        got = out.cpu().numpy()
+        np.testing.assert_allclose(got[left], ok[left], rtol=1e-5, atol=1e-6)
+        assert (got[[i for i in range(5) if i not in left]] == 7.5).all()
+    ctx.sync()
