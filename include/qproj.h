@@ -343,6 +343,33 @@ int qproj_cross_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float 
                           int64_t n_head, int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q,
                           const int32_t *pages_dev, int64_t pages_stride, float scale, float *y_dev, int64_t y_stride);
 
+/* A bias learned by buckets of the distance between a token and a row (llama.cpp's build_inp_pos_bucket_* and the kq_b of build_attn).
+ * The buckets of distances d = token - row from -reach to reach, on the HOST, as llama_relative_position_bucket gives them:
+ * both_sides: half of n_buckets for either side, the upper ones for d > 0; otherwise d > 0 counts as 0.  Of `side` buckets the
+ * first e = side / 2 are distances of their own, then e + floor(log(|d| / e) / log(reach / e) * (side - e)), at most side - 1 (powers that
+ * meet exactly begin the next bucket).  side >= 2, n_buckets even with both sides, e < reach <= 1703. */
+int qproj_relative_buckets(int64_t n_buckets, int64_t reach, int both_sides, int32_t *buckets);
+
+/* out[h][d + reach] = table[buckets[d + reach]][h]: the model's table [n_buckets][n_head] laid out by distance, once per model.  A bucket
+ * outside [0, n_buckets) gives 0 and is reported by the next qproj_sync. */
+int qproj_bias_by_distance(qproj_ctx *ctx, const float *table_dev, int64_t n_buckets, int64_t n_head, const int32_t *buckets_dev,
+                           int64_t reach, float *out_dev);
+
+/* Attention with such a bias: as qproj_attention (without a window), or with causal = 0 every row sees all tokens of its sequence, as an
+ * encoder's layers do:
+ *   y = sum_t softmax_t(scale * q . k_t + bias[h][min(max(t - p, -reach), reach) + reach]) v_t,  p the row's position: its
+ * sequence's rows are the last of its tokens either way.  by_distance_dev holds n_head rows of 2 * reach + 1 values (0 <= reach <= 1703), any finite
+ * ones or -infinity: a token that this is the bias of is not seen.  With others the rows that meet them are not finite. */
+typedef struct qproj_position_bias {
+    const float *by_distance_dev;
+    int64_t reach;
+    int causal;
+} qproj_position_bias;
+int qproj_attention_biased(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens,
+                           int64_t n_head, int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q,
+                           const int32_t *pages_dev, int64_t pages_stride, const qproj_position_bias *bias, float scale, float *y_dev,
+                           int64_t y_stride);
+
 /* Backend eligibility probe: what the reference's server asks of a GPU runtime before it offers the
  * backend pack that needs it (/root/reference/inference/crates/icn-server/src/cuda_driver.rs:343-401
  * inspect(): initialise, driver version, device count, one architecture string and one hardware label per

@@ -58,6 +58,7 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kTile = 64;            // tokens of a tile
 constexpr float kBias = 13.f;        // weights are 2^kBias at the running maximum
+constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kSlack = 2.5f;       // a score may pass it by this before the row is rescaled: 2^15.5 < 65504
 
 // Who sees what.  A kernel is compiled for one of the argument types below.
@@ -168,8 +169,9 @@ __host__ __device__ __forceinline__ Sequence sequence(const AttentionArgs &a, in
 // the rows of an item and the tokens that any of them sees
 struct Item {
     int seq, first, count;   // first row, its tokens
-    int lo, hi;              // positions of its first and last token; tokens [see, hi] are seen (hi < 0: none)
+    int lo, hi;              // positions of its first and last token; tokens [see, hi] are seen (hi < 0: none).  Where all are: both the last one
     int see;
+    int at;                  // kBiased: position of its first token
 };
 
 template <typename A>
@@ -182,6 +184,10 @@ __host__ __device__ __forceinline__ Item item_of(const A &a, int s, const Sequen
     it.hi = it.lo + it.count - 1;
     it.see = a.window && it.lo >= a.window ? it.lo - a.window + 1 : 0;     // (lo is negative where a sequence has more rows than tokens)
     if constexpr (A::kSees == kAll) it.lo = it.hi = q.len - 1;
+    if constexpr (A::kSees == kBiased) {
+        it.at = it.lo;
+        if (a.all) it.lo = it.hi = q.len - 1;
+    }
     return it;
 }
 
@@ -360,8 +366,21 @@ struct WaveLds {
 
 constexpr int meet_rounds(int dim) { return dim > 128 ? 2 : 1; }   // (so that two workgroups' LDS fit)
 
+// What a kind of attention keeps beside.
+template <Sees S>
+struct KindLds {};
+
+// Biases of the item's heads by distance, from reach + kBiasPad tokens before a row to as many behind it, those beyond reach the last ones repeated: a
+// tile of 64 tokens that some row of an item is within reach of finds all its biases at one address a lane and constant offsets.
+constexpr int kBiasPad = 96, kBiasFloats = 3600;     // (pad: 63 tokens of the tile, 31 rows of the item.  Room: eight heads at a reach of 128)
+constexpr int bias_room(int reach) { return 2 * reach + 1 + 2 * kBiasPad; }
+template <>
+struct KindLds<kBiased> {
+    float bias[kBiasFloats + 64];     // (loads write 64 at a time)
+};
+
 template <int D, int NQ, typename A>
-struct SharedLds {
+struct SharedLds : KindLds<A::kSees> {
     union {
         WaveLds<D, NQ> wave[kWaves];
         struct {
@@ -575,6 +594,13 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
     // before everything.  (No wave up 403.5 us, the younger ones 386.7, all of them 391; 512 prompt tokens 22.6, 21.5, 22.1; 48 sequences 66, 64, 64.5.
     // Where one item is cut into many parts, all of them: a token of 131072 46.0 us against 46.9, of 32768 24.1 against 24.8.)
     __builtin_amdgcn_s_setprio(3);
+    if constexpr (A::kSees == kBiased) {     // (before the queries: where those are waited for, these have come)
+        const int span = 2 * a.reach + 1, room = bias_room(a.reach);
+        for (int i = wave * 64; i < heads * room; i += kThreads) {
+            const int h = min((int)quotient(i + lane, room), heads - 1), at = i + lane - h * room;
+            global_to_lds4_unseen(a.bias + (int64_t)(head0 + h) * span + min(max(at - kBiasPad, 0), span - 1), shared.bias + i);
+        }
+    }
     Queries<D, NQ> queries;
     load_queries<D, NQ>(a, it, head0, heads, queries, wave, lane);
     if (work) {
@@ -588,11 +614,17 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
     __syncthreads();
     if (!work) return;
 
-    int pos[NQ];                // position of the column's row, -1: no row
+    int pos[NQ];                // what the column's row sees, up to this token, -1: no row
+    int own_bias[NQ];           // kBiased: its bias of token 0 is there, had the row one that far away
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
         const int slot = g * 16 + col, token = token_of(a, slot);
-        pos[g] = token < it.count && slot - token * a.split < heads ? (A::kSees == kAll ? it.hi : it.lo + token) : -1;
+        const bool live = token < it.count && slot - token * a.split < heads;
+        pos[g] = live ? (A::kSees == kAll ? it.hi : it.lo + token) : -1;
+        if constexpr (A::kSees == kBiased) {
+            if (live && a.all) pos[g] = it.hi;
+            own_bias[g] = (live ? slot - token * a.split : 0) * bias_room(a.reach) + kBiasPad + a.reach - (it.at + (live ? token : 0));
+        }
     }
 
     // (in registers, and unknown to the compiler: and-or in one instruction, half times -1 plus float in one)
@@ -742,6 +774,31 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
         u32x4 p_hi[2][NQ], p_lo[2][NQ];
 #pragma unroll
         for (int c = 0; c < NQ; ++c) {
+            float times = q_unit[c], plus = 0.f;     // kBiased: a weight's exponent is s * times + plus
+            if constexpr (A::kSees == kBiased) {
+                const bool before = t0 + kTile - 1 - it.at <= -a.reach, behind = t0 - (it.at + it.count - 1) >= a.reach;
+                if (before || behind) {              // out of reach of all rows: one bias a head
+                    const int slot = c * 16 + col, token = token_of(a, slot), head = token < it.count ? min(slot - token * a.split, heads - 1) : 0;
+                    plus = shared.bias[head * bias_room(a.reach) + (before ? 0 : bias_room(a.reach) - 1)] * kLog2e;
+                    if (__ballot(plus == -INFINITY)) {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) s[g][c][r] = plus == -INFINITY ? -INFINITY : s[g][c][r];
+                        plus = plus == -INFINITY ? 0.f : plus;
+                    }
+                } else {
+                    const float *const bias = shared.bias + (own_bias[c] + t0 + 4 * part);
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float b = bias[16 * g + r];
+                            s[g][c][r] = b == -INFINITY ? b : fmaf(b, kLog2e, s[g][c][r] * times);
+                        }
+                    times = 1.f;
+                }
+            }
             if (edge) {
                 const int last = pos[c] - t0 - 4 * part, behind = a.window ? last - a.window : -kTile;   // of the lane's tokens 16 g + r
 #pragma unroll
@@ -755,7 +812,8 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
             float top = -INFINITY;
 #pragma unroll
             for (int g = 0; g < 4; ++g) top = fmaxf(top, fmaxf(fmaxf(s[g][c][0], s[g][c][1]), fmaxf(s[g][c][2], s[g][c][3])));
-            top *= q_unit[c];
+            if constexpr (A::kSees == kBiased) top = fmaf(top, times, plus);
+            else top *= q_unit[c];
             float back = shrink;
             if (__ballot(top > st.m[c] + kSlack)) {
                 const float m = fmaxf(st.m[c], max_xor(top));
@@ -787,7 +845,7 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[g][c][r] = __builtin_amdgcn_exp2f(fmaf(s[g][c][r], q_unit[c], -base[c]));
+                for (int r = 0; r < 4; ++r) s[g][c][r] = __builtin_amdgcn_exp2f(A::kSees == kBiased ? fmaf(s[g][c][r], times, plus - base[c]) : fmaf(s[g][c][r], q_unit[c], -base[c]));
                 st.l[c] += (s[g][c][0] + s[g][c][1]) + (s[g][c][2] + s[g][c][3]);
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
@@ -1309,7 +1367,7 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
     a.kv_len = j.kv_len;
     a.pages = j.pages;
     a.error = j.error;
-    a.scale = j.scale * 1.44269504088896341f;
+    a.scale = j.scale * kLog2e;
     a.window = j.window;
     a.group = j.n_head / j.kv->n_head;
     // 16 rows an item, or 32 of them that share the work of unpacking the codes.  Few rows of work leave most of the chip waiting for a turn of
@@ -1325,6 +1383,12 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
         const int rows = 16 * cols;
         a.splits = (a.group + rows - 1) / rows;
         a.split = (a.group + a.splits - 1) / a.splits;
+        if constexpr (A::kSees == kBiased) {     // as many heads as there is room for the biases of
+            const int most = kBiasFloats / bias_room(a.reach);
+            a.splits = std::max(a.splits, (a.group + most - 1) / most);
+            a.split = (a.group + a.splits - 1) / a.splits;
+            a.splits = (a.group + a.split - 1) / a.split;
+        }
         a.split_part = (65536 + a.split - 1) / a.split;
         a.tokens = rows / a.split;
         a.row_tiles = (int32_t)std::max<int64_t>(1, (j.max_q + a.tokens - 1) / a.tokens);

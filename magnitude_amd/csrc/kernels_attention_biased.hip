@@ -1,0 +1,39 @@
+// Attention with a bias of the distance between a token and a row, learned by buckets, and the layout of such biases.
+#include "attention_device.h"
+
+namespace qproj {
+
+namespace {
+
+// out[h][i] = table[buckets[i]][h]: a thread each
+__global__ __launch_bounds__(256) void bias_by_distance_kernel(const float *table, int n_buckets, int n_head, const int32_t *buckets, int distances, float *out, int32_t *error) {
+    const int at = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+    if (at >= distances) return;
+    const int b = buckets[at];
+    if ((uint32_t)b >= (uint32_t)n_buckets && h == 0) atomicOr(error, kKvBadBucket);
+    out[(int64_t)h * distances + at] = (uint32_t)b < (uint32_t)n_buckets ? table[(int64_t)b * n_head + h] : 0.f;
+}
+
+}  // namespace
+
+int attention_most_reach() { return (kBiasFloats - 1 - 2 * kBiasPad) / 2; }
+
+hipError_t launch_bias_by_distance(const float *table, int n_buckets, int n_head, const int32_t *buckets, int reach, float *out, int32_t *error, hipStream_t s) {
+    const int distances = 2 * reach + 1;
+    if (dry_run()) {
+        plan_note("bias_by_distance_kernel: %d heads x %d distances", n_head, distances);
+        return hipSuccess;
+    }
+    hipLaunchKernelGGL(bias_by_distance_kernel, dim3((distances + 255) / 256, n_head), dim3(256), 0, s, table, n_buckets, n_head, buckets, distances, out, error);
+    return hipGetLastError();
+}
+
+hipError_t launch_attention_biased(const AttentionJob &j, const float *bias, int reach, bool all, hipStream_t s) {
+    BiasArgs a{};
+    a.bias = bias;
+    a.reach = reach;
+    a.all = all;
+    return launch_as(j, a, s);
+}
+
+}  // namespace qproj

@@ -850,8 +850,9 @@ int qproj_sync(qproj_ctx *ctx) {
         const struct { int raised; const char *what; } all[] = {{flag[0], "expert id outside [0, n_expert) in a MUL_MAT_ID batch"},
                                                                 {flag[1] & kKvBadSlot, "a slot behind the key/value cache"},
                                                                 {flag[1] & kKvBadPage, "a page outside [0, n_pages) in an attention call"},
-                                                                {flag[1] & kKvBadRows, "q_start or kv_len out of bounds in an attention call"}};
-        char buf[300] = "";     // (what several calls have met since the last time is named once each)
+                                                                {flag[1] & kKvBadRows, "q_start or kv_len out of bounds in an attention call"},
+                                                                {flag[1] & kKvBadBucket, "a bucket outside [0, n_buckets) of a bias table"}};
+        char buf[400] = "";     // (what several calls have met since the last time is named once each)
         for (const auto &f : all)
             if (f.raised) snprintf(buf + strlen(buf), sizeof buf - strlen(buf), "%s%s", *buf ? "; " : "", f.what);
         return fail(ctx, QPROJ_ERR_INVALID_ARG, buf);
@@ -1875,6 +1876,49 @@ int qproj_cross_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float 
                                  y_dev, y_stride, &j);
     if (rc != QPROJ_OK) return rc;
     QP_HIP(ctx, launch_attention_all(j, ctx->stream));
+    return QPROJ_OK;
+}
+
+int qproj_relative_buckets(int64_t n_buckets, int64_t reach, int both_sides, int32_t *buckets) {
+    if (!buckets || n_buckets > 1 << 20 || (both_sides && n_buckets % 2 != 0)) return QPROJ_ERR_INVALID_ARG;
+    const int64_t side = both_sides ? n_buckets / 2 : n_buckets, e = side / 2;
+    if (e < 1 || reach <= e || reach > attention_most_reach()) return QPROJ_ERR_INVALID_ARG;
+    for (int64_t d = -reach; d <= reach; ++d) {
+        const int64_t away = both_sides ? std::abs(d) : std::max<int64_t>(0, -d);
+        // (the logarithms' quotient is a whole number where powers meet exactly: it must not fall under it by their rounding)
+        const double far = away < e ? 0.0 : log((double)away / e) / log((double)reach / e) * (side - e);
+        const int64_t b = away < e ? away : std::min<int64_t>(side - 1, e + (int64_t)floor(far + 1e-10));
+        buckets[d + reach] = (int32_t)(b + (both_sides && d > 0 ? side : 0));
+    }
+    return QPROJ_OK;
+}
+
+static const char *bad_reach(int64_t reach) { return reach < 0 || reach > attention_most_reach() ? "reach out of range" : nullptr; }
+
+int qproj_bias_by_distance(qproj_ctx *ctx, const float *table_dev, int64_t n_buckets, int64_t n_head, const int32_t *buckets_dev, int64_t reach, float *out_dev) {
+    const char *call = "qproj_bias_by_distance";
+    if (!ctx) return QPROJ_ERR_INVALID_ARG;
+    if (!table_dev || !buckets_dev || !out_dev) return refuse(ctx, call, "null argument");
+    if (n_buckets <= 0 || n_buckets > 1 << 20 || n_head <= 0 || n_head > kMostHeads) return refuse(ctx, call, "n_buckets or n_head out of range");
+    if (const char *why = bad_reach(reach)) return refuse(ctx, call, why);
+    if (!dry_run()) QP_HIP(ctx, hipSetDevice(ctx->device));
+    QP_HIP(ctx, launch_bias_by_distance(table_dev, (int)n_buckets, (int)n_head, buckets_dev, (int)reach, out_dev, ctx->flag_dev + 1, ctx->stream));
+    return QPROJ_OK;
+}
+
+int qproj_attention_biased(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens, int64_t n_head,
+                           int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q, const int32_t *pages_dev,
+                           int64_t pages_stride, const qproj_position_bias *bias, float scale, float *y_dev, int64_t y_stride) {
+    const char *call = "qproj_attention_biased";
+    if (!ctx) return QPROJ_ERR_INVALID_ARG;
+    if (!bias || !bias->by_distance_dev) return refuse(ctx, call, "null argument");
+    if (reinterpret_cast<uintptr_t>(bias->by_distance_dev) % 4 != 0) return refuse(ctx, call, "biases must be 4-byte aligned");
+    if (const char *why = bad_reach(bias->reach)) return refuse(ctx, call, why);
+    KvView view;
+    AttentionJob j{};
+    const int rc = attention_job(ctx, call, kv, &view, q_dev, q_stride, n_tokens, n_head, n_seq, q_start_dev, kv_len_dev, max_q, pages_dev, pages_stride, scale, 0, y_dev, y_stride, &j);
+    if (rc != QPROJ_OK) return rc;
+    QP_HIP(ctx, launch_attention_biased(j, bias->by_distance_dev, (int)bias->reach, bias->causal == 0, ctx->stream));
     return QPROJ_OK;
 }
 

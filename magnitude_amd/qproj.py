@@ -68,6 +68,9 @@ SYMBOLS = {
     "qproj_kv_read": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp]),
     "qproj_attention": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, C.c_float, _i64, _vp, _i64]),
     "qproj_cross_attention": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, C.c_float, _vp, _i64]),
+    "qproj_relative_buckets": (_i32, [_i64, _i64, _i32, _vp]),
+    "qproj_bias_by_distance": (_i32, [_vp, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "qproj_attention_biased": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, C.c_float, _vp, _i64]),
     "qproj_version": (C.c_char_p, []),
     "qproj_probe_eligibility": (_i32, [_vp]),
 }
@@ -98,6 +101,11 @@ class KvPlanes(C.Structure):
     """struct qproj_kv_cache of include/qproj.h"""
     _fields_ = [("k_codes", _vp), ("k_scales", _vp), ("v_codes", _vp), ("v_scales", _vp), ("n_pages", _i64),
                 ("page_tokens", _i64), ("n_head_kv", _i64), ("head_dim", _i64)]
+
+
+class PositionBias(C.Structure):
+    """struct qproj_position_bias of include/qproj.h"""
+    _fields_ = [("by_distance_dev", _vp), ("reach", _i64), ("causal", C.c_int)]
 
 
 ROPE_MODES = {"pairs": 0, "halves": 1}
@@ -215,6 +223,16 @@ def rope_frequencies(n_dims: int, base: float = 10000.0, freq_scale: float = 1.0
     return freqs, magnitude.value
 
 
+def relative_buckets(n_buckets: int, reach: int, both_sides: bool = True) -> np.ndarray:
+    """The buckets int32 [2 * reach + 1] of a learned position bias for distances token - row from -reach to reach, half of them for
+    either side or (both_sides False) all for tokens before the row.  Needs no GPU."""
+    buckets = np.empty(2 * max(0, reach) + 1, dtype=np.int32)
+    st = load_library().qproj_relative_buckets(n_buckets, reach, 1 if both_sides else 0, buckets.ctypes.data)
+    if st:
+        raise QprojError(st, f"qproj_relative_buckets({n_buckets} buckets, reach {reach}, both_sides {both_sides})")
+    return buckets
+
+
 def row_bytes(qtype: int, k: int) -> int:
     return int(load_library().qproj_row_bytes(qtype, k))
 
@@ -290,6 +308,8 @@ class Context:
         self.device = device
         self._turn = Rotation()
         self._turn_ref = C.byref(self._turn)
+        self._bias = PositionBias()
+        self._bias_ref = C.byref(self._bias)
         self._held = []     # contiguous copies handed to launches that may still be pending (dropped in sync())
 
     def close(self) -> None:
@@ -746,6 +766,44 @@ class Context:
         if sync:
             torch.cuda.current_stream(q.device).synchronize()
         self._check(self.lib.qproj_cross_attention(*head, *tail))
+        if sync:
+            self.sync()
+        return y
+
+    def bias_by_distance(self, table: torch.Tensor, buckets: torch.Tensor, out: Optional[torch.Tensor] = None,
+                         sync: bool = True) -> torch.Tensor:
+        """A model's table of biases f32 [n_buckets, heads] laid out by distance, f32 [heads, 2 * reach + 1], for attention_biased;
+        buckets i32 [2 * reach + 1] (relative_buckets, on the device)."""
+        if table.dim() != 2 or buckets.dim() != 1 or buckets.numel() % 2 != 1:
+            raise ValueError("table must be [n_buckets, heads] and buckets [2 * reach + 1]")
+        shape = (table.shape[1], buckets.numel())
+        y = out if out is not None else torch.empty(shape, dtype=torch.float32, device=table.device)
+        if tuple(y.shape) != shape:
+            raise ValueError(f"out must be {list(shape)}")
+        tp, bp = self._on_device(table, torch.float32, "table"), self._on_device(buckets, torch.int32, "buckets")
+        yp = self._on_device(y, torch.float32, "out")
+        if sync:
+            torch.cuda.current_stream(table.device).synchronize()
+        self._check(self.lib.qproj_bias_by_distance(self.handle, tp, table.shape[0], table.shape[1], bp, buckets.numel() // 2, yp))
+        if sync:
+            self.sync()
+        return y
+
+    def attention_biased(self, kv: KvCache, q: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor,
+                         bias: torch.Tensor, causal: bool = True, max_q: Optional[int] = None, scale: Optional[float] = None,
+                         out: Optional[torch.Tensor] = None, sync: bool = True) -> torch.Tensor:
+        """As attention, with bias f32 [heads, 2 * reach + 1] (bias_by_distance) of token - row, clamped to -reach .. reach, added to the
+        scaled scores; causal False: every row sees all tokens of its sequence (an encoder's layers)."""
+        n, head, tail, y = self._attention_args(kv, q, q_start, kv_len, pages, max_q, scale, out)
+        if bias.dim() != 2 or bias.shape[0] != q.shape[1] or bias.shape[1] % 2 != 1:
+            raise ValueError("bias must be [heads, 2 * reach + 1]")
+        b = self._bias
+        b.by_distance_dev, b.reach, b.causal = self._on_device(bias, torch.float32, "bias"), bias.shape[1] // 2, 1 if causal else 0
+        if n == 0:
+            return y
+        if sync:
+            torch.cuda.current_stream(q.device).synchronize()
+        self._check(self.lib.qproj_attention_biased(*head[:-1], self._bias_ref, head[-1], *tail))
         if sync:
             self.sync()
         return y

@@ -57,6 +57,14 @@ pub struct qproj_kv_cache {
     pub head_dim: i64,
 }
 
+/// Biases by distance `[n_head][2 * reach + 1]` on the device
+#[repr(C)]
+pub struct qproj_position_bias {
+    pub by_distance_dev: *const f32,
+    pub reach: i64,
+    pub causal: c_int,
+}
+
 /// struct qproj_eligibility of include/qproj.h
 #[repr(C)]
 pub struct qproj_eligibility {
@@ -142,6 +150,13 @@ extern "C" {
                                  n_tokens: i64, n_head: i64, n_seq: i64, q_start_dev: *const i32, kv_len_dev: *const i32,
                                  max_q: i64, pages_dev: *const i32, pages_stride: i64, scale: f32, y_dev: *mut f32,
                                  y_stride: i64) -> c_int;
+    pub fn qproj_relative_buckets(n_buckets: i64, reach: i64, both_sides: c_int, buckets: *mut i32) -> c_int;
+    pub fn qproj_bias_by_distance(ctx: *mut qproj_ctx, table_dev: *const f32, n_buckets: i64, n_head: i64,
+                                  buckets_dev: *const i32, reach: i64, out_dev: *mut f32) -> c_int;
+    pub fn qproj_attention_biased(ctx: *mut qproj_ctx, kv: *const qproj_kv_cache, q_dev: *const f32, q_stride: i64,
+                                  n_tokens: i64, n_head: i64, n_seq: i64, q_start_dev: *const i32, kv_len_dev: *const i32,
+                                  max_q: i64, pages_dev: *const i32, pages_stride: i64, bias: *const qproj_position_bias,
+                                  scale: f32, y_dev: *mut f32, y_stride: i64) -> c_int;
     pub fn qproj_version() -> *const c_char;
     pub fn qproj_probe_eligibility(out: *mut qproj_eligibility) -> c_int;
 }

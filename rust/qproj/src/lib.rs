@@ -194,6 +194,18 @@ impl Context {
         })
     }
 
+    /// Attention with a bias of the distance between token and row; see `qproj_attention_biased`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn attention_biased(&self, kv: &sys::qproj_kv_cache, q: DevicePtr, n: i64, n_head: i64, n_seq: i64, q_start: DevicePtr,
+                            kv_len: DevicePtr, max_q: i64, pages: DevicePtr, pages_stride: i64, bias: &sys::qproj_position_bias,
+                            scale: f32, y: DevicePtr) -> Result<()> {
+        let row = n_head * kv.head_dim;
+        self.check(unsafe {
+            sys::qproj_attention_biased(self.raw, kv, q.0.cast(), row, n, n_head, n_seq, q_start.0.cast(), kv_len.0.cast(), max_q,
+                                        pages.0.cast(), pages_stride, bias, scale, y.0.cast(), row)
+        })
+    }
+
     /// Attention of rows that see all tokens of their sequence, an encoder's states say; see `qproj_cross_attention`.
     #[allow(clippy::too_many_arguments)]
     pub fn cross_attention(&self, kv: &sys::qproj_kv_cache, q: DevicePtr, n: i64, n_head: i64, n_seq: i64, q_start: DevicePtr,
@@ -203,6 +215,17 @@ impl Context {
             sys::qproj_cross_attention(self.raw, kv, q.0.cast(), row, n, n_head, n_seq, q_start.0.cast(), kv_len.0.cast(), max_q,
                                        pages.0.cast(), pages_stride, scale, y.0.cast(), row)
         })
+    }
+}
+
+/// The buckets of the distances from `-reach` to `reach`; see `qproj_relative_buckets`.
+pub fn relative_buckets(n_buckets: i64, reach: i64, both_sides: bool) -> Result<Vec<i32>> {
+    let mut buckets = vec![0i32; (2 * reach.max(0) + 1) as usize];
+    let st = unsafe { sys::qproj_relative_buckets(n_buckets, reach, both_sides as i32, buckets.as_mut_ptr()) };
+    if st == sys::QPROJ_OK {
+        Ok(buckets)
+    } else {
+        Err(QprojError { status: st, message: "relative_buckets".into() })
     }
 }
 

@@ -51,10 +51,11 @@ def attention(cache, q, q_start, kv_len, pages, scale, sees_all=False, bias=None
 
 
 def allowed(sizes, dim, tokens):
-    """kv_ref.allowed, and what a bias adds: its product with log2(e) is rounded twice (the constant, the product), its sum with the score once, of at
-    most both: delta <= |bias| * 3 * 2^-24 + |score| * 2^-24 more, and the score stays under `steep`."""
+    """kv_ref.allowed, and what a bias adds: its product with log2(e) is rounded twice (the constant, the product), its sum with the score or with what is
+    taken off the score (the row's largest, which is a score and a bias too, and 13 + 2.5 in powers of two) once, of at most both: delta <=
+    |bias| * 2 * 2^-24 + (2 * |bias| + |score| + 11) * 2^-24 more, and the score stays under `steep`."""
     weight, steep, spread, lift = sizes
-    more = lift * 3 * 2.0 ** -24 + np.where(lift > 0, steep, 0) * 2.0 ** -24
+    more = np.where(lift > 0, 4 * lift + steep + 11, 0) * 2.0 ** -24
     return kv_ref.allowed((weight, steep, spread), dim, tokens) + weight * np.expm1(2 * more)[..., None] * 1.01
 
 

@@ -125,3 +125,126 @@ def test_cross_bad_pages_and_bounds_are_reported(ctx):
         np.testing.assert_allclose(got[left], ok[left], rtol=1e-5, atol=1e-6)
         assert (got[[i for i in range(5) if i not in left]] == 7.5).all()
     ctx.sync()
+
+
+# ---- a bias of the distance -------------------------------------------------------------------------------------------------
+def make_bias(rng, heads, reach, n_buckets=None, both=True, size=3.0):
+    """(by distance, and where there are buckets the table)"""
+    from magnitude_amd import relative_buckets
+    if n_buckets is None:
+        return (rng.standard_normal((heads, 2 * reach + 1)) * size).astype(np.float32), None
+    table = (rng.standard_normal((n_buckets, heads)) * size).astype(np.float32)
+    return np.ascontiguousarray(table[relative_buckets(n_buckets, reach, both)].T), table
+
+
+def check_biased(ctx, kv, pages, q, q_start, kv_len, bias, causal, scale=None, **kw):
+    s = kv.head_dim ** -0.5 if scale is None else scale
+    args = numpy_cache(kv), q, q_start, kv_len, pages, s
+    want, sizes = forms_ref.attention(*args, sees_all=not causal, bias=bias)
+    plain = forms_ref.attention(*args, sees_all=not causal, bias=bias, dtype=np.float32)[0]
+    for table in (wide(pages, kv), pages):
+        out = torch.full(q.shape, 7.5, device="cuda")
+        got = ctx.attention_biased(kv, dev(q), i32(q_start), i32(kv_len), dev(table), dev(bias), causal=causal, scale=scale, out=out, **kw).cpu().numpy()
+        compare(got, want, plain, sizes, kv.head_dim, max([1] + list(kv_len)))
+    return got
+
+
+BIASED = [  # dim, page, kv heads, group, [(tokens, rows)], reach
+    (64, 64, 1, 1, [(1, 1)], 128),
+    (64, 64, 12, 1, [(300, 1), (64, 1), (65, 1), (1, 1)], 128),
+    (64, 16, 2, 1, [(200, 200), (33, 33), (1, 1)], 20),
+    (64, 64, 2, 1, [(700, 700)], 128),
+    (128, 32, 1, 8, [(500, 90), (40, 40)], 128),
+    (128, 64, 2, 3, [(1000, 1), (90, 7), (0, 0), (0, 3), (5, 9)], 64),
+    (96, 128, 1, 16, [(600, 20)], 40),
+    (256, 16, 1, 4, [(400, 70)], 30),
+    (64, 256, 1, 71, [(100, 2)], 128),                    # as many heads an item as there is room for
+    (64, 32, 1, 5, [(3000, 40)], 500),
+    (128, 64, 1, 2, [(2500, 33)], 1703),
+    (64, 64, 1, 1, [(9000, 1)], 0),
+    (64, 64, 1, 2, [(20000, 3)], 128),                    # many parts, joined by a launch of their own
+    (128, 16, 4, 4, [(1 + 37 * i % 301, 1) for i in range(90)], 10),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim,page,kv_heads,group,seqs,reach", BIASED)
+def test_biased_attention(ctx, dim, page, kv_heads, group, seqs, reach, causal):
+    tell("biased", dim, page, kv_heads, group, seqs, reach, causal)
+    rng = np.random.default_rng(dim + page + len(seqs) + causal)
+    lens = [n for n, _ in seqs]
+    kv, pages = make_cache(rng, lens, page, kv_heads, dim)
+    q_start = np.cumsum([0] + [m for _, m in seqs])
+    q = rng.standard_normal((q_start[-1], kv_heads * group, dim)).astype(np.float32)
+    bias, _ = make_bias(rng, kv_heads * group, reach)
+    check_biased(ctx, kv, pages, q, q_start, lens, bias, causal)
+    check_biased(ctx, kv, pages, q, q_start, lens, bias, causal, scale=0.25, max_q=max(m for _, m in seqs))
+
+
+@pytest.mark.parametrize("both", [True, False])
+@pytest.mark.parametrize("n_buckets,reach,heads", [(32, 128, 12), (8, 20, 1), (64, 500, 3)])
+def test_bias_by_distance(ctx, n_buckets, reach, heads, both):
+    from magnitude_amd import QprojError, relative_buckets
+    rng = np.random.default_rng(n_buckets)
+    bias, table = make_bias(rng, heads, reach, n_buckets, both)
+    buckets = relative_buckets(n_buckets, reach, both)
+    assert np.array_equal(ctx.bias_by_distance(dev(table), dev(buckets)).cpu().numpy(), bias)
+    for bad in (-1, n_buckets, 2147483647):
+        wrong = buckets.copy()
+        wrong[3] = bad
+        out = torch.full(bias.shape, 7.5, device="cuda")
+        with pytest.raises(QprojError, match="bucket"):
+            ctx.bias_by_distance(dev(table), dev(wrong), out=out)
+        got = out.cpu().numpy()
+        assert not got[:, 3].any() and np.array_equal(np.delete(got, 3, 1), np.delete(bias, 3, 1))
+    ctx.sync()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("reach", [3, 60, 128])
+def test_a_bias_of_minus_infinity_hides_tokens(ctx, reach, causal):
+    """at single distances, at all beyond reach on either side, at all but a row's own, at all: as masks; rows that see nothing are zeros"""
+    rng = np.random.default_rng(reach)
+    lens, q_start = [400, 90, 5], [0, 70, 160, 162]
+    kv, pages = make_cache(rng, lens, 16, 2, 64)
+    q = rng.standard_normal((162, 4, 64)).astype(np.float32)
+    whole, _ = make_bias(rng, 4, reach)
+    for cut in (slice(0, 1), slice(2 * reach, None), slice(0, 2 * reach + 1, 2), np.r_[0:reach, reach + 1:2 * reach + 1]):
+        bias = whole.copy()
+        bias[:, cut] = -np.inf
+        check_biased(ctx, kv, pages, q, q_start, lens, bias, causal)
+    bias = whole.copy()
+    bias[2] = -np.inf
+    got = check_biased(ctx, kv, pages, q, q_start, lens, bias, causal)
+    assert not got[:, 2].any() and got[:, 1].any(-1).all()
+
+
+def test_biased_what_is_not_seen_is_not_looked_at(ctx):
+    """blocks that are not finite, hidden by the bias or by the rows' own positions"""
+    rng = np.random.default_rng(31)
+    kv, pages = make_cache(rng, [300], 16, 1, 64)
+    q = dev(rng.standard_normal((20, 2, 64)).astype(np.float32))
+    bias, _ = make_bias(rng, 2, 50)
+    bias[:, :30] = -np.inf                      # more than 20 tokens back: not seen, from 29 on by distances of their own
+    args = kv, q, i32([0, 20]), i32([300]), dev(pages), dev(bias)
+    base = ctx.attention_biased(*args).cpu().numpy()
+    for t in list(range(0, 259)):               # 280 - 21 and before: out of every row's sight
+        for plane in (1, 3):
+            kv.tensors[plane][int(pages[0, t // 16]), :, t % 16] = float("nan")
+    np.testing.assert_array_equal(ctx.attention_biased(*args).cpu().numpy(), base)
+    bias[0, 50 - 1] = np.nan                    # met by the rows that have a token before them
+    got = ctx.attention_biased(kv, q, i32([0, 20]), i32([300]), dev(pages), dev(bias)).cpu().numpy()
+    assert np.isnan(got[:, 0]).all()
+    np.testing.assert_array_equal(got[:, 1], base[:, 1])
+
+
+def test_a_bias_of_nothing_changes_nothing(ctx):
+    rng = np.random.default_rng(32)
+    kv, pages = make_cache(rng, [700, 20], 64, 2, 128)
+    q = dev(rng.standard_normal((41, 8, 128)).astype(np.float32))
+    args = kv, q, i32([0, 40, 41]), i32([700, 20]), dev(pages)
+    none = torch.zeros((8, 257), device="cuda")
+    assert (ctx.attention_biased(*args, none) - ctx.attention(*args)).abs().max() < 1e-5
+    assert (ctx.attention_biased(*args, none, causal=False) - ctx.cross_attention(*args)).abs().max() < 1e-5
+    same = torch.full((8, 257), 7.25, device="cuda")       # softmax does not see what all tokens have
+    assert (ctx.attention_biased(*args, same) - ctx.attention(*args)).abs().max() < 1e-5
