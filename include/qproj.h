@@ -332,6 +332,22 @@ int qproj_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev
                     const int32_t *pages_dev, int64_t pages_stride, float scale, int64_t window, float *y_dev,
                     int64_t y_stride);
 
+/* Attention of a batch whose sequences share their first tokens (requests behind one system prompt, samples of one prompt): the results of
+ * qproj_attention for the same arguments, what is shared read and multiplied once for several sequences.
+ *   sequences group_start_dev[g] .. group_start_dev[g + 1] - 1 (at most max_group of them) are a group, whose first
+ *   shared_len_dev[g] tokens lie in the same places: their rows of pages_dev begin with the same pages.  (Sequences that share nothing are groups of
+ *   one, or have shared_len 0.)
+ * Any of a group's tables may be read for what is shared.  shared_len may pass a sequence's tokens: what lies before the newest rows of all
+ * sequences that are taken together is shared, in steps of 64 tokens.  group_start_dev has to ascend from 0 to n_seq by at most
+ * max_group, shared_len_dev to be at least 0; a group that breaks this is left out, sequences of no group are too, and the next qproj_sync reports
+ * it.  Bounds, errors, workspace and capture otherwise as for qproj_attention, of which a row's result differs in the order of its sums only.
+ * A call that would gain nothing is qproj_attention's and does not look at the groups: with a window, with max_group under two, or where
+ * max_q rows of a sequence times n_head / n_head_kv leave no room for another's among 32 (16 where a head is 256 wide). */
+int qproj_attention_shared(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens,
+                           int64_t n_head, int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q,
+                           const int32_t *pages_dev, int64_t pages_stride, int64_t n_groups, const int32_t *group_start_dev,
+                           const int32_t *shared_len_dev, int64_t max_group, float scale, int64_t window, float *y_dev, int64_t y_stride);
+
 /* Attention of rows over tokens of another length: llama.cpp's build_attn over an encoder's states (llm_graph_input_attn_cross), and an
  * encoder's own layers.  As qproj_attention, but every row q_start_dev[s] .. q_start_dev[s + 1] - 1 sees all kv_len_dev[s] tokens of its
  * sequence, of which there may be fewer than rows:

@@ -183,6 +183,12 @@ __host__ __device__ __forceinline__ Item item_of(const A &a, int s, const Sequen
     it.lo = q.len - q.count + row_tile * a.tokens;
     it.hi = it.lo + it.count - 1;
     it.see = a.window && it.lo >= a.window ? it.lo - a.window + 1 : 0;     // (lo is negative where a sequence has more rows than tokens)
+    if constexpr (A::kSees == kPrefix) {     // (of a group: its first sequence, sequences, tokens they share)
+        it.seq = q.start + row_tile * a.together;
+        it.count = min(a.together, q.count - row_tile * a.together);
+        it.first = it.lo = it.hi = 0;
+        it.see = q.len;
+    }
     if constexpr (A::kSees == kAll) it.lo = it.hi = q.len - 1;
     if constexpr (A::kSees == kBiased) {
         it.at = it.lo;
@@ -195,6 +201,59 @@ __host__ __device__ __forceinline__ int item_tiles(const Item &it) { return it.h
 // what an item takes of the line: a turn of the waves for every kWaves tiles
 __host__ __device__ __forceinline__ int item_turns(const Item &it) { return it.count <= 0 ? 0 : (item_tiles(it) + kWaves - 1) / kWaves; }
 
+// What lies behind the line's places: sequences, or groups of them.  Of a group: its first sequence, sequences, the tokens that they share.
+template <typename A>
+__host__ __device__ __forceinline__ int units_of(const A &a) {
+    if constexpr (A::kSees == kPrefix) return a.n_groups * a.row_tiles;
+    else return a.n_seq * a.row_tiles;
+}
+template <typename A>
+__host__ __device__ __forceinline__ int each_of(const A &a) {     // what an item takes of a unit
+    if constexpr (A::kSees == kPrefix) return a.together;
+    else return a.tokens;
+}
+template <typename A>
+__host__ __device__ __forceinline__ Sequence unit_of(const A &a, int s, bool &bad) {
+    if constexpr (A::kSees == kPrefix) {
+        Sequence g;
+        g.start = a.group_start[s];
+        const int end = a.group_start[s + 1];
+        g.len = a.shared_len[s];
+        g.count = end - g.start;
+        bad = g.start < 0 || end < g.start || end > a.n_seq || g.count > a.max_group || g.len < 0;
+        if (bad) g.count = 0;
+        bad = bad || (s == 0 && g.start != 0) || (s == a.n_groups - 1 && end != a.n_seq);     // (sequences of no group: reported, left out)
+        return g;
+    } else {
+        return sequence(a, s, bad);
+    }
+}
+
+// Tiles of an item of several sequences: those that they share, then every sequence's own.  A sequence shares no more than lies before its rows, and
+// whole tiles only.
+__host__ __device__ __forceinline__ int shared_tiles(int shared, int before) { return max(0, min(shared, before)) / kTile; }
+__host__ __device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len - 1) / kTile + 1 : 0; }
+template <typename A>
+__host__ __device__ __forceinline__ int turns_of(const A &a, int s, const Sequence &q, int row_tile) {
+    const Item it = item_of(a, s, q, row_tile);
+    if constexpr (A::kSees == kPrefix) {
+        int before = 0x7fffffff, tiles = 0, with_rows = 0;
+        for (int i = 0; i < it.count; ++i) {
+            bool bad;
+            const Sequence m = sequence(a, it.seq + i, bad);
+            if (m.count == 0) continue;
+            before = min(before, m.len - m.count);
+            tiles += tiles_of(m.len);
+            ++with_rows;
+        }
+        const int shared = with_rows ? shared_tiles(it.see, before) : 0;
+        tiles -= (with_rows - 1) * shared;
+        return (max(1, tiles) + kWaves - 1) / kWaves;
+    } else {
+        return item_turns(it);
+    }
+}
+
 // Thread `id`'s places of the line of one head's items, `per` of them: f(sequence, row tile, rows, turns) of those that hold an item (a sequence has
 // as many places as max_q allows), until one returns true.  outside(sequence) of sequences that break the bounds.
 template <typename A, typename F, typename G>
@@ -202,10 +261,10 @@ __host__ __device__ __forceinline__ void each_item(const A &a, int id, int units
     for (int u = id * per; u < min(units, (id + 1) * per);) {
         const int s = a.row_tiles == 1 ? u : (int)quotient(u, a.row_tiles), tile0 = u - s * a.row_tiles, tile1 = min(a.row_tiles, tile0 + min(units, (id + 1) * per) - u);
         bool bad;
-        const Sequence q = sequence(a, s, bad);
+        const Sequence q = unit_of(a, s, bad);
         if (bad && tile0 == 0) outside(s);
-        for (int tile = tile0; tile < tile1 && tile * a.tokens < q.count; ++tile)
-            if (f(s, tile, q, item_turns(item_of(a, s, q, tile)))) return;
+        for (int tile = tile0; tile < tile1 && tile * each_of(a) < q.count; ++tile)
+            if (f(s, tile, q, turns_of(a, s, q, tile))) return;
         u += tile1 - tile0;
     }
 }
@@ -379,6 +438,15 @@ struct KindLds<kBiased> {
     float bias[kBiasFloats + 64];     // (loads write 64 at a time)
 };
 
+// The item's sequences, a copy for every wave, which keeps itself in order.
+constexpr int kTogether = 32;        // at most
+template <>
+struct KindLds<kPrefix> {
+    int32_t first[kWaves][kTogether], count[kWaves][kTogether], before[kWaves][kTogether];   // first row, rows, tokens before them
+    int32_t newest[kWaves][64];      // its last token
+    int32_t ends[kWaves][64];        // tiles of the item up to the sequence's last one
+};
+
 template <int D, int NQ, typename A>
 struct SharedLds : KindLds<A::kSees> {
     union {
@@ -405,6 +473,61 @@ struct Running {
     float m[NQ], l[NQ];    // of the lane's column; l of the lane's own tokens only until the end
 };
 
+// kPrefix: what is the same for all lanes of the item's sequences
+struct Members {
+    int lead;            // a sequence whose pages hold what is shared
+    int shared, tiles;   // tiles that are shared, all of them
+};
+
+template <int D, int NQ, typename A>
+__device__ __forceinline__ Members members(const A &a, const Item &it, SharedLds<D, NQ, A> &lds, int wave, int lane) {
+    Members m{};
+    if constexpr (A::kSees == kPrefix) {
+        Sequence q{0, 0, 0};
+        bool bad = false;
+        if (lane < it.count) q = sequence(a, it.seq + lane, bad);
+        if (bad) atomicOr(a.error, kKvBadRows);
+        const uint64_t rows = __ballot(q.count > 0);
+        const int before = 0x7fffffff - (int)wave_max(q.count > 0 ? 0x7fffffffu - (uint32_t)max(0, q.len - q.count) : 0u);
+        m.shared = rows ? shared_tiles(it.see, before) : 0;
+        m.lead = it.seq + (rows ? __builtin_ctzll(rows) : 0);
+        const int ends = wave_scan(q.count > 0 ? tiles_of(q.len) - m.shared : 0) + m.shared;
+        m.tiles = __builtin_amdgcn_readlane(ends, 63);
+        if (lane < kTogether) {
+            lds.first[wave][lane] = q.count > 0 ? q.start : 0;     // (a row that there is: columns without one load it)
+            lds.count[wave][lane] = q.count;
+            lds.before[wave][lane] = q.len - q.count;
+        }
+        lds.newest[wave][lane] = q.len - 1;
+        lds.ends[wave][lane] = ends;
+        wave_sync();
+    }
+    return m;
+}
+
+// A column's row: whether there is one, its number, and of kPrefix the sequence within the item and the last token that it sees.
+struct Row {
+    bool live;
+    int row, head, seq, last;
+};
+template <int D, int NQ, typename A>
+__device__ __forceinline__ Row row_of(const A &a, const Item &it, int heads, int slot, const SharedLds<D, NQ, A> &lds, int wave) {
+    Row r{};
+    const int token = token_of(a, slot);
+    r.head = slot - token * a.split;
+    if constexpr (A::kSees == kPrefix) {
+        const int seq = token < a.tokens ? (int)((uint32_t)token * a.row_part >> 16) : 0, i = token - seq * a.max_q;
+        r.live = token < a.tokens && i < lds.count[wave][seq] && r.head < heads;
+        r.row = lds.first[wave][seq] + (r.live ? i : 0);
+        r.seq = r.live ? seq : -1;
+        r.last = r.live ? lds.before[wave][seq] + i : -1;
+    } else {
+        r.live = token < it.count && r.head < heads;
+        r.row = it.first + (r.live ? token : 0);
+    }
+    return r;
+}
+
 // 16 queries of an item for the matrix cores: 22 bits of q * scale * log2(e), the row scaled by a power of two.  A wave takes the blocks
 // wave, wave + 4, ... of all rows.  (All blocks in every wave, for want of a meeting about the rows' largest values, kept the loads of
 // keys and values waiting: 512 prompt tokens took 23.5 us instead of 21.7, 4096 402 instead of 388.)
@@ -415,12 +538,11 @@ struct Queries {
 };
 
 template <int D, int NQ, typename A>
-__device__ __forceinline__ void load_queries(const A &a, const Item &it, int head0, int heads, Queries<D, NQ> &q, int wave, int lane) {
+__device__ __forceinline__ void load_queries(const A &a, const Item &it, int head0, int heads, Queries<D, NQ> &q, const SharedLds<D, NQ, A> &lds, int wave, int lane) {
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
-        const int slot = g * 16 + (lane & 15), token = token_of(a, slot), head = slot - token * a.split;
-        const bool live = token < it.count && head < heads;
-        const float *row = a.q + (int64_t)(it.first + (live ? token : 0)) * a.q_stride + (int64_t)(head0 + (live ? head : 0)) * D + 8 * (lane >> 4);
+        const Row r = row_of(a, it, heads, g * 16 + (lane & 15), lds, wave);
+        const float *row = a.q + (int64_t)r.row * a.q_stride + (int64_t)(head0 + (r.live ? r.head : 0)) * D + 8 * (lane >> 4);
 #pragma unroll
         for (int i = 0; i < q.kMine; ++i)
 #pragma unroll
@@ -435,8 +557,7 @@ __device__ __forceinline__ void stage_queries(const A &a, const Item &it, int he
     const int col = lane & 15;
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
-        const int slot = g * 16 + col, token = token_of(a, slot);
-        const bool live = token < it.count && slot - token * a.split < heads;
+        const bool live = row_of(a, it, heads, g * 16 + col, lds, wave).live;
         float most = 0.f;
         bool whole = true;
 #pragma unroll
@@ -482,7 +603,7 @@ __device__ __forceinline__ void stage_queries(const A &a, const Item &it, int he
 // Tiles [from, to) of an item (in tiles from token 0 on), every kWaves-th of them.  Two barriers of the workgroup, before and
 // behind the staged queries, whatever there is to do.
 template <int D, int NQ, typename A>
-__device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, int head0, int heads, int from, int to, SharedLds<D, NQ, A> &shared,
+__device__ __forceinline__ void walk(const A &a, const Item &it, const Members &members, int kv_head, int head0, int heads, int from, int to, SharedLds<D, NQ, A> &shared,
                                      int wave, Running<D, NQ> &st, int lane) {
     WaveLds<D, NQ> &lds = shared.wave[wave];
     constexpr int B = D / 32, RB = D / 2, T = D / 16;
@@ -498,16 +619,33 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
 #pragma unroll
         for (int t = 0; t < T; ++t) st.o[t][g] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const bool work = from < to && it.hi >= 0;
+    const bool work = from < to && (A::kSees == kPrefix ? members.tiles > 0 : it.hi >= 0);
 
+    // Where a tile's tokens are: whose (of the item's sequences; -1: shared, or the only one's), which pages, its first token, the first and the last one that is seen.
+    struct Place {
+        int own, seq, t0, see, hi;
+    };
+    const auto find = [&](int tile) {
+        if constexpr (A::kSees == kPrefix) {
+            if (tile < members.shared) return Place{-1, members.lead, tile * kTile, 0, members.shared * kTile - 1};
+            const int ends = shared.ends[wave][lane], last = shared.newest[wave][lane];
+            const int own = min((int)__popcll(__ballot(ends <= tile)), it.count - 1);
+            const int start = own ? __builtin_amdgcn_readlane(ends, max(own - 1, 0)) : members.shared;
+            return Place{own, it.seq + own, (members.shared + tile - start) * kTile, 0, __builtin_amdgcn_readlane(last, own)};
+        } else {
+            return Place{-1, it.seq, tile * kTile, it.see, it.hi};
+        }
+    };
     // page of the lane's token of a tile (a token outside what is seen: of the nearest one that is)
     const int32_t *table = a.pages + (int64_t)it.seq * a.pages_stride;
-    const auto page_of = [&](int tile) {
-        const int t = min(max(tile * kTile + lane, it.see), it.hi);
-        return table[t >> shift];
+    const auto page_of = [&](const Place &p) {
+        const int t = min(max(p.t0 + lane, p.see), p.hi);
+        return (A::kSees == kPrefix ? a.pages + (int64_t)p.seq * a.pages_stride : table)[t >> shift];
     };
     const int last_tile = work ? from + (to - 1 - from) / kWaves * kWaves : from;   // of this wave
-    int page = work ? page_of(from) : 0, page_next = work ? page_of(min(from + kWaves, last_tile)) : 0;
+    Place now{}, next{};        // kPrefix: this tile's and the wave's next one's (otherwise known from their numbers)
+    if (A::kSees == kPrefix && work) now = find(from), next = find(min(from + kWaves, last_tile));
+    int page = work ? page_of(A::kSees == kPrefix ? now : find(from)) : 0, page_next = work ? page_of(A::kSees == kPrefix ? next : find(min(from + kWaves, last_tile))) : 0;
     bool bad_page = false;
 
     uint32_t k_raw[4][B];
@@ -515,8 +653,8 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
     int bad_groups;      // of the tile whose loads are in flight
     uint32_t rows[4];    // first row of its groups of 16 tokens
 
-    const auto place = [&](int tile) {   // rows of the tile whose pages have come
-        const int own = tile * kTile + lane, t = min(max(own, it.see), it.hi);
+    const auto place = [&](const Place &p) {   // rows of the tile whose pages have come
+        const int own = p.t0 + lane, t = min(max(own, p.see), p.hi);
         const bool bad = (uint32_t)page >= (uint32_t)kv.n_pages;
         bad_page = bad_page || (bad && t == own);
         bad_groups = 0;
@@ -602,9 +740,9 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
         }
     }
     Queries<D, NQ> queries;
-    load_queries<D, NQ>(a, it, head0, heads, queries, wave, lane);
+    load_queries<D, NQ>(a, it, head0, heads, queries, shared, wave, lane);
     if (work) {
-        place(from);
+        place(A::kSees == kPrefix ? now : find(from));
         if (kAhead) load_v(0, rows);
         load_scales();
         load_k();
@@ -616,11 +754,17 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
 
     int pos[NQ];                // what the column's row sees, up to this token, -1: no row
     int own_bias[NQ];           // kBiased: its bias of token 0 is there, had the row one that far away
+    int own_seq[NQ];            // kPrefix: of the item's sequences
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
         const int slot = g * 16 + col, token = token_of(a, slot);
         const bool live = token < it.count && slot - token * a.split < heads;
         pos[g] = live ? (A::kSees == kAll ? it.hi : it.lo + token) : -1;
+        if constexpr (A::kSees == kPrefix) {
+            const Row r = row_of(a, it, heads, slot, shared, wave);
+            pos[g] = r.last;
+            own_seq[g] = r.seq;
+        }
         if constexpr (A::kSees == kBiased) {
             if (live && a.all) pos[g] = it.hi;
             own_bias[g] = (live ? slot - token * a.split : 0) * bias_room(a.reach) + kBiasPad + a.reach - (it.at + (live ? token : 0));
@@ -642,13 +786,14 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
     const bool young = (int)blockIdx.x >= a.young;
     bool up = false;
     for (int tile = from; tile < to; tile += kWaves) {
-        const int t0 = tile * kTile;
+        const Place here = A::kSees == kPrefix ? now : find(tile);
+        const int t0 = here.t0;
         const int bad_now = bad_groups;
         up = young && !up;
         if (up) __builtin_amdgcn_s_setprio(2); else __builtin_amdgcn_s_setprio(0);
         // ---- scales to LDS ----
         const int t = t0 + lane;
-        const bool live = t >= it.see && t <= it.hi && !((bad_now >> part) & 1);
+        const bool live = t >= here.see && t <= here.hi && !((bad_now >> part) & 1);
         uint32_t most = 0;
         bool tiny = false;
         uint16_t vs[B];
@@ -692,8 +837,15 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
         // ---- the next tile's values and scales, and the page of the one behind ----
         // (behind the wave's last tile that tile again: loads that no branch surrounds are waited for one by one)
         page = page_next;
-        page_next = page_of(min(tile + 2 * kWaves, last_tile));
-        place(min(tile + kWaves, last_tile));
+        if constexpr (A::kSees == kPrefix) {
+            now = next;
+            next = find(min(tile + 2 * kWaves, last_tile));
+            page_next = page_of(next);
+            place(now);
+        } else {
+            page_next = page_of(find(min(tile + 2 * kWaves, last_tile)));
+            place(find(min(tile + kWaves, last_tile)));
+        }
         load_scales();
         // ---- scores ----
         f32x4 s[4][NQ];
@@ -770,7 +922,8 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
         else load_v(0, rows_now);
         load_k();
         // ---- weights ----
-        const bool edge = t0 + kTile - 1 > it.lo || (a.window && t0 <= it.hi - a.window) || t0 < it.see || bad_now;
+        const bool edge = A::kSees == kPrefix ? here.own >= 0 || bad_now
+                                              : t0 + kTile - 1 > it.lo || (a.window && t0 <= it.hi - a.window) || t0 < it.see || bad_now;
         u32x4 p_hi[2][NQ], p_lo[2][NQ];
 #pragma unroll
         for (int c = 0; c < NQ; ++c) {
@@ -800,7 +953,9 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, int kv_head, in
                 }
             }
             if (edge) {
-                const int last = pos[c] - t0 - 4 * part, behind = a.window ? last - a.window : -kTile;   // of the lane's tokens 16 g + r
+                int last = pos[c] - t0 - 4 * part;                             // of the lane's tokens 16 g + r
+                if constexpr (A::kSees == kPrefix) last = here.own >= 0 && own_seq[c] != here.own ? -1 : last;
+                const int behind = A::kSees != kPrefix && a.window ? last - a.window : -kTile;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const bool there = !((bad_now >> g) & 1);
@@ -1005,10 +1160,8 @@ constexpr uint32_t kFirstCall = 0x9e3779b9u;     // (the number of a call that f
 
 // rows of an item from sums: lane's column of 16 queries, 4 dimensions of 16
 template <int D, int NQ, typename A>
-__device__ __forceinline__ float *out_row(const A &a, const Item &it, int head0, int heads, int g, int lane, bool &live) {
-    const int slot = g * 16 + (lane & 15), token = token_of(a, slot), head = slot - token * a.split;
-    live = token < it.count && head < heads;
-    return a.y + (int64_t)(it.first + (live ? token : 0)) * a.y_stride + (int64_t)(head0 + (live ? head : 0)) * D + 4 * (lane >> 4);
+__device__ __forceinline__ float *out_row(const A &a, const Row &r, int head0, int lane) {
+    return a.y + (int64_t)r.row * a.y_stride + (int64_t)(head0 + (r.live ? r.head : 0)) * D + 4 * (lane >> 4);
 }
 
 // The waves' sums of an item: every wave adds a quarter of the dimensions, and writes rows of the result, or a part of one.
@@ -1018,8 +1171,9 @@ __device__ __forceinline__ void meet(const A &a, const Item &it, int head0, int 
     constexpr int T = D / 16, kMeet = T / meet_rounds(D);
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
-        bool live;
-        float *y = out_row<D, NQ>(a, it, head0, heads, g, lane, live);
+        const Row r = row_of(a, it, heads, g * 16 + (lane & 15), lds, wave);
+        const bool live = r.live;
+        float *y = out_row<D, NQ>(a, r, head0, lane);
 #pragma unroll
         for (int t0 = 0; t0 < T; t0 += kMeet) {
             __syncthreads();
@@ -1073,8 +1227,9 @@ __device__ __forceinline__ void join_parts(const A &a, const Item &it, int head0
     const auto part = [&](int w) { return a.parts + ((int64_t)(first + w) * 2 + (w ? 0 : 1)) * size; };   // (the first is a stretch's second)
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
-        bool live;
-        float *y = out_row<D, NQ>(a, it, head0, heads, g, lane, live);
+        const Row r = row_of(a, it, heads, g * 16 + (lane & 15), lds, wave);
+        const bool live = r.live;
+        float *y = out_row<D, NQ>(a, r, head0, lane);
         float m = -INFINITY;
         for (int w = wave * 4 + (lane >> 4); live && w < parts; w += 4 * kWaves) m = fmaxf(m, load_part(part(w) + kM + g * 16 + col));
         m = max_xor(m);
@@ -1125,7 +1280,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const A) {
     fetch_arguments<void(A), sizeof(A)>();
     __shared__ __align__(16) SharedLds<D, NQ, A> lds;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), id = threadIdx.x;
-    const int units = a.n_seq * a.row_tiles, per = (units + kThreads - 1) / kThreads;
+    const int units = units_of(a), per = (units + kThreads - 1) / kThreads;
     // ---- the line of turns ----
     int turns_mine = 0, items_mine = 0, longest = 0;
     each_item(a, id, units, per, [&](int s, int tile, const Sequence &q, int n) {
@@ -1139,7 +1294,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const A) {
         longest = max(longest, n);
         return false;
     }, [&](int) {
-        if (blockIdx.x == 0) atomicOr(a.error, kKvBadRows);
+        if (blockIdx.x == 0) atomicOr(a.error, A::kSees == kPrefix ? kKvBadGroups : kKvBadRows);
     });
     int turns_before = wave_scan(turns_mine), items_before = wave_scan(items_mine);
     longest = (int)wave_max((uint32_t)longest);
@@ -1176,7 +1331,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const A) {
     if (__builtin_expect(head_items > a.most_items, 0)) {      // (q_start falls somewhere: reported above)
         const A &a = fresh_arguments<A>();
         if (!a.arrived)                                        // nothing is to be joined
-            for (int i = id; i < a.n_seq * a.row_tiles * a.kv.n_head * a.splits; i += kThreads) a.joins[2 * i] = -1;
+            for (int i = id; i < units_of(a) * a.kv.n_head * a.splits; i += kThreads) a.joins[2 * i] = -1;
         return leave(a);
     }
     const Line line = line_of(head_turns, head_items, longest, a.kv.n_head * a.splits, gridDim.x);
@@ -1228,10 +1383,12 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const A) {
         const int skip = off - first;
         const Piece piece = piece_of(line, skip, turns, end - at);
         if (piece.to <= 0) break;
-        const int tile0 = it.hi < 0 ? 0 : it.see / kTile, tile1 = tile0 + min(piece.to * kWaves, item_tiles(it));
+        const Members seqs = members<D, NQ>(a, it, lds, wave, lane);
+        const int tile0 = A::kSees == kPrefix || it.hi < 0 ? 0 : it.see / kTile;
+        const int tile1 = tile0 + min(piece.to * kWaves, A::kSees == kPrefix ? max(1, seqs.tiles) : item_tiles(it));
 
         Running<D, NQ> st;
-        walk<D, NQ>(a, it, kv_head, head0, heads, tile0 + piece.from * kWaves + wave, tile1, lds, wave, st, lane);
+        walk<D, NQ>(a, it, seqs, kv_head, head0, heads, tile0 + piece.from * kWaves + wave, tile1, lds, wave, st, lane);
         leave(a);                       // (here, so that nothing waits for it)
         // ---- the waves' sums ----
         const bool starts = piece.from == 0, ends = piece.to == turns;
@@ -1239,7 +1396,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const A) {
         const A &c = fresh_arguments<A>();
         if (!c.arrived) {            // whoever writes an item's end says what is to be joined
             if (ends && id == 0) {
-                int32_t *const join = c.joins + 2 * ((int64_t)hv * c.n_seq * c.row_tiles + seq * c.row_tiles + row_tile);
+                int32_t *const join = c.joins + 2 * ((int64_t)hv * units_of(c) + seq * c.row_tiles + row_tile);
                 join[0] = starts ? -1 : (int32_t)stretch_at(line, at - skip + line.start);
                 join[1] = (int32_t)me;
             }
@@ -1275,11 +1432,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const A
     __shared__ __align__(16) f32x4 sums[kJoinWaves][64];
     __shared__ float tops[kJoinWaves][16], weights[kJoinWaves][16];
     const int32_t *j = a.joins + 2 * (int64_t)blockIdx.x;
-    const int first = j[0], last = j[1], units = a.n_seq * a.row_tiles;
+    const int first = j[0], last = j[1], units = units_of(a);
     const int hv = blockIdx.x / units, s = (blockIdx.x - hv * units) / a.row_tiles, row_tile = blockIdx.x - hv * units - s * a.row_tiles;
-    bool bad, live;
-    const Sequence q = sequence(a, s, bad);
-    const Item it = item_of(a, s, q, row_tile);
+    bool bad;
+    const Item it = item_of(a, s, unit_of(a, s, bad), row_tile);
     if (it.count <= 0 || first < 0) return;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15;
     const int x = blockIdx.y / NQ, g = blockIdx.y % NQ, parts = last - first + 1;
@@ -1318,9 +1474,22 @@ __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const A
     sums[wave][lane] = o;
     __syncthreads();
     if (wave != 0) return;
-    const int kv_head = hv / a.splits, go = hv - kv_head * a.splits;
-    float *y = out_row<D, NQ>(a, it, kv_head * a.group + go * a.split, min(a.split, a.group - go * a.split), g, lane, live);
-    if (!live) return;
+    const int kv_head = hv / a.splits, go = hv - kv_head * a.splits, heads = min(a.split, a.group - go * a.split);
+    const int token = token_of(a, g * 16 + col);
+    Row r{};
+    r.head = g * 16 + col - token * a.split;
+    if constexpr (A::kSees == kPrefix) {
+        const int member = (int)((uint32_t)token * a.row_part >> 16), i = token - member * a.max_q;
+        if (token >= a.tokens || member >= it.count || r.head >= heads) return;
+        const Sequence q = sequence(a, it.seq + member, bad);
+        r.live = i < q.count;
+        r.row = q.start + i;
+    } else {
+        r.live = token < it.count && r.head < heads;
+        r.row = it.first + token;
+    }
+    if (!r.live) return;
+    float *y = out_row<D, NQ>(a, r, kv_head * a.group + go * a.split, lane);
     const int used = min(kJoinWaves, parts);
     m = -INFINITY, l = 0.f;
     for (int w = 0; w < used; ++w) m = fmaxf(m, tops[w][col]);
@@ -1394,11 +1563,22 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
         a.row_tiles = (int32_t)std::max<int64_t>(1, (j.max_q + a.tokens - 1) / a.tokens);
         a.most_items = a.n_tokens / a.tokens + a.n_seq;
         items = std::min((double)a.n_seq * a.row_tiles, (double)a.n_tokens / a.tokens + a.n_seq) * j.kv->n_head * a.splits;
+        if constexpr (A::kSees == kPrefix) {     // sequences that an item has the rows of, alike for all items of the largest group
+            a.together = std::min({(int32_t)(a.tokens / j.max_q), a.max_group, (int32_t)kTogether});
+            if (a.together < 2 && cols == 1 && a.kv.dim <= 128) continue;
+            a.row_tiles = (a.max_group + a.together - 1) / a.together;
+            a.together = (a.max_group + a.row_tiles - 1) / a.row_tiles;
+            a.tokens = a.together * a.max_q;
+            a.row_part = (65536 + a.max_q - 1) / a.max_q;
+            a.most_items = a.n_seq / a.together + a.n_groups;
+            items = std::min((double)a.n_groups * a.row_tiles, (double)a.most_items) * j.kv->n_head * a.splits;
+            if (a.max_group * a.max_q * a.group <= 16) break;
+        }
         const int64_t seen = j.window ? std::min<int64_t>(most_len, (int64_t)j.window + a.tokens) : most_len;
-        if (cols == 2 || a.kv.dim > 128 || j.max_q * a.group <= 16 || items * ((double)seen / (kWaves * kTile) + 2) <= 6. * groups_most) break;
+        if (cols == 2 || a.kv.dim > 128 || (A::kSees != kPrefix && j.max_q * a.group <= 16) || items * ((double)seen / (kWaves * kTile) + 2) <= 6. * groups_most) break;
     }
     // no more workgroups than there can be turns
-    const int64_t most = (most_len + kTile - 1) / kTile + 1;
+    const int64_t most = ((most_len + kTile - 1) / kTile + 1) * (A::kSees == kPrefix ? kTogether : 1);
     const int groups = (int)std::max(1., std::min<double>(groups_most, items * ((double)most / kWaves + 1)));
     a.parts = reinterpret_cast<float *>(j.scratch + head_bytes(j.cus));
     a.slots = groups_most;
@@ -1408,7 +1588,7 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
     // of 8192 13.8 against 19.0, for eight rows behind 6000 17.2 against 22.1; a short chat's token, with two, 14.0 against 11.9.  (Up to five
     // instead of eight: 0.6% more over 50 drawn calls, up to three 2%.)
     // (the joins' list has a place for every item there could be, fewer than groups / 8)
-    const int64_t places = (int64_t)a.n_seq * a.row_tiles * j.kv->n_head * a.splits;
+    const int64_t places = (int64_t)units_of(a) * j.kv->n_head * a.splits;
     const bool few_parts = groups <= 8 * places;
     a.arrived = few_parts ? reinterpret_cast<uint64_t *>(j.scratch) : nullptr;
     a.calls = reinterpret_cast<uint32_t *>(j.scratch + counts_bytes(j.cus));
@@ -1429,6 +1609,83 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
     if (a.kv.dim == 64) return launch<64, 2, A>(a, groups, (int)places, s);
     if (a.kv.dim == 96) return launch<96, 2, A>(a, groups, (int)places, s);
     return launch<128, 2, A>(a, groups, (int)places, s);
+}
+
+// For the tests: the pieces of the line that every workgroup of a call takes, in the order in which it takes them, worked out on the host by the
+// kernel's own arithmetic.  A piece is {workgroup, head, sequence, row tile, its turns from, to, all the item's turns, first and last stretch of the item}.
+// Their number, or -1 where a workgroup would not come to an end.  kv_len_later: what the lengths are when an item is looked for.
+template <typename A>
+int64_t pieces_of(A a, const int32_t *kv_len_later, int heads, int groups, int32_t *out, int64_t room) {
+    const int units = units_of(a), per = (units + kThreads - 1) / kThreads;
+    struct Thread { int turns_before, items_before, turns, items, only[3]; } threads[kThreads];
+    int head_turns = 0, head_items = 0, longest = 0;
+    for (int id = 0; id < kThreads; ++id) {
+        Thread &t = threads[id];
+        t = Thread{head_turns, head_items, 0, 0, {0, 0, 0}};
+        each_item(a, id, units, per, [&](int s, int tile, const Sequence &, int n) {
+            t.only[0] = s, t.only[1] = tile, t.only[2] = n;
+            t.turns += n;
+            ++t.items;
+            longest = max(longest, n);
+            return false;
+        }, [](int) {});
+        head_turns += t.turns, head_items += t.items;
+    }
+    if (head_items > a.most_items) return 0;
+    const Line line = line_of(head_turns, head_items, longest, heads, groups);
+    a.kv_len = kv_len_later;
+    int64_t pieces = 0;
+    for (int block = 0; block < groups; ++block) {
+        const uint32_t me = line.whole ? block : stretch_of_block(block, line.active);
+        if (me >= line.active) continue;
+        uint32_t at = line.whole ? me : me * line.length + std::min(me, line.longer);
+        const uint32_t end = line.whole ? line.total : at + line.length + (me < line.longer ? 1 : 0);
+        uint32_t round = 0;
+        int found[4] = {0, 0, 0, 0};
+        for (int64_t steps = 0; at < end; ++steps) {
+            if (steps > line.total) return -1;
+            const int hv = (int)quotient(at, (uint32_t)line.head_length), off = (int)(at - (uint32_t)hv * line.head_length);
+            for (int id = 0; id < kThreads; ++id) {
+                const Thread &t = threads[id];
+                int b = line.whole ? t.items_before : t.turns_before + line.start * t.items_before;
+                if (off < b || off >= b + (line.whole ? t.items : t.turns + line.start * t.items)) continue;
+                if (per == 1) {
+                    found[0] = t.only[0], found[1] = t.only[1], found[2] = t.only[2];
+                } else {
+                    bool there = false;
+                    each_item(a, id, units, per, [&](int s, int tile, const Sequence &, int n) {
+                        const int weight = line.whole ? 1 : n + line.start;
+                        if (off >= b + weight) {
+                            b += weight;
+                            return false;
+                        }
+                        found[0] = s, found[1] = tile, found[2] = n;
+                        there = true;
+                        return true;
+                    }, [](int) {});
+                    if (!there) b = -1;
+                }
+                found[3] = b;
+            }
+            if (found[3] < 0) break;
+            const int turns = found[2], skip = off - found[3];
+            const Piece piece = piece_of(line, skip, turns, end - at);
+            if (piece.to <= 0) break;
+            const uint32_t first = line.whole ? me : stretch_at(line, at - skip + line.start), last = line.whole ? me : stretch_at(line, at - skip + line.start + turns - 1);
+            if (pieces < room) {
+                const int32_t row[9] = {block, hv, found[0], found[1], piece.from, piece.to, turns, (int32_t)first, (int32_t)last};
+                for (int i = 0; i < 9; ++i) out[9 * pieces + i] = row[i];
+            }
+            ++pieces;
+            if (line.whole) {
+                ++round;
+                at = round * line.active + (round & 1 ? line.active - 1 - me : me);
+            } else {
+                at += piece.take;
+            }
+        }
+    }
+    return pieces;
 }
 
 }  // namespace

@@ -37,6 +37,6 @@ __device__ __forceinline__ int key_word(int blocks, int block, int eighth) { ret
 __device__ __forceinline__ int value_word(int block, int eighth) { return block * 4 + eighth; }
 
 // bits of the error word that kernels raise (the context's second flag)
-constexpr int kKvBadSlot = 1, kKvBadPage = 2, kKvBadRows = 4, kKvBadBucket = 8;
+constexpr int kKvBadSlot = 1, kKvBadPage = 2, kKvBadRows = 4, kKvBadBucket = 8, kKvBadGroups = 16;
 
 }  // namespace qproj

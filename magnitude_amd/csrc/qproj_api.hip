@@ -851,8 +851,9 @@ int qproj_sync(qproj_ctx *ctx) {
                                                                 {flag[1] & kKvBadSlot, "a slot behind the key/value cache"},
                                                                 {flag[1] & kKvBadPage, "a page outside [0, n_pages) in an attention call"},
                                                                 {flag[1] & kKvBadRows, "q_start or kv_len out of bounds in an attention call"},
-                                                                {flag[1] & kKvBadBucket, "a bucket outside [0, n_buckets) of a bias table"}};
-        char buf[400] = "";     // (what several calls have met since the last time is named once each)
+                                                                {flag[1] & kKvBadBucket, "a bucket outside [0, n_buckets) of a bias table"},
+                                                                {flag[1] & kKvBadGroups, "group_start or shared_len out of bounds in an attention call"}};
+        char buf[500] = "";     // (what several calls have met since the last time is named once each)
         for (const auto &f : all)
             if (f.raised) snprintf(buf + strlen(buf), sizeof buf - strlen(buf), "%s%s", *buf ? "; " : "", f.what);
         return fail(ctx, QPROJ_ERR_INVALID_ARG, buf);
@@ -1879,6 +1880,23 @@ int qproj_cross_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float 
     return QPROJ_OK;
 }
 
+int qproj_attention_shared(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens, int64_t n_head,
+                           int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q, const int32_t *pages_dev,
+                           int64_t pages_stride, int64_t n_groups, const int32_t *group_start_dev, const int32_t *shared_len_dev, int64_t max_group,
+                           float scale, int64_t window, float *y_dev, int64_t y_stride) {
+    const char *call = "qproj_attention_shared";
+    if (!ctx) return QPROJ_ERR_INVALID_ARG;
+    if (n_groups < 0 || n_groups > 65536 || max_group < 0) return refuse(ctx, call, "n_groups or max_group out of range");
+    if (n_groups == 0 && n_seq > 0) return refuse(ctx, call, "sequences of no group");
+    if (n_groups && (!group_start_dev || !shared_len_dev)) return refuse(ctx, call, "null argument");
+    KvView view;
+    AttentionJob j{};
+    const int rc = attention_job(ctx, call, kv, &view, q_dev, q_stride, n_tokens, n_head, n_seq, q_start_dev, kv_len_dev, max_q, pages_dev, pages_stride, scale, window, y_dev, y_stride, &j);
+    if (rc != QPROJ_OK) return rc;
+    QP_HIP(ctx, launch_attention_shared(j, {group_start_dev, shared_len_dev, n_groups, std::min(max_group, n_seq)}, ctx->stream));
+    return QPROJ_OK;
+}
+
 int qproj_relative_buckets(int64_t n_buckets, int64_t reach, int both_sides, int32_t *buckets) {
     if (!buckets || n_buckets > 1 << 20 || (both_sides && n_buckets % 2 != 0)) return QPROJ_ERR_INVALID_ARG;
     const int64_t side = both_sides ? n_buckets / 2 : n_buckets, e = side / 2;
@@ -1956,6 +1974,20 @@ int64_t qproj_internal_attention_pieces(const int32_t *q_start, const int32_t *k
     j.max_q = max_q;
     j.window = (int32_t)window;
     return attention_pieces(j, kv_len_later ? kv_len_later : kv_len, most_len, (int)tokens, (int)heads, (int)groups, out, room);
+}
+
+// The same of a call with groups of sequences that share their first tokens, `together` sequences an item.
+int64_t qproj_internal_attention_shared_pieces(const int32_t *q_start, const int32_t *kv_len, const int32_t *kv_len_later, int64_t n_seq, int64_t n_tokens, int64_t max_q,
+                                               const int32_t *group_start, const int32_t *shared_len, int64_t n_groups, int64_t max_group, int64_t most_len, int64_t together,
+                                               int64_t heads, int64_t groups, int32_t *out, int64_t room) {
+    AttentionJob j{};
+    j.q_start = q_start;
+    j.kv_len = kv_len;
+    j.n_seq = n_seq;
+    j.n_tokens = n_tokens;
+    j.max_q = max_q;
+    const SharedGroups g{group_start, shared_len, n_groups, max_group};
+    return attention_shared_pieces(j, g, kv_len_later ? kv_len_later : kv_len, most_len, (int)together, (int)heads, (int)groups, out, room);
 }
 
 // For the tests: sets the counts of parts of a context whose attention has run to `words`, over and over where there are more of them.

@@ -349,9 +349,15 @@ size_t attention_scratch_bytes(int cus);
 size_t attention_counts_bytes(int cus);   // of its beginning: 64-bit counts of parts
 hipError_t launch_attention(const AttentionJob &j, hipStream_t s);
 hipError_t launch_attention_all(const AttentionJob &j, hipStream_t s);
+struct SharedGroups {           // sequences start[g] .. start[g + 1] - 1 have their first shared[g] tokens in common; at most max_group of them
+    const int32_t *start, *shared;
+    int64_t n_groups, max_group;
+};
+hipError_t launch_attention_shared(const AttentionJob &j, const SharedGroups &g, hipStream_t s);
 int attention_most_reach();
 hipError_t launch_attention_biased(const AttentionJob &j, const float *bias, int reach, bool all, hipStream_t s);   // bias [n_head][2 * reach + 1]
 hipError_t launch_bias_by_distance(const float *table, int n_buckets, int n_head, const int32_t *buckets, int reach, float *out, int32_t *error, hipStream_t s);
 int64_t attention_pieces(const AttentionJob &j, const int32_t *kv_len_later, int64_t most_len, int tokens, int heads, int groups, int32_t *out, int64_t room);   // for the tests
+int64_t attention_shared_pieces(const AttentionJob &j, const SharedGroups &g, const int32_t *kv_len_later, int64_t most_len, int together, int heads, int groups, int32_t *out, int64_t room);   // too
 
 }  // namespace qproj

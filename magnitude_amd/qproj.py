@@ -68,6 +68,8 @@ SYMBOLS = {
     "qproj_kv_read": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp]),
     "qproj_attention": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, C.c_float, _i64, _vp, _i64]),
     "qproj_cross_attention": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, C.c_float, _vp, _i64]),
+    "qproj_attention_shared": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64,
+                                      C.c_float, _i64, _vp, _i64]),
     "qproj_relative_buckets": (_i32, [_i64, _i64, _i32, _vp]),
     "qproj_bias_by_distance": (_i32, [_vp, _vp, _i64, _i64, _vp, _i64, _vp]),
     "qproj_attention_biased": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, C.c_float, _vp, _i64]),
@@ -752,6 +754,27 @@ class Context:
         if sync:
             torch.cuda.current_stream(q.device).synchronize()
         self._check(self.lib.qproj_attention(*head, window, *tail))
+        if sync:
+            self.sync()
+        return y
+
+    def attention_shared(self, kv: KvCache, q: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor,
+                         group_start: torch.Tensor, shared_len: torch.Tensor, max_q: Optional[int] = None, max_group: Optional[int] = None,
+                         scale: Optional[float] = None, window: int = 0, out: Optional[torch.Tensor] = None,
+                         sync: bool = True) -> torch.Tensor:
+        """attention of a batch whose sequences share their first tokens, with what is shared computed once for several of them:
+        sequences group_start[g] .. group_start[g + 1] - 1 (i32 [n_groups + 1], from 0 to n_seq) have the same pages for their first
+        shared_len[g] (i32 [n_groups]) tokens.  max_group: the most sequences a group has (default: all of them could be one's)."""
+        n, head, tail, y = self._attention_args(kv, q, q_start, kv_len, pages, max_q, scale, out)
+        if group_start.numel() != shared_len.numel() + 1:
+            raise ValueError("group_start must be [n_groups + 1] and shared_len [n_groups]")
+        gp, sp = self._on_device(group_start, torch.int32, "group_start"), self._on_device(shared_len, torch.int32, "shared_len")
+        if n == 0:
+            return y
+        if sync:
+            torch.cuda.current_stream(q.device).synchronize()
+        self._check(self.lib.qproj_attention_shared(*head[:-1], shared_len.numel(), gp, sp, pages.shape[0] if max_group is None else max_group,
+                                                    head[-1], window, *tail))
         if sync:
             self.sync()
         return y

@@ -6,7 +6,7 @@ const SOURCES: &[&str] = &[
     "qproj_api.hip", "kernels_dequant.hip", "kernels_actquant.hip", "kernels_gemv.hip", "kernels_decode.hip",
     "kernels_gemv_mfma.hip", "kernels_gemv_f32.hip", "kernels_moe.hip", "kernels_moe_decode.hip", "kernels_moe_stream.hip", "kernels_gemm.hip", "kernels_gemm_q6k.hip", "kernels_gemm_q8_0.hip",
     "kernels_gemm_stream.hip", "kernels_rmsnorm.hip", "kernels_rope_kv.hip", "kernels_attention.hip",
-    "kernels_attention_all.hip", "kernels_attention_biased.hip",
+    "kernels_attention_all.hip", "kernels_attention_biased.hip", "kernels_attention_shared.hip",
 ];
 const HEADERS: &[&str] = &[
     "qproj_internal.h", "qproj_device.h", "gemv_frags.h", "actquant_device.h", "gemm_tiles.h", "gemm_convert.h", "lds_direct.h", "kv_cache.h", "attention_device.h",

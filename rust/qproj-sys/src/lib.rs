@@ -150,6 +150,11 @@ extern "C" {
                                  n_tokens: i64, n_head: i64, n_seq: i64, q_start_dev: *const i32, kv_len_dev: *const i32,
                                  max_q: i64, pages_dev: *const i32, pages_stride: i64, scale: f32, y_dev: *mut f32,
                                  y_stride: i64) -> c_int;
+    pub fn qproj_attention_shared(ctx: *mut qproj_ctx, kv: *const qproj_kv_cache, q_dev: *const f32, q_stride: i64,
+                                  n_tokens: i64, n_head: i64, n_seq: i64, q_start_dev: *const i32, kv_len_dev: *const i32,
+                                  max_q: i64, pages_dev: *const i32, pages_stride: i64, n_groups: i64,
+                                  group_start_dev: *const i32, shared_len_dev: *const i32, max_group: i64, scale: f32,
+                                  window: i64, y_dev: *mut f32, y_stride: i64) -> c_int;
     pub fn qproj_relative_buckets(n_buckets: i64, reach: i64, both_sides: c_int, buckets: *mut i32) -> c_int;
     pub fn qproj_bias_by_distance(ctx: *mut qproj_ctx, table_dev: *const f32, n_buckets: i64, n_head: i64,
                                   buckets_dev: *const i32, reach: i64, out_dev: *mut f32) -> c_int;

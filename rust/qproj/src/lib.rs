@@ -194,6 +194,20 @@ impl Context {
         })
     }
 
+    /// Attention of a batch in groups that share their first tokens; see `qproj_attention_shared`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn attention_shared(&self, kv: &sys::qproj_kv_cache, q: DevicePtr, n: i64, n_head: i64, n_seq: i64, q_start: DevicePtr,
+                            kv_len: DevicePtr, max_q: i64, pages: DevicePtr, pages_stride: i64, n_groups: i64,
+                            group_start: DevicePtr, shared_len: DevicePtr, max_group: i64, scale: f32, window: i64,
+                            y: DevicePtr) -> Result<()> {
+        let row = n_head * kv.head_dim;
+        self.check(unsafe {
+            sys::qproj_attention_shared(self.raw, kv, q.0.cast(), row, n, n_head, n_seq, q_start.0.cast(), kv_len.0.cast(), max_q,
+                                        pages.0.cast(), pages_stride, n_groups, group_start.0.cast(), shared_len.0.cast(), max_group,
+                                        scale, window, y.0.cast(), row)
+        })
+    }
+
     /// Attention with a bias of the distance between token and row; see `qproj_attention_biased`.
     #[allow(clippy::too_many_arguments)]
     pub fn attention_biased(&self, kv: &sys::qproj_kv_cache, q: DevicePtr, n: i64, n_head: i64, n_seq: i64, q_start: DevicePtr,

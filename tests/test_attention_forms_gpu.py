@@ -248,3 +248,164 @@ def test_a_bias_of_nothing_changes_nothing(ctx):
     assert (ctx.attention_biased(*args, none, causal=False) - ctx.cross_attention(*args)).abs().max() < 1e-5
     same = torch.full((8, 257), 7.25, device="cuda")       # softmax does not see what all tokens have
     assert (ctx.attention_biased(*args, same) - ctx.attention(*args)).abs().max() < 1e-5
+
+
+# ---- sequences that share their first tokens ----------------------------------------------------------------------------------
+def share(pages, lens, groups, page):
+    """The table with whole pages of `shared` tokens the same in every group [(shared, sequences)], (table, group_start, shared_len)"""
+    pages, at = pages.copy(), 0
+    for shared, n in groups:
+        for s in range(at + 1, at + n):
+            whole = min(shared, lens[at]) // page
+            pages[s, :whole] = pages[at, :whole]
+        at += n
+    return pages, np.cumsum([0] + [n for _, n in groups]).astype(np.int32), np.array([min(m, lens[s]) // page * page for (m, _), s in
+                                                                                       zip(groups, np.cumsum([0] + [n for _, n in groups]))], np.int32)
+
+
+def check_shared(ctx, kv, pages, q, q_start, kv_len, group_start, shared, scale=None, **kw):
+    s = kv.head_dim ** -0.5 if scale is None else scale
+    want, sizes = forms_ref.attention(numpy_cache(kv), q, q_start, kv_len, pages, s)
+    plain = forms_ref.attention(numpy_cache(kv), q, q_start, kv_len, pages, s, dtype=np.float32)[0]
+    for table in (wide(pages, kv), pages):
+        out = torch.full(q.shape, 7.5, device="cuda")
+        got = ctx.attention_shared(kv, dev(q), i32(q_start), i32(kv_len), dev(table), i32(group_start), i32(shared), scale=scale, out=out, **kw).cpu().numpy()
+        compare(got, want, plain, sizes, kv.head_dim, max([1] + list(kv_len)))
+    return got
+
+
+SHARED = [  # dim, page, kv heads, group, [(shared, [(tokens, rows)])], the most rows
+    (128, 64, 1, 4, [(64, [(65, 1), (100, 1)])], 1),
+    (128, 64, 8, 4, [(1024, [(1024 + 37 * i % 300 + 1, 1) for i in range(20)])], 1),
+    (64, 16, 2, 7, [(80, [(90, 2), (83, 3), (400, 1)]), (16, [(33, 2), (17, 1)]), (0, [(50, 1), (3, 2)])], 3),
+    (96, 32, 2, 1, [(320, [(320 + i, 1) for i in range(1, 41)])], 1),             # 32 sequences an item
+    (256, 128, 1, 2, [(384, [(400, 2), (700, 2), (385, 1)]), (128, [(129, 1), (130, 2)])], 2),
+    (128, 16, 1, 16, [(160, [(200, 1), (170, 1), (300, 1)])], 1),                 # two sequences fill an item
+    (128, 64, 2, 4, [(8192, [(8200 + 11 * i, 1) for i in range(9)])], 1),         # many parts
+    (64, 64, 1, 4, [(20032, [(20040, 1), (20400, 4), (21000, 2)])], 4),           # many parts, joined by a launch of their own
+    (128, 64, 4, 2, [(128 * (i % 4), [(130 + 128 * (i % 4) + 7 * j, 1 + (i + j) % 2) for j in range(1 + i % 6)]) for i in range(40)], 2),
+    (128, 256, 2, 4, [(512, [(600, 1), (520, 0), (513, 1), (0, 0)]), (256, []), (256, [(300, 0)]), (256, [(299, 1), (700, 4)])], 4),
+    (64, 32, 8, 1, [(96, [(97 + 5 * i, 1) for i in range(150)])], 1),             # far more items than can stay whole
+    (128, 32, 2, 4, [(640, [(650, 8), (700, 5)])], 8),                            # nothing to gain: the causal kernel
+]
+
+
+@pytest.mark.parametrize("dim,page,kv_heads,group,groups,most", SHARED)
+def test_shared_attention(ctx, dim, page, kv_heads, group, groups, most):
+    tell("shared", dim, page, kv_heads, group, [(m, len(g)) for m, g in groups], most)
+    rng = np.random.default_rng(dim + page + len(groups))
+    seqs = [s for _, g in groups for s in g]
+    lens, q_start = [n for n, _ in seqs], np.cumsum([0] + [m for _, m in seqs])
+    kv, pages = make_cache(rng, lens, page, kv_heads, dim)
+    table, group_start, shared = share(np.pad(pages, ((0, 1), (0, 0))), lens + [0], [(m, len(g)) for m, g in groups], page)
+    table = table[:len(lens)]
+    q = rng.standard_normal((q_start[-1], kv_heads * group, dim)).astype(np.float32)
+    sizes = dict(max_q=most, max_group=max(len(g) for _, g in groups))
+    check_shared(ctx, kv, table, q, q_start, lens, group_start, shared, **sizes)
+    check_shared(ctx, kv, table, q, q_start, lens, group_start, shared, scale=0.3, max_q=most)      # any number a group
+    for other in (0, 1, 63, 64, 65):      # less shared than could be
+        if group_start[-1] < 20:
+            check_shared(ctx, kv, table, q, q_start, lens, group_start, np.minimum(shared, other), **sizes)
+
+
+def test_shared_tokens_that_reach_into_the_newest_are_each_row_s_own(ctx):
+    """shared_len up to and past the sequences' ends: what lies at and behind the rows is not taken as seen"""
+    rng = np.random.default_rng(41)
+    lens, q_start = [200, 130, 129, 64, 5], [0, 2, 3, 5, 6, 8]
+    kv, pages = make_cache(rng, lens, 16, 2, 64)
+    pages[:, :] = pages[0]                       # the same pages from the first to the last
+    q = rng.standard_normal((8, 8, 64)).astype(np.float32)
+    for shared in (64, 128, 129, 200, 100000, 2147483647):
+        check_shared(ctx, kv, pages, q, q_start, lens, [0, 5], [shared], max_q=2)
+        check_shared(ctx, kv, pages, q, q_start, lens, [0, 3, 5], [shared, shared], max_q=2)
+
+
+def test_shared_rows_of_no_sequence_stay_and_rows_that_see_nothing_are_zeros(ctx):
+    rng = np.random.default_rng(42)
+    lens, q_start = [3, 0, 300, 290, 0], [2, 6, 8, 10, 11, 12]        # four rows of three tokens
+    kv, pages = make_cache(rng, lens, 16, 1, 128)
+    q = rng.standard_normal((20, 4, 128)).astype(np.float32)
+    pages[3, :16] = pages[2, :16]
+    got = check_shared(ctx, kv, pages, q, q_start, lens, [0, 2, 4, 5], [0, 256, 0], max_q=4)
+    assert not got[2].any() and got[3:6].any(-1).all() and not got[6:8].any() and got[8:11].any(-1).all() and not got[11].any()
+
+
+def test_shared_blocks_that_are_not_finite(ctx):
+    """shared ones reach all rows of the group, a sequence's own its rows, others nobody"""
+    rng = np.random.default_rng(43)
+    lens, q_start = [300, 280, 270, 100], [0, 1, 3, 4, 5]
+    kv, pages = make_cache(rng, lens, 16, 2, 128)
+    pages[1, :16], pages[2, :16] = pages[0, :16], pages[0, :16]
+    q = dev(rng.standard_normal((5, 8, 128)).astype(np.float32))
+    args = kv, q, i32(q_start), i32(lens), dev(pages), i32([0, 3, 4]), i32([256, 0])
+    base = ctx.attention_shared(*args, max_q=2).cpu().numpy()
+    clean = [t.clone() for t in kv.tensors]
+    for s, t, rows in ((0, 255, [0, 1, 2, 3]), (0, 299, [0]), (1, 279, [2]), (1, 270, [1, 2]), (2, 256, [3]), (3, 99, [4])):
+        for u, c in zip(kv.tensors, clean):
+            u.copy_(c)
+        p = int(pages[s, t // 16])
+        kv.tensors[1][p, 0, t % 16, 0] = float("nan")         # a key of head 0
+        kv.tensors[3][p, 1, t % 16, 1] = float("inf")         # a block of a value of head 1
+        for i in range(t % 16 + 1, 16):                       # and what lies behind the last token
+            if t + i - t % 16 >= lens[s]:
+                kv.tensors[1][p, :, i] = float("nan")
+        got = ctx.attention_shared(*args, max_q=2).cpu().numpy()
+        assert np.isnan(got[rows, :4]).all() and not np.isfinite(got[rows, 4:, 32:64]).any()
+        others = [r for r in range(5) if r not in rows]
+        np.testing.assert_array_equal(got[others], base[others])
+        np.testing.assert_array_equal(got[rows, 4:, :32], base[rows, 4:, :32])
+
+
+def test_shared_bad_pages_bounds_and_groups_are_reported(ctx):
+    from magnitude_amd import QprojError
+    rng = np.random.default_rng(44)
+    lens, q_start = [200, 180, 190, 90, 60], [0, 1, 2, 3, 4, 5]
+    kv, pages = make_cache(rng, lens, 16, 1, 64)
+    pages[1, :10], pages[2, :10] = pages[0, :10], pages[0, :10]
+    q = rng.standard_normal((5, 4, 64)).astype(np.float32)
+    call = lambda p=pages, s=q_start, n=lens, g=(0, 3, 5), m=(160, 0), out=None, **kw: ctx.attention_shared(
+        kv, dev(q), i32(s), i32(n), dev(p), i32(g), i32(m), out=out, **{"max_q": 1, "max_group": 3, **kw}).cpu().numpy()
+    ok = call()
+    for bad in (-1, kv.n_pages, 2147483647, -2147483648):
+        wrong = pages.copy()
+        wrong[:3, 2] = bad                    # of what is shared (a sequence's tokens of a bad page are not seen)
+        wrong[4, 1] = bad
+        out = torch.full(q.shape, 7.5, device="cuda")
+        with pytest.raises(QprojError, match="page"):
+            call(wrong, out=out)
+        want, sizes = forms_ref.attention(numpy_cache(kv), q, q_start, lens, wrong, 64 ** -0.5)
+        assert (np.abs(out.cpu().numpy() - want) <= forms_ref.allowed(sizes, 64, 200)).all()
+    for kw, what, left in ((dict(s=[0, 1, 2, 3, 4, 6]), "q_start", [0, 1, 2, 3]), (dict(s=[0, 1, 0, 3, 4, 5]), "q_start", [0, 3, 4]), (dict(n=[200, -1, 190, 90, 60]), "q_start", [0, 2, 3, 4]),
+                           (dict(n=[1 << 20, 180, 190, 90, 60]), "q_start", [1, 2, 3, 4]), (dict(s=[-1, 1, 2, 3, 4, 5]), "q_start", [1, 2, 3, 4]),
+                           (dict(g=(0, 3, 6)), "group_start", [0, 1, 2]), (dict(g=(1, 3, 5)), "group_start", [1, 2, 3, 4]), (dict(g=(0, 3, 4)), "group_start", [0, 1, 2, 3]),
+                           (dict(g=(0, 3, 2)), "group_start", [0, 1, 2]), (dict(g=(-1, 3, 5)), "group_start", [3, 4]), (dict(m=(-1, 0)), "group_start", [3, 4]),
+                           (dict(g=(0, 2, 5), m=(160, 0), max_group=2), "group_start", [0, 1])):
+        out = torch.full(q.shape, 7.5, device="cuda")
+        with pytest.raises(QprojError, match=what):
+            call(out=out, **kw)
+        got = out.cpu().numpy()
+        np.testing.assert_allclose(got[left], ok[left], rtol=1e-5, atol=1e-6)
+        assert (got[[i for i in range(5) if i not in left]] == 7.5).all()
+    ctx.sync()
+    np.testing.assert_array_equal(call(), ok)
+
+
+def test_shared_rows_that_lie_apart_and_the_same_bits(ctx):
+    rng = np.random.default_rng(45)
+    lens = [3000, 2900, 2600, 70, 3100, 2700]
+    kv, pages = make_cache(rng, lens, 64, 2, 128)
+    pages[[1, 2, 4, 5], :40] = pages[0, :40]
+    order = [0, 1, 2, 4, 5, 3]
+    pages, lens = pages[order], [lens[i] for i in order]
+    wide_rows = rng.standard_normal((9, 12 * 128)).astype(np.float32)
+    q = dev(wide_rows)[:, 256: 256 + 1024].unflatten(1, (8, 128))
+    out = torch.full((9, 1100), 7.5, device="cuda")
+    y = out[:, 8: 8 + 1024].unflatten(1, (8, 128))
+    args = i32([0, 1, 3, 4, 6, 8, 9]), i32(lens), dev(pages), i32([0, 5, 6]), i32([2560, 0])
+    ctx.attention_shared(kv, q, *args, max_q=2, max_group=5, out=y)
+    first = ctx.attention_shared(kv, q.contiguous(), *args, max_q=2, max_group=5)
+    assert torch.equal(y, first) and (out[:, :8] == 7.5).all() and (out[:, 8 + 1024:] == 7.5).all()
+    for _ in range(5):
+        assert torch.equal(first, ctx.attention_shared(kv, q, *args, max_q=2, max_group=5))
+    want = ctx.attention(kv, q, *args[:3], max_q=2)
+    assert (first - want).abs().max() < 1e-5
