@@ -148,6 +148,16 @@ def test_every_turn_of_groups_has_one_workgroup(heads, together, groups, grid):
         assert len({r[0] for r in parts}) == len(parts)
 
 
+@pytest.mark.parametrize("items,grid", [(9, 8), (10, 8), (15, 8), (16, 8), (616, 512), (1025, 512)])
+def test_no_workgroup_has_an_item_more_than_the_others(items, grid):
+    """items of 20 turns, some grids full and a little more: cut where whole ones would leave workgroups more than two turns from each other"""
+    lens, n = [20 * 256] * items, list(range(items + 1))
+    got = shared_pieces(n, lens, 1, n, [0] * items, max(lens), 2, 1, grid, 1)
+    turns = np.bincount(got[:, 0], weights=got[:, 5] - got[:, 4], minlength=grid)
+    assert turns.sum() == 20 * items and turns.max() <= 20 * items / grid + 3 + 2 * -(-items // grid)
+    assert (len(got) == items) == (items == 16)
+
+
 def test_groups_and_lengths_that_are_wrong_come_to_an_end():
     """bounds that do not hold, and lengths that change between the count and the search: pieces are any, but every workgroup ends"""
     rng = np.random.default_rng(3)
