@@ -98,6 +98,13 @@ def test_an_item_takes_sequences_alike():
     assert m(plan(seqs=2, n=2, max_q=1, ps=20, max_group=2)) == (2, 1)
 
 
+def test_long_caches_have_items_of_32_columns():
+    for ps in (64, 511, 512, 1024):
+        kw = dict(seqs=48, n=48, max_q=1, max_group=48, ps=ps)
+        assert ("attention_kernel<128, 2, prefix>" in plan(**kw)) == (ps >= 512) and ("attention_kernel<128, 1, prefix>" in plan(**kw)) == (ps < 512), ps
+    assert "attention_kernel<128, 2, prefix>" in plan(group=12, seqs=8, n=8, max_q=1, max_group=8, ps=64)      # (16 hold one sequence)
+
+
 def shared_pieces(q_start, kv_len, max_q, group_start, shared, most_len, together, heads, grid, max_group, later=None, n=None):
     f = qproj.load_library().qproj_internal_attention_shared_pieces
     f.restype, f.argtypes = C.c_int64, [C.c_void_p] * 3 + [C.c_int64] * 3 + [C.c_void_p] * 2 + [C.c_int64] * 6 + [C.c_void_p, C.c_int64]
