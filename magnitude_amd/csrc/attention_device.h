@@ -1590,8 +1590,17 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
         if (cols == 2 || a.kv.dim > 128 || (A::kSees != kPrefix && j.max_q * a.group <= 16) || items * ((double)seen / (kWaves * kTile) + 2) <= 6. * groups_most) break;
     }
     // no more workgroups than there can be turns
-    const int64_t most = ((most_len + kTile - 1) / kTile + 1) * (A::kSees == kPrefix ? kTogether : 1);
-    const int groups = (int)std::max(1., std::min<double>(groups_most, items * ((double)most / kWaves + 1)));
+    const int64_t most = (most_len + kTile - 1) / kTile + 1;
+    const int64_t places = (int64_t)units_of(a) * j.kv->n_head * a.splits;
+    int groups;
+    if constexpr (A::kSees == kPrefix) {
+        // (an item's sequences may share next to nothing; where they share nearly everything its turns are one's, and if eight parts an item are enough
+        // for those, one launch does: two sequences behind 1024 tokens 13.6 us instead of 14.4)
+        groups = (int)std::max(1., std::min<double>(groups_most, items * ((double)most * a.together / kWaves + 1)));
+        if (groups > 8 * places && items * ((double)most / kWaves + 1) <= 8. * places) groups = (int)(8 * places);
+    } else {
+        groups = (int)std::max(1., std::min<double>(groups_most, items * ((double)most / kWaves + 1)));
+    }
     a.parts = reinterpret_cast<float *>(j.scratch + head_bytes(j.cus));
     a.slots = groups_most;
     a.slots_each = (groups_most - groups + groups - 1) / groups;
@@ -1600,7 +1609,6 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
     // of 8192 13.8 against 19.0, for eight rows behind 6000 17.2 against 22.1; a short chat's token, with two, 14.0 against 11.9.  (Up to five
     // instead of eight: 0.6% more over 50 drawn calls, up to three 2%.)
     // (the joins' list has a place for every item there could be, fewer than groups / 8)
-    const int64_t places = (int64_t)units_of(a) * j.kv->n_head * a.splits;
     const bool few_parts = groups <= 8 * places;
     a.arrived = few_parts ? reinterpret_cast<uint64_t *>(j.scratch) : nullptr;
     a.calls = reinterpret_cast<uint32_t *>(j.scratch + counts_bytes(j.cus));
