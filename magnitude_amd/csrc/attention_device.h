@@ -1300,7 +1300,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const A) {
         turns_mine += n;
         ++items_mine;
         longest = max(longest, n);
-        return false;
+        return A::kSees == kPrefix && items_mine > a.most_items;     // (groups that do not ascend could have any number of items, whose sequences are looked at)
     }, [&](int) {
         if (blockIdx.x == 0) atomicOr(a.error, A::kSees == kPrefix ? kKvBadGroups : kKvBadRows);
     });
@@ -1647,7 +1647,7 @@ int64_t pieces_of(A a, const int32_t *kv_len_later, int heads, int groups, int32
             t.turns += n;
             ++t.items;
             longest = max(longest, n);
-            return false;
+            return A::kSees == kPrefix && t.items > a.most_items;
         }, [](int) {});
         head_turns += t.turns, head_items += t.items;
     }

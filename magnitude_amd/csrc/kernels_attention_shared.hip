@@ -15,6 +15,7 @@ static bool sharing_pays(const AttentionJob &j, const SharedGroups &g) {
     const int rows = j.kv->dim > 128 ? 16 : 32, group = j.n_head / j.kv->n_head;
     const int splits = (group + rows - 1) / rows, split = (group + splits - 1) / splits;
     if (j.max_q > rows / split / 2) return false;
+    if ((double)g.n_groups * (g.max_group + 1) > 2e9) return false;      // places of the line, in 32 bits
     // the line's turns are counted in 32 bits: groups that do not ascend may have any item hold the most sequences
     const double turns = ((double)(j.pages_stride << j.kv->page_shift) / (kWaves * kTile) + 4) * ((double)j.n_seq + (double)kTogether * g.n_groups);
     return turns * j.n_head <= 2e9;

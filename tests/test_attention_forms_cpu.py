@@ -98,6 +98,12 @@ def test_an_item_takes_sequences_alike():
     assert m(plan(seqs=2, n=2, max_q=1, ps=20, max_group=2)) == (2, 1)
 
 
+def test_more_places_than_32_bits_hold_are_the_causal_kernel_s():
+    most = dict(heads_kv=1, group=2, page=16, seqs=65536, n=65536, max_q=4, ps=4)
+    assert ", prefix>" not in plan(groups=65536, max_group=65536, **most)
+    assert ", prefix>" in plan(groups=65536, max_group=16, **most) and ", prefix>" in plan(groups=16, max_group=65536, **most)
+
+
 def test_long_caches_have_items_of_32_columns():
     for ps in (64, 511, 512, 1024):
         kw = dict(seqs=48, n=48, max_q=1, max_group=48, ps=ps)
@@ -175,6 +181,12 @@ def test_groups_and_lengths_that_are_wrong_come_to_an_end():
         group_start = np.sort(rng.integers(0, n_seq + 1, n_groups + 1)) if rng.random() < 0.5 else rng.integers(-2, n_seq + 3, n_groups + 1)
         shared_pieces(q_start.tolist(), lens, 2, group_start, rng.integers(-5, 4000, n_groups), 2900, int(rng.integers(2, 9)), int(rng.integers(1, 5)), int(rng.integers(1, 200)),
                       int(rng.integers(1, n_seq + 1)), later, n=2 * n_seq)
+
+
+def test_groups_that_repeat_sequences_are_not_counted_to_their_end():
+    n = 3000
+    groups = [0, n, n, 0] * 4000                           # every other good one has all sequences
+    assert len(shared_pieces(list(range(n + 1)), [100] * n, 1, groups + [0], [0] * len(groups), 100, 2, 1, 8, n)) == 0
 
 
 # ---- buckets --------------------------------------------------------------------------------------------------------------
