@@ -1800,7 +1800,7 @@ static int attention_job(qproj_ctx *ctx, const char *call, const qproj_kv_cache 
     if (!q_start_dev || (!kv_len_dev && n_seq) || (!pages_dev && n_seq && pages_stride)) return refuse(ctx, call, "null argument");
     if (n_tokens < 0 || n_tokens > kMostTokens || n_seq < 0 || n_seq > 65536 || max_q < 0 || pages_stride < 0)
         return refuse(ctx, call, "n_tokens, n_seq, max_q or pages_stride out of range");
-    if (pages_stride * kv->page_tokens > 0x7fffffff) return refuse(ctx, call, "a sequence must stay under 2^31 tokens");
+    if (pages_stride > 0x7fffffff / kv->page_tokens) return refuse(ctx, call, "a sequence must stay under 2^31 tokens");
     if (n_head <= 0 || n_head > kMostHeads || n_head % kv->n_head_kv != 0) return refuse(ctx, call, "n_head must be a multiple of n_head_kv");
     if (window < 0) return refuse(ctx, call, "negative window");
     // The device numbers places for rows of a head, and turns of four tiles of 64 tokens of all heads, in 32 bits.  A sequence's rows of a

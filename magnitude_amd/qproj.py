@@ -228,7 +228,7 @@ def rope_frequencies(n_dims: int, base: float = 10000.0, freq_scale: float = 1.0
 def relative_buckets(n_buckets: int, reach: int, both_sides: bool = True) -> np.ndarray:
     """The buckets int32 [2 * reach + 1] of a learned position bias for distances token - row from -reach to reach, half of them for
     either side or (both_sides False) all for tokens before the row.  Needs no GPU."""
-    buckets = np.empty(2 * max(0, reach) + 1, dtype=np.int32)
+    buckets = np.empty(2 * min(max(0, reach), 1 << 16) + 1, dtype=np.int32)     # (a longer reach is refused)
     st = load_library().qproj_relative_buckets(n_buckets, reach, 1 if both_sides else 0, buckets.ctypes.data)
     if st:
         raise QprojError(st, f"qproj_relative_buckets({n_buckets} buckets, reach {reach}, both_sides {both_sides})")

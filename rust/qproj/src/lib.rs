@@ -234,7 +234,7 @@ impl Context {
 
 /// The buckets of the distances from `-reach` to `reach`; see `qproj_relative_buckets`.
 pub fn relative_buckets(n_buckets: i64, reach: i64, both_sides: bool) -> Result<Vec<i32>> {
-    let mut buckets = vec![0i32; (2 * reach.max(0) + 1) as usize];
+    let mut buckets = vec![0i32; (2 * reach.clamp(0, 1 << 16) + 1) as usize];
     let st = unsafe { sys::qproj_relative_buckets(n_buckets, reach, both_sides as i32, buckets.as_mut_ptr()) };
     if st == sys::QPROJ_OK {
         Ok(buckets)

@@ -41,6 +41,14 @@ def test_bad_arguments_are_refused(name, bad):
     assert "kernel" not in dry.plan
 
 
+@pytest.mark.parametrize("ps", [1 << 60, (1 << 60) + 2, (1 << 63) - 1])
+def test_page_tables_that_pass_64_bits_are_refused(ps):
+    with Dry() as dry:
+        for name in ("cross", "biased", "shared"):
+            assert call(dry, name, cache(page_tokens=16), ps=ps) == 1 and "2^31" in dry.error()
+    assert "kernel" not in dry.plan
+
+
 @pytest.mark.parametrize("bad", CACHE_BAD, ids=str)
 def test_bad_caches_are_refused(bad):
     with Dry() as dry:
