@@ -41,6 +41,7 @@
 #include "qproj_internal.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace qproj {
 
@@ -71,6 +72,7 @@ enum Sees {
 
 struct AttentionArgs {
     static constexpr Sees kSees = kBefore;
+    static constexpr bool kApart = false;     // every wave has rows of its own and goes through all tiles of an item, instead of some tiles of rows that are all waves'
     KvView kv;
     const float *q;
     float *y;
@@ -104,6 +106,14 @@ struct BiasArgs : AttentionArgs {
     const float *bias;       // [query heads][2 * reach + 1], of tokens `reach` before a row to `reach` behind it
     int32_t reach;
     int32_t all;             // rows see all tokens
+};
+
+struct AllApartArgs : AllArgs {
+    static constexpr bool kApart = true;
+};
+
+struct BiasApartArgs : BiasArgs {
+    static constexpr bool kApart = true;
 };
 
 struct PrefixArgs : AttentionArgs {
@@ -198,8 +208,24 @@ __host__ __device__ __forceinline__ Item item_of(const A &a, int s, const Sequen
 }
 
 __host__ __device__ __forceinline__ int item_tiles(const Item &it) { return it.hi < 0 ? 1 : it.hi / kTile - it.see / kTile + 1; }
-// what an item takes of the line: a turn of the waves for every kWaves tiles
-__host__ __device__ __forceinline__ int item_turns(const Item &it) { return it.count <= 0 ? 0 : (item_tiles(it) + kWaves - 1) / kWaves; }
+// what an item takes of the line: a turn of the waves for every kWaves tiles, or where they are apart for every one
+template <typename A>
+__host__ __device__ __forceinline__ int item_turns(const Item &it) { return it.count <= 0 ? 0 : A::kApart ? item_tiles(it) : (item_tiles(it) + kWaves - 1) / kWaves; }
+// a wave's rows of an item where they are apart
+template <typename A>
+__device__ __forceinline__ Item item_of_wave(const A &a, const Item &it, int wave) {
+    Item mine = it;
+    if constexpr (A::kApart) {
+        const int skip = wave * (a.tokens / kWaves);
+        mine.count = max(0, min(a.tokens / kWaves, it.count - skip));
+        if (mine.count) mine.first += skip;      // (otherwise a row that there is: queries are loaded all the same)
+        if constexpr (A::kSees == kBiased) {
+            mine.at += skip;
+            if (!a.all) mine.lo += skip, mine.hi = mine.lo + mine.count - 1;
+        }
+    }
+    return mine;
+}
 
 // What lies behind the line's places: sequences, or groups of them.  Of a group: its first sequence, sequences, the tokens that they share.
 template <typename A>
@@ -250,7 +276,7 @@ __host__ __device__ __forceinline__ int turns_of(const A &a, int s, const Sequen
         tiles -= (with_rows - 1) * shared;
         return (max(1, tiles) + kWaves - 1) / kWaves;
     } else {
-        return item_turns(it);
+        return item_turns<A>(it);
     }
 }
 
@@ -278,8 +304,8 @@ struct Line {
     uint32_t length, longer; // a stretch's; the first `longer` have one more
 };
 
-// (spread: of the forms other than the causal one)
-__host__ __device__ __forceinline__ Line line_of(int head_turns, int head_items, int longest, uint32_t heads, uint32_t groups, bool spread) {
+// (spread: of the forms other than the causal one; apart: of items whose waves are, which stay whole)
+__host__ __device__ __forceinline__ Line line_of(int head_turns, int head_items, int longest, uint32_t heads, uint32_t groups, bool spread, bool apart) {
     // Where there are more turns than workgroups, beginning an item (staging its queries, adding its sums) counts as two turns.  Where no item
     // is longer than a workgroup's share, items stay whole and are dealt out, forwards and backwards in turn: an item is as long as its
     // rows are far from the start of their sequence, so that long ones meet short ones.  Otherwise every workgroup has a stretch of the
@@ -294,7 +320,9 @@ __host__ __device__ __forceinline__ Line line_of(int head_turns, int head_items,
     // The other forms cut items too where whole ones, a few a workgroup, would leave most workgroups waiting for those that have one more: where that is
     // over two turns of the average item.  (616 items on 512 workgroups, rows over five images' states: 60.8 us instead of 71.8; prompts
     // with a bias 64.9 instead of 67.8, a drawn one 124 instead of 177; where it is less than two, level.)
-    if (spread && l.whole && l.start) {
+    if (apart) {
+        l.whole = true;
+    } else if (spread && l.whole && l.start) {
         const uint32_t items = (uint32_t)head_items * heads, turns = (uint32_t)(head_turns + l.start * head_items) * heads, rounds = (items + groups - 1) / groups;
         l.whole = (float)rounds * (float)turns / (float)items - (float)turns / (float)groups <= 2.f;
     }
@@ -464,7 +492,7 @@ struct SharedLds : KindLds<A::kSees> {
             float m[kWaves][16], l[kWaves][16];
         } meet;
     };
-    u32x4 q[D / 32][NQ][2][64];   // the item's queries as the matrix cores take them: high halves, low halves
+    u32x4 q[A::kApart ? kWaves : 1][D / 32][NQ][2][64];   // the item's queries as the matrix cores take them: high halves, low halves
     float q_most[kWaves][NQ][16]; // of the waves' blocks, the rows' largest queries
     int32_t line[kThreads][2];    // a thread's items on a head's line: turns before them, theirs
     int32_t only[6][kThreads];    // where a thread has one place of the line: its item, as in `found`
@@ -539,14 +567,14 @@ __device__ __forceinline__ Row row_of(const A &a, const Item &it, int heads, int
 // 16 queries of an item for the matrix cores: 22 bits of q * scale * log2(e), the row scaled by a power of two.  A wave takes the blocks
 // wave, wave + 4, ... of all rows.  (All blocks in every wave, for want of a meeting about the rows' largest values, kept the loads of
 // keys and values waiting: 512 prompt tokens took 23.5 us instead of 21.7, 4096 402 instead of 388.)
-template <int D, int NQ>
+template <int D, int NQ, typename A>
 struct Queries {
-    static constexpr int kMine = (D / 32 + kWaves - 1) / kWaves;
+    static constexpr int kEvery = A::kApart ? 1 : kWaves, kMine = (D / 32 + kEvery - 1) / kEvery;
     f32x4 x[NQ][kMine][2];
 };
 
 template <int D, int NQ, typename A>
-__device__ __forceinline__ void load_queries(const A &a, const Item &it, int head0, int heads, Queries<D, NQ> &q, const SharedLds<D, NQ, A> &lds, int wave, int lane) {
+__device__ __forceinline__ void load_queries(const A &a, const Item &it, int head0, int heads, Queries<D, NQ, A> &q, const SharedLds<D, NQ, A> &lds, int wave, int lane) {
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
         const Row r = row_of(a, it, heads, g * 16 + (lane & 15), lds, wave);
@@ -554,15 +582,16 @@ __device__ __forceinline__ void load_queries(const A &a, const Item &it, int hea
 #pragma unroll
         for (int i = 0; i < q.kMine; ++i)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) q.x[g][i][k] = *reinterpret_cast<const f32x4 *>(row + 32 * min(wave + kWaves * i, D / 32 - 1) + 4 * k);
+            for (int k = 0; k < 2; ++k) q.x[g][i][k] = *reinterpret_cast<const f32x4 *>(row + 32 * min((A::kApart ? 0 : wave) + q.kEvery * i, D / 32 - 1) + 4 * k);
     }
 }
 
 // One barrier, about the rows' largest values; the staged queries need another.  q_unit: what sums are multiplied by, of the lane's columns.
 template <int D, int NQ, typename A>
-__device__ __forceinline__ void stage_queries(const A &a, const Item &it, int heads, Queries<D, NQ> &q, SharedLds<D, NQ, A> &lds, float (&q_unit)[NQ], int wave,
+__device__ __forceinline__ void stage_queries(const A &a, const Item &it, int heads, Queries<D, NQ, A> &q, SharedLds<D, NQ, A> &lds, float (&q_unit)[NQ], int wave,
                                               int lane) {
     const int col = lane & 15;
+    float mosts[NQ];
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
         const bool live = row_of(a, it, heads, g * 16 + col, lds, wave).live;
@@ -580,20 +609,25 @@ __device__ __forceinline__ void stage_queries(const A &a, const Item &it, int he
                     whole = whole && fabsf(x) <= 3.402823466e38f;
                 }
         most = max_xor(whole ? most : INFINITY);
-        if (lane < 16) lds.q_most[wave][g][lane] = most;
+        if (A::kApart) mosts[g] = most;
+        else if (lane < 16) lds.q_most[wave][g][lane] = most;
     }
-    __syncthreads();
+    if (!A::kApart) __syncthreads();
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
         float most = 0.f;
+        if (A::kApart) {
+            most = mosts[g];
+        } else {
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, lds.q_most[w][g][col]);
+            for (int w = 0; w < kWaves; ++w) most = fmaxf(most, lds.q_most[w][g][col]);
+        }
         // (frexp: most = f * 2^e with f in [0.5, 1); where a value is not finite the row stays as it is: NaN comes of it)
         const int e = most > 0.f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
         q_unit[g] = ldexpf(1.f, max(e - 15, -126));    // (not 0, which masked scores are multiplied by; such scores are 0)
 #pragma unroll
         for (int i = 0; i < q.kMine; ++i) {
-            const int b = wave + kWaves * i;
+            const int b = (A::kApart ? 0 : wave) + q.kEvery * i;
             if (b >= D / 32) continue;
             u32x4 hi, lo;
 #pragma unroll
@@ -602,13 +636,13 @@ __device__ __forceinline__ void stage_queries(const A &a, const Item &it, int he
                 hi[j] = half_pair(u, v);
                 lo[j] = half_pair(u - low_half(hi[j]), v - high_half(hi[j]));
             }
-            lds.q[b][g][0][lane] = hi;
-            lds.q[b][g][1][lane] = lo;
+            lds.q[A::kApart ? wave : 0][b][g][0][lane] = hi;
+            lds.q[A::kApart ? wave : 0][b][g][1][lane] = lo;
         }
     }
 }
 
-// Tiles [from, to) of an item (in tiles from token 0 on), every kWaves-th of them.  Two barriers of the workgroup, before and
+// Tiles [from, to) of an item (in tiles from token 0 on), every kWaves-th of them (all of them where the waves are apart).  Two barriers of the workgroup, before and
 // behind the staged queries, whatever there is to do.
 template <int D, int NQ, typename A>
 __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &members, int kv_head, int head0, int heads, int from, int to, SharedLds<D, NQ, A> &shared,
@@ -616,6 +650,7 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
     WaveLds<D, NQ> &lds = shared.wave[wave];
     constexpr int B = D / 32, RB = D / 2, T = D / 16;
     constexpr bool kAhead = values_ahead(D);
+    constexpr int kEvery = A::kApart ? 1 : kWaves;
     const int col = lane & 15, part = lane >> 4;
     const KvView &kv = a.kv;
     const int shift = kv.page_shift, mask = (1 << shift) - 1;
@@ -627,7 +662,7 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
 #pragma unroll
         for (int t = 0; t < T; ++t) st.o[t][g] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const bool work = from < to && (A::kSees == kPrefix ? members.tiles > 0 : it.hi >= 0);
+    const bool work = from < to && (A::kSees == kPrefix ? members.tiles > 0 : it.hi >= 0) && (!A::kApart || it.count > 0);
 
     // Where a tile's tokens are: whose (of the item's sequences; -1: shared, or the only one's), which pages, its first token, the first and the last one that is seen.
     struct Place {
@@ -650,10 +685,10 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
         const int t = min(max(p.t0 + lane, p.see), p.hi);
         return (A::kSees == kPrefix ? a.pages + (int64_t)p.seq * a.pages_stride : table)[t >> shift];
     };
-    const int last_tile = work ? from + (to - 1 - from) / kWaves * kWaves : from;   // of this wave
+    const int last_tile = work ? from + (to - 1 - from) / kEvery * kEvery : from;   // of this wave
     Place now{}, next{};        // kPrefix: this tile's and the wave's next one's (otherwise known from their numbers)
-    if (A::kSees == kPrefix && work) now = find(from), next = find(min(from + kWaves, last_tile));
-    int page = work ? page_of(A::kSees == kPrefix ? now : find(from)) : 0, page_next = work ? page_of(A::kSees == kPrefix ? next : find(min(from + kWaves, last_tile))) : 0;
+    if (A::kSees == kPrefix && work) now = find(from), next = find(min(from + kEvery, last_tile));
+    int page = work ? page_of(A::kSees == kPrefix ? now : find(from)) : 0, page_next = work ? page_of(A::kSees == kPrefix ? next : find(min(from + kEvery, last_tile))) : 0;
     bool bad_page = false;
 
     uint32_t k_raw[4][B];
@@ -747,7 +782,7 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
             global_to_lds4_unseen(a.bias + (int64_t)(head0 + h) * span + min(max(at - kBiasPad, 0), span - 1), shared.bias + i);
         }
     }
-    Queries<D, NQ> queries;
+    Queries<D, NQ, A> queries;
     load_queries<D, NQ>(a, it, head0, heads, queries, shared, wave, lane);
     if (work) {
         place(A::kSees == kPrefix ? now : find(from));
@@ -793,7 +828,7 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
     int buffer = 0;
     const bool young = (int)blockIdx.x >= a.young;
     bool up = false;
-    for (int tile = from; tile < to; tile += kWaves) {
+    for (int tile = from; tile < to; tile += kEvery) {
         const Place here = A::kSees == kPrefix ? now : find(tile);
         const int t0 = here.t0;
         const int bad_now = bad_groups;
@@ -847,12 +882,12 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
         page = page_next;
         if constexpr (A::kSees == kPrefix) {
             now = next;
-            next = find(min(tile + 2 * kWaves, last_tile));
+            next = find(min(tile + 2 * kEvery, last_tile));
             page_next = page_of(next);
             place(now);
         } else {
-            page_next = page_of(find(min(tile + 2 * kWaves, last_tile)));
-            place(find(min(tile + kWaves, last_tile)));
+            page_next = page_of(find(min(tile + 2 * kEvery, last_tile)));
+            place(find(min(tile + kEvery, last_tile)));
         }
         load_scales();
         // ---- scores ----
@@ -889,8 +924,8 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
                 if (g0 == 0) {
 #pragma unroll
                     for (int c = 0; c < NQ; ++c) {
-                        qh[c] = __builtin_bit_cast(half8, shared.q[b][c][0][lane]);
-                        ql[c] = __builtin_bit_cast(half8, shared.q[b][c][1][lane]);
+                        qh[c] = __builtin_bit_cast(half8, shared.q[A::kApart ? wave : 0][b][c][0][lane]);
+                        ql[c] = __builtin_bit_cast(half8, shared.q[A::kApart ? wave : 0][b][c][1][lane]);
                     }
                 }
 #pragma unroll
@@ -1225,6 +1260,20 @@ __device__ __forceinline__ void meet(const A &a, const Item &it, int head0, int 
     }
 }
 
+// Rows of a wave that is apart.
+template <int D, int NQ, typename A>
+__device__ __forceinline__ void finish(const A &a, const Item &it, int head0, int heads, const Running<D, NQ> &st, SharedLds<D, NQ, A> &lds, int wave, int lane) {
+#pragma unroll
+    for (int g = 0; g < NQ; ++g) {
+        const Row r = row_of(a, it, heads, g * 16 + (lane & 15), lds, wave);
+        float *const y = out_row<D, NQ>(a, r, head0, lane);
+        const float unit = st.l[g] != 0.f ? 1.f / st.l[g] : 0.f;
+        if (!r.live) continue;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) *reinterpret_cast<f32x4 *>(y + 16 * t) = f32x4{st.o[t][g][0] * unit, st.o[t][g][1] * unit, st.o[t][g][2] * unit, st.o[t][g][3] * unit};
+    }
+}
+
 // An item that was cut into a few parts, which stretches first .. first + parts - 1 wrote: their sums.  The waves share the dimensions; a part
 // comes from far away, so several are asked for at a time.
 template <int D, int NQ, typename A>
@@ -1342,7 +1391,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const A) {
             for (int i = id; i < units_of(a) * a.kv.n_head * a.splits; i += kThreads) a.joins[2 * i] = -1;
         return leave(a);
     }
-    const Line line = line_of(head_turns, head_items, longest, a.kv.n_head * a.splits, gridDim.x, A::kSees != kBefore);
+    const Line line = line_of(head_turns, head_items, longest, a.kv.n_head * a.splits, gridDim.x, A::kSees != kBefore, A::kApart);
     lds.line[id][0] = line.whole ? items_before : turns_before + line.start * items_before;   // (each thread's own: kept out of the registers
     lds.line[id][1] = line.whole ? items_mine : turns_mine + line.start * items_mine;         // that the tiles want)
     const uint32_t me = line.whole ? blockIdx.x : stretch_of_block(blockIdx.x, line.active);
@@ -1396,6 +1445,16 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const A) {
         const int tile1 = tile0 + min(piece.to * kWaves, A::kSees == kPrefix ? max(1, seqs.tiles) : item_tiles(it));
 
         Running<D, NQ> st;
+        if constexpr (A::kApart) {      // whole items only
+            const Item mine = item_of_wave(a, it, wave);
+            walk<D, NQ>(a, mine, seqs, kv_head, head0, heads, tile0, min(tile0 + turns, mine.hi / kTile + 1), lds, wave, st, lane);
+            leave(a);
+            finish<D, NQ>(fresh_arguments<A>(), mine, head0, heads, st, lds, wave, lane);
+            ++round;
+            at = round * line.active + (round & 1 ? line.active - 1 - me : me);
+            if (at < end) __syncthreads();
+            continue;
+        }
         walk<D, NQ>(a, it, seqs, kv_head, head0, heads, tile0 + piece.from * kWaves + wave, tile1, lds, wave, st, lane);
         leave(a);                       // (here, so that nothing waits for it)
         // ---- the waves' sums ----
@@ -1555,7 +1614,7 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
     const int groups_most = kPerCu * j.cus;
     const int64_t most_len = j.pages_stride << j.kv->page_shift;
     double items = 0;
-    int cols = 1;
+    int cols = A::kApart ? 2 : 1;
     for (;; ++cols) {
         const int rows = 16 * cols;
         a.splits = (a.group + rows - 1) / rows;
@@ -1567,7 +1626,7 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
             a.splits = (a.group + a.split - 1) / a.split;
         }
         a.split_part = (65536 + a.split - 1) / a.split;
-        a.tokens = rows / a.split;
+        a.tokens = (A::kApart ? kWaves : 1) * (rows / a.split);
         a.row_tiles = (int32_t)std::max<int64_t>(1, (j.max_q + a.tokens - 1) / a.tokens);
         a.most_items = a.n_tokens / a.tokens + a.n_seq;
         items = std::min((double)a.n_seq * a.row_tiles, (double)a.n_tokens / a.tokens + a.n_seq) * j.kv->n_head * a.splits;
@@ -1599,7 +1658,7 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
         groups = (int)std::max(1., std::min<double>(groups_most, items * ((double)most * a.together / kWaves + 1)));
         if (groups > 8 * places && items * ((double)most / kWaves + 1) <= 8. * places) groups = (int)(8 * places);
     } else {
-        groups = (int)std::max(1., std::min<double>(groups_most, items * ((double)most / kWaves + 1)));
+        groups = (int)std::max(1., std::min<double>(groups_most, items * (A::kApart ? 1. : (double)most / kWaves + 1)));
     }
     a.parts = reinterpret_cast<float *>(j.scratch + head_bytes(j.cus));
     a.slots = groups_most;
@@ -1609,26 +1668,43 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
     // of 8192 13.8 against 19.0, for eight rows behind 6000 17.2 against 22.1; a short chat's token, with two, 14.0 against 11.9.  (Up to five
     // instead of eight: 0.6% more over 50 drawn calls, up to three 2%.)
     // (the joins' list has a place for every item there could be, fewer than groups / 8)
-    const bool few_parts = groups <= 8 * places;
+    const bool few_parts = A::kApart || groups <= 8 * places;
     a.arrived = few_parts ? reinterpret_cast<uint64_t *>(j.scratch) : nullptr;
     a.calls = reinterpret_cast<uint32_t *>(j.scratch + counts_bytes(j.cus));
     a.young = few_parts ? j.cus : 0;      // (the second workgroups of the compute units, or all: see walk)
     a.joins = reinterpret_cast<int32_t *>(j.scratch + counts_bytes(j.cus) + calls_bytes(j.cus));
     if (dry_run()) {
         const char *const sees[] = {"", ", all", ", biased", ", prefix"};
-        plan_note("attention_kernel<%d, %d%s>: %d heads in %d x %d of %d, %d tokens x %d a sequence of rows, grid %d x %d, first from %d on", a.kv.dim, cols, sees[A::kSees], j.n_head,
+        plan_note("attention_kernel<%d, %d%s%s>: %d heads in %d x %d of %d, %d tokens x %d a sequence of rows, grid %d x %d, first from %d on", a.kv.dim, cols, sees[A::kSees], A::kApart ? ", apart" : "", j.n_head,
                   a.kv.n_head, a.splits, a.split, a.tokens, a.row_tiles, groups, kThreads, a.young);
         return hipSuccess;
     }
-    if (cols == 1) {
-        if (a.kv.dim == 64) return launch<64, 1, A>(a, groups, (int)places, s);
-        if (a.kv.dim == 96) return launch<96, 1, A>(a, groups, (int)places, s);
-        if (a.kv.dim == 128) return launch<128, 1, A>(a, groups, (int)places, s);
-        return launch<256, 1, A>(a, groups, (int)places, s);
+    if constexpr (A::kApart) {
+        return launch<64, 2, A>(a, groups, (int)places, s);
+    } else {
+        if (cols == 1) {
+            if (a.kv.dim == 64) return launch<64, 1, A>(a, groups, (int)places, s);
+            if (a.kv.dim == 96) return launch<96, 1, A>(a, groups, (int)places, s);
+            if (a.kv.dim == 128) return launch<128, 1, A>(a, groups, (int)places, s);
+            return launch<256, 1, A>(a, groups, (int)places, s);
+        }
+        if (a.kv.dim == 64) return launch<64, 2, A>(a, groups, (int)places, s);
+        if (a.kv.dim == 96) return launch<96, 2, A>(a, groups, (int)places, s);
+        return launch<128, 2, A>(a, groups, (int)places, s);
     }
-    if (a.kv.dim == 64) return launch<64, 2, A>(a, groups, (int)places, s);
-    if (a.kv.dim == 96) return launch<96, 2, A>(a, groups, (int)places, s);
-    return launch<128, 2, A>(a, groups, (int)places, s);
+}
+
+// Whether every wave is to have rows of its own, 32 of an item of 128, and go through all tiles.  Otherwise four waves share 32 rows and the tiles, and
+// meet: an item of a short sequence is one or two tiles a wave between finding it, staging its queries and adding the waves' sums, some 10000 cycles
+// of 17000.  Apart the queries are found and staged once for 128 rows and nothing is added; an item is as long as the tokens it sees, though, stays
+// whole, and there are a quarter as many.  So: where there are items enough for how long they can be, at least 32 for every tile, and beyond eight tiles four times as
+// many as tiles.  Over 46 batches of rows with a bias, alike / of all lengths, and cross attention, heads of 64, at the best 2.0 times as fast, inside the rule 1.3 in the mean
+// and 0.95 at worst: 64 sequences of 128 on 8 heads 40.4 -> 19.9 us, 16 of 512 on 16 98 -> 72, 8 of up to 512 39.5 -> 35.3; outside it 2 of 1024 on 8
+// 24.0 -> 47.4.  Wider heads' queries, of four waves, leave no room in LDS for a second workgroup.
+inline bool rows_apart(const AttentionJob &j) {
+    if (j.n_tokens == 0 || j.n_seq == 0 || j.kv->dim != 64) return false;
+    const double rows = (double)j.n_tokens * j.n_head / j.kv->n_head, tiles = std::ceil((double)(j.pages_stride << j.kv->page_shift) / kTile);
+    return rows >= 32. * j.n_seq && rows * j.kv->n_head / (32 * kWaves) >= tiles * std::max(32., 4 * tiles);
 }
 
 // For the tests: the pieces of the line that every workgroup of a call takes, in the order in which it takes them, worked out on the host by the
@@ -1652,7 +1728,7 @@ int64_t pieces_of(A a, const int32_t *kv_len_later, int heads, int groups, int32
         head_turns += t.turns, head_items += t.items;
     }
     if (head_items > a.most_items) return 0;
-    const Line line = line_of(head_turns, head_items, longest, heads, groups, A::kSees != kBefore);
+    const Line line = line_of(head_turns, head_items, longest, heads, groups, A::kSees != kBefore, A::kApart);
     a.kv_len = kv_len_later;
     int64_t pieces = 0;
     for (int block = 0; block < groups; ++block) {

@@ -3,6 +3,9 @@
 
 namespace qproj {
 
-hipError_t launch_attention_all(const AttentionJob &j, hipStream_t s) { return launch_as(j, AllArgs{}, s); }
+hipError_t launch_attention_all(const AttentionJob &j, hipStream_t s) {
+    if (rows_apart(j)) return launch_as(j, AllApartArgs{}, s);
+    return launch_as(j, AllArgs{}, s);
+}
 
 }  // namespace qproj

@@ -29,11 +29,13 @@ hipError_t launch_bias_by_distance(const float *table, int n_buckets, int n_head
 }
 
 hipError_t launch_attention_biased(const AttentionJob &j, const float *bias, int reach, bool all, hipStream_t s) {
-    BiasArgs a{};
-    a.bias = bias;
-    a.reach = reach;
-    a.all = all;
-    return launch_as(j, a, s);
+    const auto with = [&](auto a) {
+        a.bias = bias;
+        a.reach = reach;
+        a.all = all;
+        return launch_as(j, a, s);
+    };
+    return rows_apart(j) ? with(BiasApartArgs{}) : with(BiasArgs{});
 }
 
 }  // namespace qproj

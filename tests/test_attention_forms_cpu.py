@@ -8,6 +8,7 @@ import pytest
 
 import forms_ref
 from magnitude_amd import qproj
+from test_attention_forms_gpu import APART
 from test_attention_cpu import ATTENTION_BAD, BUF, CACHE_BAD, Dry, cache
 
 
@@ -68,6 +69,27 @@ def test_calls_that_are_taken_note_their_launches():
         assert dry.lib.qproj_bias_by_distance(dry.ctx, BUF, 32, 12, BUF, 128, BUF) == 0
     assert dry.plan.count(", all>:") == 20 and dry.plan.count(", biased>:") == 20 and dry.plan.count("attention_kernel<") == 40
     assert dry.plan.count("bias_by_distance_kernel: 12 heads x 257 distances") == 1
+
+
+def short(name, page, kv_heads, group, seqs, dim=64, columns=None, **kw):
+    """The plan of a call with such sequences [(tokens, rows)] in a table as wide as the tests make it"""
+    h, rows = kv_heads * group, [m for _, m in seqs]
+    ps = max(-(-n // page) for n, _ in seqs) + 1 if columns is None else columns
+    with Dry() as dry:
+        assert call(dry, name, cache(page_tokens=page, n_head_kv=kv_heads, head_dim=dim, n_pages=4000), h=h, qs=h * dim, ys=h * dim, n=sum(rows), seqs=len(seqs), max_q=max(rows), ps=ps, **kw) == 0
+    return dry.plan
+
+
+def test_many_rows_of_short_sequences_are_taken_by_waves_of_their_own():
+    for page, kv_heads, group, seqs in APART:
+        for name in ("cross", "biased"):
+            assert "attention_kernel<64, 2, " + {"cross": "all", "biased": "biased"}[name] + ", apart>" in short(name, page, kv_heads, group, seqs), (name, page)
+            assert "apart" not in short(name, page, kv_heads, group, seqs, dim=128)
+    many = [(128, 128)] * 64                                            # 512 items of 128 rows
+    assert "grid 512 x 256" in short("cross", 64, 8, 1, many, columns=2) and ", apart>" in short("cross", 64, 8, 1, many, columns=11)
+    assert "apart" not in short("cross", 64, 8, 1, many, columns=12)    # (twelve tiles: 576 items)
+    assert "apart" not in short("cross", 64, 16, 1, [(64, 1)] * 4000, columns=1)       # single rows
+    assert "apart" not in short("shared", 64, 8, 1, many, columns=2)
 
 
 @pytest.mark.parametrize("reach,group,heads", [(0, 16, 16), (128, 16, 8), (128, 9, 5), (128, 4, 4), (500, 8, 3), (1703, 7, 1)])

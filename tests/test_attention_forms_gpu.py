@@ -65,6 +65,17 @@ CROSS = [  # dim, page, kv heads, group, [(states, rows)]
 ]
 
 
+APART = [  # of heads of 64, so many rows of short sequences that every wave has some of its own: page, kv heads, group, [(tokens, rows)]
+    (64, 64, 1, [(200, 200), (129, 129), (60, 60), (190, 130)]),
+    (16, 64, 2, [(100, 250), (1, 130), (0, 140), (65, 65), (64, 33)]),       # more rows than tokens, none at all
+    (256, 32, 5, [(500, 500)]),                                               # 6 of 32 rows a token
+    (32, 128, 1, [(90 + 7 * i, 130 + 3 * i) for i in range(3)]),
+    (128, 1, 71, [(200, 1000)]),
+    (128, 64, 1, [(900 - 10 * i, 600) for i in range(5)]),
+]
+CROSS += [(64, page, kv_heads, group, seqs) for page, kv_heads, group, seqs in APART]
+
+
 @pytest.mark.parametrize("dim,page,kv_heads,group,seqs", CROSS)
 def test_cross_attention(ctx, dim, page, kv_heads, group, seqs):
     tell("cross", dim, page, kv_heads, group, seqs)
@@ -165,6 +176,9 @@ BIASED = [  # dim, page, kv heads, group, [(tokens, rows)], reach
     (64, 64, 1, 2, [(20000, 3)], 128),                    # many parts, joined by a launch of their own
     (128, 16, 4, 4, [(1 + 37 * i % 301, 1) for i in range(90)], 10),
 ]
+
+
+BIASED += [(64, page, kv_heads, group, seqs, reach) for (page, kv_heads, group, seqs), reach in zip(APART, (128, 30, 400, 128, 1, 200))]
 
 
 @pytest.mark.parametrize("causal", [True, False])

@@ -222,6 +222,63 @@ def test_a_table_of_biases_laid_out_in_a_graph(ctx):
     own.close()
 
 
+@pytest.mark.parametrize("form", ["cross", "causal", "both"])
+def test_a_captured_encoder_follows_the_lengths(ctx, form):
+    """many rows of short sequences, recorded once, replayed with other sequences' lengths and rows, some of none, eager work between"""
+    from magnitude_amd import Context, QprojError
+    tell("captured encoder", form)
+    stream = torch.cuda.Stream()
+    own = Context(0, stream=stream.cuda_stream)
+    rng = np.random.default_rng(62)
+    seqs, heads, most, rows = 8, 64, 180, 600
+    kv, pages = make_cache(rng, [most] * seqs, 64, heads, 64)
+    q_host, bias_host = rng.standard_normal((rows, heads, 64)).astype(np.float32), make_bias(rng, heads, 100)[0]
+    q, bias, table, y = dev(q_host), dev(bias_host), dev(pages), torch.zeros((rows, heads, 64), device="cuda")
+    start, lens = i32(np.arange(seqs + 1) * 75), i32([75] * seqs)
+
+    def step(c, out):
+        if form == "cross":
+            return c.cross_attention(kv, q, start, lens, table, max_q=300, out=out, sync=False)
+        return c.attention_biased(kv, q, start, lens, table, bias, causal=form == "causal", max_q=300, out=out, sync=False)
+
+    torch.cuda.synchronize()
+    step(own, y)
+    own.sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step(own, y)
+    for i in range(6):
+        count = [[75] * 8, [300, 0, 1, 299, 0, 0, 0, 0], [128, 129, 31, 32, 33, 96, 97, 54], [0] * 8, [1] * 8, [64, 128, 200, 100, 7, 1, 0, 100]][i]
+        n = [most, 0, 1, 64, 65, 128, 33, most] if i % 2 else rng.integers(0, most + 1, seqs)
+        with torch.cuda.stream(stream):
+            start.copy_(i32(np.cumsum([0] + count)))
+            lens.copy_(i32(n))
+            y.fill_(7.5)
+            graph.replay()
+        stream.synchronize()
+        other = torch.full_like(y, 7.5)
+        torch.cuda.synchronize()
+        step(ctx, other)
+        ctx.sync()
+        assert torch.equal(y, other), f"replay {i}"
+        args = ctx, kv, pages, q_host, np.cumsum([0] + count), [int(v) for v in n]
+        got = check_cross(*args, max_q=300) if form == "cross" else check_biased(*args, bias_host, form == "causal", max_q=300)
+        assert np.abs(got[:sum(count)] - y.cpu().numpy()[:sum(count)]).max(initial=0) < 1e-5
+        if i % 2:
+            step(own, other)
+    ok = y.clone()
+    for bad_start, bad_len, what, left in (([64, 128, 200, 100, 7, 1, 0, 101], 33, "q_start", 500), ([64, 128, 200, 100, 7, 1, 0, 100], -1, "q_start", 500)):
+        start.copy_(i32(np.cumsum([0] + bad_start)))
+        lens[7] = bad_len
+        y.fill_(7.5)
+        torch.cuda.synchronize()
+        step(ctx, y)
+        with pytest.raises(QprojError, match=what):
+            ctx.sync()
+        assert torch.equal(y[:left], ok[:left]) and (y[left:] == 7.5).all()
+    own.close()
+
+
 def test_contexts_of_all_forms_at_once():
     """calls on streams of their own, cut into few parts and into many, do not meet"""
     from magnitude_amd import Context
