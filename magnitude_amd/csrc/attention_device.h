@@ -1,6 +1,6 @@
-// Attention over the paged 4-bit cache on the matrix cores.
+// Attention over the paged 4-bit cache on the matrix cores: the kernel of every form, which differ in who sees what.
 //
-//   y = sum_t softmax_t(scale * q . k_t) v_t over the tokens t <= p (the last `window` of them) of a sequence.
+//   y = sum_t softmax_t(scale * q . k_t [+ bias of t - p]) v_t over the tokens t <= p (the last `window` of them) of a sequence, or over all of its tokens.
 //
 // Work.  An item is 16 or 32 rows (some new tokens x the query heads that share a key/value head) against the
 // tokens they see, in tiles of 64 tokens.  All tiles of all items lie in one line, head by head, and the workgroups of one round
@@ -9,7 +9,8 @@
 // many parts, a second kernel.  Items that are all short stay whole.  The line is laid out
 // on the device (a scan over the lengths in every workgroup), so that a captured call follows the lengths.  Inside a
 // workgroup the four waves take tiles in turn, each with its own running maximum, sum and result; they meet once, at the
-// end of an item.  No barrier in the loop over tiles.
+// end of an item.  No barrier in the loop over tiles.  (Rows of several sequences that share tokens, and waves with rows of their own: see
+// PrefixArgs and rows_apart.)
 //
 // A tile.  v_mfma_f32_16x16x32_f16 with tokens (then dimensions) as rows and queries as columns, so that a lane's column is
 // one query throughout: row statistics are a lane's own, and the probabilities come out of the first product in the
@@ -67,7 +68,7 @@ enum Sees {
     kBefore,     // a row at position p: tokens up to p, the last `window` of them
     kAll,        // every row: all tokens of its sequence
     kBiased,     // either, with a bias of the distance added to the scores
-    kPrefix,     // tokens up to p; several sequences an item, whose first tokens are the same
+    kPrefix,     // tokens up to p; several sequences an item, which share their first tokens
 };
 
 struct AttentionArgs {
@@ -1697,10 +1698,11 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
 // Whether every wave is to have rows of its own, 32 of an item of 128, and go through all tiles.  Otherwise four waves share 32 rows and the tiles, and
 // meet: an item of a short sequence is one or two tiles a wave between finding it, staging its queries and adding the waves' sums, some 10000 cycles
 // of 17000.  Apart the queries are found and staged once for 128 rows and nothing is added; an item is as long as the tokens it sees, though, stays
-// whole, and there are a quarter as many.  So: where there are items enough for how long they can be, at least 32 for every tile, and beyond eight tiles four times as
-// many as tiles.  Over 46 batches of rows with a bias, alike / of all lengths, and cross attention, heads of 64, at the best 2.0 times as fast, inside the rule 1.3 in the mean
-// and 0.95 at worst: 64 sequences of 128 on 8 heads 40.4 -> 19.9 us, 16 of 512 on 16 98 -> 72, 8 of up to 512 39.5 -> 35.3; outside it 2 of 1024 on 8
-// 24.0 -> 47.4.  Wider heads' queries, of four waves, leave no room in LDS for a second workgroup.
+// whole, and there are a quarter as many.  So: where there are items enough for how long they can be, at least 32 for every tile, and beyond
+// eight tiles four times as many as tiles for each.  Over 125 batches inside the rule (heads of 64, a bias on both sides or causal and cross attention, rows
+// alike and of all lengths) 1.32 times as fast in the mean, 2.07 at best, 0.90 at worst: 64 sequences of 128 on 8 heads 40.4 us -> 19.9, 16 of 512
+// on 16 98 -> 72, 8 of up to 512 on 16 39.5 -> 34.7; outside it 2 of 1024 on 8 24.0 -> 47.4.  Wider heads' queries, of four waves, leave no room in LDS
+// for a second workgroup.
 inline bool rows_apart(const AttentionJob &j) {
     if (j.n_tokens == 0 || j.n_seq == 0 || j.kv->dim != 64) return false;
     const double rows = (double)j.n_tokens * j.n_head / j.kv->n_head, tiles = std::ceil((double)(j.pages_stride << j.kv->page_shift) / kTile);
