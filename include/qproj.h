@@ -354,7 +354,8 @@ int qproj_attention_shared(qproj_ctx *ctx, const qproj_kv_cache *kv, const float
  *   y = sum_t softmax_t(scale * q . k_t) v_t,  t < kv_len.
  * The states' keys and values are appended without a rotation; rows that look at the same states (beams of a request) are
  * best given as rows of one sequence, which reads them once.  Bounds, errors, workspace and capture as for qproj_attention; rows of a
- * sequence without tokens are zeros. */
+ * sequence without tokens are zeros.  How work is laid out follows from n_tokens, max_q and pages_stride, not from the lengths on the
+ * device: a table no wider than the longest sequence needs is best (here, and with qproj_attention_biased for an encoder's layers). */
 int qproj_cross_attention(qproj_ctx *ctx, const qproj_kv_cache *kv, const float *q_dev, int64_t q_stride, int64_t n_tokens,
                           int64_t n_head, int64_t n_seq, const int32_t *q_start_dev, const int32_t *kv_len_dev, int64_t max_q,
                           const int32_t *pages_dev, int64_t pages_stride, float scale, float *y_dev, int64_t y_stride);
