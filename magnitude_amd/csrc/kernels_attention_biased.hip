@@ -6,7 +6,7 @@
 //
 // What bounds it, as of every kind: issue slots, and where sequences are short the finding and staging of items.  Encoders of 16 heads of 64, reach 128: eight
 // texts of up to 512 tokens 34.7 us; one of 4096 231 us, 68.7 Gflop (2.5 times that on the matrix cores, as pairs of halves: 740 Tflop/s).  Two prompts of 500 behind
-// 100 to 900, 24 heads of 96 on 8, reach 400, 65 us, of which the biases are 5 (with a reach of 1 58, without a bias 62).  A token of 16 sequences of up to
+// 100 to 900, 24 heads of 96 on 8, reach 400, 60.8 us, of which the biases are some 5.  A token of 16 sequences of up to
 // 512, 16 heads of 64, 10.9.
 #include "attention_device.h"
 
