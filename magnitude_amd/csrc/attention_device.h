@@ -1476,6 +1476,7 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const A) {
             walk<D, NQ>(a, mine, seqs, kv_head, head0, heads, tile0, min(tile0 + turns, mine.hi / kTile + 1), lds, wave, st, lane);
             leave(a);
             finish<D, NQ>(fresh_arguments<A>(), mine, head0, heads, st, lds, wave, lane);
+            if (!kEarly) move_on();
             if (at < end) __syncthreads();
             continue;
         }
@@ -1633,7 +1634,7 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
     const int groups_most = kPerCu * j.cus;
     const int64_t most_len = j.pages_stride << j.kv->page_shift;
     double items = 0;
-    int cols = A::kApart ? 2 : 1;
+    int cols = A::kApart && a.kv.dim == 64 ? 2 : 1;
     for (;; ++cols) {
         const int rows = 16 * cols;
         a.splits = (a.group + rows - 1) / rows;
@@ -1665,7 +1666,7 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
             if (a.max_group * a.max_q * a.group <= 16 || (a.together >= 2 && most_len < 32768)) break;
         }
         const int64_t seen = j.window ? std::min<int64_t>(most_len, (int64_t)j.window + a.tokens) : most_len;
-        if (cols == 2 || a.kv.dim > 128 || (A::kSees != kPrefix && j.max_q * a.group <= 16) || items * ((double)seen / (kWaves * kTile) + 2) <= 6. * groups_most) break;
+        if (A::kApart || cols == 2 || a.kv.dim > 128 || (A::kSees != kPrefix && j.max_q * a.group <= 16) || items * ((double)seen / (kWaves * kTile) + 2) <= 6. * groups_most) break;
     }
     // no more workgroups than there can be turns
     const int64_t most = (most_len + kTile - 1) / kTile + 1;
@@ -1699,7 +1700,10 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
         return hipSuccess;
     }
     if constexpr (A::kApart) {
-        return launch<64, 2, A>(a, groups, (int)places, s);
+        if (a.kv.dim == 64) return launch<64, 2, A>(a, groups, (int)places, s);
+        if (a.kv.dim == 96) return launch<96, 1, A>(a, groups, (int)places, s);
+        if constexpr (A::kSees == kAll) return launch<128, 1, A>(a, groups, (int)places, s);
+        return hipErrorInvalidValue;
     } else {
         if (cols == 1) {
             if (a.kv.dim == 64) return launch<64, 1, A>(a, groups, (int)places, s);
@@ -1713,18 +1717,21 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
     }
 }
 
-// Whether every wave is to have rows of its own, 32 of an item of 128, and go through all tiles.  Otherwise four waves share 32 rows and the tiles, and
-// meet: an item of a short sequence is one or two tiles a wave between finding it, staging its queries and adding the waves' sums, some 10000 cycles
-// of 17000.  Apart the queries are found and staged once for 128 rows and nothing is added; an item is as long as the tokens it sees, though, stays
-// whole, and there are a quarter as many.  So: where there are items enough for how long they can be, at least 32 for every tile, and beyond
-// eight tiles four times as many as tiles for each.  Over 125 batches inside the rule (heads of 64, a bias on both sides or causal and cross attention, rows
-// alike and of all lengths) 1.32 times as fast in the mean, 2.07 at best, 0.90 at worst: 64 sequences of 128 on 8 heads 40.4 us -> 19.9, 16 of 512
-// on 16 98 -> 72, 8 of up to 512 on 16 39.5 -> 34.7; outside it 2 of 1024 on 8 24.0 -> 47.4.  Wider heads' queries, of four waves, leave no room in LDS
-// for a second workgroup.
-inline bool rows_apart(const AttentionJob &j) {
-    if (j.n_tokens == 0 || j.n_seq == 0 || j.kv->dim != 64) return false;
+// Whether every wave is to have rows of its own, 32 of an item of 128 (of heads wider than 64 16 of one of 64), and go through all tiles.  Otherwise four waves
+// share the rows and the tiles, and meet: an item of a short sequence is one or two tiles a wave between finding it, staging its queries and adding the
+// waves' sums, some 10000 cycles of 17000.  Apart the queries are found and staged once for four times the rows and nothing is added; an item is as
+// long as the tokens it sees, though, stays whole, and there are a quarter as many.  So: where there are items enough for how long they can be, at least
+// 32 for every tile, and beyond eight tiles four times as many as tiles for each.  Over 125 batches inside the rule (heads of 64, a bias on both sides or
+// causal and cross attention, rows alike and of all lengths) 1.32 times as fast in the mean, 2.07 at best, 0.90 at worst: 64 sequences of 128 on 8 heads 40.4 us ->
+// 19.9, 16 of 512 on 16 98 -> 72, 8 of up to 512 on 16 39.5 -> 34.7; outside it 2 of 1024 on 8 24.0 -> 47.4.
+// The queries of four waves have to leave room in LDS for a second workgroup: 32 rows a wave of heads of 64, 16 of 96 and, without biases, of 128.  Those tiles' codes are
+// unpacked twice as often, which pays up to six tiles: 1.29 times as fast in the mean of 116 batches, 1.04 to 1.77 (64 sequences of 128 on 8 heads of 128 52.8 us ->
+// 35.6, 32 of 384 on 16 193 -> 143); of eight tiles 0.8 to 1.34.
+inline bool rows_apart(const AttentionJob &j, bool biased) {
+    if (j.n_tokens == 0 || j.n_seq == 0 || j.kv->dim > (biased ? 96 : 128)) return false;
     const double rows = (double)j.n_tokens * j.n_head / j.kv->n_head, tiles = std::ceil((double)(j.pages_stride << j.kv->page_shift) / kTile);
-    return rows >= 32. * j.n_seq && rows * j.kv->n_head / (32 * kWaves) >= tiles * std::max(32., 4 * tiles);
+    if (j.kv->dim > 64 && tiles > 6) return false;
+    return rows >= (j.kv->dim > 64 ? 16. : 32.) * j.n_seq && rows * j.kv->n_head / 128 >= tiles * std::max(32., 4 * tiles);
 }
 
 // For the tests: the pieces of the line that every workgroup of a call takes, in the order in which it takes them, worked out on the host by the

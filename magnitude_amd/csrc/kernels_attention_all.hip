@@ -9,7 +9,7 @@
 namespace qproj {
 
 hipError_t launch_attention_all(const AttentionJob &j, hipStream_t s) {
-    if (rows_apart(j)) return launch_as(j, AllApartArgs{}, s);
+    if (rows_apart(j, false)) return launch_as(j, AllApartArgs{}, s);
     return launch_as(j, AllArgs{}, s);
 }
 

@@ -44,7 +44,7 @@ hipError_t launch_attention_biased(const AttentionJob &j, const float *bias, int
         a.all = all;
         return launch_as(j, a, s);
     };
-    return rows_apart(j) ? with(BiasApartArgs{}) : with(BiasArgs{});
+    return rows_apart(j, true) ? with(BiasApartArgs{}) : with(BiasArgs{});
 }
 
 }  // namespace qproj

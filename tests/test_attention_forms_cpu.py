@@ -8,7 +8,7 @@ import pytest
 
 import forms_ref
 from magnitude_amd import qproj
-from test_attention_forms_gpu import APART
+from test_attention_forms_gpu import APART, APART_WIDE
 from test_attention_cpu import ATTENTION_BAD, BUF, CACHE_BAD, Dry, cache
 
 
@@ -84,7 +84,12 @@ def test_many_rows_of_short_sequences_are_taken_by_waves_of_their_own():
     for page, kv_heads, group, seqs in APART:
         for name in ("cross", "biased"):
             assert "attention_kernel<64, 2, " + {"cross": "all", "biased": "biased"}[name] + ", apart>" in short(name, page, kv_heads, group, seqs), (name, page)
-            assert "apart" not in short(name, page, kv_heads, group, seqs, dim=128)
+            assert "apart" not in short(name, page, kv_heads, group, seqs, dim=256)
+    for page, kv_heads, group, seqs in APART_WIDE:
+        assert "attention_kernel<96, 1, biased, apart>" in short("biased", page, kv_heads, group, seqs, dim=96) and "apart" not in short("biased", page, kv_heads, group, seqs, dim=128)
+        for dim in (96, 128):
+            assert f"attention_kernel<{dim}, 1, all, apart>" in short("cross", page, kv_heads, group, seqs, dim=dim)
+            assert "apart" not in short("cross", page, kv_heads, group, seqs, dim=dim, columns=-(-7 * 64 // page))      # (seven tiles)
     many = [(128, 128)] * 64                                            # 512 items of 128 rows
     assert "grid 512 x 256" in short("cross", 64, 8, 1, many, columns=2) and ", apart>" in short("cross", 64, 8, 1, many, columns=11)
     assert "apart" not in short("cross", 64, 8, 1, many, columns=12)    # (twelve tiles: 576 items)

@@ -73,7 +73,9 @@ APART = [  # of heads of 64, so many rows of short sequences that every wave has
     (128, 1, 71, [(200, 1000)]),
     (128, 64, 1, [(900 - 10 * i, 600) for i in range(5)]),
 ]
+APART_WIDE = [APART[i] for i in (0, 1, 3, 4)]      # of wider heads too
 CROSS += [(64, page, kv_heads, group, seqs) for page, kv_heads, group, seqs in APART]
+CROSS += [(dim, page, kv_heads, group, seqs) for dim in (96, 128) for page, kv_heads, group, seqs in APART_WIDE]
 
 
 @pytest.mark.parametrize("dim,page,kv_heads,group,seqs", CROSS)
@@ -179,6 +181,7 @@ BIASED = [  # dim, page, kv heads, group, [(tokens, rows)], reach
 
 
 BIASED += [(64, page, kv_heads, group, seqs, reach) for (page, kv_heads, group, seqs), reach in zip(APART, (128, 30, 400, 128, 1, 200))]
+BIASED += [(96, page, kv_heads, group, seqs, reach) for (page, kv_heads, group, seqs), reach in zip(APART_WIDE, (128, 30, 128, 500))]
 
 
 @pytest.mark.parametrize("causal", [True, False])
