@@ -26,7 +26,10 @@
 //            of two that the result is kept in.  Probabilities split into two halves too: three products (low x low is under 2^-22).
 //   A lane needs eight tokens' codes of one dimension, memory holds one token's of all: ds_read_b64_tr_b4 turns 16 x 16 nibbles.
 // The running maximum of a row moves only when a score passes it by 2^2.5; until then nothing is rescaled.  Weights are 2^13 at
-// the maximum, so that as pairs of halves they keep 22 bits down to 2^-26 of it, and steps of 2^-37 of it below.
+// the maximum, so that as pairs of halves they keep 22 bits down to 2^-26 of it, and steps of 2^-37 of it below.  A weight's
+// exponent is its score less (the maximum less 13), in one fma.  From maxima of 2^20 on fp32 would round what is in parentheses by too much (from 2^26 on
+// 13 may become 16, and weights pass fp16): there the maximum is taken off first, then 13 is added.  Such rows are rescaled every tile, and that branch does it, so
+// that others pay for it with the compiler's registers only (0.3 % in the mean of 12 calls, 1.3 % at most; as a branch of its own up to 3.5 %).
 //
 // Weights, sums, maxima and results are fp32; every value that goes to the matrix cores has 22 bits.
 //
@@ -62,6 +65,7 @@ constexpr int kTile = 64;            // tokens of a tile
 constexpr float kBias = 13.f;        // weights are 2^kBias at the running maximum
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kSlack = 2.5f;       // a score may pass it by this before the row is rescaled: 2^15.5 < 65504
+constexpr float kFar = 0x1p20f;      // a running maximum this large is taken off the scores before kBias is added
 
 // Who sees what.  A kernel is compiled for one of the argument types below.
 enum Sees {
@@ -821,10 +825,11 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
     asm volatile("" : "+v"(mask0), "+v"(mask1), "+s"(magic), "+s"(minus));
 
     int unit = 0;               // results are in units of 2^unit
+    float limit[NQ];            // a row is rescaled where a score passes this
     float base[NQ];             // what is taken off a score
     uint32_t poison = 0;        // blocks of values that are not finite and were seen, 8 bits a column
 #pragma unroll
-    for (int g = 0; g < NQ; ++g) base[g] = -kBias;
+    for (int g = 0; g < NQ; ++g) base[g] = -kBias, limit[g] = -INFINITY;
 
     int buffer = 0;
     const bool young = (int)blockIdx.x >= a.young;
@@ -1008,26 +1013,6 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
                         s[g][c][r] = 16 * g + r <= last && 16 * g + r > behind && there ? s[g][c][r] : -INFINITY;
                 }
             }
-            float top = -INFINITY;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) top = fmaxf(top, fmaxf(fmaxf(s[g][c][0], s[g][c][1]), fmaxf(s[g][c][2], s[g][c][3])));
-            if constexpr (A::kSees == kBiased) top = fmaf(top, times, plus);
-            else top *= q_unit[c];
-            float back = shrink;
-            if (__ballot(top > st.m[c] + kSlack)) {
-                const float m = fmaxf(st.m[c], max_xor(top));
-                const float f = m == st.m[c] ? 1.f : __builtin_amdgcn_exp2f(st.m[c] - m);
-                st.l[c] *= f;
-                back *= f;
-                st.m[c] = m;
-                base[c] = (m == -INFINITY ? 0.f : m) - kBias;
-            }
-            if (__ballot(back != 1.f)) {
-#pragma unroll
-                for (int x = 0; x < T; ++x)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) st.o[x][c][r] *= back;
-            }
             if (strange) {
                 uint32_t seen = 0;      // bit 4 g + r: the lane's token r of group g
 #pragma unroll
@@ -1041,10 +1026,41 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
                     poison |= (seen & bits ? 1u : 0u) << (8 * c + b);
                 }
             }
+            float top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) top = fmaxf(top, fmaxf(fmaxf(s[g][c][0], s[g][c][1]), fmaxf(s[g][c][2], s[g][c][3])));
+            if constexpr (A::kSees == kBiased) top = fmaf(top, times, plus);
+            else top *= q_unit[c];
+            float back = shrink;
+            if (__ballot(top > limit[c])) {
+                const float m = fmaxf(st.m[c], max_xor(top));
+                const float f = m == st.m[c] ? 1.f : __builtin_amdgcn_exp2f(st.m[c] - m);
+                st.l[c] *= f;
+                back *= f;
+                st.m[c] = m;
+                const bool plain = fabsf(m) < kFar, far = !plain && m != -INFINITY;
+                base[c] = plain ? m - kBias : -kBias;
+                limit[c] = plain ? m + kSlack : -INFINITY;
+                if (__builtin_expect(__ballot(far) != 0, 0)) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[g][c][r] = far ? fmaf(s[g][c][r], times, plus) - m : s[g][c][r];
+                    times = far ? 1.f : times;
+                    plus = far ? 0.f : plus;
+                }
+            }
+            if (__ballot(back != 1.f)) {
+#pragma unroll
+                for (int x = 0; x < T; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) st.o[x][c][r] *= back;
+            }
+            const float off = A::kSees == kBiased ? plus - base[c] : -base[c];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[g][c][r] = __builtin_amdgcn_exp2f(A::kSees == kBiased ? fmaf(s[g][c][r], times, plus - base[c]) : fmaf(s[g][c][r], q_unit[c], -base[c]));
+                for (int r = 0; r < 4; ++r) s[g][c][r] = __builtin_amdgcn_exp2f(fmaf(s[g][c][r], times, off));
                 st.l[c] += (s[g][c][0] + s[g][c][1]) + (s[g][c][2] + s[g][c][3]);
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
