@@ -318,7 +318,7 @@ int qproj_kv_read(qproj_ctx *ctx, const qproj_kv_cache *kv, const int64_t *slots
  * rows, all of them may be), the tokens of a bad page are not seen, and the next qproj_sync reports it.  Where n_tokens or
  * n_seq is 0 nothing is looked at.  Every value accumulates in fp32; queries, weights and values go to the matrix cores as
  * fp16 pairs of 22 bits (of a row's largest query, down to 2^-37 of its largest weight and 2^-36 of the largest value near
- * it).  A score past fp32 and a cached block that is not finite can make the rows that see them not finite, and no others.
+ * it).  A score (or a query times scale) past 2^127 and a cached block that is not finite can make the rows that see them not finite, and no others.
  * The result of a row depends on what else is in the call only in the order of its sums; the same call gives the same bits.
  * y must not overlap q.  max_q should be what it says: it sizes the launch.  A call is refused where
  * min(n_seq * max_q, n_tokens) * n_head / 8 + n_seq * n_head times pages_stride * page_tokens / 256 + 4 passes 2 * 10^9.
@@ -377,7 +377,9 @@ int qproj_bias_by_distance(qproj_ctx *ctx, const float *table_dev, int64_t n_buc
  * encoder's layers do:
  *   y = sum_t softmax_t(scale * q . k_t + bias[h][min(max(t - p, -reach), reach) + reach]) v_t,  p the row's position: its
  * sequence's rows are the last of its tokens either way.  by_distance_dev holds n_head rows of 2 * reach + 1 values (0 <= reach <= 1703), any finite
- * ones or -infinity: a token that this is the bias of is not seen.  With others the rows that meet them are not finite. */
+ * ones or -infinity: a token that this is the bias of is not seen.  With others the rows that meet them are not finite.  A score and its bias are added
+ * in fp32: a large negative bias (-1e9, or -FLT_MAX) hides its token from every row that sees one with an ordinary bias, and a row that sees only such
+ * tokens is their mean with scores rounded as fp32 rounds them beside that bias. */
 typedef struct qproj_position_bias {
     const float *by_distance_dev;
     int64_t reach;

@@ -89,7 +89,7 @@ struct AttentionArgs {
     uint64_t *arrived;       // [2][slots] parts written of the item that a stretch begins and does not end, and above them the call that counts them;
                              // calls use either half in turn.  Null: attention_join_kernel adds the parts
     int32_t *joins;          // [heads][n_seq][row_tiles][2] for it: of every item its first stretch (-1: nothing to join) and its last
-    float scale;             // times log2(e)
+    float scale;             // times log2(e) / kScoreBits
     int32_t n_tokens, n_seq, max_q, window;
     int32_t group;           // query heads of a key/value head
     int32_t splits, split;   // they are served `split` at a time, in `splits` goes
@@ -128,6 +128,10 @@ struct PrefixArgs : AttentionArgs {
     int32_t together;        // sequences of an item
     uint32_t row_part;       // 2^16 / max_q, rounded up
 };
+
+// Scores, their maxima and biases are in powers of 2^kScoreBits: log2(e) takes the largest biases of fp32 past it otherwise.
+template <typename A>
+constexpr float kScoreBits = A::kSees == kBiased ? 4.f : 1.f;
 
 // The kernel's arguments, loaded where they are used from here on.  Kept in registers from the start they are more scalars than there are, and
 // the kernel's phases use different ones.
@@ -976,12 +980,12 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
         u32x4 p_hi[2][NQ], p_lo[2][NQ];
 #pragma unroll
         for (int c = 0; c < NQ; ++c) {
-            float times = q_unit[c], plus = 0.f;     // kBiased: a weight's exponent is s * times + plus
+            float times = q_unit[c], plus = 0.f, lift = 0.f;     // a score is s * times + plus; lift: plus in powers of two, under infinity
             if constexpr (A::kSees == kBiased) {
                 const bool before = t0 + kTile - 1 - it.at <= -a.reach, behind = t0 - (it.at + it.count - 1) >= a.reach;
                 if (before || behind) {              // out of reach of all rows: one bias a head
                     const int slot = c * 16 + col, token = token_of(a, slot), head = token < it.count ? min(slot - token * a.split, heads - 1) : 0;
-                    plus = shared.bias[head * bias_room(a.reach) + (before ? 0 : bias_room(a.reach) - 1)] * kLog2e;
+                    plus = shared.bias[head * bias_room(a.reach) + (before ? 0 : bias_room(a.reach) - 1)] * (kLog2e / kScoreBits<A>);
                     if (__ballot(plus == -INFINITY)) {
 #pragma unroll
                         for (int g = 0; g < 4; ++g)
@@ -989,6 +993,8 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
                             for (int r = 0; r < 4; ++r) s[g][c][r] = plus == -INFINITY ? -INFINITY : s[g][c][r];
                         plus = plus == -INFINITY ? 0.f : plus;
                     }
+                    lift = plus * kScoreBits<A>;         // (a row with a larger bias that has seen any of its tokens is far, see below; of others all are masked here)
+                    lift = lift > 3.402823466e38f ? 3.402823466e38f : lift;
                 } else {
                     const float *const bias = shared.bias + (own_bias[c] + t0 + 4 * part);
 #pragma unroll
@@ -996,7 +1002,7 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const float b = bias[16 * g + r];
-                            s[g][c][r] = b == -INFINITY ? b : fmaf(b, kLog2e, s[g][c][r] * times);
+                            s[g][c][r] = b == -INFINITY ? b : fmaf(b, kLog2e / kScoreBits<A>, s[g][c][r] * times);
                         }
                     times = 1.f;
                 }
@@ -1034,20 +1040,20 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
             float back = shrink;
             if (__ballot(top > limit[c])) {
                 const float m = fmaxf(st.m[c], max_xor(top));
-                const float f = m == st.m[c] ? 1.f : __builtin_amdgcn_exp2f(st.m[c] - m);
+                const float f = m == st.m[c] ? 1.f : __builtin_amdgcn_exp2f((st.m[c] - m) * kScoreBits<A>);
                 st.l[c] *= f;
                 back *= f;
                 st.m[c] = m;
-                const bool plain = fabsf(m) < kFar, far = !plain && m != -INFINITY;
-                base[c] = plain ? m - kBias : -kBias;
-                limit[c] = plain ? m + kSlack : -INFINITY;
+                const bool plain = fabsf(m) < kFar / kScoreBits<A>, far = !plain && m != -INFINITY;
+                base[c] = plain ? m * kScoreBits<A> - kBias : -kBias;
+                limit[c] = plain ? m + kSlack / kScoreBits<A> : -INFINITY;
                 if (__builtin_expect(__ballot(far) != 0, 0)) {
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) s[g][c][r] = far ? fmaf(s[g][c][r], times, plus) - m : s[g][c][r];
                     times = far ? 1.f : times;
-                    plus = far ? 0.f : plus;
+                    lift = far ? 0.f : lift;
                 }
             }
             if (__ballot(back != 1.f)) {
@@ -1056,11 +1062,11 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
 #pragma unroll
                     for (int r = 0; r < 4; ++r) st.o[x][c][r] *= back;
             }
-            const float off = A::kSees == kBiased ? plus - base[c] : -base[c];
+            const float off = A::kSees == kBiased ? lift - base[c] : -base[c], by = times * kScoreBits<A>;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[g][c][r] = __builtin_amdgcn_exp2f(fmaf(s[g][c][r], times, off));
+                for (int r = 0; r < 4; ++r) s[g][c][r] = __builtin_amdgcn_exp2f(fmaf(s[g][c][r], by, off));
                 st.l[c] += (s[g][c][0] + s[g][c][1]) + (s[g][c][2] + s[g][c][3]);
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
@@ -1251,7 +1257,7 @@ __device__ __forceinline__ void meet(const A &a, const Item &it, int head0, int 
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) {
                     const float mw = lds.meet.m[w][lane & 15];
-                    f[w] = mw == m ? 1.f : __builtin_amdgcn_exp2f(mw - m);
+                    f[w] = mw == m ? 1.f : __builtin_amdgcn_exp2f((mw - m) * kScoreBits<A>);
                     l += lds.meet.l[w][lane & 15] * f[w];
                 }
                 const float unit = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
@@ -1331,7 +1337,7 @@ __device__ __forceinline__ void join_parts(const A &a, const Item &it, int head0
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
                     if (w0 + k >= parts) break;
-                    const float f = mw[k] == m ? 1.f : __builtin_amdgcn_exp2f(mw[k] - m);
+                    const float f = mw[k] == m ? 1.f : __builtin_amdgcn_exp2f((mw[k] - m) * kScoreBits<A>);
                     l += lw[k] * f;
 #pragma unroll
                     for (int t = 0; t < kMine; ++t)
@@ -1559,7 +1565,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const A
         float top = m;
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) top = fmaxf(top, mw[k]);
-        const float back = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        const float back = m == top ? 1.f : __builtin_amdgcn_exp2f((m - top) * kScoreBits<A>);
         m = top;
         l *= back;
 #pragma unroll
@@ -1567,7 +1573,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const A
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
             if (w0 + k * kJoinWaves >= parts) break;
-            const float f = mw[k] == m ? 1.f : __builtin_amdgcn_exp2f(mw[k] - m);
+            const float f = mw[k] == m ? 1.f : __builtin_amdgcn_exp2f((mw[k] - m) * kScoreBits<A>);
             l += lw[k] * f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] += v[k][r] * f;
@@ -1598,7 +1604,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const A
     for (int w = 0; w < used; ++w) m = fmaxf(m, tops[w][col]);
     o = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int w = 0; w < used; ++w) {
-        const float f = tops[w][col] == m ? 1.f : __builtin_amdgcn_exp2f(tops[w][col] - m);
+        const float f = tops[w][col] == m ? 1.f : __builtin_amdgcn_exp2f((tops[w][col] - m) * kScoreBits<A>);
         const f32x4 v = sums[w][lane];
         l += weights[w][col] * f;
 #pragma unroll
@@ -1639,7 +1645,7 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
     a.kv_len = j.kv_len;
     a.pages = j.pages;
     a.error = j.error;
-    a.scale = j.scale * kLog2e;
+    a.scale = j.scale * kLog2e / kScoreBits<A>;
     a.window = j.window;
     a.group = j.n_head / j.kv->n_head;
     // 16 rows an item, or 32 of them that share the work of unpacking the codes.  Few rows of work leave most of the chip waiting for a turn of

@@ -11,10 +11,12 @@ from test_attention_gpu import dev, make_cache, numpy_cache, tell, wide
 
 pytestmark = pytest.mark.gpu
 
+MOST = float(np.finfo(np.float32).max)
 SHAPES = [  # dim, page, kv heads, group, [(tokens, rows)], reach
     (64, 16, 2, 2, [(400, 70), (90, 90), (5, 2)], 60),
     (128, 64, 2, 4, [(300, 1), (65, 1), (1, 1)], 128),
     (128, 32, 1, 3, [(500, 40), (70, 90)], 3),                     # more rows than tokens
+    (64, 16, 1, 2, [(100, 40), (30, 50), (0, 3)], 0),              # one bias a head: tiles that are out of reach and not seen
     (96, 32, 1, 3, [(500, 40)], 20),
     (256, 16, 1, 4, [(400, 33)], 30),
     (64, 64, 1, 2, [(20000, 3)], 128),                             # many parts, joined by a launch of their own
@@ -75,7 +77,7 @@ def test_a_large_negative_bias_is_a_mask(ctx, shape, causal):
         hidden[:, cut] = -np.inf
         want, sizes = forms_ref.attention(numpy_cache(kv), q, q_start, lens, pages, kv.head_dim ** -0.5, sees_all=not causal, bias=hidden)
         bound, some = forms_ref.allowed(sizes, kv.head_dim, max(lens)), sizes[2].any(-1)
-        for size in (-1e6, -6e7, -1e8, -1e9, -1e10, -1e30):
+        for size in (-1e6, -6e7, -1e8, -1e9, -1e10, -1e30, -2.5e38, -MOST):
             bias_now = hidden.copy()
             bias_now[:, cut] = size
             for table in tables(kv, pages):
@@ -91,10 +93,10 @@ def test_biases_of_any_size_weigh_alike(ctx, shape, causal):
     """scores of next to nothing: the tokens with the largest bias that a row sees have the same weight, others none"""
     tell("alike", shape, causal)
     rng, kv, pages, q, q_start, lens, reach = make(shape, 72)
-    for size in (6e7, 7e7, 1e8, 3.3e8, 1e9, 1e10, 1e30):
+    for size in (6e7, 7e7, 1e8, 3.3e8, 1e9, 1e10, 1e30, 2.3e38, 2.5e38, MOST):
         for sign in (1, -1):
             bias = np.full((q.shape[1], 2 * reach + 1), sign * size, np.float32)
-            bias[:, rng.random(2 * reach + 1) < 0.5] *= np.float32(0.95 if sign > 0 else 1.05)
+            bias[:, rng.random(2 * reach + 1) < 0.5] *= np.float32(0.95 if sign > 0 else 1.0 if size == MOST else 1.05)
             args = numpy_cache(kv), q, q_start, lens, pages, 1e-30
             want, sizes = forms_ref.attention(*args, sees_all=not causal, bias=bias)
             bound = kv_ref.allowed(sizes[:3], kv.head_dim, max(lens))      # (equal biases are rounded alike)
@@ -109,7 +111,7 @@ def test_biases_that_are_not_finite_reach_who_meets_them(ctx):
     rng = np.random.default_rng(73)
     kv, pages = make_cache(rng, [300], 16, 1, 64)
     q = dev(rng.standard_normal((20, 2, 64)).astype(np.float32))
-    for ordinary in (1.0, -1e8):
+    for ordinary in (1.0, -1e8, -MOST):
         bias = np.full((2, 101), ordinary, np.float32)
         base = ctx.attention_biased(kv, q, i32([0, 20]), i32([300]), dev(pages), dev(bias)).cpu().numpy()
         for bad in (np.inf, np.nan):
@@ -138,6 +140,8 @@ def test_scores_of_every_size(ctx, shape, kind):
     want, lead, steep = np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape[:2])
     scales = numpy_cache(kv)[1]
     for s, (k, v) in enumerate(zip(decoded(kv, pages, lens, 0), decoded(kv, pages, lens, 1))):
+        if not lens[s]:
+            continue
         t = np.arange(lens[s])
         most = 8 * np.repeat(np.abs(scales[pages[s][t // kv.page_tokens], :, t % kv.page_tokens].astype(np.float64)), 32, -1)
         r = np.arange(q_start[s], q_start[s + 1])
