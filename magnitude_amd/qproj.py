@@ -764,7 +764,12 @@ class Context:
                          sync: bool = True) -> torch.Tensor:
         """attention of a batch whose sequences share their first tokens, with what is shared computed once for several of them:
         sequences group_start[g] .. group_start[g + 1] - 1 (i32 [n_groups + 1], from 0 to n_seq) have the same pages for their first
-        shared_len[g] (i32 [n_groups]) tokens.  max_group: the most sequences a group has (default: all of them could be one's)."""
+        shared_len[g] (i32 [n_groups]) tokens.  max_group: the most sequences a group has (default: all of them could be one's).
+        max_q decides whether anything is shared: two sequences' rows have to fit an item (qproj_attention_shared in include/qproj.h).  By
+        default it is read from q_start, a copy to the host; with sync False, where there is none, all rows could be one sequence's and nothing
+        is shared, so give it there."""
+        if max_q is None and sync and q_start.numel() > 1:
+            max_q = max(0, min(q.shape[0], int(q_start.long().diff().max())))     # (bounds that do not hold are reported by the call)
         n, head, tail, y = self._attention_args(kv, q, q_start, kv_len, pages, max_q, scale, out)
         if group_start.numel() != shared_len.numel() + 1:
             raise ValueError("group_start must be [n_groups + 1] and shared_len [n_groups]")
