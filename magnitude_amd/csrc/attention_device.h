@@ -652,7 +652,7 @@ __device__ __forceinline__ void stage_queries(const A &a, const Item &it, int he
 }
 
 // Tiles [from, to) of an item (in tiles from token 0 on), every kWaves-th of them (all of them where the waves are apart).  Two barriers of the workgroup, before and
-// behind the staged queries, whatever there is to do.
+// behind the staged queries (the second alone where the waves are apart), whatever there is to do.
 template <int D, int NQ, typename A>
 __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &members, int kv_head, int head0, int heads, int from, int to, SharedLds<D, NQ, A> &shared,
                                      int wave, Running<D, NQ> &st, int lane) {
@@ -1498,32 +1498,30 @@ __global__ __launch_bounds__(kThreads, kPerCu) void attention_kernel(const A) {
             walk<D, NQ>(a, mine, seqs, kv_head, head0, heads, tile0, min(tile0 + turns, mine.hi / kTile + 1), lds, wave, st, lane);
             leave(a);
             finish<D, NQ>(fresh_arguments<A>(), mine, head0, heads, st, lds, wave, lane);
-            if (!kEarly) move_on();
-            if (at < end) __syncthreads();
-            continue;
-        }
-        walk<D, NQ>(a, it, seqs, kv_head, head0, heads, tile0 + piece.from * kWaves + wave, tile1, lds, wave, st, lane);
-        leave(a);                       // (here, so that nothing waits for it)
-        // ---- the waves' sums ----
-        const bool starts = piece.from == 0, ends = piece.to == turns;
-        meet<D, NQ>(fresh_arguments<A>(), it, head0, heads, st, starts && ends, fresh_arguments<A>().parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ), lds, wave, lane);
-        const A &c = fresh_arguments<A>();
-        if (!c.arrived) {            // whoever writes an item's end says what is to be joined
-            if (ends && id == 0) {
-                int32_t *const join = c.joins + 2 * ((int64_t)hv * units_of(c) + seq * c.row_tiles + row_tile);
-                join[0] = starts ? -1 : (int32_t)stretch_at(line, begin + line.start);
-                join[1] = (int32_t)me;
+        } else {
+            walk<D, NQ>(a, it, seqs, kv_head, head0, heads, tile0 + piece.from * kWaves + wave, tile1, lds, wave, st, lane);
+            leave(a);                       // (here, so that nothing waits for it)
+            // ---- the waves' sums ----
+            const bool starts = piece.from == 0, ends = piece.to == turns;
+            meet<D, NQ>(fresh_arguments<A>(), it, head0, heads, st, starts && ends, fresh_arguments<A>().parts + ((int64_t)me * 2 + (starts ? 1 : 0)) * part_floats(D, NQ), lds, wave, lane);
+            const A &c = fresh_arguments<A>();
+            if (!c.arrived) {            // whoever writes an item's end says what is to be joined
+                if (ends && id == 0) {
+                    int32_t *const join = c.joins + 2 * ((int64_t)hv * units_of(c) + seq * c.row_tiles + row_tile);
+                    join[0] = starts ? -1 : (int32_t)stretch_at(line, begin + line.start);
+                    join[1] = (int32_t)me;
+                }
+            } else if (!(starts && ends)) {
+                // The part is in memory before it is counted (the wait is for the stores); whoever counts the last one loads them after that.
+                const int first = (int)stretch_at(line, begin + line.start), parts = (int)stretch_at(line, begin + line.start + turns - 1) - first + 1;
+                const uint32_t number = call();
+                uint64_t *const word = c.arrived + (number & 1 ? c.slots : 0) + first;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (id == 0) lds.last = arrive(word, number) == (uint32_t)parts;
+                __syncthreads();
+                if (lds.last) join_parts<D, NQ>(c, it, head0, heads, first, parts, lds, wave, lane);
             }
-        } else if (!(starts && ends)) {
-            // The part is in memory before it is counted (the wait is for the stores); whoever counts the last one loads them after that.
-            const int first = (int)stretch_at(line, begin + line.start), parts = (int)stretch_at(line, begin + line.start + turns - 1) - first + 1;
-            const uint32_t number = call();
-            uint64_t *const word = c.arrived + (number & 1 ? c.slots : 0) + first;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (id == 0) lds.last = arrive(word, number) == (uint32_t)parts;
-            __syncthreads();
-            if (lds.last) join_parts<D, NQ>(c, it, head0, heads, first, parts, lds, wave, lane);
         }
         if (!kEarly) move_on();
         if (at < end) __syncthreads();
@@ -1617,10 +1615,13 @@ __global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const A
 template <int D, int NQ, typename A>
 hipError_t launch(const A &a, int groups, int places, hipStream_t s) {
     hipLaunchKernelGGL((attention_kernel<D, NQ, A>), dim3(groups), dim3(kThreads), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.arrived) return e;
-    hipLaunchKernelGGL((attention_join_kernel<D, NQ, A>), dim3(places, D / 16 * NQ), dim3(64 * kJoinWaves), 0, s, a);
-    return hipGetLastError();
+    const hipError_t e = hipGetLastError();
+    if constexpr (!A::kApart) {      // (whose items stay whole)
+        if (e != hipSuccess || a.arrived) return e;
+        hipLaunchKernelGGL((attention_join_kernel<D, NQ, A>), dim3(places, D / 16 * NQ), dim3(64 * kJoinWaves), 0, s, a);
+        return hipGetLastError();
+    }
+    return e;
 }
 
 // numbers of calls and counts of parts, what the joining kernel is to do, then the parts; zeros before the first call
