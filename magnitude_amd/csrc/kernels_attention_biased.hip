@@ -47,4 +47,17 @@ hipError_t launch_attention_biased(const AttentionJob &j, const float *bias, int
     return rows_apart(j, true) ? with(BiasApartArgs{}) : with(BiasArgs{});
 }
 
+// For the tests: as attention_pieces, where every wave has rows of its own; rows see what lies before them, or all.
+int64_t attention_apart_pieces(const AttentionJob &j, bool all, const int32_t *kv_len_later, int64_t most_len, int tokens, int heads, int groups, int32_t *out, int64_t room) {
+    BiasApartArgs a{};
+    a.all = all;
+    a.pages_stride = most_len;      // (pages of one token)
+    a.n_tokens = (int32_t)j.n_tokens, a.n_seq = (int32_t)j.n_seq, a.max_q = (int32_t)j.max_q;
+    a.q_start = j.q_start, a.kv_len = j.kv_len;
+    a.tokens = tokens;
+    a.row_tiles = std::max(1, (a.max_q + tokens - 1) / tokens);
+    a.most_items = a.n_tokens / tokens + a.n_seq;
+    return pieces_of(a, kv_len_later, heads, groups, out, room);
+}
+
 }  // namespace qproj

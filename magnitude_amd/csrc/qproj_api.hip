@@ -1976,6 +1976,18 @@ int64_t qproj_internal_attention_pieces(const int32_t *q_start, const int32_t *k
     return attention_pieces(j, kv_len_later ? kv_len_later : kv_len, most_len, (int)tokens, (int)heads, (int)groups, out, room);
 }
 
+// The same of a call whose waves have rows of their own; `all`: rows see all tokens.
+int64_t qproj_internal_attention_apart_pieces(const int32_t *q_start, const int32_t *kv_len, const int32_t *kv_len_later, int64_t n_seq, int64_t n_tokens, int64_t max_q, int32_t all,
+                                              int64_t most_len, int64_t tokens, int64_t heads, int64_t groups, int32_t *out, int64_t room) {
+    AttentionJob j{};
+    j.q_start = q_start;
+    j.kv_len = kv_len;
+    j.n_seq = n_seq;
+    j.n_tokens = n_tokens;
+    j.max_q = max_q;
+    return attention_apart_pieces(j, all != 0, kv_len_later ? kv_len_later : kv_len, most_len, (int)tokens, (int)heads, (int)groups, out, room);
+}
+
 // The same of a call with groups of sequences that share their first tokens, `together` sequences an item.
 int64_t qproj_internal_attention_shared_pieces(const int32_t *q_start, const int32_t *kv_len, const int32_t *kv_len_later, int64_t n_seq, int64_t n_tokens, int64_t max_q,
                                                const int32_t *group_start, const int32_t *shared_len, int64_t n_groups, int64_t max_group, int64_t most_len, int64_t together,

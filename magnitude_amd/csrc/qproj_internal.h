@@ -358,6 +358,7 @@ int attention_most_reach();
 hipError_t launch_attention_biased(const AttentionJob &j, const float *bias, int reach, bool all, hipStream_t s);   // bias [n_head][2 * reach + 1]
 hipError_t launch_bias_by_distance(const float *table, int n_buckets, int n_head, const int32_t *buckets, int reach, float *out, int32_t *error, hipStream_t s);
 int64_t attention_pieces(const AttentionJob &j, const int32_t *kv_len_later, int64_t most_len, int tokens, int heads, int groups, int32_t *out, int64_t room);   // for the tests
+int64_t attention_apart_pieces(const AttentionJob &j, bool all, const int32_t *kv_len_later, int64_t most_len, int tokens, int heads, int groups, int32_t *out, int64_t room);   // too
 int64_t attention_shared_pieces(const AttentionJob &j, const SharedGroups &g, const int32_t *kv_len_later, int64_t most_len, int together, int heads, int groups, int32_t *out, int64_t room);   // too
 
 }  // namespace qproj
