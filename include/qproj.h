@@ -379,7 +379,7 @@ int qproj_bias_by_distance(qproj_ctx *ctx, const float *table_dev, int64_t n_buc
  * sequence's rows are the last of its tokens either way.  by_distance_dev holds n_head rows of 2 * reach + 1 values (0 <= reach <= 1703), any finite
  * ones or -infinity: a token that this is the bias of is not seen.  With others the rows that meet them are not finite.  A score and its bias are added
  * in fp32: a large negative bias (-1e9, or -FLT_MAX) hides its token from every row that sees one with an ordinary bias, and a row that sees only such
- * tokens is their mean with scores rounded as fp32 rounds them beside that bias. */
+ * tokens is their mean with scores rounded at most as fp32 rounds them beside that bias. */
 typedef struct qproj_position_bias {
     const float *by_distance_dev;
     int64_t reach;

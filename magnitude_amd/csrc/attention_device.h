@@ -1051,7 +1051,11 @@ __device__ __forceinline__ void walk(const A &a, const Item &it, const Members &
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[g][c][r] = far ? fmaf(s[g][c][r], times, plus) - m : s[g][c][r];
+                        for (int r = 0; r < 4; ++r) {
+                            // (plus - m is exact where it matters.  m is rounded, scores beside a large bias are not: they may pass it by half a step of fp32)
+                            const float x = fmaf(s[g][c][r], times, plus - m);
+                            s[g][c][r] = !far ? s[g][c][r] : x > kSlack / kScoreBits<A> ? kSlack / kScoreBits<A> : x;
+                        }
                     times = far ? 1.f : times;
                     lift = far ? 0.f : lift;
                 }

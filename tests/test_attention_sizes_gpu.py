@@ -106,6 +106,23 @@ def test_biases_of_any_size_weigh_alike(ctx, shape, causal):
                 assert (np.abs(got - want) <= bound).all(), (size, sign)
 
 
+@pytest.mark.parametrize("dim,page,kv_heads,group,lens", [(64, 64, 2, 4, [1024, 640, 128]), (128, 32, 8, 4, [4096, 192]), (256, 16, 1, 2, [448]), (64, 64, 1, 2, [20480])])
+def test_a_bias_that_all_tokens_have_changes_nothing(ctx, dim, page, kv_heads, group, lens):
+    """tiles that are out of reach take their one bias off without rounding scores beside it, as long as steps of fp32 there are under what a score may pass
+    the row's largest by: (largest, rounded by 2) up to 2^26 in powers of two"""
+    rng, kv, pages, q, q_start, lens, reach = make((dim, page, kv_heads, group, [(n, 1) for n in lens], 64), 75)
+    bias = np.full((q.shape[1], 2 * reach + 1), -np.inf, np.float32)      # the last 64 tokens, a tile, are not seen
+    bias[:, 0] = 0
+    want, sizes = forms_ref.attention(numpy_cache(kv), q, q_start, lens, pages, dim ** -0.5, bias=bias)
+    bound = kv_ref.allowed(sizes[:3], dim, max(lens))
+    for size in (0, 300, 1e5, 8e5, 1e6, 3e6, 1e7, 3e7, 4.6e7):
+        for sign in (1, -1):
+            bias[:, 0] = sign * size
+            for table in tables(kv, pages):
+                got = ctx.attention_biased(kv, dev(q), i32(q_start), i32(lens), dev(table), dev(bias), max_q=1).cpu().numpy()
+                assert (np.abs(got - want) <= bound).all(), sign * size
+
+
 def test_biases_that_are_not_finite_reach_who_meets_them(ctx):
     """among others of any size: +infinity and NaN make the rows that see their tokens not finite, no others"""
     rng = np.random.default_rng(73)
