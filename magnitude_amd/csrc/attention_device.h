@@ -1687,8 +1687,8 @@ hipError_t launch_as(const AttentionJob &j, A a, hipStream_t s) {
             a.most_items = a.n_seq / a.together + a.n_groups;
             items = std::min((double)a.n_groups * a.row_tiles, (double)a.most_items) * j.kv->n_head * a.splits;
             // 16 columns, where they hold two sequences: a tile of 32 takes 1.77 times as long, and of a sequence's own tokens only its columns are any use.  32
-            // save where what is shared is about 26 times as long as what is not (four heads a key/value head, one row): taken for so where a
-            // sequence can have 32768 tokens.  48 sequences behind 8192 tokens with 30 to 1500 of their own 45.0 us in sixteens and 50.2 in 32s, four groups of
+            // save where what is shared is about 26 times as long as what is not (four heads a key/value head, one row).  The host knows neither, only how
+            // wide the table is: taken for so where a sequence can have 32768 tokens, so that short ones in such a table pay for the width.  48 sequences behind 8192 tokens with 30 to 1500 of their own 45.0 us in sixteens and 50.2 in 32s, four groups of
             // nine with up to four rows 26.8 and 31.4, 32 sequences behind 65536 with 10 to 400 of their own 126 and 105.
             if (a.max_group * a.max_q * a.group <= 16 || (a.together >= 2 && most_len < 32768)) break;
         }

@@ -5,9 +5,9 @@
 // at constant offsets from one address, any other tile has one a head.  (A bias of -infinity hides its token, also where the key is not finite: the choice costs 1 to 2 %.)
 //
 // What bounds it, as of every kind: issue slots, and where sequences are short the finding and staging of items.  Encoders of 16 heads of 64, reach 128: eight
-// texts of up to 512 tokens 34.7 us; one of 4096 231 us, 68.7 Gflop (2.5 times that on the matrix cores, as pairs of halves: 740 Tflop/s).  Two prompts of 500 behind
-// 100 to 900, 24 heads of 96 on 8, reach 400, 60.8 us, of which the biases are some 5.  A token of 16 sequences of up to
-// 512, 16 heads of 64, 10.9.
+// texts of up to 512 tokens 35.0 us; one of 4096 233 us, 68.7 Gflop (2.5 times that on the matrix cores, as pairs of halves: 735 Tflop/s).  Two prompts of 500 behind
+// 100 to 900, 24 heads of 96 on 8, reach 400, 61.2 us, of which the biases are some 5.  A token of 16 sequences of up to
+// 512, 16 heads of 64, 11.0.
 #include "attention_device.h"
 
 namespace qproj {

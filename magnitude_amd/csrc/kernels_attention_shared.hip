@@ -6,10 +6,10 @@
 // of that sequence alone and as many columns.
 //
 // What bounds it, as of every kind: the vector units' and the matrix cores' issue slots, 690 vector instructions and 80 products a tile and 16 columns.  48
-// sequences behind 8192 tokens with 30 to 1500 of their own (32 heads of 128 on 8, one row) 45.2 us, 54 MB that have to be read; 48 % of a SIMD's
-// cycles issue vector instructions, 17 % matrix ones.  The causal kernel, which reads what is shared 48 times, takes 98 us.  32
-// behind 65536 with 10 to 400 of their own 105 us (84 MB, 34 Gflop); two behind 1024 13.6; four groups of nine, up to four rows,
-// 14 heads of 64 on 7, 26.3.  (Batches of the loads of an item's sequences in the scan, four or eight at a time: level or up to 5 % more.)
+// sequences behind 8192 tokens with 30 to 1500 of their own (32 heads of 128 on 8, one row) 45.7 us, 54 MB that have to be read; 48 % of a SIMD's
+// cycles issue vector instructions, 17 % matrix ones.  The causal kernel, which reads what is shared 48 times, takes 98 us (and where nothing is shared 98 against 107).  32
+// behind 65536 with 10 to 400 of their own 106 us (84 MB, 34 Gflop); two behind 1024 13.8; four groups of nine, up to four rows,
+// 14 heads of 64 on 7, 26.8.  (Batches of the loads of an item's sequences in the scan, four or eight at a time: level or up to 5 % more.)
 #include "attention_device.h"
 
 namespace qproj {

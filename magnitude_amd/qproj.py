@@ -821,7 +821,8 @@ class Context:
                          bias: torch.Tensor, causal: bool = True, max_q: Optional[int] = None, scale: Optional[float] = None,
                          out: Optional[torch.Tensor] = None, sync: bool = True) -> torch.Tensor:
         """As attention, with bias f32 [heads, 2 * reach + 1] (bias_by_distance) of token - row, clamped to -reach .. reach, added to the
-        scaled scores; causal False: every row sees all tokens of its sequence (an encoder's layers)."""
+        scaled scores; causal False: every row sees all tokens of its sequence (an encoder's layers).  A model that does not scale its
+        scores wants scale=1 (the default is 1 / sqrt(head_dim), as in attention)."""
         n, head, tail, y = self._attention_args(kv, q, q_start, kv_len, pages, max_q, scale, out)
         if bias.dim() != 2 or bias.shape[0] != q.shape[1] or bias.shape[1] % 2 != 1:
             raise ValueError("bias must be [heads, 2 * reach + 1]")
