@@ -769,7 +769,7 @@ class Context:
         default it is read from q_start, a copy to the host; with sync False, where there is none, all rows could be one sequence's and nothing
         is shared, so give it there."""
         if max_q is None and sync and q_start.numel() > 1:
-            max_q = max(0, min(q.shape[0], int(q_start.long().diff().max())))     # (bounds that do not hold are reported by the call)
+            max_q = max(0, int(q_start.flatten().long().diff().max()))     # (bounds that do not hold are reported by the call)
         n, head, tail, y = self._attention_args(kv, q, q_start, kv_len, pages, max_q, scale, out)
         if group_start.numel() != shared_len.numel() + 1:
             raise ValueError("group_start must be [n_groups + 1] and shared_len [n_groups]")
